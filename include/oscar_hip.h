@@ -555,6 +555,73 @@ int oscar_calibrated_rotations(const float* covariances, int32_t batch, int32_t 
                                int64_t workspace_bytes, float* rotations, float* eigenvalues,
                                float* info, void* stream);
 
+/*
+ * qk_norm_rope -- norms of the queries and keys of each head and the position rotation in one
+ * pass (no reference counterpart: the reference's layer starts behind them). Per (token, head) row
+ * of 256: y = x / sqrt(mean(x^2) + eps) * w, w = weight (+ 1 with unit_offset); then the pairs of
+ * the first rotary_dim dims (even, 0..256; dims i and i + rotary_dim / 2, or 2 i and 2 i + 1 when
+ * interleaved) are turned by the angles of the token's position: cos_sin row `position` holds the
+ * cosines of the pairs, then their sines (rows table_stride elements apart). fp32 arithmetic, one
+ * rounding to bf16. query [n][hq][256], key [n][hk][256]: bf16, strides multiples of 8, rows
+ * contiguous and 16-byte aligned. Weights [256] and cos_sin: bf16 or fp32 (the flags). q_out, k_out:
+ * contiguous bf16. counts (optional, as for the other entry points): rows of tokens at or past
+ * counts[1] are zeroed and their positions not read. A live token whose position is outside
+ * [0, table_rows) gets NaN rows. rk_t and q_rot (both or neither): q_rot [n][hq][256] receives
+ * rotate(q_out, R_k), with the bits of oscar_rotate (rk_t: R_k^T, contiguous bf16 [256][256]).
+ */
+int oscar_qk_norm_rope(const void* query, int64_t q_s0, int64_t q_s1, const void* key,
+                       int64_t k_s0, int64_t k_s1, int64_t n, int64_t hq, int64_t hk,
+                       const void* q_weight, const void* k_weight, int32_t weight_fp32,
+                       int32_t unit_offset, float eps, const void* cos_sin, int64_t table_rows,
+                       int64_t table_stride, int32_t table_fp32, int32_t rotary_dim,
+                       int32_t interleaved, const int64_t* positions, const int32_t* counts,
+                       void* q_out, void* k_out, const void* rk_t, void* q_rot, void* stream);
+
+/*
+ * Pages of the caches of a model's layers (no reference counterpart). `stripes`: device array of
+ * `layers` pairs of addresses, the K stripe (INT2 records) and the V stripe (BF16 windows) of each
+ * layer, num_pages physical pages each, 16-byte aligned; `table`: int32 block table (rows of
+ * table_stride elements) whose entry j holds kernel block j of a request; seq_lens: tokens per row.
+ * A page is in use when a row below counts[0] maps one of its seq_lens tokens to it; table entries
+ * outside the pool are skipped.
+ *
+ * free_pages: `pages` [num_pages] receives the free pages in ascending order, then -1; count [1]
+ * their number. `used`: scratch of num_pages.
+ */
+int oscar_free_pages(int64_t num_pages, const int32_t* table, int64_t table_stride,
+                     int64_t table_columns, int64_t rows, const int32_t* seq_lens,
+                     const int32_t* counts, const oscar_layout* layout, int32_t* used,
+                     int32_t* pages, int32_t* count, void* stream);
+
+/*
+ * fork_requests -- row children[i] becomes a request that continues the tokens of row parents[i]:
+ * it maps the parent's full pages, except the first, which is copied into page fresh[i][0] with the
+ * BF16 window (the page has one owner), and an unfinished last page (of several), which is copied
+ * into fresh[i][1]. Only records and window rows of the parent's tokens are copied; table columns
+ * past its last page keep their values. status[i]: 1, or 0 for a fork that was refused and wrote
+ * nothing: a row outside the table, a parent that is some fork's child, a child row or a needed
+ * fresh page that an earlier entry lists too, a needed fresh page outside the pool or among the
+ * parent's, a parent's page outside the pool. Fresh pages must be free. forks <= 4096.
+ */
+int oscar_fork_requests(const void* stripes, int64_t layers, int64_t num_pages, int32_t* table,
+                        int64_t table_stride, int64_t table_columns, int64_t rows,
+                        int32_t* seq_lens, const int32_t* parents, const int32_t* children,
+                        const int32_t* fresh, int64_t forks, const oscar_layout* layout,
+                        int32_t* status, void* stream);
+
+/*
+ * compact_pages -- moves the pages in use to the pool's start: with `live` pages in use, those
+ * below page `live` stay and the k-th one above moves to the k-th free one below (records and window
+ * rows in use only; the old page keeps its bytes). new_table [rows][table_columns] receives the table
+ * with the entries of live tokens' pages changed; live [1] the number of pages in use: every page
+ * from there on is free. scratch: 5 num_pages + 1 values.
+ */
+int oscar_compact_pages(const void* stripes, int64_t layers, int64_t num_pages,
+                        const int32_t* table, int64_t table_stride, int64_t table_columns,
+                        int64_t rows, const int32_t* seq_lens, const int32_t* counts,
+                        const oscar_layout* layout, int32_t* scratch, int32_t* new_table,
+                        int32_t* live, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -183,6 +183,17 @@ SIGNATURES = {
     "oscar_normalize": [_P, _I64, _P, _F, _P, _P],
     "oscar_calibration_workspace_bytes": [_I32, _I32],
     "oscar_calibrated_rotations": [_P, _I32, _I32, _I32, _F, _P, _I64, _P, _P, _P, _P],
+    "oscar_qk_norm_rope": [
+        _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64,  # query, key (+ strides), n, hq, hk
+        _P, _P, _I32, _I32, _F,  # q weight, k weight, weight fp32, unit offset, eps
+        _P, _I64, _I64, _I32, _I32, _I32,  # cos_sin, rows, stride, fp32, rotary dim, interleaved
+        _P, _P, _P, _P, _P, _P, _P,  # positions, counts, q out, k out, rk_t, q rot, stream
+    ],
+    "oscar_free_pages": [_I64, _P, _I64, _I64, _I64, _P, _P, POINTER(OscarLayout), _P, _P, _P, _P],
+    "oscar_fork_requests": [_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64,
+                            POINTER(OscarLayout), _P, _P],
+    "oscar_compact_pages": [_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, POINTER(OscarLayout), _P,
+                            _P, _P, _P],
 }
 RESTYPES = {"oscar_noalloc_scratch_bytes": c_int64, "oscar_calibration_workspace_bytes": c_int64,
             "oscar_history_chunk_tiles": c_int64}

@@ -25,6 +25,7 @@ __all__ = [
     "merge_paths",
     "store_windows",
     "dequant_inverse_rotate",
+    "qk_norm_rope",
     "pre_attention",
     "post_attention",
     "history_post",
@@ -409,6 +410,84 @@ def dequant_inverse_rotate(history, slots, rk, rv, layout):
             "dequant_inverse_rotate",
         )
     return rotate(k, rk.T), rotate(v, rv.T)
+
+
+def _same_device(first, **others):
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} must be on {first.device}, got {t.device}")
+
+
+def _vector(t, name):
+    """A contiguous 16-byte aligned bf16 or fp32 vector of one head."""
+    if t.dtype not in (torch.bfloat16, torch.float32) or tuple(t.shape) != (256,):
+        raise ValueError(f"{name} must be a bf16 or fp32 vector of 256, got {t.dtype} "
+                         f"{tuple(t.shape)}")
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None, eps=1e-6,
+                 unit_offset=False, interleaved=False, rk_t=None):
+    """Norms of the queries and keys of each head with the position rotation in the same pass (no
+    reference counterpart; what a model computes ahead of backend.py:125-140).
+
+    ``query`` [n, hq, 256], ``key`` [n, hk, 256]: bf16, any strides (rows that are contiguous and
+    16-byte aligned, such as slices of a packed projection output, are read in place). Per row
+    ``y = x / sqrt(mean(x^2) + eps) * w`` with w the weight (bf16 or fp32 [256]; ``1 + weight`` with
+    ``unit_offset``), then the pairs of the first ``cos_sin.shape[1]`` dims, (i, i + half) or, with
+    ``interleaved``, (2 i, 2 i + 1), are turned by row ``positions[token]`` (int64) of ``cos_sin``
+    (bf16 or fp32 [positions, rotary]: the pairs' cosines, then their sines). With ``counts`` the
+    rows of tokens at or past ``counts[1]`` are zeros; a live token whose position is outside the
+    table gets NaN rows.
+
+    Returns ``(query, key)``, contiguous bf16; with ``rk_t`` (R_k^T, contiguous bf16 [256, 256])
+    ``(query, key, rotate(query, R_k))``, the third with the bits of ``rotate``.
+    """
+    _device_check(query, key, q_weight, k_weight, cos_sin, positions, counts, rk_t)
+    _same_device(query, key=key, q_weight=q_weight, k_weight=k_weight, cos_sin=cos_sin,
+                 positions=positions, counts=counts, rk_t=rk_t)
+    n, hq, d = query.shape
+    hk = key.shape[1]
+    if d != 256 or tuple(key.shape) != (n, hk, 256):
+        raise ValueError("query and key must be [n, heads, 256] of the same tokens")
+    if cos_sin.dim() != 2 or cos_sin.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("cos_sin must be a bf16 or fp32 [positions, rotary] table")
+    rows, rotary = cos_sin.shape
+    if rotary % 2 or rotary > 256 or (rotary and not rows):
+        raise ValueError(f"the rotary dims must be even and at most 256, got {rotary} of {rows} "
+                         "positions")
+    if rotary and cos_sin.stride(1) != 1 or rows > 1 and cos_sin.stride(0) < rotary:
+        cos_sin = cos_sin.contiguous()
+    if positions.dtype != torch.int64 or tuple(positions.shape) != (n,):
+        raise ValueError("positions must be int64, one per token")
+    if counts is not None and (_int32(counts, "counts").numel() < 2 or not counts.is_contiguous()):
+        raise ValueError("counts must hold (requests, tokens)")
+    if rk_t is not None and (rk_t.dtype != torch.bfloat16 or not rk_t.is_contiguous()
+                             or tuple(rk_t.shape) != (256, 256)):
+        raise ValueError("rk_t must be contiguous bf16 [256, 256] (R_k transposed)")
+    q_weight, k_weight = _vector(q_weight, "q_weight"), _vector(k_weight, "k_weight")
+    if q_weight.dtype != k_weight.dtype:
+        q_weight, k_weight = q_weight.float(), k_weight.float()
+    out = [torch.empty((n, h, 256), dtype=torch.bfloat16, device=query.device)
+           for h in ((hq, hk) if rk_t is None else (hq, hk, hq))]
+    if n:
+        query, key = (t if t.data_ptr() % 16 == 0 else t.clone()
+                      for t in (_rows_contiguous(query), _rows_contiguous(key)))
+        positions = positions.contiguous()
+        with torch.cuda.device(query.device):
+            _ext.check(
+                _ext.library().oscar_qk_norm_rope(
+                    _ptr(query), *query.stride()[:2], _ptr(key), *key.stride()[:2], n, hq, hk,
+                    _ptr(q_weight), _ptr(k_weight), int(q_weight.dtype == torch.float32),
+                    int(unit_offset), float(eps), _ptr(cos_sin), rows,
+                    max(cos_sin.stride(0), rotary), int(cos_sin.dtype == torch.float32), rotary,
+                    int(interleaved), _ptr(positions), _ptr(counts), _ptr(out[0]), _ptr(out[1]),
+                    _ptr(rk_t), _ptr(out[2]) if rk_t is not None else None, _stream(query),
+                ),
+                "qk_norm_rope",
+            )
+    return tuple(out)
 
 
 # --------------------------------------------------------------------------- fused launches

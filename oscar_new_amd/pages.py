@@ -1,0 +1,152 @@
+"""Pages of a model's caches: free pages, forked requests, compaction (``csrc/pages.hip``).
+
+No reference counterpart: the reference refuses page copies (backend.py:30-38), because the first
+page of a request holds its BF16 window and so has one owner. Its other pages hold INT2 records that
+nothing writes again once a page is full, so requests that continue the same tokens may map them
+together. A fork does that: it copies the first page and an unfinished last one and shares the rest.
+``kernels.shared_history`` then computes the attention over the shared positions once for all of
+them.
+
+Everything stays on the device: no call reads back, synchronizes or allocates anything but its
+outputs, so calls can be captured in a graph. Page numbers are physical pages (a block table's entry
+divided by the kernel blocks of a page). All calls take the block table and the token counts of the
+scheduler's rows: row r holds ``seq_lens[r]`` tokens in the blocks of ``block_tables[r]``, and the
+rows below ``counts[0]`` are live.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _ext
+from .kernels import _device_check, _int32, _ptr, _same_device, _stream, layout_struct
+
+__all__ = ["PageCaches", "free_pages", "fork_requests", "compact_pages"]
+
+
+class PageCaches:
+    """The caches of a model's layers, for page copies in all of them with one launch.
+
+    ``kv_caches``: one native ``(K, V)`` cache view pair per layer (``CacheLayout.tensor_views``),
+    all of the same page count on one device. Keeps the views and a device table of their
+    addresses.
+    """
+
+    def __init__(self, kv_caches, layout):
+        views = [layout.tensor_views(pair) for pair in kv_caches]
+        if not views:
+            raise ValueError("PageCaches needs at least one layer's cache")
+        history, window = views[0]
+        _device_check(*(t for pair in views for t in pair))
+        for pair in views:
+            if any(t.device != history.device for t in pair):
+                raise ValueError("all layers' caches must be on one device")
+            if pair[0].numel() != history.numel():
+                raise ValueError("all layers' caches must have the same number of pages")
+            if any(t.data_ptr() % 16 for t in pair):
+                raise ValueError("cache stripes must be 16-byte aligned")
+        self.layout = layout
+        self.views = views
+        self.device = history.device
+        self.num_pages = history.numel() // layout.stripe_page_bytes
+        if not self.num_pages:
+            raise ValueError("the caches hold no pages")
+        self.stripes = torch.tensor([[t.data_ptr() for t in pair] for pair in views],
+                                    dtype=torch.int64, device=self.device)
+
+
+def _table(caches, block_tables, seq_lens, counts=None, **others):
+    """Checks of the scheduler's tensors; the arguments of the block table."""
+    _device_check(block_tables, seq_lens, counts, *others.values())
+    _same_device(caches.stripes, block_tables=block_tables, seq_lens=seq_lens, counts=counts,
+                 **others)
+    if block_tables.dim() != 2 or 0 in block_tables.shape:
+        raise ValueError("block_tables must be [rows, columns]")
+    if _int32(block_tables, "block_tables").stride(1) != 1 and block_tables.shape[1] > 1:
+        raise ValueError("block table rows must be contiguous")
+    rows, columns = block_tables.shape
+    stride = block_tables.stride(0) if rows > 1 else max(block_tables.stride(0), columns)
+    if stride < columns:
+        raise ValueError("block table rows must not overlap")
+    if _int32(seq_lens, "seq_lens").dim() != 1 or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be a contiguous vector")
+    if seq_lens.shape[0] < rows:
+        raise ValueError("seq_lens must hold one count per block table row")
+    if counts is not None and (_int32(counts, "counts").numel() < 1 or not counts.is_contiguous()):
+        raise ValueError("counts must hold the number of live rows first")
+    return _ptr(block_tables), stride, columns, rows
+
+
+def free_pages(caches, block_tables, seq_lens, counts):
+    """Pages that no token of a live row is mapped to: ``(pages, count)``, int32 ``[num_pages]`` with
+    the free pages in ascending order and -1 behind them, and int32 ``[1]``."""
+    table = _table(caches, block_tables, seq_lens, counts)
+    used = torch.empty(caches.num_pages, dtype=torch.int32, device=caches.device)
+    pages = torch.empty_like(used)
+    count = torch.empty(1, dtype=torch.int32, device=caches.device)
+    with torch.cuda.device(caches.device):
+        _ext.check(
+            _ext.library().oscar_free_pages(
+                caches.num_pages, *table, _ptr(seq_lens), _ptr(counts),
+                layout_struct(caches.layout), _ptr(used), _ptr(pages), _ptr(count),
+                _stream(used)),
+            "free_pages",
+        )
+    return pages, count
+
+
+def fork_requests(caches, block_tables, seq_lens, parents, children, fresh):
+    """Rows ``children[i]`` become requests that continue the tokens of rows ``parents[i]``.
+
+    ``parents``, ``children``: int32 ``[forks]`` rows of ``block_tables``, which is changed in place,
+    as is ``seq_lens``; ``fresh``: int32 ``[forks, 2]`` free pages (such as the first ones of
+    ``free_pages``), the child's first page and its copy of an unfinished last page (not used when
+    the parent's tokens end with a page, or in the first one). In every layer the parent's records
+    and window rows of those pages are copied, nothing else of them is written; table columns past
+    the parent's last page keep their values.
+
+    Returns int32 ``[forks]``: 1, or 0 for a fork that was refused and wrote nothing (a row outside
+    the table, a parent that is also some fork's child, a child row or a needed page that an earlier
+    fork lists too, a needed page outside the pool or among the parent's own, a parent's page
+    outside the pool). At most 4096 forks a call.
+    """
+    table = _table(caches, block_tables, seq_lens, parents=parents, children=children, fresh=fresh)
+    forks = parents.numel()
+    for name, t, shape in (("parents", parents, (forks,)), ("children", children, (forks,)),
+                           ("fresh", fresh, (forks, 2))):
+        if tuple(_int32(t, name).shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}")
+    status = torch.empty(forks, dtype=torch.int32, device=caches.device)
+    with torch.cuda.device(caches.device):
+        _ext.check(
+            _ext.library().oscar_fork_requests(
+                _ptr(caches.stripes), len(caches.views), caches.num_pages, *table,
+                _ptr(seq_lens), _ptr(parents), _ptr(children), _ptr(fresh), forks,
+                layout_struct(caches.layout), _ptr(status), _stream(status)),
+            "fork_requests",
+        )
+    return status
+
+
+def compact_pages(caches, block_tables, seq_lens, counts):
+    """Moves the pages in use to the pool's start in every layer.
+
+    Returns ``(tables, live)``: int32 ``[1]`` the number of pages in use, and the block table with
+    every live token's blocks where they are now, all below page ``live``; the pages from there on
+    are free. Pages below ``live`` that were in use stay, the k-th one above moves to the k-th free
+    one below. ``block_tables`` is not changed (a caller with fixed buffers copies the new one in),
+    slot mappings made from it are stale.
+    """
+    table = _table(caches, block_tables, seq_lens, counts)
+    scratch = torch.empty(5 * caches.num_pages + 1, dtype=torch.int32, device=caches.device)
+    tables = torch.empty(tuple(block_tables.shape), dtype=torch.int32, device=caches.device)
+    live = torch.empty(1, dtype=torch.int32, device=caches.device)
+    with torch.cuda.device(caches.device):
+        _ext.check(
+            _ext.library().oscar_compact_pages(
+                _ptr(caches.stripes), len(caches.views), caches.num_pages, *table,
+                _ptr(seq_lens), _ptr(counts), layout_struct(caches.layout), _ptr(scratch),
+                _ptr(tables), _ptr(live), _stream(scratch)),
+            "compact_pages",
+        )
+    return tables, live
