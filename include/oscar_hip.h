@@ -622,6 +622,39 @@ int oscar_compact_pages(const void* stripes, int64_t layers, int64_t num_pages,
                         const oscar_layout* layout, int32_t* scratch, int32_t* new_table,
                         int32_t* live, void* stream);
 
+/*
+ * shared_plan / shared_history -- the history branch of a step whose requests share long prefixes,
+ * with each group's shared positions computed once for all its rows, merged: what
+ * oscar_attention_partials (raw = 0) followed by oscar_merge_splits gives, within rounding (no
+ * reference counterpart as one call: kernels.py:290-482 and 485-511, oscar_ascend).
+ *
+ * shared_plan, once per step: group g is the requests group_starts[g] .. group_starts[g + 1] - 1
+ * (int32 [groups + 1], ascending; requests of no group share nothing), whose first
+ * prefix_tokens[g] positions hold the same records (pages may differ: the first member's are
+ * read). It writes the step's units (int32 [capacity][8], 16-byte aligned), their number and the
+ * partial rows of every token below counts[1] (token_slots, int32 [tokens]). `slots` (4..64) bounds
+ * the partial rows of a row; tokens the query tokens of the step; capacity at least 256 / kv_heads
+ * + 2 (tokens * (hq / kv_heads) / 128) + groups + min(max_reqs, tokens). groups + max_reqs <= 8192
+ * and hq / kv_heads <= 32, else OSCAR_E_UNSUPPORTED. Starts that descend share nothing.
+ *
+ * shared_history, per layer: query is the rotated query, partials fp32 [n][hq][slots][256] and lse
+ * [n][hq][slots] scratch, out bf16 [n][hq][256] (fp32 with fp32_out, the layout of one split's
+ * partials), out_lse fp32 [n][hq]. Rows of tokens at or past counts[1] get 0 and -inf. n may not
+ * exceed the plan's tokens.
+ */
+int oscar_shared_plan(const int32_t* qstarts, const int32_t* seq_lens, const int32_t* counts,
+                      const int32_t* group_starts, const int32_t* prefix_tokens, int64_t groups,
+                      int64_t max_reqs, int64_t tokens, int64_t hq, int32_t slots,
+                      const oscar_layout* layout, int32_t* units, int64_t capacity,
+                      int32_t* unit_count, int32_t* token_slots, void* stream);
+int oscar_shared_history(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_s2,
+                         const void* history, int64_t history_bytes, const int32_t* block_tables,
+                         int64_t table_stride, int64_t table_columns, const int32_t* counts,
+                         const int32_t* units, int64_t capacity, const int32_t* unit_count,
+                         const int32_t* token_slots, int64_t n, int64_t hq, int32_t slots,
+                         float scale, const oscar_layout* layout, float* partials, float* lse,
+                         int32_t fp32_out, void* out, float* out_lse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -194,6 +194,13 @@ SIGNATURES = {
                             POINTER(OscarLayout), _P, _P],
     "oscar_compact_pages": [_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, POINTER(OscarLayout), _P,
                             _P, _P, _P],
+    "oscar_shared_plan": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, POINTER(OscarLayout),
+                          _P, _I64, _P, _P, _P],
+    "oscar_shared_history": [
+        _P, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P,  # query, history, table, counts
+        _P, _I64, _P, _P, _I64, _I64, _I32, _F,  # units, capacity, count, slots of tokens, n ...
+        POINTER(OscarLayout), _P, _P, _I32, _P, _P, _P,  # layout, partials, lse, fp32, outs, stream
+    ],
 }
 RESTYPES = {"oscar_noalloc_scratch_bytes": c_int64, "oscar_calibration_workspace_bytes": c_int64,
             "oscar_history_chunk_tiles": c_int64}

@@ -366,12 +366,25 @@ class OscarAttentionImpl:
         return output
 
     def _fused_step(self, q, k, v, meta, splits, split_tokens, rows, lse):
-        """The whole step in one launch (``layer_step``, where it applies); else, with
+        """With a plan of shared prefixes (``meta.shared``): pre-attention -> shared history ->
+        post. Otherwise the whole step in one launch (``layer_step``, where it applies); else, with
         ``overlap``, the history launch carrying the pre-attention work (BF16 branch, K/V INT2
         store and, with ``rotate_in_history``, the q rotation) -> post (split merge, inverse V
         rotation, path merge, windows); else pre-attention -> history -> post, the last two in
         one launch with ``one_launch_post``."""
         layout = meta.layout
+        shared = getattr(meta, "shared", None)
+        if shared is not None:
+            # Requests with common prefixes: the history branch computes the shared positions
+            # once for all of them and comes merged, as one split.
+            qrot, rp, rl = kernels.pre_attention(q, k, v, self.history, self.window, meta, layout,
+                                                 self.scale, self.rk_t, self.rv_t,
+                                                 raw=not kernels.chunk_raw_preferred(meta))
+            hp, hl = kernels.shared_history(qrot, self.history, meta, shared, layout, self.scale,
+                                            merged=False)
+            kernels.post_attention(hp, hl, rp, rl, self.rv, k, v, self.window, meta, layout, rows,
+                                   lse)
+            return
         if self.layer_step and kernels.layer_step_supported(meta, layout, self.num_heads, splits,
                                                             q.shape[0]):
             kernels.layer_step(q, k, v, self.history, self.window, meta, layout, self.scale,
@@ -419,10 +432,15 @@ class OscarAttentionImpl:
         layout = meta.layout
         kernels.store_int2(kernels.rotate(k, self.rk_cols), kernels.rotate(v, self.rv_cols),
                            self.history, meta.slot_mapping, meta.counts, layout)
-        hp, hl = kernels.attention_partials(kernels.rotate(q, self.rk_cols), k, v, self.history,
-                                            self.window, meta, layout, self.scale, splits,
-                                            raw=False, split_tokens=split_tokens)
-        merged, merged_lse = kernels.merge_splits(hp, hl, meta.counts)
+        qrot, shared = kernels.rotate(q, self.rk_cols), getattr(meta, "shared", None)
+        if shared is not None:
+            merged, merged_lse = kernels.shared_history(qrot, self.history, meta, shared, layout,
+                                                        self.scale)
+        else:
+            hp, hl = kernels.attention_partials(qrot, k, v, self.history, self.window, meta,
+                                                layout, self.scale, splits, raw=False,
+                                                split_tokens=split_tokens)
+            merged, merged_lse = kernels.merge_splits(hp, hl, meta.counts)
         hout = kernels.rotate(merged, self.rv.T)
         rp, rl = kernels.attention_partials(q, k, v, self.history, self.window, meta, layout,
                                             self.scale, 1, raw=True)

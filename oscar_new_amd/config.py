@@ -326,6 +326,13 @@ def chunk_kernel_pays(tokens, requests, num_kv_heads, q_heads, splits, max_seq_l
     return tile < task
 
 
+def choose_shared_slots(tokens, q_heads, most=64, scratch_bytes=128 << 20):
+    """Partial rows per query row of a step with shared prefixes (no reference counterpart): the
+    pieces that a row's positions may be cut into, one per lane of the wavefront that merges them
+    and within ``scratch_bytes`` of rows, but at least 4."""
+    return max(4, min(most, scratch_bytes // max(1, tokens * q_heads * SPLIT_ROW_BYTES)))
+
+
 def percentile_selection(ratio, dim=256):
     """Descending ranks and interpolation weight of a linear quantile (config.py:92-97).
 

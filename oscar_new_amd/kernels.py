@@ -10,10 +10,12 @@ as in the reference.
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from . import _ext
-from .config import CLIP_MODES, attention_programs, chunk_kernel_pays
+from .config import CLIP_MODES, attention_programs, choose_shared_slots, chunk_kernel_pays
 
 __all__ = [
     "rotate",
@@ -26,6 +28,8 @@ __all__ = [
     "store_windows",
     "dequant_inverse_rotate",
     "qk_norm_rope",
+    "prepare_shared",
+    "shared_history",
     "pre_attention",
     "post_attention",
     "history_post",
@@ -488,6 +492,113 @@ def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None
                 "qk_norm_rope",
             )
     return tuple(out)
+
+
+@dataclass
+class SharedPlan:
+    """A step's units for ``shared_history`` (``prepare_shared``), in device buffers."""
+
+    units: torch.Tensor  # int32 [capacity, 8]
+    unit_count: torch.Tensor  # int32 [1]
+    token_slots: torch.Tensor  # int32 [tokens]: partial rows of each token
+    slots: int
+    query_heads: int
+    requests: int  # rows of the block table that the units may name
+
+
+def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, out=None):
+    """The plan of a step whose requests share prefixes, for every layer's ``shared_history``: one
+    launch per step (no reference counterpart).
+
+    Group g is the requests ``group_starts[g] .. group_starts[g + 1] - 1`` (int32 [groups + 1] on
+    the device, ascending), whose first ``prefix_tokens[g]`` tokens (int32 [groups]) are the same:
+    their history records are equal, in the same pages or in copies (``pages.fork_requests``).
+    Requests of no group, and groups of one, share nothing; so does a step whose starts descend.
+    ``hq``: query heads; ``tokens``: most query tokens the plan's layers pass (default
+    ``meta.num_actual_tokens``; a padded graph step passes its rows). ``out``: a plan of the same
+    sizes to fill again, so that a captured graph reads the new one.
+    """
+    _device_check(meta.query_start_loc, group_starts, prefix_tokens)
+    _same_device(meta.query_start_loc, group_starts=group_starts, prefix_tokens=prefix_tokens)
+    for name, t in (("group_starts", group_starts), ("prefix_tokens", prefix_tokens)):
+        if _int32(t, name).dim() != 1 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous vector")
+    groups = prefix_tokens.shape[0]
+    if group_starts.shape[0] != groups + 1:
+        raise ValueError("group_starts must hold one start per group and the end of the last")
+    tokens = int(meta.num_actual_tokens if tokens is None else tokens)
+    reqs, heads = int(meta.max_num_reqs), layout.kv_heads
+    if meta.query_start_loc.shape[0] < reqs + 1 or meta.seq_lens.shape[0] < reqs:
+        raise ValueError("the metadata holds fewer requests than max_num_reqs")
+    if hq <= 0 or hq % heads:
+        raise ValueError("the query head count must be a multiple of the KV head count")
+    slots = choose_shared_slots(tokens, hq)
+    capacity = (max(1, 256 // heads) + 2 * (tokens * (hq // heads) // 128) + groups
+                + min(reqs, tokens))
+    device = meta.query_start_loc.device
+    if out is None:
+        sizes = (8 * capacity, 8, max(tokens, 1))
+        buffer = torch.empty(sum(sizes), dtype=torch.int32, device=device)
+        units, count, used = buffer.split(sizes)
+        out = SharedPlan(units.view(capacity, 8), count[:1], used, slots, hq, reqs)
+    elif (out.units.shape[0] != capacity or out.token_slots.shape[0] != max(tokens, 1)
+          or out.slots != slots or out.query_heads != hq or out.requests != reqs
+          or out.units.device != device):
+        raise ValueError("the plan to fill again was made for other sizes")
+    with torch.cuda.device(device):
+        _ext.check(
+            _ext.library().oscar_shared_plan(
+                _ptr(_int32(meta.query_start_loc, "query_start_loc")),
+                _ptr(_int32(meta.seq_lens, "seq_lens")), _ptr(_int32(meta.counts, "counts")),
+                _ptr(group_starts), _ptr(prefix_tokens), groups, reqs, tokens, hq, slots,
+                layout_struct(layout), _ptr(out.units), capacity, _ptr(out.unit_count),
+                _ptr(out.token_slots), _stream(meta.query_start_loc)),
+            "prepare_shared",
+        )
+    return out
+
+
+def shared_history(query, history, meta, shared, layout, scale, merged=True):
+    """The history branch of a step whose requests share prefixes, each group's shared positions
+    computed once for all its rows (no reference counterpart as one call).
+
+    ``query``: the rotated query [n, hq, 256]; ``shared``: the step's plan (``prepare_shared``).
+    Returns ``(out bf16 [n, hq, 256], lse fp32 [n, hq])``, what ``merge_splits`` of
+    ``attention_partials(raw=False)`` gives, within rounding; with ``merged=False`` the rows as one
+    split's partials, ``(fp32 [n, hq, 1, 256], lse [n, hq, 1])``, for ``post_attention``.
+    """
+    _device_check(query, history)
+    n, hq, d = query.shape
+    if hq != shared.query_heads or n > shared.token_slots.shape[0]:
+        raise ValueError(f"the plan covers {shared.token_slots.shape[0]} tokens of "
+                         f"{shared.query_heads} heads, got {n} of {hq}")
+    table = _int32(meta.block_tables, "block_tables")
+    _same_device(query, history=history, block_tables=table, units=shared.units)
+    if table.shape[0] < shared.requests or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("block_tables must have contiguous rows, one per request of the plan")
+    if history.dtype != torch.uint8 or not history.is_contiguous():
+        raise ValueError("history must be the contiguous bytes of the K stripe")
+    device = query.device
+    partials = torch.empty((n, hq, shared.slots, d), dtype=torch.float32, device=device)
+    lse = torch.empty((n, hq, shared.slots), dtype=torch.float32, device=device)
+    shape = (n, hq, d) if merged else (n, hq, 1, d)
+    out = torch.empty(shape, dtype=torch.bfloat16 if merged else torch.float32, device=device)
+    out_lse = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+    if n == 0:
+        return out, out_lse
+    query = _rows_contiguous(query)
+    with torch.cuda.device(device):
+        _ext.check(
+            _ext.library().oscar_shared_history(
+                _ptr(query), *query.stride(), _ptr(history), history.numel(), _ptr(table),
+                table.stride(0), table.shape[1], _ptr(_int32(meta.counts, "counts")),
+                _ptr(shared.units), shared.units.shape[0], _ptr(shared.unit_count),
+                _ptr(shared.token_slots), n, hq, shared.slots, float(scale),
+                layout_struct(layout), _ptr(partials), _ptr(lse), int(not merged), _ptr(out),
+                _ptr(out_lse), _stream(query)),
+            "shared_history",
+        )
+    return out, out_lse
 
 
 # --------------------------------------------------------------------------- fused launches

@@ -51,6 +51,7 @@ class OscarMetadata:
     merged_lse: torch.Tensor | None = None  # optional [n, hq] output of the merged LSE
     finish_counters: torch.Tensor | None = None  # zeroed int32 slots of one-launch post
     queue_counters: torch.Tensor | None = None  # two zeroed int32 work-queue counters
+    shared: object = None  # kernels.SharedPlan of a step whose requests share prefixes
 
     @property
     def query_ends(self):
