@@ -632,16 +632,18 @@ int oscar_compact_pages(const void* stripes, int64_t layers, int64_t num_pages,
  * (int32 [groups + 1], ascending; requests of no group share nothing), whose first
  * prefix_tokens[g] positions hold the same records (pages may differ: the first member's are
  * read). It writes the step's units (int32 [capacity][8], 16-byte aligned), their number and the
- * partial rows of every token below counts[1] (token_slots, int32 [tokens]). `slots` (4..64) bounds
- * the partial rows of a row; tokens the query tokens of the step; capacity at least 256 / kv_heads
- * + 2 (tokens * (hq / kv_heads) / 128) + groups + min(max_reqs, tokens). groups + max_reqs <= 8192
- * and hq / kv_heads <= 32, else OSCAR_E_UNSUPPORTED. Starts that descend share nothing.
+ * partial rows of every token below counts[1] (token_slots, int32 [tokens]). `slots` (4..256) bounds
+ * the partial rows of a row; tokens the query tokens of the step; capacity at least
+ * oscar_shared_capacity of the same sizes. groups + max_reqs <= 6144 and hq / kv_heads <= 32, else
+ * OSCAR_E_UNSUPPORTED. Starts that descend share nothing.
  *
  * shared_history, per layer: query is the rotated query, partials fp32 [n][hq][slots][256] and lse
  * [n][hq][slots] scratch, out bf16 [n][hq][256] (fp32 with fp32_out, the layout of one split's
  * partials), out_lse fp32 [n][hq]. Rows of tokens at or past counts[1] get 0 and -inf. n may not
  * exceed the plan's tokens.
  */
+int64_t oscar_shared_capacity(int64_t tokens, int64_t hq, int64_t groups, int64_t max_reqs,
+                              int32_t kv_heads);
 int oscar_shared_plan(const int32_t* qstarts, const int32_t* seq_lens, const int32_t* counts,
                       const int32_t* group_starts, const int32_t* prefix_tokens, int64_t groups,
                       int64_t max_reqs, int64_t tokens, int64_t hq, int32_t slots,

@@ -194,6 +194,7 @@ SIGNATURES = {
                             POINTER(OscarLayout), _P, _P],
     "oscar_compact_pages": [_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, POINTER(OscarLayout), _P,
                             _P, _P, _P],
+    "oscar_shared_capacity": [_I64, _I64, _I64, _I64, _I32],
     "oscar_shared_plan": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, POINTER(OscarLayout),
                           _P, _I64, _P, _P, _P],
     "oscar_shared_history": [
@@ -203,7 +204,7 @@ SIGNATURES = {
     ],
 }
 RESTYPES = {"oscar_noalloc_scratch_bytes": c_int64, "oscar_calibration_workspace_bytes": c_int64,
-            "oscar_history_chunk_tiles": c_int64}
+            "oscar_history_chunk_tiles": c_int64, "oscar_shared_capacity": c_int64}
 NOALLOC_SCRATCH_BYTES = 32 << 20  # OSCAR_NOALLOC_SCRATCH_BYTES
 
 _lib = None

@@ -326,9 +326,9 @@ def chunk_kernel_pays(tokens, requests, num_kv_heads, q_heads, splits, max_seq_l
     return tile < task
 
 
-def choose_shared_slots(tokens, q_heads, most=64, scratch_bytes=128 << 20):
+def choose_shared_slots(tokens, q_heads, most=256, scratch_bytes=128 << 20):
     """Partial rows per query row of a step with shared prefixes (no reference counterpart): the
-    pieces that a row's positions may be cut into, one per lane of the wavefront that merges them
+    pieces that a row's positions may be cut into, four per lane of the wavefront that merges them
     and within ``scratch_bytes`` of rows, but at least 4."""
     return max(4, min(most, scratch_bytes // max(1, tokens * q_heads * SPLIT_ROW_BYTES)))
 

@@ -9,27 +9,33 @@
 // before E, the first one that some member does not share, rounded down to a chunk. They form one
 // long matrix product: `rows` is the members' query tokens times the heads of a KV head.
 //
-// Units. A step's work is (row tile, position range) units of the 128-row tile of chunk_tile.h:
-// the group's rows against [sink, E) through its first member's pages, and each request's own rows
-// against [E, recent_begin) through its own. The plan kernel cuts every tile's positions into pieces
-// of about T chunks, T from the whole step's lengths so that the units fill the CUs once, and writes
-// the list; it runs once per step, before every layer's launch. Partial rows of a tile's pieces go to
-// slots that the merge kernel joins by their LSEs, as many as the plan says for each token.
-#include "chunk_tile.h"
+// Units. A step's work is (row tile, position range) units: the group's rows against [sink, E)
+// through its first member's pages, and each request's own rows against [E, recent_begin) through
+// its own. Up to kSmallRows rows a tile is 16 rows whose positions the wavefronts of a workgroup
+// divide (row_tile.h), above that 128 rows that share the codes (chunk_tile.h). The plan kernel cuts
+// every tile's positions into pieces from the whole step's lengths, so that the launch ends early on
+// 256 CUs, and writes the list, once per step and before every layer's launch. Partial rows of a
+// tile's pieces go to slots that the merge kernel joins by their LSEs, as many as the plan says for
+// each token.
 #include "merge.h"
+#include "row_tile.h"
 
 namespace oscar {
 namespace {
 
 constexpr int kSharedThreads = 1024;
-constexpr int kSharedEntries = 8192;  // groups and requests whose counts live in LDS
-constexpr int kSharedSlots = 64;      // partial rows of a row: one per lane of the merging wavefront
+constexpr int kSharedEntries = 6144;  // groups and requests whose counts live in LDS
+constexpr int kSharedSlots = 256;     // partial rows of a row: four per lane of a merging wavefront
 constexpr int kUnitWords = 8;
+// Rows up to which a tile is 16 rows; 128-token chunks such a unit takes at least.
+constexpr int kSmallRows = 48, kSmallPiece = 8;
+// A unit's time in us: its start and end, and each 128-token chunk.
+constexpr float kTileStart = 10.f, kTileChunk = 4.5f, kSmallStart = 10.f, kSmallChunk = 1.2f;
 
 // A unit: rows [row_base, row_end) of tokens token0 .. (row r is token token0 + r / g), positions
-// [p_lo, p_hi) through block-table row req, partials to `slot`.
+// [p_lo, p_hi) through block-table row req, partials to `slot`; small: at most 16 rows, row_tile.h.
 struct Unit {
-  int32_t req, token0, row_end, row_base, p_lo, p_hi, slot, reserved;
+  int32_t req, token0, row_end, row_base, p_lo, p_hi, slot, small;
 };
 static_assert(sizeof(Unit) == kUnitWords * 4, "one unit is eight words");
 
@@ -69,6 +75,10 @@ __device__ __forceinline__ void plan_reduce(int64_t& sum, int& most) {
   }
 }
 
+// Tiles of an entry of `rows` rows (small entries: 16-row tiles, kept negative).
+__device__ __forceinline__ int tiles_of(int rows) {
+  return rows <= kSmallRows ? -((rows + 15) / 16) : (rows + kRowsC - 1) / kRowsC;
+}
 __device__ __forceinline__ int chunks_of(int lo, int hi) {
   return lo < hi ? ((hi - 1) >> 7) - (lo >> 7) + 1 : 0;
 }
@@ -77,6 +87,7 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
   // Entries: the groups, then the requests.
   __shared__ int s_chunks[kSharedEntries], s_tiles[kSharedEntries], s_start[kSharedEntries + 1];
   __shared__ int s_own[kSharedEntries];  // first history position of a request's own part
+  __shared__ int s_group[kSharedEntries];  // the group whose positions a request shares, or -1
   __shared__ int s_wave[kSharedThreads / kWave];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int reqs = max(min(a.counts[0], a.max_reqs), 0);
@@ -104,7 +115,7 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
   };
   auto clip = [&](int r) { return min(max(r, 0), reqs); };
 
-  for (int r = tid; r < reqs; r += kSharedThreads) s_own[r] = -1;
+  for (int r = tid; r < reqs; r += kSharedThreads) s_own[r] = s_group[r] = -1;
   __syncthreads();
   for (int i = wave; i < groups; i += kSharedThreads / kWave) {
     const int r0 = clip(a.group_starts[i]), r1 = clip(a.group_starts[i + 1]);
@@ -116,49 +127,76 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
     // Past the sink every member's recent part starts behind it, so all begin at `sink`.
     const bool shared = r1 - r0 > 1 && end > a.sink;
     if (shared)
-      for (int r = r0 + lane; r < r1; r += kWave) s_own[r] = end;
+      for (int r = r0 + lane; r < r1; r += kWave) {
+        s_own[r] = end;
+        s_group[r] = i;
+      }
     if (lane == 0) {
       const int rows = shared ? max(token(r1) - token(r0), 0) * a.g : 0;
       s_chunks[i] = shared ? chunks_of(a.sink, end) : 0;
-      s_tiles[i] = (rows + kRowsC - 1) / kRowsC;
+      s_tiles[i] = tiles_of(rows);
     }
   }
   __syncthreads();
-  int64_t work = 0;
   int most = 0;  // chunks of one row's positions
   for (int r = tid; r < reqs; r += kSharedThreads) {
     const Span s = span(r);
-    const int own = s_own[r];
-    const int lo = own >= 0 ? own : s.sink_len;
+    const int group = s_group[r];
+    const int lo = group >= 0 ? s_own[r] : s.sink_len;
     s_own[r] = lo;
     s_chunks[groups + r] = chunks_of(lo, s.recent);
-    s_tiles[groups + r] = (s.rows + kRowsC - 1) / kRowsC;
+    s_tiles[groups + r] = tiles_of(s.rows);
     if (s.rows > 0)
-      most = max(most, s_chunks[groups + r] + (lo > a.sink ? chunks_of(a.sink, lo) : 0));
+      most = max(most, s_chunks[groups + r] + (group >= 0 ? s_chunks[group] : 0));
   }
   __syncthreads();
-  int64_t tiles = 0;
+  int64_t work = 0, small = 0, small_tiles = 0;  // chunks of 128-row tiles and of 16-row tiles
   for (int e = tid; e < entries; e += kSharedThreads) {
-    work += static_cast<int64_t>(s_tiles[e]) * s_chunks[e];
-    tiles += s_chunks[e] ? s_tiles[e] : 0;
+    const int64_t w = static_cast<int64_t>(abs(s_tiles[e])) * s_chunks[e];
+    work += s_tiles[e] > 0 ? w : 0;
+    small += s_tiles[e] < 0 ? w : 0;
+    small_tiles += s_tiles[e] < 0 && s_chunks[e] ? -s_tiles[e] : 0;
   }
   int none = 0;
   plan_reduce(work, most);
-  plan_reduce(tiles, none);
-  // Chunks per unit: at most about `budget` units, and no row in more than `slots` pieces (a row's
-  // positions are two ranges, each with one uneven piece).
-  int per = static_cast<int>(max(static_cast<int64_t>(1), (work + a.budget - 1) / a.budget));
-  per = max(per, (most + a.slots - 3) / (a.slots - 2));
-  auto count_units = [&](int t) {
-    int64_t units = 0;
-    for (int e = tid; e < entries; e += kSharedThreads)
-      units += static_cast<int64_t>(s_tiles[e]) * cdiv(s_chunks[e], t);
-    int unused = 0;
-    plan_reduce(units, unused);
-    return units;
+  plan_reduce(small, none);
+  plan_reduce(small_tiles, none);
+  // Chunks of a piece: no row in more than `slots` pieces (a row's positions are two ranges, each
+  // with one uneven piece), at most `budget` units by the average, and then the first count, of 16
+  // tried by the wavefronts at once, with which the 128-row units and the others' load, in units of
+  // the same time, fit the budget: they run side by side, one per CU, and a second round would
+  // cost more than longer units do.
+  const int least = (most + a.slots - 3) / (a.slots - 2);
+  const int small_least = max(max(kSmallPiece, least),
+                              static_cast<int>((small + a.budget - 1) / a.budget));
+  int per = max(max(1, least), static_cast<int>((work + a.budget - 1) / a.budget));
+  const float load = small_tiles * kSmallStart + small * kSmallChunk;
+  auto small_per = [&](int t) {
+    return max(small_least, static_cast<int>(t * (kTileChunk / kSmallChunk)));
   };
-  // Uneven pieces may pass the budget: a second round of workgroups costs more than longer units.
-  for (int i = 0; i < 8 && tiles < a.budget && count_units(per) > a.budget; ++i) ++per;
+  __shared__ int s_fits;
+  for (int round = 0; round < 16; ++round) {
+    const int t = per + wave;
+    int64_t units = 0;
+    for (int e = lane; e < entries; e += kWave)
+      units += s_tiles[e] > 0 ? static_cast<int64_t>(s_tiles[e]) * cdiv(s_chunks[e], t) : 0;
+    units = wave_sum_i64(units);
+    if (tid == 0) s_fits = kSharedThreads / kWave;
+    __syncthreads();
+    if (lane == 0 && units + load / (kTileStart + kTileChunk * t) <= a.budget)
+      atomicMin(&s_fits, wave);
+    __syncthreads();
+    const int fits = s_fits;
+    __syncthreads();
+    per += fits;
+    if (fits < kSharedThreads / kWave || per >= most) break;
+  }
+  per = max(1, min(per, most));
+  const int per_small = small_per(per);
+  auto pieces = [&](int e) {
+    return cdiv(s_chunks[e], s_tiles[e] < 0 ? per_small : per);
+  };
+  auto units_of = [&](int e) { return abs(s_tiles[e]) * pieces(e); };
 
   // Exclusive scan of the entries' units, eight entries a thread.
   constexpr int kPer = kSharedEntries / kSharedThreads;
@@ -166,7 +204,7 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
     const int e = kPer * tid + k;
-    if (e < entries) mine += s_tiles[e] * cdiv(s_chunks[e], per);
+    if (e < entries) mine += units_of(e);
   }
   int incl = mine;
 #pragma unroll
@@ -183,7 +221,7 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
     const int e = kPer * tid + k;
     if (e >= entries) break;
     s_start[e] = at;
-    at += s_tiles[e] * cdiv(s_chunks[e], per);
+    at += units_of(e);
   }
   int total = 0;
 #pragma unroll
@@ -201,7 +239,8 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
       else
         hi = mid;
     }
-    const int e = lo, tile_count = s_tiles[e], pieces = cdiv(s_chunks[e], per);
+    const int e = lo, tile_count = abs(s_tiles[e]);
+    const int64_t count = pieces(e);
     const int local = u - s_start[e], piece = local / tile_count, tile = local - piece * tile_count;
     Unit x;
     int begin, end, rows;
@@ -221,31 +260,32 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
       rows = s.rows;
       begin = s_own[r];
       end = s.recent;
-      x.slot = piece + (begin > a.sink ? cdiv(chunks_of(a.sink, begin), per) : 0);
+      x.slot = piece + (s_group[r] >= 0 ? pieces(s_group[r]) : 0);
     }
     // Tiles of equal numbers of 16-row groups, pieces of equal numbers of chunks.
     const int share = ((rows + 15) / 16 + tile_count - 1) / tile_count * 16;
     x.row_base = tile * share;
     x.row_end = min(x.row_base + share, rows);
-    const int c0 = (begin >> 7) + static_cast<int>(static_cast<int64_t>(piece) * s_chunks[e] / pieces);
+    const int c0 = (begin >> 7) + static_cast<int>(static_cast<int64_t>(piece) * s_chunks[e] / count);
     const int c1 =
-        (begin >> 7) + static_cast<int>(static_cast<int64_t>(piece + 1) * s_chunks[e] / pieces);
+        (begin >> 7) + static_cast<int>(static_cast<int64_t>(piece + 1) * s_chunks[e] / count);
     x.p_lo = max(begin, c0 << 7);
     x.p_hi = min(end, c1 << 7);
-    x.reserved = 0;
+    x.small = s_tiles[e] < 0;
     a.units[u] = x;
   }
   for (int r = wave; r < reqs; r += kSharedThreads / kWave) {
-    const int own = s_own[r];
-    const int used = cdiv(s_chunks[groups + r], per) +
-                     (own > a.sink ? cdiv(chunks_of(a.sink, own), per) : 0);
+    const int used = pieces(groups + r) + (s_group[r] >= 0 ? pieces(s_group[r]) : 0);
     const int t1 = token(r + 1);
     for (int t = token(r) + lane; t < t1; t += kWave) a.token_slots[t] = used;
   }
 }
 
 __global__ __launch_bounds__(kThreadsC, 2) void shared_history_kernel(const AttnArgs a) {
-  __shared__ ChunkLds lds;
+  __shared__ union {
+    ChunkLds chunk;
+    RowTileLds row;
+  } lds;
   const int heads = a.L.kv_heads;
   const int index = static_cast<int>(blockIdx.x) / heads;
   if (index >= a.task_count[0]) return;
@@ -254,8 +294,11 @@ __global__ __launch_bounds__(kThreadsC, 2) void shared_history_kernel(const Attn
   Task t{};
   t.req = u.req;
   t.qstart = u.token0;
-  chunk_tile(a, t, static_cast<int>(blockIdx.x) - index * heads, u.row_end, u.row_base, u.p_lo,
-             u.p_hi, u.slot, lds);
+  const int head = static_cast<int>(blockIdx.x) - index * heads;
+  if (u.small)
+    row_tile(a, t, head, u.row_end, u.row_base, u.p_lo, u.p_hi, u.slot, lds.row);
+  else
+    chunk_tile(a, t, head, u.row_end, u.row_base, u.p_lo, u.p_hi, u.slot, lds.chunk);
 }
 
 struct SharedMergeArgs {
@@ -268,7 +311,7 @@ struct SharedMergeArgs {
   int32_t hq, slots;
 };
 
-// One workgroup per row: every wavefront holds all LSEs (one per lane) and adds every fourth slot,
+// One workgroup per row: every wavefront holds all LSEs (four per lane) and adds every fourth slot,
 // eight loads in flight; the four sums are added in wavefront order.
 template <bool kFloat>
 __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedMergeArgs a) {
@@ -276,27 +319,40 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedMerg
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int64_t row = blockIdx.x, token = row / a.hq;
   const int used = token < a.counts[1] ? min(max(a.token_slots[token], 0), a.slots) : 0;
-  const float l = lane < used ? a.lse[row * a.slots + lane] : -INFINITY;
-  const float mx = wave_max_dpp(l);
-  const float w = l == -INFINITY ? 0.f : expf(l - mx);
-  const float den = wave_tree_sum_dpp(w);
+  float w[kSharedSlots / kWave];
+  float mx = -INFINITY, den = 0.f;
+#pragma unroll
+  for (int i = 0; i < kSharedSlots / kWave; ++i) {
+    w[i] = kWave * i + lane < used ? a.lse[row * a.slots + kWave * i + lane] : -INFINITY;
+    mx = fmaxf(mx, w[i]);
+  }
+  mx = wave_max_dpp(mx);
+#pragma unroll
+  for (int i = 0; i < kSharedSlots / kWave; ++i) {
+    w[i] = w[i] == -INFINITY ? 0.f : expf(w[i] - mx);
+    den += w[i];
+  }
+  den = wave_tree_sum_dpp(den);
   const f32x4* part = reinterpret_cast<const f32x4*>(a.partials + row * a.slots * kHeadDim) + lane;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = wave; s0 < used; s0 += 32) {
-    f32x4 v[8];
-    float ws[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int s = s0 + 4 * k;
-      v[k] = s < used ? part[static_cast<int64_t>(s) * (kHeadDim / 4)] : f32x4{0.f, 0.f, 0.f, 0.f};
-      ws[k] = lane_value(w, min(s, kWave - 1));
-    }
+  for (int i = 0; i < kSharedSlots / kWave; ++i)
+    for (int s0 = wave; s0 < min(used - kWave * i, kWave); s0 += 32) {
+      f32x4 v[8];
+      float ws[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (s0 + 4 * k < used)
+      for (int k = 0; k < 8; ++k) {
+        const int s = s0 + 4 * k;
+        const bool in = kWave * i + s < used;
+        v[k] = in ? part[static_cast<int64_t>(kWave * i + s) * (kHeadDim / 4)]
+                  : f32x4{0.f, 0.f, 0.f, 0.f};
+        ws[k] = in ? lane_value(w[i], s) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] = fmaf(ws[k], v[k][e], sum[e]);
-  }
+    }
   if (wave) s_sum[wave - 1][lane] = sum;
   __syncthreads();
   if (wave) return;
@@ -312,8 +368,26 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedMerg
   if (lane == 0) a.out_lse[row] = den > 0.f ? mx + logf(den) : -INFINITY;
 }
 
+// Units that a plan may hold: a tile's pieces pass its share of the budget by less than one, for
+// 128-row tiles (one per 128 rows and one more per entry) and for 16-row tiles (at most three per
+// entry, and one per 16 rows and one more per entry).
+int64_t shared_capacity(int64_t tokens, int64_t g, int64_t groups, int64_t max_reqs,
+                        int64_t budget) {
+  const int64_t entries = groups + (max_reqs < tokens ? max_reqs : tokens);
+  const int64_t tiles = 2 * (tokens * g / kRowsC) + entries;
+  const int64_t by_rows = 2 * (tokens * g / 16) + entries;
+  return 2 * budget + tiles + (by_rows < 3 * entries ? by_rows : 3 * entries);
+}
+
 }  // namespace
 }  // namespace oscar
+
+extern "C" int64_t oscar_shared_capacity(int64_t tokens, int64_t hq, int64_t groups,
+                                         int64_t max_reqs, int32_t kv_heads) {
+  if (tokens < 0 || hq <= 0 || kv_heads <= 0 || groups < 0 || max_reqs < 0) return -1;
+  return oscar::shared_capacity(tokens, hq / kv_heads, groups, max_reqs,
+                                kv_heads < 256 ? 256 / kv_heads : 1);
+}
 
 extern "C" int oscar_shared_plan(const int32_t* qstarts, const int32_t* seq_lens,
                                  const int32_t* counts, const int32_t* group_starts,
@@ -331,9 +405,7 @@ extern "C" int oscar_shared_plan(const int32_t* qstarts, const int32_t* seq_lens
   if (groups + max_reqs > kSharedEntries || hq / L.kv_heads > 32) return OSCAR_E_UNSUPPORTED;
   if (slots < 4 || slots > kSharedSlots) return OSCAR_E_SHAPE;
   const int64_t g = hq / L.kv_heads, budget = L.kv_heads < 256 ? 256 / L.kv_heads : 1;
-  const int64_t reqs = max_reqs < tokens ? max_reqs : tokens;
-  // A tile per 128 rows and one more per group or request, a piece more than its share per tile.
-  if (capacity < budget + 2 * (tokens * g / kRowsC) + groups + reqs || capacity > 0x7fffffffll)
+  if (capacity < shared_capacity(tokens, g, groups, max_reqs, budget) || capacity > 0x7fffffffll)
     return OSCAR_E_SHAPE;
   if (!qstarts || !seq_lens || !counts || !units || !unit_count || !token_slots ||
       (groups && (!group_starts || !prefix_tokens)))

@@ -533,8 +533,7 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
     if hq <= 0 or hq % heads:
         raise ValueError("the query head count must be a multiple of the KV head count")
     slots = choose_shared_slots(tokens, hq)
-    capacity = (max(1, 256 // heads) + 2 * (tokens * (hq // heads) // 128) + groups
-                + min(reqs, tokens))
+    capacity = _ext.library().oscar_shared_capacity(tokens, hq, groups, reqs, heads)
     device = meta.query_start_loc.device
     if out is None:
         sizes = (8 * capacity, 8, max(tokens, 1))

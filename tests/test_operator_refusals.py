@@ -65,25 +65,27 @@ def test_pages():
 def test_shared_prefixes():
     lib = _ext.library()
 
-    def plan(groups=2, reqs=8, tokens=8, hq=6, slots=64, lay=layout(), units=A, capacity=400,
+    def plan(groups=2, reqs=8, tokens=8, hq=6, slots=64, lay=layout(), units=A, capacity=600,
              starts=A):
         return lib.oscar_shared_plan(A, A, A, starts, A, groups, reqs, tokens, hq, slots, lay,
                                      units, capacity, A, A, None)
 
-    def attend(q=A, history=A, units=A, capacity=400, used=A, n=8, hq=6, slots=64, scale=1 / 16,
+    def attend(q=A, history=A, units=A, capacity=600, used=A, n=8, hq=6, slots=64, scale=1 / 16,
                lay=layout(), out=A, history_bytes=1 << 24):
         return lib.oscar_shared_history(q, 1536, 256, 1, history, history_bytes, A, 64, 64, A, units,
                                         capacity, A, used, n, hq, slots, scale, lay, A, A, 0, out,
                                         A, None)
 
     assert plan(groups=-1) == -2 and plan(reqs=0) == -2 and plan(tokens=-1) == -2
-    assert plan(hq=0) == -2 and plan(slots=3) == -2 and plan(slots=65) == -2
+    assert plan(hq=0) == -2 and plan(slots=3) == -2 and plan(slots=257) == -2
     assert plan(groups=8000, reqs=200) == -5 and plan(hq=33) == -5
-    assert plan(capacity=256) == -2  # below what the plan may write
+    least = lib.oscar_shared_capacity(8, 6, 2, 8, 1)
+    assert plan(capacity=least - 1) == -2  # below what the plan may write
+    assert lib.oscar_shared_capacity(8, 0, 2, 8, 1) == -1
     assert plan(units=None) == -1 and plan(starts=None) == -1 and plan(units=A + 4) == -4
     assert plan(lay=layout(page=1)) == -3
     assert attend(n=0) == 0
-    assert attend(slots=3) == -2 and attend(slots=65) == -2 and attend(capacity=0) == -2
+    assert attend(slots=3) == -2 and attend(slots=257) == -2 and attend(capacity=0) == -2
     assert attend(n=-1) == -2 and attend(hq=0) == -2 and attend(history_bytes=64) == -2
     assert attend(q=None) == -1 and attend(used=None) == -1 and attend(out=None) == -1
     assert attend(q=A + 2) == -4 and attend(out=A + 4) == -4 and attend(history=A + 4) == -4
