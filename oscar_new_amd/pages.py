@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import _ext
-from .kernels import _device_check, _int32, _ptr, _same_device, _stream, layout_struct
+from .kernels import _device_check, _int32, _launch, _same_device, layout_struct
 
 __all__ = ["PageCaches", "free_pages", "fork_requests", "compact_pages"]
 
@@ -46,6 +46,7 @@ class PageCaches:
             if any(t.data_ptr() % 16 for t in pair):
                 raise ValueError("cache stripes must be 16-byte aligned")
         self.layout = layout
+        self.layout_struct = layout_struct(layout)
         self.views = views
         self.device = history.device
         self.num_pages = history.numel() // layout.stripe_page_bytes
@@ -57,7 +58,6 @@ class PageCaches:
 
 def _table(caches, block_tables, seq_lens, counts=None, **others):
     """Checks of the scheduler's tensors; the arguments of the block table."""
-    _device_check(block_tables, seq_lens, counts, *others.values())
     _same_device(caches.stripes, block_tables=block_tables, seq_lens=seq_lens, counts=counts,
                  **others)
     if block_tables.dim() != 2 or 0 in block_tables.shape:
@@ -74,7 +74,7 @@ def _table(caches, block_tables, seq_lens, counts=None, **others):
         raise ValueError("seq_lens must hold one count per block table row")
     if counts is not None and (_int32(counts, "counts").numel() < 1 or not counts.is_contiguous()):
         raise ValueError("counts must hold the number of live rows first")
-    return _ptr(block_tables), stride, columns, rows
+    return block_tables.data_ptr(), stride, columns, rows
 
 
 def free_pages(caches, block_tables, seq_lens, counts):
@@ -82,16 +82,12 @@ def free_pages(caches, block_tables, seq_lens, counts):
     the free pages in ascending order and -1 behind them, and int32 ``[1]``."""
     table = _table(caches, block_tables, seq_lens, counts)
     used = torch.empty(caches.num_pages, dtype=torch.int32, device=caches.device)
-    pages = torch.empty_like(used)
-    count = torch.empty(1, dtype=torch.int32, device=caches.device)
-    with torch.cuda.device(caches.device):
-        _ext.check(
-            _ext.library().oscar_free_pages(
-                caches.num_pages, *table, _ptr(seq_lens), _ptr(counts),
-                layout_struct(caches.layout), _ptr(used), _ptr(pages), _ptr(count),
-                _stream(used)),
-            "free_pages",
-        )
+    pages, count = used.new_empty(caches.num_pages), used.new_empty(1)
+    _launch(
+        _ext.library().oscar_free_pages, "free_pages", caches.device, caches.num_pages, *table,
+        seq_lens.data_ptr(), counts.data_ptr(), caches.layout_struct, used.data_ptr(),
+        pages.data_ptr(), count.data_ptr(),
+    )
     return pages, count
 
 
@@ -114,17 +110,15 @@ def fork_requests(caches, block_tables, seq_lens, parents, children, fresh):
     forks = parents.numel()
     for name, t, shape in (("parents", parents, (forks,)), ("children", children, (forks,)),
                            ("fresh", fresh, (forks, 2))):
-        if tuple(_int32(t, name).shape) != shape or not t.is_contiguous():
+        if _int32(t, name).shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}")
-    status = torch.empty(forks, dtype=torch.int32, device=caches.device)
-    with torch.cuda.device(caches.device):
-        _ext.check(
-            _ext.library().oscar_fork_requests(
-                _ptr(caches.stripes), len(caches.views), caches.num_pages, *table,
-                _ptr(seq_lens), _ptr(parents), _ptr(children), _ptr(fresh), forks,
-                layout_struct(caches.layout), _ptr(status), _stream(status)),
-            "fork_requests",
-        )
+    status = children.new_empty(forks)
+    _launch(
+        _ext.library().oscar_fork_requests, "fork_requests", caches.device,
+        caches.stripes.data_ptr(), len(caches.views), caches.num_pages, *table,
+        seq_lens.data_ptr(), parents.data_ptr(), children.data_ptr(), fresh.data_ptr(), forks,
+        caches.layout_struct, status.data_ptr(),
+    )
     return status
 
 
@@ -139,14 +133,11 @@ def compact_pages(caches, block_tables, seq_lens, counts):
     """
     table = _table(caches, block_tables, seq_lens, counts)
     scratch = torch.empty(5 * caches.num_pages + 1, dtype=torch.int32, device=caches.device)
-    tables = torch.empty(tuple(block_tables.shape), dtype=torch.int32, device=caches.device)
-    live = torch.empty(1, dtype=torch.int32, device=caches.device)
-    with torch.cuda.device(caches.device):
-        _ext.check(
-            _ext.library().oscar_compact_pages(
-                _ptr(caches.stripes), len(caches.views), caches.num_pages, *table,
-                _ptr(seq_lens), _ptr(counts), layout_struct(caches.layout), _ptr(scratch),
-                _ptr(tables), _ptr(live), _stream(scratch)),
-            "compact_pages",
-        )
+    tables, live = scratch.new_empty(block_tables.shape), scratch.new_empty(1)
+    _launch(
+        _ext.library().oscar_compact_pages, "compact_pages", caches.device,
+        caches.stripes.data_ptr(), len(caches.views), caches.num_pages, *table,
+        seq_lens.data_ptr(), counts.data_ptr(), caches.layout_struct, scratch.data_ptr(),
+        tables.data_ptr(), live.data_ptr(),
+    )
     return tables, live
