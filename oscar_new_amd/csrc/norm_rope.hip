@@ -14,6 +14,8 @@
 // through DPP moves and one lane swap. A pair's other half is read again from memory (the row is
 // in the cache by then) rather than moved between lanes: one 16-byte load, in flight with the
 // lane's own, against four cross-lane moves behind it.
+#include <type_traits>
+
 #include "rotate.h"
 
 namespace oscar {
@@ -38,11 +40,10 @@ struct NormRopeArgs {
   const int64_t* positions;
   const int32_t* counts;  // null: every token is live
   int64_t n;
-  int32_t rotary, weight_fp32, table_fp32, adjacent;
+  int32_t rotary, weight_fp32, adjacent;
   float offset, eps;
   const uint16_t* rk_t;  // R_k^T [256][256]
   uint16_t* q_rot;
-  int32_t q_groups;  // workgroups of the query rows (kRotate)
 };
 
 __device__ __forceinline__ float load_value(const void* p, int64_t i, int fp32) {
@@ -76,11 +77,6 @@ __device__ __forceinline__ void unpack_eight(u32x4 w, float (&v)[8]) {
   }
 }
 
-// The lane's dims 8 l .. 8 l + 7 within a row: weights of its own dims and of their partners.
-struct LaneWeights {
-  float own[8], pair[8];
-};
-
 // Partner of dim d, the index of its angle and the sign of the partner's term.
 __device__ __forceinline__ void pair_of(const NormRopeArgs& a, int d, int& pair, int& angle,
                                         float& sign) {
@@ -96,73 +92,59 @@ __device__ __forceinline__ void pair_of(const NormRopeArgs& a, int d, int& pair,
   }
 }
 
-template <int kMode>
-__device__ __forceinline__ void load_weights(const NormRopeArgs& a, const void* weight, int l,
-                                             LaneWeights& w) {
-  load_eight(weight, 8 * l, a.weight_fp32, w.own);
+// The weight of every dim (with the offset), in LDS: sixteen values a lane would cost the walking
+// kernel registers that it needs. Threads from .. from + 31 of the workgroup write it.
+__device__ __forceinline__ void stage_weights(const NormRopeArgs& a, const void* weight,
+                                              float* s_weight, int from) {
+  const int i = static_cast<int>(threadIdx.x) - from;
+  if (i < 0 || i >= 32) return;
+  float w[8];
+  load_eight(weight, 8 * i, a.weight_fp32, w);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w.own[e] += a.offset;
-  const int half = a.rotary >> 1;
-  if (kMode == kPairHalves) {
-    const int d = 8 * l < half ? 8 * l + half : 8 * l - half;
-    load_eight(weight, 8 * l < a.rotary ? d : 0, a.weight_fp32, w.pair);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w.pair[e] += a.offset;
-  } else if (kMode == kPairAdjacent) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w.pair[e] = w.own[e ^ 1];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      int p = 0, j;
-      float s;
-      if (8 * l + e < a.rotary) pair_of(a, 8 * l + e, p, j, s);
-      w.pair[e] = load_value(weight, p, a.weight_fp32) + a.offset;
-    }
-  }
+  for (int e = 0; e < 8; ++e) s_weight[8 * i + e] = w[e] + a.offset;
 }
 
-// What a row needs from memory: its lane's values, their partners and the angles.
-struct RowLoads {
-  u32x4 x;
-  float pair[8], c[8], s[8];
+// A token's angles for the lane's dims, as they lie in the table: bf16 or fp32 words of the
+// cosines and sines, or (generic) the fp32 values themselves. They stay packed while a load is in
+// flight, as do the rows: a conversion waits for it.
+template <int kMode, bool kFp32>
+struct Angles {
+  static constexpr int kWords = kMode == kPairGeneric || (kMode == kPairHalves && kFp32) ? 2 : 1;
+  u32x4 c[kWords], s[kWords];
   bool live, bad;  // a live token; its position is outside the table
 };
+struct RowLoads {
+  u32x4 x, pair;  // the lane's values and, where halves are paired, their partners
+};
 
-template <int kMode>
-__device__ __forceinline__ void load_row(const NormRopeArgs& a, const NormArgs& t, int64_t row,
-                                         int64_t active, int l, RowLoads& r) {
-  const int64_t safe = row < t.rows ? row : 0;
-  const int64_t token = fastdiv(static_cast<uint32_t>(safe), t.h_div);
-  const uint16_t* x = t.x + token * t.s0 + (safe - token * t.heads) * t.s1;
-  r.live = row < t.rows && token < active;
-  r.x = *reinterpret_cast<const u32x4*>(x + 8 * l);
-  const int64_t pos = r.live ? a.positions[token] : 0;
+template <int kMode, bool kFp32>
+__device__ __forceinline__ void load_angles(const NormRopeArgs& a, int64_t token, int64_t position,
+                                            int64_t active, int l, Angles<kMode, kFp32>& r) {
+  r.live = token < active;
+  const int64_t pos = r.live ? position : 0;
   r.bad = a.rotary > 0 && (pos < 0 || pos >= a.table_rows);
+  if (8 * l >= a.rotary) return;  // nothing is read
   const int64_t at = (r.bad ? 0 : pos) * a.table_stride;
   const int half = a.rotary >> 1;
-  if (8 * l >= a.rotary) return;  // nothing else is read
-  if (kMode == kPairHalves) {
-    const bool low = 8 * l < half;
-    const int d = low ? 8 * l : 8 * l - half;
-    unpack_eight(*reinterpret_cast<const u32x4*>(x + (low ? 8 * l + half : 8 * l - half)), r.pair);
-    load_eight(a.table, at + d, a.table_fp32, r.c);
-    load_eight(a.table, at + half + d, a.table_fp32, r.s);
+  if constexpr (kMode == kPairHalves) {
+    const int64_t c = at + (8 * l < half ? 8 * l : 8 * l - half);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r.s[e] = low ? -r.s[e] : r.s[e];
-  } else if (kMode == kPairAdjacent) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float c = load_value(a.table, at + 4 * l + e, a.table_fp32);
-      const float s = load_value(a.table, at + half + 4 * l + e, a.table_fp32);
-      r.c[2 * e] = r.c[2 * e + 1] = c;
-      r.s[2 * e] = -s;
-      r.s[2 * e + 1] = s;
+    for (int w = 0; w < r.kWords; ++w) {
+      const char* p = static_cast<const char*>(a.table) + 16 * w;
+      r.c[w] = *reinterpret_cast<const u32x4*>(p + c * (kFp32 ? 4 : 2));
+      r.s[w] = *reinterpret_cast<const u32x4*>(p + (c + half) * (kFp32 ? 4 : 2));
     }
-    float v[8];
-    unpack_eight(r.x, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r.pair[e] = v[e ^ 1];
+  } else if constexpr (kMode == kPairAdjacent) {  // four pairs a lane
+    if constexpr (kFp32) {
+      r.c[0] = *reinterpret_cast<const u32x4*>(static_cast<const float*>(a.table) + at + 4 * l);
+      r.s[0] = *reinterpret_cast<const u32x4*>(static_cast<const float*>(a.table) + at + half + 4 * l);
+    } else {
+      const uint16_t* t = static_cast<const uint16_t*>(a.table) + at + 4 * l;
+      const uint2 c = *reinterpret_cast<const uint2*>(t);
+      const uint2 s = *reinterpret_cast<const uint2*>(t + half);
+      r.c[0] = u32x4{c.x, c.y, 0u, 0u};
+      r.s[0] = u32x4{s.x, s.y, 0u, 0u};
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -170,19 +152,88 @@ __device__ __forceinline__ void load_row(const NormRopeArgs& a, const NormArgs& 
       int p, j;
       float sign;
       pair_of(a, 8 * l + e, p, j, sign);
-      r.pair[e] = bf16_to_float(x[p]);
-      r.c[e] = load_value(a.table, at + j, a.table_fp32);
-      r.s[e] = sign * load_value(a.table, at + half + j, a.table_fp32);
+      r.c[e >> 2][e & 3] = __float_as_uint(load_value(a.table, at + j, kFp32));
+      r.s[e >> 2][e & 3] = __float_as_uint(load_value(a.table, at + half + j, kFp32));
+    }
+  }
+}
+
+// Cosine and sine of the lane's dim 8 l + e, the sine with the sign of the partner's term.
+template <int kMode, bool kFp32>
+__device__ __forceinline__ void angle_of(const NormRopeArgs& a, const Angles<kMode, kFp32>& r, int l,
+                                         int e, float& c, float& s) {
+  auto half_word = [](uint32_t w, int i) { return bf16_to_float(i & 1 ? w >> 16 : w & 0xffffu); };
+  if constexpr (kMode == kPairAdjacent) {
+    const int j = e >> 1;
+    c = kFp32 ? __uint_as_float(r.c[0][j]) : half_word(r.c[0][j >> 1], j);
+    s = kFp32 ? __uint_as_float(r.s[0][j]) : half_word(r.s[0][j >> 1], j);
+    s = e & 1 ? s : -s;
+  } else if constexpr (kMode == kPairHalves) {
+    c = kFp32 ? __uint_as_float(r.c[e >> 2 & (r.kWords - 1)][e & 3]) : half_word(r.c[0][e >> 1], e);
+    s = kFp32 ? __uint_as_float(r.s[e >> 2 & (r.kWords - 1)][e & 3]) : half_word(r.s[0][e >> 1], e);
+    s = 8 * l < (a.rotary >> 1) ? -s : s;
+  } else {
+    int p, j;
+    float sign = 1.f;
+    pair_of(a, 8 * l + e, p, j, sign);
+    c = __uint_as_float(r.c[e >> 2][e & 3]);
+    s = sign * __uint_as_float(r.s[e >> 2][e & 3]);
+  }
+}
+
+template <int kMode>
+__device__ __forceinline__ void load_row(const NormRopeArgs& a, const uint16_t* x, int l,
+                                         RowLoads& r) {
+  r.x = *reinterpret_cast<const u32x4*>(x + 8 * l);
+  if (kMode == kPairAdjacent || 8 * l >= a.rotary) return;
+  const int half = a.rotary >> 1;
+  if (kMode == kPairHalves) {
+    r.pair = *reinterpret_cast<const u32x4*>(x + (8 * l < half ? 8 * l + half : 8 * l - half));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (8 * l + e >= a.rotary) break;
+      int p, j;
+      float sign;
+      pair_of(a, 8 * l + e, p, j, sign);
+      const uint32_t bits = x[p];
+      r.pair[e >> 1] = e & 1 ? (r.pair[e >> 1] & 0xffffu) | bits << 16
+                             : (r.pair[e >> 1] & 0xffff0000u) | bits;
     }
   }
 }
 
 // The row's 8 dims of this lane as bf16: zeros past the live tokens, NaN at a position outside the
 // table (never a row of wrong angles).
-__device__ __forceinline__ u32x4 finish_row(const NormRopeArgs& a, const LaneWeights& w,
-                                            const RowLoads& r, int l) {
-  float v[8], sum = 0.f;
+template <int kMode, bool kFp32>
+__device__ __forceinline__ u32x4 finish_row(const NormRopeArgs& a, const float* s_weight,
+                                            const Angles<kMode, kFp32>& t, const RowLoads& r,
+                                            int l) {
+  float v[8], pair[8], own_w[8], pair_w[8], sum = 0.f;
   unpack_eight(r.x, v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) own_w[e] = s_weight[8 * l + e];
+  const int half = a.rotary >> 1;
+  const int partner = 8 * l >= a.rotary ? 0 : 8 * l < half ? 8 * l + half : 8 * l - half;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (kMode == kPairAdjacent) {
+      pair_w[e] = own_w[e ^ 1];
+    } else if (kMode == kPairHalves) {
+      pair_w[e] = s_weight[partner + e];
+    } else {
+      int p = 0, j;
+      float sign;
+      if (8 * l + e < a.rotary) pair_of(a, 8 * l + e, p, j, sign);
+      pair_w[e] = s_weight[p];
+    }
+  }
+  if (kMode == kPairAdjacent) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pair[e] = v[e ^ 1];
+  } else {
+    unpack_eight(r.pair, pair);
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
   sum += dpp<kDppQuadXor1>(sum);
@@ -190,17 +241,25 @@ __device__ __forceinline__ u32x4 finish_row(const NormRopeArgs& a, const LaneWei
   sum += dpp<kDppRowHalfMirror>(sum);
   sum += dpp<kDppRowMirror>(sum);
   sum = sum_xor16(sum);
-  const float inv = r.bad ? __uint_as_float(0x7fc00000u)
-                          : 1.0f / sqrtf(fmaf(sum, 1.0f / kHeadDim, a.eps));
+  // The hardware's reciprocal root (within one unit of the last place), whose argument may not be
+  // subnormal.
+  float mean = fmaf(sum, 1.0f / kHeadDim, a.eps);
+  const bool tiny = mean < 0x1p-96f;
+  mean = tiny ? mean * 0x1p96f : mean;
+  float inv = __builtin_amdgcn_rsqf(mean);
+  inv = tiny ? inv * 0x1p48f : inv;
+  inv = t.bad ? __uint_as_float(0x7fc00000u) : inv;
   float o[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float y = v[e] * inv * w.own[e], p = r.pair[e] * inv * w.pair[e];
-    o[e] = 8 * l + e < a.rotary ? fmaf(y, r.c[e], p * r.s[e]) : y;
+    const float y = v[e] * inv * own_w[e], p = pair[e] * inv * pair_w[e];
+    float c, s;
+    angle_of(a, t, l, e, c, s);
+    o[e] = 8 * l + e < a.rotary ? fmaf(y, c, p * s) : y;
   }
   u32x4 bits;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) bits[e] = r.live ? pack_bf16x2(o[2 * e], o[2 * e + 1]) : 0u;
+  for (int e = 0; e < 4; ++e) bits[e] = t.live ? pack_bf16x2(o[2 * e], o[2 * e + 1]) : 0u;
   return bits;
 }
 
@@ -208,118 +267,166 @@ __device__ __forceinline__ int64_t live_tokens(const NormRopeArgs& a) {
   return a.counts ? min(static_cast<int64_t>(max(a.counts[1], 0)), a.n) : a.n;
 }
 
-// ---- no rotation by R_k: 8 rows per workgroup, query rows first.
-template <int kMode>
+// ---- no rotation by R_k. Half a wavefront takes one token's rows of up to kRopeHeads heads: their
+// loads and the token's angles are in flight together (one row per half wavefront, the angles read
+// again for each, keeps half as many bytes in flight: 16384 tokens x 7 heads 30 us).
+constexpr int kRopeHeads = 4;
+
+template <int kMode, bool kFp32>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeArgs a,
-                                                             int64_t q_blocks) {
+                                                             int64_t q_blocks, FastDiv q_div,
+                                                             FastDiv k_div) {
+  __shared__ float s_weight[kHeadDim];
   const int l = threadIdx.x & 31;
   const bool is_q = blockIdx.x < q_blocks;
   const NormArgs& t = is_q ? a.q : a.k;
-  const int64_t row = (blockIdx.x - (is_q ? 0 : q_blocks)) * 8 + (threadIdx.x >> 5);
-  RowLoads r;
-  LaneWeights w;
-  load_row<kMode>(a, t, row, live_tokens(a), l, r);
-  load_weights<kMode>(a, t.weight, l, w);
-  const u32x4 bits = finish_row(a, w, r, l);
-  if (row < t.rows) *reinterpret_cast<u32x4*>(t.out + row * kHeadDim + 8 * l) = bits;
+  stage_weights(a, t.weight, s_weight, 0);
+  __syncthreads();
+  const FastDiv div = is_q ? q_div : k_div;  // items per token
+  const uint32_t item =
+      static_cast<uint32_t>((blockIdx.x - (is_q ? 0 : q_blocks)) * 8 + (threadIdx.x >> 5));
+  const uint32_t index = fastdiv(item, div);
+  if (index >= a.n) return;
+  const int64_t token = index;
+  const int h0 = static_cast<int>(item - index * div.divisor) * kRopeHeads;
+  const int count = min(kRopeHeads, t.heads - h0);
+  const int64_t active = live_tokens(a);
+  const int64_t position = token < active ? a.positions[token] : 0;
+  const uint16_t* x = t.x + token * t.s0 + h0 * t.s1;
+  RowLoads r[kRopeHeads];
+#pragma unroll
+  for (int i = 0; i < kRopeHeads; ++i)
+    if (i < count) load_row<kMode>(a, x + i * t.s1, l, r[i]);
+  Angles<kMode, kFp32> angles;
+  load_angles(a, token, position, active, l, angles);
+  uint16_t* out = t.out + (token * t.heads + h0) * kHeadDim + 8 * l;
+#pragma unroll
+  for (int i = 0; i < kRopeHeads; ++i)
+    if (i < count)
+      *reinterpret_cast<u32x4*>(out + i * kHeadDim) = finish_row(a, s_weight, angles, r[i], l);
 }
 
-// ---- with the rotation: workgroups of 8 wavefronts walk 16-row blocks of the queries. A wavefront
-// keeps its 16 kTiles columns of R_k in registers for the whole walk (kTiles 2: the workgroup holds
-// R_k once, 64 registers a lane; kTiles 1: two workgroups share the columns of a block, for the few
-// rows of a decode step). The block's rows go through LDS (16-byte piece p of row r at p ^ r) as the
-// B operand; the columns are the A operand, so that a lane ends with 4 kTiles consecutive columns
-// of one row and stores them at once. Key rows are workgroups of their own behind the queries'.
-constexpr int kRopeWaves = 8;
-
-template <int kMode, int kTiles>
-__global__ __launch_bounds__(kRopeWaves * kWave, kTiles == 2 || kMode == kPairGeneric ? 2 : 4) void norm_rope_rotate_kernel(
-    const NormRopeArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t s_rows[2][16 * kHeadDim * 2];
-  const int tid = threadIdx.x, l = tid & 31, r16 = tid >> 5;
+// ---- with the rotation: workgroups of kWaves wavefronts walk blocks of 2 kWaves query rows, one per
+// half wavefront. A wavefront keeps 16 columns of R_k in registers for the whole walk (32 a lane): 16
+// wavefronts hold all of R_k, 8 half of it (the rows of a decode step, few blocks: two workgroups
+// share a block and each reads half as much of R_k). The block's rows go through LDS (16-byte piece p
+// of row r at p ^ r % 16) as the B operand; the columns are the A operand, so that a lane ends with
+// four consecutive columns of a row. While a block is multiplied, the next one's rows are normed and
+// the loads of the one after are in flight, with its positions read a block earlier. The keys' blocks
+// follow the queries' in the walk.
+template <int kMode, bool kFp32, int kWaves>
+__global__ __launch_bounds__(kWaves * kWave, 4) void norm_rope_rotate_kernel(const NormRopeArgs a) {
+  constexpr int kRows = 2 * kWaves, kSets = kWaves / 8;
+  __shared__ __attribute__((aligned(16))) uint8_t s_rows[2][kRows * kHeadDim * 2];
+  __shared__ float s_weight[2][kHeadDim];
+  const int tid = threadIdx.x, l = tid & 31, mine = tid >> 5;
   const int64_t active = live_tokens(a);
-  const bool is_q = static_cast<int>(blockIdx.x) < a.q_groups;
-  LaneWeights w;
-  if (!is_q) {
-    if (blockIdx.y) return;
-    const int64_t row = static_cast<int64_t>(blockIdx.x - a.q_groups) * 16 + r16;
-    RowLoads r;
-    load_row<kMode>(a, a.k, row, active, l, r);
-    load_weights<kMode>(a, a.k.weight, l, w);
-    const u32x4 bits = finish_row(a, w, r, l);
-    if (row < a.k.rows) *reinterpret_cast<u32x4*>(a.k.out + row * kHeadDim + 8 * l) = bits;
-    return;
-  }
-  const int lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  // A row n of tile t is column base + 4 kTiles (n / 4) + 4 t + n % 4.
-  const int base = 16 * kTiles * (kRopeWaves * blockIdx.y + wave);
-  const int64_t blocks = (a.q.rows + 15) / 16;
+  const int64_t q_blocks = (a.q.rows + kRows - 1) / kRows;
+  const int64_t blocks = q_blocks + (a.k.rows + kRows - 1) / kRows;
+  const int64_t first = blockIdx.x, step = gridDim.x;
   RowLoads r;
-  load_row<kMode>(a, a.q, static_cast<int64_t>(blockIdx.x) * 16 + r16, active, l, r);
-  load_weights<kMode>(a, a.q.weight, l, w);
-  u32x4 rk[kTiles][8];
+  Angles<kMode, kFp32> angles;
+  int64_t position;
+  auto rows_of = [&](int64_t b) -> const NormArgs& { return b < q_blocks ? a.q : a.k; };
+  auto my_row = [&](int64_t b) { return (b < q_blocks ? b : b - q_blocks) * kRows + mine; };
+  // This half wavefront's row of block b; rows past the last are no live token's (and read row 0).
+  auto load_position = [&](int64_t b) {
+    const NormArgs& t = rows_of(b);
+    const int64_t row = my_row(b);
+    const int64_t token = row < t.rows ? fastdiv(static_cast<uint32_t>(row), t.h_div) : a.n;
+    position = token < active ? a.positions[token] : 0;
+  };
+  auto load_block = [&](int64_t b) {
+    const NormArgs& t = rows_of(b);
+    const int64_t row = my_row(b);
+    const uint32_t safe = row < t.rows ? static_cast<uint32_t>(row) : 0u;
+    const uint32_t token = fastdiv(safe, t.h_div);
+    load_row<kMode>(a, t.x + static_cast<int64_t>(token) * t.s0 +
+                           static_cast<int64_t>(safe - token * static_cast<uint32_t>(t.heads)) * t.s1,
+                    l, r);
+    load_angles(a, row < t.rows ? static_cast<int64_t>(token) : a.n, position, active, l, angles);
+  };
+  auto finish_block = [&](int64_t b, int buf) {
+    const NormArgs& t = rows_of(b);
+    const int64_t row = my_row(b);
+    const u32x4 bits = finish_row(a, s_weight[b < q_blocks ? 0 : 1], angles, r, l);
+    *reinterpret_cast<u32x4*>(&s_rows[buf][mine * 512 + 16 * (l ^ (mine & 15))]) = bits;
+    if (blockIdx.y == 0 && row < t.rows)
+      *reinterpret_cast<u32x4*>(t.out + row * kHeadDim + 8 * l) = bits;
+  };
+  load_position(first);
+  stage_weights(a, a.q.weight, s_weight[0], 0);
+  stage_weights(a, a.k.weight, s_weight[1], 32);
+  load_block(first);
+  const int lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int base = 16 * (kWaves * blockIdx.y + wave);
+  u32x4 rk[8];
+  if (first < q_blocks) {
+    const uint16_t* col = a.rk_t + static_cast<int64_t>(base + n) * kHeadDim + 8 * g;
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    const uint16_t* col =
-        a.rk_t + static_cast<int64_t>(base + 4 * kTiles * (n >> 2) + 4 * t + (n & 3)) * kHeadDim;
-#pragma unroll
-    for (int m = 0; m < 8; ++m) rk[t][m] = *reinterpret_cast<const u32x4*>(col + 32 * m + 8 * g);
+    for (int m = 0; m < 8; ++m) rk[m] = *reinterpret_cast<const u32x4*>(col + 32 * m);
   }
+  __syncthreads();  // the weights
+  finish_block(first, 0);
+  if (first + step < blocks) {
+    load_position(first + step);
+    load_block(first + step);
+    load_position(first + 2 * step);
+  }
+  __syncthreads();
   int buf = 0;
-  for (int64_t b = blockIdx.x; b < blocks; b += a.q_groups, buf ^= 1) {
-    const int64_t row = b * 16 + r16;
-    const u32x4 bits = finish_row(a, w, r, l);
-    *reinterpret_cast<u32x4*>(&s_rows[buf][r16 * 512 + 16 * (l ^ r16)]) = bits;
-    if (blockIdx.y == 0 && row < a.q.rows)
-      *reinterpret_cast<u32x4*>(a.q.out + row * kHeadDim + 8 * l) = bits;
-    // The next block's rows are in flight while this one's are multiplied.
-    if (b + a.q_groups < blocks) load_row<kMode>(a, a.q, row + 16ll * a.q_groups, active, l, r);
-    __syncthreads();  // one barrier per block: the other buffer's readers are a block behind it
-    f32x4 acc[kTiles];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int m = 0; m < 8; ++m) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(&s_rows[buf][n * 512 + 16 * ((4 * m + g) ^ n)]);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) acc[t] = mfma16x16x32(rk[t][m], x, acc[t]);
-    }
-    const int64_t orow = b * 16 + n;
-    if (orow < a.q.rows) {
-      uint16_t* out = a.q_rot + orow * kHeadDim + base + 4 * kTiles * g;
-      if constexpr (kTiles == 2) {
-        *reinterpret_cast<u32x4*>(out) =
-            u32x4{pack_bf16x2(acc[0][0], acc[0][1]), pack_bf16x2(acc[0][2], acc[0][3]),
-                  pack_bf16x2(acc[1][0], acc[1][1]), pack_bf16x2(acc[1][2], acc[1][3])};
-      } else {
-        *reinterpret_cast<uint2*>(out) =
-            make_uint2(pack_bf16x2(acc[0][0], acc[0][1]), pack_bf16x2(acc[0][2], acc[0][3]));
+  for (int64_t b = first; b < blocks; b += step, buf ^= 1) {
+    if (b + step < blocks) {
+      finish_block(b + step, buf ^ 1);
+      if (b + 2 * step < blocks) {
+        load_block(b + 2 * step);
+        load_position(b + 3 * step);
       }
     }
+    if (b < q_blocks) {
+#pragma unroll
+      for (int i = 0; i < kSets; ++i) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+          acc = mfma16x16x32(rk[m], *reinterpret_cast<const u32x4*>(
+                                        &s_rows[buf][(16 * i + n) * 512 + 16 * ((4 * m + g) ^ n)]),
+                             acc);
+        const int64_t row = b * kRows + 16 * i + n;
+        if (row < a.q.rows)
+          *reinterpret_cast<uint2*>(a.q_rot + row * kHeadDim + base + 4 * g) =
+              make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
+      }
+    }
+    __syncthreads();  // this block's rows are read, the next one's are written
   }
 }
 
-// Query blocks up to which two workgroups share a block's columns: with fewer blocks than CUs the
-// second workgroup halves what each reads of R_k.
-constexpr int64_t kSharedColumnBlocks = 128;
-constexpr int64_t kRotateGroups = 256;  // one workgroup per CU walks the blocks
+// 16-row blocks up to which workgroups of 8 wavefronts take them; above, 256 workgroups of 16 (one
+// per CU) walk blocks of 32.
+constexpr int64_t kFewBlocks = 128, kRotateGroups = 256;
 
-template <int kMode>
+template <int kMode, bool kFp32>
 void launch_norm_rope(NormRopeArgs& a, hipStream_t s) {
   if (!a.rk_t) {
-    const int64_t q_blocks = (a.q.rows + 7) / 8, k_blocks = (a.k.rows + 7) / 8;
-    hipLaunchKernelGGL((norm_rope_kernel<kMode>), dim3(static_cast<unsigned>(q_blocks + k_blocks)),
-                       dim3(kThreads), 0, s, a, q_blocks);
+    const int64_t per_q = (a.q.heads + kRopeHeads - 1) / kRopeHeads;
+    const int64_t per_k = (a.k.heads + kRopeHeads - 1) / kRopeHeads;
+    const int64_t q_blocks = (a.n * per_q + 7) / 8, k_blocks = (a.n * per_k + 7) / 8;
+    hipLaunchKernelGGL((norm_rope_kernel<kMode, kFp32>),
+                       dim3(static_cast<unsigned>(q_blocks + k_blocks)), dim3(kThreads), 0, s, a,
+                       q_blocks, make_fastdiv(static_cast<uint32_t>(per_q)),
+                       make_fastdiv(static_cast<uint32_t>(per_k)));
     return;
   }
-  const int64_t blocks = (a.q.rows + 15) / 16;
-  a.q_groups = static_cast<int32_t>(blocks < kRotateGroups ? blocks : kRotateGroups);
-  const unsigned x = static_cast<unsigned>(a.q_groups + (a.k.rows + 15) / 16);
-  if (blocks <= kSharedColumnBlocks)
-    hipLaunchKernelGGL((norm_rope_rotate_kernel<kMode, 1>), dim3(x, 2), dim3(kRopeWaves * kWave), 0,
-                       s, a);
+  const bool few = (a.q.rows + 15) / 16 <= kFewBlocks;
+  const int64_t rows = few ? 16 : 32;
+  const int64_t blocks = (a.q.rows + rows - 1) / rows + (a.k.rows + rows - 1) / rows;
+  const unsigned x = static_cast<unsigned>(few || blocks < kRotateGroups ? blocks : kRotateGroups);
+  if (few)
+    hipLaunchKernelGGL((norm_rope_rotate_kernel<kMode, kFp32, 8>), dim3(x, 2), dim3(8 * kWave), 0, s,
+                       a);
   else
-    hipLaunchKernelGGL((norm_rope_rotate_kernel<kMode, 2>), dim3(x, 1), dim3(kRopeWaves * kWave), 0,
+    hipLaunchKernelGGL((norm_rope_rotate_kernel<kMode, kFp32, 16>), dim3(x, 1), dim3(16 * kWave), 0,
                        s, a);
 }
 
@@ -363,20 +470,25 @@ extern "C" int oscar_qk_norm_rope(const void* query, int64_t q_s0, int64_t q_s1,
   a.n = n;
   a.rotary = rotary_dim;
   a.weight_fp32 = weight_fp32 ? 1 : 0;
-  a.table_fp32 = table_fp32 ? 1 : 0;
   a.adjacent = interleaved ? 1 : 0;
   a.offset = unit_offset ? 1.f : 0.f;
   a.eps = eps;
   a.rk_t = static_cast<const uint16_t*>(rk_t);
   a.q_rot = static_cast<uint16_t*>(q_rot);
-  a.q_groups = 0;
   hipStream_t s = as_stream(stream);
   const bool rows16 = aligned16(cos_sin) && table_stride % 8 == 0;
-  if (interleaved && rotary_dim % 8 == 0)
-    launch_norm_rope<kPairAdjacent>(a, s);
+  auto launch = [&](auto mode) {
+    constexpr int kMode = decltype(mode)::value;
+    if (table_fp32)
+      launch_norm_rope<kMode, true>(a, s);
+    else
+      launch_norm_rope<kMode, false>(a, s);
+  };
+  if (interleaved && rotary_dim % 8 == 0 && rows16)
+    launch(std::integral_constant<int, kPairAdjacent>());
   else if (!interleaved && rotary_dim % 16 == 0 && rows16)
-    launch_norm_rope<kPairHalves>(a, s);
+    launch(std::integral_constant<int, kPairHalves>());
   else
-    launch_norm_rope<kPairGeneric>(a, s);
+    launch(std::integral_constant<int, kPairGeneric>());
   return static_cast<int>(hipGetLastError());
 }
