@@ -102,6 +102,9 @@ __device__ __forceinline__ void stage_weights(const NormRopeArgs& a, const void*
   load_eight(weight, 8 * i, a.weight_fp32, w);
 #pragma unroll
   for (int e = 0; e < 8; ++e) s_weight[8 * i + e] = w[e] + a.offset;
+  if (i == 0)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_weight[kHeadDim + e] = 0.f;
 }
 
 // A token's angles for the lane's dims, as they lie in the table: bf16 or fp32 words of the
@@ -123,7 +126,7 @@ __device__ __forceinline__ void load_angles(const NormRopeArgs& a, int64_t token
   r.live = token < active;
   const int64_t pos = r.live ? position : 0;
   r.bad = a.rotary > 0 && (pos < 0 || pos >= a.table_rows);
-  if (8 * l >= a.rotary) return;  // nothing is read
+  if (8 * l >= a.rotary) return;  // keeps its identity turn (start_row)
   const int64_t at = (r.bad ? 0 : pos) * a.table_stride;
   const int half = a.rotary >> 1;
   if constexpr (kMode == kPairHalves) {
@@ -158,26 +161,45 @@ __device__ __forceinline__ void load_angles(const NormRopeArgs& a, int64_t token
   }
 }
 
-// Cosine and sine of the lane's dim 8 l + e, the sine with the sign of the partner's term.
+// A lane past the rotary dims turns by cosine 1, sine 0 and a partner of 0 times 0: set once, since
+// the loads leave such lanes alone. (A lane that ends inside them, as generic dims may, is selected
+// per element.)
 template <int kMode, bool kFp32>
-__device__ __forceinline__ void angle_of(const NormRopeArgs& a, const Angles<kMode, kFp32>& r, int l,
-                                         int e, float& c, float& s) {
+__device__ __forceinline__ void start_row(Angles<kMode, kFp32>& t, RowLoads& r) {
+  const bool fp32 = kFp32 || kMode == kPairGeneric;
+#pragma unroll
+  for (int w = 0; w < t.kWords; ++w)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      t.c[w][e] = fp32 ? 0x3f800000u : 0x3f803f80u;
+      t.s[w][e] = 0u;
+      r.pair[e] = 0u;
+    }
+}
+
+// Cosine and sine of the lane's dim 8 l + e; the partner's term has the sign of partner_sign.
+template <int kMode>
+__device__ __forceinline__ float partner_sign(const NormRopeArgs& a, int l, int e, float v) {
+  if (kMode == kPairAdjacent) return e & 1 ? v : -v;
+  if (kMode == kPairHalves) return v;  // one sign a lane, taken before (finish_row)
+  int p, j;
+  float sign;
+  pair_of(a, 8 * l + e, p, j, sign);
+  return sign * v;
+}
+template <int kMode, bool kFp32>
+__device__ __forceinline__ void angle_of(const Angles<kMode, kFp32>& r, int e, float& c, float& s) {
   auto half_word = [](uint32_t w, int i) { return bf16_to_float(i & 1 ? w >> 16 : w & 0xffffu); };
   if constexpr (kMode == kPairAdjacent) {
     const int j = e >> 1;
     c = kFp32 ? __uint_as_float(r.c[0][j]) : half_word(r.c[0][j >> 1], j);
     s = kFp32 ? __uint_as_float(r.s[0][j]) : half_word(r.s[0][j >> 1], j);
-    s = e & 1 ? s : -s;
   } else if constexpr (kMode == kPairHalves) {
     c = kFp32 ? __uint_as_float(r.c[e >> 2 & (r.kWords - 1)][e & 3]) : half_word(r.c[0][e >> 1], e);
     s = kFp32 ? __uint_as_float(r.s[e >> 2 & (r.kWords - 1)][e & 3]) : half_word(r.s[0][e >> 1], e);
-    s = 8 * l < (a.rotary >> 1) ? -s : s;
   } else {
-    int p, j;
-    float sign = 1.f;
-    pair_of(a, 8 * l + e, p, j, sign);
     c = __uint_as_float(r.c[e >> 2][e & 3]);
-    s = sign * __uint_as_float(r.s[e >> 2][e & 3]);
+    s = __uint_as_float(r.s[e >> 2][e & 3]);
   }
 }
 
@@ -214,7 +236,8 @@ __device__ __forceinline__ u32x4 finish_row(const NormRopeArgs& a, const float* 
 #pragma unroll
   for (int e = 0; e < 8; ++e) own_w[e] = s_weight[8 * l + e];
   const int half = a.rotary >> 1;
-  const int partner = 8 * l >= a.rotary ? 0 : 8 * l < half ? 8 * l + half : 8 * l - half;
+  // Past the rotary dims: the zeros behind the weights.
+  const int partner = 8 * l >= a.rotary ? kHeadDim : 8 * l < half ? 8 * l + half : 8 * l - half;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     if (kMode == kPairAdjacent) {
@@ -222,7 +245,7 @@ __device__ __forceinline__ u32x4 finish_row(const NormRopeArgs& a, const float* 
     } else if (kMode == kPairHalves) {
       pair_w[e] = s_weight[partner + e];
     } else {
-      int p = 0, j;
+      int p = kHeadDim, j;
       float sign;
       if (8 * l + e < a.rotary) pair_of(a, 8 * l + e, p, j, sign);
       pair_w[e] = s_weight[p];
@@ -249,13 +272,15 @@ __device__ __forceinline__ u32x4 finish_row(const NormRopeArgs& a, const float* 
   float inv = __builtin_amdgcn_rsqf(mean);
   inv = tiny ? inv * 0x1p48f : inv;
   inv = t.bad ? __uint_as_float(0x7fc00000u) : inv;
+  const float pair_inv = kMode == kPairHalves && 8 * l < half ? -inv : inv;
   float o[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float y = v[e] * inv * own_w[e], p = pair[e] * inv * pair_w[e];
+    const float y = v[e] * inv * own_w[e], p = pair[e] * pair_inv * pair_w[e];
     float c, s;
-    angle_of(a, t, l, e, c, s);
-    o[e] = 8 * l + e < a.rotary ? fmaf(y, c, p * s) : y;
+    angle_of(t, e, c, s);
+    const float turned = fmaf(y, c, partner_sign<kMode>(a, l, e, p) * s);
+    o[e] = kMode == kPairHalves || 8 * l + e < a.rotary ? turned : y;
   }
   u32x4 bits;
 #pragma unroll
@@ -276,7 +301,7 @@ template <int kMode, bool kFp32>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeArgs a,
                                                              int64_t q_blocks, FastDiv q_div,
                                                              FastDiv k_div) {
-  __shared__ float s_weight[kHeadDim];
+  __shared__ float s_weight[kHeadDim + 8];
   const int l = threadIdx.x & 31;
   const bool is_q = blockIdx.x < q_blocks;
   const NormArgs& t = is_q ? a.q : a.k;
@@ -294,10 +319,12 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeArgs 
   const int64_t position = token < active ? a.positions[token] : 0;
   const uint16_t* x = t.x + token * t.s0 + h0 * t.s1;
   RowLoads r[kRopeHeads];
+  Angles<kMode, kFp32> angles;
+#pragma unroll
+  for (int i = 0; i < kRopeHeads; ++i) start_row(angles, r[i]);
 #pragma unroll
   for (int i = 0; i < kRopeHeads; ++i)
     if (i < count) load_row<kMode>(a, x + i * t.s1, l, r[i]);
-  Angles<kMode, kFp32> angles;
   load_angles(a, token, position, active, l, angles);
   uint16_t* out = t.out + (token * t.heads + h0) * kHeadDim + 8 * l;
 #pragma unroll
@@ -318,7 +345,7 @@ template <int kMode, bool kFp32, int kWaves>
 __global__ __launch_bounds__(kWaves * kWave, 4) void norm_rope_rotate_kernel(const NormRopeArgs a) {
   constexpr int kRows = 2 * kWaves, kSets = kWaves / 8;
   __shared__ __attribute__((aligned(16))) uint8_t s_rows[2][kRows * kHeadDim * 2];
-  __shared__ float s_weight[2][kHeadDim];
+  __shared__ float s_weight[2][kHeadDim + 8];
   const int tid = threadIdx.x, l = tid & 31, mine = tid >> 5;
   const int64_t active = live_tokens(a);
   const int64_t q_blocks = (a.q.rows + kRows - 1) / kRows;
@@ -326,6 +353,7 @@ __global__ __launch_bounds__(kWaves * kWave, 4) void norm_rope_rotate_kernel(con
   const int64_t first = blockIdx.x, step = gridDim.x;
   RowLoads r;
   Angles<kMode, kFp32> angles;
+  start_row(angles, r);
   int64_t position;
   auto rows_of = [&](int64_t b) -> const NormArgs& { return b < q_blocks ? a.q : a.k; };
   auto my_row = [&](int64_t b) { return (b < q_blocks ? b : b - q_blocks) * kRows + mine; };
