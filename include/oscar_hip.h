@@ -634,7 +634,7 @@ int oscar_compact_pages(const void* stripes, int64_t layers, int64_t num_pages,
  * read). It writes the step's units (int32 [capacity][8], 16-byte aligned), their number and the
  * partial rows of every token below counts[1] (token_slots, int32 [tokens]). `slots` (4..256) bounds
  * the partial rows of a row; tokens the query tokens of the step; capacity at least
- * oscar_shared_capacity of the same sizes. groups + max_reqs <= 6144 and hq / kv_heads <= 32, else
+ * oscar_shared_capacity of the same sizes. groups + max_reqs <= 4096 and hq / kv_heads <= 32, else
  * OSCAR_E_UNSUPPORTED. Starts that descend share nothing.
  *
  * shared_history, per layer: query is the rotated query, partials fp32 [n][hq][slots][256] and lse

@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kThreadsC, 2) void history_chunk_kernel(const AttnA
   int begin, end;
   split_range(t.recent_begin - t.sink_len, a.block_n, a.splits, split, begin, end);
   const int p_lo = max(t.sink_len + begin, 0), p_hi = t.sink_len + end;
-  chunk_tile(a, t, head, rows, row_base, p_lo, p_hi, split, lds);
+  chunk_tile<false>(a, t, head, rows, row_base, p_lo, p_hi, split, lds);
 }
 
 }  // namespace

@@ -5,7 +5,9 @@
 // Wavefront w takes chunks w, w + 8, ... through a private two-stage LDS ring, keeps its own
 // online-softmax state, and the eight states are merged once at the end, so the token loop has no
 // barrier. In chunk_tile.h such a tile would leave seven wavefronts waiting for one. Operand layouts
-// and arithmetic per chunk are those of history.hip's one-tile kernel (four wavefronts there).
+// and arithmetic per chunk are those of history.hip's one-tile kernel (four wavefronts there), but
+// for the values being centred as in chunk_tile.h, here by P's own sum: one more MFMA against ones
+// gives the sum of the rounded P, and sum P c - 1.5 sum P + sum p (z + 1.5 s) is the row.
 #pragma once
 
 #include <type_traits>
@@ -20,7 +22,7 @@ constexpr int kRowTileTable = 512;  // kernel blocks whose offsets live in LDS
 struct RowTileLds {
   uint8_t ring[kWavesC][2][kStageBytes] __attribute__((aligned(16)));
   uint32_t off[kRowTileTable];
-  float red[3][kWavesC][16];  // per wavefront: row max, sum p, sum p z_v
+  float red[4][kWavesC][16];  // per wavefront: row max, sum p, sum p (z_v + 1.5 s_v), P's sum
 };
 static_assert(kWavesC * 16 * kHeadDim * 4 <= sizeof(RowTileLds::ring), "the merge fits the ring");
 
@@ -134,6 +136,7 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
   f32x4 o[16];  // o[2 c + par]: rows 4 g + v, dim 32 c + 2 n + par (units of code / 2)
 #pragma unroll
   for (int c = 0; c < 16; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 ones_o = {0.f, 0.f, 0.f, 0.f};  // P's sums of rows 4 g + v
 
   auto process = [&](int j, auto stage_tag) {
     constexpr int S = decltype(stage_tag)::value;
@@ -195,6 +198,7 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
         const float av = __shfl(alpha, 4 * g + v, kWave);
 #pragma unroll
         for (int c = 0; c < 16; ++c) o[c][v] *= av;
+        ones_o[v] *= av;
       }
     }
     const float nm = m == -INFINITY ? 0.f : -m;
@@ -204,7 +208,7 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
     for (int e = 0; e < 16; ++e) {
       const float p = __builtin_amdgcn_exp2f(fmaf(r2[e], fq, nm));
       psum += p;
-      zsum = fmaf(p, h16hi(vsz[e]), zsum);
+      zsum = fmaf(p, fmaf(1.5f, h16lo(vsz[e]), h16hi(vsz[e])), zsum);
       av[e] = p * h16lo(vsz[e]);
       amax = fmaxf(amax, av[e]);
     }
@@ -222,6 +226,8 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
     const i32x8 pa = {(int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3],
                       (int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3]};
     const int sa = static_cast<int>(eb) - 6;
+    constexpr int kOnes = 0x22222222;  // FP4 1.0
+    ones_o = mfma_pv(pa, i32x8{kOnes, kOnes, kOnes, kOnes, 0, 0, 0, 0}, ones_o, sa);
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       const i32x2 r0 = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2_ptr_t)(st + v_off + 8 * c));
@@ -259,11 +265,13 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
     lds.red[1][wave][n] = psum;
     lds.red[2][wave][n] = zsum;
   }
+  if (n == 0) *reinterpret_cast<f32x4*>(&lds.red[3][wave][4 * g]) = ones_o;
   __syncthreads();  // every chunk consumed; the ring is free for the merge
   float* s_o = reinterpret_cast<float*>(&lds.ring[0][0][0]);  // [wavefront][row][256]
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
     const int row = 4 * g + v;
+    if (row_base + row >= rows) break;  // no row: nothing reads its part of the area
     float mx = lds.red[0][0][row];
 #pragma unroll
     for (int w = 1; w < kWavesC; ++w) mx = fmaxf(mx, lds.red[0][w][row]);
@@ -291,7 +299,7 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
     const float mw = lds.red[0][w][row16];
     const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx);
     den = fmaf(f, lds.red[1][w][row16], den);
-    zs = fmaf(f, lds.red[2][w][row16], zs);
+    zs = fmaf(f, fmaf(-1.5f, lds.red[3][w][row16], lds.red[2][w][row16]), zs);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       sum[h] += *reinterpret_cast<const f32x4*>(s_o + (w * 16 + row16) * kHeadDim + d0 + 128 * h);

@@ -24,13 +24,13 @@ namespace oscar {
 namespace {
 
 constexpr int kSharedThreads = 1024;
-constexpr int kSharedEntries = 6144;  // groups and requests whose counts live in LDS
+constexpr int kSharedEntries = 4096;  // groups and requests whose counts live in LDS
 constexpr int kSharedSlots = 256;     // partial rows of a row: four per lane of a merging wavefront
 constexpr int kUnitWords = 8;
 // Rows up to which a tile is 16 rows; 128-token chunks such a unit takes at least.
-constexpr int kSmallRows = 48, kSmallPiece = 8;
+constexpr int kSmallRows = 48, kSmallPiece = 4;
 // A unit's time in us: its start and end, and each 128-token chunk.
-constexpr float kTileStart = 10.f, kTileChunk = 4.5f, kSmallStart = 10.f, kSmallChunk = 1.2f;
+constexpr float kTileStart = 11.f, kTileChunk = 4.1f, kSmallStart = 11.f, kSmallChunk = 0.8f;
 
 // A unit: rows [row_base, row_end) of tokens token0 .. (row r is token token0 + r / g), positions
 // [p_lo, p_hi) through block-table row req, partials to `slot`; small: at most 16 rows, row_tile.h.
@@ -52,25 +52,25 @@ struct SharedPlanArgs {
   int64_t tokens;
 };
 
-// Sum and maximum over the workgroup (every thread gets both).
-__device__ __forceinline__ void plan_reduce(int64_t& sum, int& most) {
-  __shared__ int64_t s_sum[kSharedThreads / kWave];
+// Sums of two counts and a maximum over the workgroup (every thread gets them).
+__device__ __forceinline__ void plan_reduce(int64_t (&sum)[2], int& most) {
+  __shared__ int64_t s_sum[2][kSharedThreads / kWave];
   __shared__ int s_most[kSharedThreads / kWave];
-  sum = wave_sum_i64(sum);
+  const int wave = threadIdx.x >> 6;
+  for (int i = 0; i < 2; ++i) sum[i] = wave_sum_i64(sum[i]);
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) most = max(most, __shfl_xor(most, m, kWave));
-  const int wave = threadIdx.x >> 6;
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) {
-    s_sum[wave] = sum;
+    s_sum[0][wave] = sum[0];
+    s_sum[1][wave] = sum[1];
     s_most[wave] = most;
   }
   __syncthreads();
-  sum = 0;
-  most = 0;
+  sum[0] = sum[1] = 0;
 #pragma unroll
   for (int w = 0; w < kSharedThreads / kWave; ++w) {
-    sum += s_sum[w];
+    sum[0] += s_sum[0][w];
+    sum[1] += s_sum[1][w];
     most = max(most, s_most[w]);
   }
 }
@@ -86,41 +86,38 @@ __device__ __forceinline__ int chunks_of(int lo, int hi) {
 __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const SharedPlanArgs a) {
   // Entries: the groups, then the requests.
   __shared__ int s_chunks[kSharedEntries], s_tiles[kSharedEntries], s_start[kSharedEntries + 1];
-  __shared__ int s_own[kSharedEntries];  // first history position of a request's own part
-  __shared__ int s_group[kSharedEntries];  // the group whose positions a request shares, or -1
+  // Requests: first token, end of the history, first position of the request's own part, and the
+  // group whose positions it shares, or -1.
+  __shared__ int s_token[kSharedEntries + 1], s_end[kSharedEntries], s_own[kSharedEntries];
+  __shared__ int s_group[kSharedEntries];
   __shared__ int s_wave[kSharedThreads / kWave];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int reqs = max(min(a.counts[0], a.max_reqs), 0);
   const int active = static_cast<int>(
       min(static_cast<int64_t>(max(a.counts[1], 0)), a.tokens));
+  for (int r = tid; r < reqs; r += kSharedThreads) {
+    const int t0 = min(max(a.qstarts[r], 0), active), t1 = min(max(a.qstarts[r + 1], 0), active);
+    const int prefix = a.seq_lens[r] - max(t1 - t0, 0);
+    const int sink_len = max(min(a.sink, prefix), 0);
+    s_token[r] = t0;
+    if (r + 1 == reqs) s_token[reqs] = t1;
+    s_end[r] = max(sink_len, prefix - a.recent);
+    s_own[r] = sink_len;
+    s_group[r] = -1;
+  }
   // Starts that descend are no partition: then nothing is shared.
   bool bad = false;
   for (int i = tid; i < a.groups; i += kSharedThreads)
     bad |= a.group_starts[i + 1] < a.group_starts[i];
   const int groups = __syncthreads_or(bad) ? 0 : a.groups;
   const int entries = groups + reqs;
-
-  struct Span {
-    int prefix, sink_len, recent, rows;
-  };
-  auto token = [&](int r) { return min(max(a.qstarts[r], 0), active); };
-  auto span = [&](int r) {
-    Span s;
-    const int qlen = max(token(r + 1) - token(r), 0);
-    s.prefix = a.seq_lens[r] - qlen;
-    s.sink_len = max(min(a.sink, s.prefix), 0);
-    s.recent = max(s.sink_len, s.prefix - a.recent);
-    s.rows = qlen * a.g;
-    return s;
-  };
+  auto rows_of = [&](int r0, int r1) { return max(s_token[r1] - s_token[r0], 0) * a.g; };
   auto clip = [&](int r) { return min(max(r, 0), reqs); };
 
-  for (int r = tid; r < reqs; r += kSharedThreads) s_own[r] = s_group[r] = -1;
-  __syncthreads();
   for (int i = wave; i < groups; i += kSharedThreads / kWave) {
     const int r0 = clip(a.group_starts[i]), r1 = clip(a.group_starts[i + 1]);
     int end = a.prefix_tokens[i];
-    for (int r = r0 + lane; r < r1; r += kWave) end = min(end, span(r).recent);
+    for (int r = r0 + lane; r < r1; r += kWave) end = min(end, s_end[r]);
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) end = min(end, __shfl_xor(end, m, kWave));
     end &= ~(kTokC - 1);
@@ -132,35 +129,30 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
         s_group[r] = i;
       }
     if (lane == 0) {
-      const int rows = shared ? max(token(r1) - token(r0), 0) * a.g : 0;
       s_chunks[i] = shared ? chunks_of(a.sink, end) : 0;
-      s_tiles[i] = tiles_of(rows);
+      s_tiles[i] = tiles_of(shared ? rows_of(r0, r1) : 0);
     }
   }
   __syncthreads();
   int most = 0;  // chunks of one row's positions
   for (int r = tid; r < reqs; r += kSharedThreads) {
-    const Span s = span(r);
-    const int group = s_group[r];
-    const int lo = group >= 0 ? s_own[r] : s.sink_len;
-    s_own[r] = lo;
-    s_chunks[groups + r] = chunks_of(lo, s.recent);
-    s_tiles[groups + r] = tiles_of(s.rows);
-    if (s.rows > 0)
-      most = max(most, s_chunks[groups + r] + (group >= 0 ? s_chunks[group] : 0));
+    const int rows = rows_of(r, r + 1);
+    s_chunks[groups + r] = chunks_of(s_own[r], s_end[r]);
+    s_tiles[groups + r] = tiles_of(rows);
+    if (rows > 0)
+      most = max(most, s_chunks[groups + r] + (s_group[r] >= 0 ? s_chunks[s_group[r]] : 0));
   }
   __syncthreads();
-  int64_t work = 0, small = 0, small_tiles = 0;  // chunks of 128-row tiles and of 16-row tiles
+  int64_t work = 0, small = 0;  // chunks of 128-row tiles and of 16-row tiles
   for (int e = tid; e < entries; e += kSharedThreads) {
     const int64_t w = static_cast<int64_t>(abs(s_tiles[e])) * s_chunks[e];
     work += s_tiles[e] > 0 ? w : 0;
     small += s_tiles[e] < 0 ? w : 0;
-    small_tiles += s_tiles[e] < 0 && s_chunks[e] ? -s_tiles[e] : 0;
   }
-  int none = 0;
-  plan_reduce(work, most);
-  plan_reduce(small, none);
-  plan_reduce(small_tiles, none);
+  int64_t sums[2] = {work, small};
+  plan_reduce(sums, most);
+  work = sums[0];
+  small = sums[1];
   // Chunks of a piece: no row in more than `slots` pieces (a row's positions are two ranges, each
   // with one uneven piece), at most `budget` units by the average, and then the first count, of 16
   // tried by the wavefronts at once, with which the 128-row units and the others' load, in units of
@@ -170,17 +162,24 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
   const int small_least = max(max(kSmallPiece, least),
                               static_cast<int>((small + a.budget - 1) / a.budget));
   int per = max(max(1, least), static_cast<int>((work + a.budget - 1) / a.budget));
-  const float load = small_tiles * kSmallStart + small * kSmallChunk;
   auto small_per = [&](int t) {
     return max(small_least, static_cast<int>(t * (kTileChunk / kSmallChunk)));
   };
   __shared__ int s_fits;
   for (int round = 0; round < 16; ++round) {
     const int t = per + wave;
-    int64_t units = 0;
-    for (int e = lane; e < entries; e += kWave)
-      units += s_tiles[e] > 0 ? static_cast<int64_t>(s_tiles[e]) * cdiv(s_chunks[e], t) : 0;
+    const int t_small = small_per(t);
+    int64_t units = 0, small_units = 0;
+    for (int e = lane; e < entries; e += kWave) {
+      const int64_t count = abs(s_tiles[e]);
+      if (s_tiles[e] > 0)
+        units += count * cdiv(s_chunks[e], t);
+      else
+        small_units += count * cdiv(s_chunks[e], t_small);
+    }
     units = wave_sum_i64(units);
+    small_units = wave_sum_i64(small_units);
+    const float load = small_units * kSmallStart + small * kSmallChunk;
     if (tid == 0) s_fits = kSharedThreads / kWave;
     __syncthreads();
     if (lane == 0 && units + load / (kTileStart + kTileChunk * t) <= a.budget)
@@ -247,21 +246,19 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
     if (e < groups) {
       const int r0 = clip(a.group_starts[e]), r1 = clip(a.group_starts[e + 1]);
       x.req = r0;
-      x.token0 = token(r0);
-      rows = max(token(r1) - x.token0, 0) * a.g;
+      rows = rows_of(r0, r1);
       begin = a.sink;
       end = s_own[r0];
       x.slot = piece;
     } else {
       const int r = e - groups;
-      const Span s = span(r);
       x.req = r;
-      x.token0 = token(r);
-      rows = s.rows;
+      rows = rows_of(r, r + 1);
       begin = s_own[r];
-      end = s.recent;
+      end = s_end[r];
       x.slot = piece + (s_group[r] >= 0 ? pieces(s_group[r]) : 0);
     }
+    x.token0 = s_token[x.req];
     // Tiles of equal numbers of 16-row groups, pieces of equal numbers of chunks.
     const int share = ((rows + 15) / 16 + tile_count - 1) / tile_count * 16;
     x.row_base = tile * share;
@@ -274,10 +271,10 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
     x.small = s_tiles[e] < 0;
     a.units[u] = x;
   }
-  for (int r = wave; r < reqs; r += kSharedThreads / kWave) {
+  // Eight threads per request.
+  for (int r = tid >> 3; r < reqs; r += kSharedThreads / 8) {
     const int used = pieces(groups + r) + (s_group[r] >= 0 ? pieces(s_group[r]) : 0);
-    const int t1 = token(r + 1);
-    for (int t = token(r) + lane; t < t1; t += kWave) a.token_slots[t] = used;
+    for (int t = s_token[r] + (tid & 7); t < s_token[r + 1]; t += 8) a.token_slots[t] = used;
   }
 }
 
@@ -288,9 +285,9 @@ __global__ __launch_bounds__(kThreadsC, 2) void shared_history_kernel(const Attn
   } lds;
   const int heads = a.L.kv_heads;
   const int index = static_cast<int>(blockIdx.x) / heads;
-  if (index >= a.task_count[0]) return;
-  const Unit u = reinterpret_cast<const Unit*>(a.tasks)[index];
-  if (u.row_base >= u.row_end) return;
+  const int count = a.task_count[0];
+  const Unit u = reinterpret_cast<const Unit*>(a.tasks)[index];  // below the capacity: one wait for both
+  if (index >= count || u.row_base >= u.row_end) return;
   Task t{};
   t.req = u.req;
   t.qstart = u.token0;
@@ -298,7 +295,7 @@ __global__ __launch_bounds__(kThreadsC, 2) void shared_history_kernel(const Attn
   if (u.small)
     row_tile(a, t, head, u.row_end, u.row_base, u.p_lo, u.p_hi, u.slot, lds.row);
   else
-    chunk_tile(a, t, head, u.row_end, u.row_base, u.p_lo, u.p_hi, u.slot, lds.chunk);
+    chunk_tile<true>(a, t, head, u.row_end, u.row_base, u.p_lo, u.p_hi, u.slot, lds.chunk);
 }
 
 struct SharedMergeArgs {

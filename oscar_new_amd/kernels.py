@@ -491,8 +491,13 @@ def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None
     Returns ``(query, key)``, contiguous bf16; with ``rk_t`` (R_k^T, contiguous bf16 [256, 256])
     ``(query, key, rotate(query, R_k))``, the third with the bits of ``rotate``.
     """
-    device = _same_device(query, key=key, q_weight=q_weight, k_weight=k_weight, cos_sin=cos_sin,
-                          positions=positions, counts=counts, rk_t=rk_t)
+    device = query.device
+    if (device.type != "cuda" or key.device != device or q_weight.device != device
+            or k_weight.device != device or cos_sin.device != device
+            or positions.device != device or counts is not None and counts.device != device
+            or rk_t is not None and rk_t.device != device):
+        _same_device(query, key=key, q_weight=q_weight, k_weight=k_weight, cos_sin=cos_sin,
+                     positions=positions, counts=counts, rk_t=rk_t)
     n, hq, d = query.shape
     hk = key.shape[1]
     if d != 256 or key.shape != (n, hk, 256):
