@@ -11,8 +11,8 @@
 //
 // Units. A step's work is (row tile, position range) units: the group's rows against [sink, E)
 // through its first member's pages, and each request's own rows against [E, recent_begin) through
-// its own. Up to kSmallRows rows a tile is 16 rows whose positions the wavefronts of a workgroup
-// divide (row_tile.h), above that 128 rows that share the codes (chunk_tile.h). The plan kernel cuts
+// its own. A tile is 16 rows whose positions the wavefronts of a workgroup divide
+// (row_tile.h), or of many rows 128 that share the codes (chunk_tile.h). The plan kernel cuts
 // every tile's positions into pieces from the whole step's lengths, so that the launch ends early on
 // 256 CUs, and writes the list, once per step and before every layer's launch. Partial rows of a
 // tile's pieces go to slots that the merge kernel joins by their LSEs, as many as the plan says for
@@ -27,10 +27,16 @@ constexpr int kSharedThreads = 1024;
 constexpr int kSharedEntries = 4096;  // groups and requests whose counts live in LDS
 constexpr int kSharedSlots = 256;     // partial rows of a row: four per lane of a merging wavefront
 constexpr int kUnitWords = 8;
-// Rows up to which a tile is 16 rows; 128-token chunks such a unit takes at least.
-constexpr int kSmallRows = 48, kSmallPiece = 4;
-// A unit's time in us: its start and end, and each 128-token chunk.
-constexpr float kTileStart = 11.f, kTileChunk = 4.1f, kSmallStart = 11.f, kSmallChunk = 0.8f;
+// Rows up to which an entry's tiles are 16 rows: always, and where the plan finds that faster for the
+// step (32 samples of 32000 tokens, 192 rows: 28.2 us a layer against 34.5 with 128-row tiles, 96 of
+// 16000: 40.1 and 43.7, 128 of 32000: 62.6 and 59.1).
+constexpr int kSmallRows[2] = {48, 1024};
+// A unit's time in us: its start and end, a 128-token chunk of a 128-row tile, and a round of a 16-row
+// tile, in which each of the eight wavefronts takes 64 tokens (kRound chunks); what a short unit
+// behind another on its CU adds, and a partial row that is written and merged.
+constexpr float kUnitStart = 11.f, kTileChunk = 4.1f, kSmallRound = 2.75f, kSecond = 7.f;
+constexpr float kPartialRow = 5.5e-4f;
+constexpr int kRound = kWavesC * 64 / kTokC;
 
 // A unit: rows [row_base, row_end) of tokens token0 .. (row r is token token0 + r / g), positions
 // [p_lo, p_hi) through block-table row req, partials to `slot`; small: at most 16 rows, row_tile.h.
@@ -48,36 +54,37 @@ struct SharedPlanArgs {
   Unit* units;
   int32_t* unit_count;
   int32_t* token_slots;
-  int32_t groups, max_reqs, sink, recent, g, budget, capacity, slots;
+  int32_t groups, max_reqs, sink, recent, g, heads, budget, capacity, slots;
   int64_t tokens;
 };
 
-// Sums of two counts and a maximum over the workgroup (every thread gets them).
-__device__ __forceinline__ void plan_reduce(int64_t (&sum)[2], int& most) {
-  __shared__ int64_t s_sum[2][kSharedThreads / kWave];
+// Sums of four counts and a maximum over the workgroup (every thread gets them).
+__device__ __forceinline__ void plan_reduce(int64_t (&sum)[4], int& most) {
+  __shared__ int64_t s_sum[4][kSharedThreads / kWave];
   __shared__ int s_most[kSharedThreads / kWave];
   const int wave = threadIdx.x >> 6;
-  for (int i = 0; i < 2; ++i) sum[i] = wave_sum_i64(sum[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] = wave_sum_i64(sum[i]);
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) most = max(most, __shfl_xor(most, m, kWave));
   if ((threadIdx.x & 63) == 0) {
-    s_sum[0][wave] = sum[0];
-    s_sum[1][wave] = sum[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_sum[i][wave] = sum[i];
     s_most[wave] = most;
   }
   __syncthreads();
-  sum[0] = sum[1] = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] = 0;
 #pragma unroll
   for (int w = 0; w < kSharedThreads / kWave; ++w) {
-    sum[0] += s_sum[0][w];
-    sum[1] += s_sum[1][w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += s_sum[i][w];
     most = max(most, s_most[w]);
   }
 }
 
-// Tiles of an entry of `rows` rows (small entries: 16-row tiles, kept negative).
-__device__ __forceinline__ int tiles_of(int rows) {
-  return rows <= kSmallRows ? -((rows + 15) / 16) : (rows + kRowsC - 1) / kRowsC;
+__device__ __forceinline__ int tiles_of(int rows, bool small) {
+  return small ? (rows + 15) / 16 : (rows + kRowsC - 1) / kRowsC;
 }
 __device__ __forceinline__ int chunks_of(int lo, int hi) {
   return lo < hi ? ((hi - 1) >> 7) - (lo >> 7) + 1 : 0;
@@ -85,7 +92,7 @@ __device__ __forceinline__ int chunks_of(int lo, int hi) {
 
 __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const SharedPlanArgs a) {
   // Entries: the groups, then the requests.
-  __shared__ int s_chunks[kSharedEntries], s_tiles[kSharedEntries], s_start[kSharedEntries + 1];
+  __shared__ int s_chunks[kSharedEntries], s_rows[kSharedEntries], s_start[kSharedEntries + 1];
   // Requests: first token, end of the history, first position of the request's own part, and the
   // group whose positions it shares, or -1.
   __shared__ int s_token[kSharedEntries + 1], s_end[kSharedEntries], s_own[kSharedEntries];
@@ -130,7 +137,7 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
       }
     if (lane == 0) {
       s_chunks[i] = shared ? chunks_of(a.sink, end) : 0;
-      s_tiles[i] = tiles_of(shared ? rows_of(r0, r1) : 0);
+      s_rows[i] = shared ? rows_of(r0, r1) : 0;
     }
   }
   __syncthreads();
@@ -138,64 +145,81 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
   for (int r = tid; r < reqs; r += kSharedThreads) {
     const int rows = rows_of(r, r + 1);
     s_chunks[groups + r] = chunks_of(s_own[r], s_end[r]);
-    s_tiles[groups + r] = tiles_of(rows);
+    s_rows[groups + r] = rows;
     if (rows > 0)
       most = max(most, s_chunks[groups + r] + (s_group[r] >= 0 ? s_chunks[s_group[r]] : 0));
   }
   __syncthreads();
-  int64_t work = 0, small = 0;  // chunks of 128-row tiles and of 16-row tiles
-  for (int e = tid; e < entries; e += kSharedThreads) {
-    const int64_t w = static_cast<int64_t>(abs(s_tiles[e])) * s_chunks[e];
-    work += s_tiles[e] > 0 ? w : 0;
-    small += s_tiles[e] < 0 ? w : 0;
-  }
-  int64_t sums[2] = {work, small};
-  plan_reduce(sums, most);
-  work = sums[0];
-  small = sums[1];
-  // Chunks of a piece: no row in more than `slots` pieces (a row's positions are two ranges, each
-  // with one uneven piece), at most `budget` units by the average, and then the first count, of 16
-  // tried by the wavefronts at once, with which the 128-row units and the others' load, in units of
-  // the same time, fit the budget: they run side by side, one per CU, and a second round would
-  // cost more than longer units do.
-  const int least = (most + a.slots - 3) / (a.slots - 2);
-  const int small_least = max(max(kSmallPiece, least),
-                              static_cast<int>((small + a.budget - 1) / a.budget));
-  int per = max(max(1, least), static_cast<int>((work + a.budget - 1) / a.budget));
-  auto small_per = [&](int t) {
-    return max(small_least, static_cast<int>(t * (kTileChunk / kSmallChunk)));
-  };
-  __shared__ int s_fits;
-  for (int round = 0; round < 16; ++round) {
-    const int t = per + wave;
-    const int t_small = small_per(t);
-    int64_t units = 0, small_units = 0;
-    for (int e = lane; e < entries; e += kWave) {
-      const int64_t count = abs(s_tiles[e]);
-      if (s_tiles[e] > 0)
-        units += count * cdiv(s_chunks[e], t);
-      else
-        small_units += count * cdiv(s_chunks[e], t_small);
+  // Tiles times chunks of either kind of tile, with the one and the other limit of small entries.
+  int64_t sums[4] = {};
+  for (int e = tid; e < entries; e += kSharedThreads)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const bool small = s_rows[e] <= kSmallRows[k];
+      sums[2 * k + (small ? 1 : 0)] +=
+          static_cast<int64_t>(tiles_of(s_rows[e], small)) * s_chunks[e];
     }
-    units = wave_sum_i64(units);
-    small_units = wave_sum_i64(small_units);
-    const float load = small_units * kSmallStart + small * kSmallChunk;
-    if (tid == 0) s_fits = kSharedThreads / kWave;
-    __syncthreads();
-    if (lane == 0 && units + load / (kTileStart + kTileChunk * t) <= a.budget)
-      atomicMin(&s_fits, wave);
-    __syncthreads();
-    const int fits = s_fits;
-    __syncthreads();
-    per += fits;
-    if (fits < kSharedThreads / kWave || per >= most) break;
-  }
-  per = max(1, min(per, most));
-  const int per_small = small_per(per);
-  auto pieces = [&](int e) {
-    return cdiv(s_chunks[e], s_tiles[e] < 0 ? per_small : per);
+  plan_reduce(sums, most);
+  // Chunks of a piece of either kind of tile, from a time that grows by half chunks: no row in more
+  // than `slots` pieces (its positions are two ranges, each with one uneven piece), and neither kind
+  // in more than `budget` units by the average.
+  const int least = max(1, (most + a.slots - 3) / (a.slots - 2));
+  int average[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    average[k] = max(least, static_cast<int>((sums[k] + a.budget - 1) / a.budget));
+  auto tile_piece = [&](int k, int i) { return max(average[2 * k], i >> 1); };
+  auto small_piece = [&](int k, int i) {
+    const int rounds = max(1, static_cast<int>(i * (0.5f * kTileChunk / kSmallRound)));
+    return (max(average[2 * k + 1], kRound * rounds) + kRound - 1) / kRound * kRound;
   };
-  auto units_of = [&](int e) { return abs(s_tiles[e]) * pieces(e); };
+  // The choice of least estimated time; the wavefronts estimate 16 at once, until the growing time
+  // itself passes the best. Units that fit the CUs run side by side, one per CU, in the time of the
+  // longest; more of them take their load and a short one's time behind another.
+  __shared__ uint64_t s_best;  // the estimate's bits, then 2 i + k
+  if (tid == 0) s_best = ~0ull;
+  __syncthreads();
+  for (int i0 = max(1, 2 * min(average[0], average[2]) - 6), end = i0 + 4096; i0 < end;
+       i0 += kSharedThreads / kWave) {
+    const int i = i0 + wave;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int t = tile_piece(k, i), ts = small_piece(k, i);
+      float tiles = 0.f, smalls = 0.f, rows = 0.f;
+      const float per_t = 1.0f / t, per_ts = 1.0f / ts;
+      for (int e = lane; e < entries; e += kWave) {
+        const bool small = s_rows[e] <= kSmallRows[k];
+        const float pieces = ceilf(s_chunks[e] * (small ? per_ts : per_t));
+        const float units = tiles_of(s_rows[e], small) * pieces;
+        tiles += small ? 0.f : units;
+        smalls += small ? units : 0.f;
+        rows += s_rows[e] * pieces;
+      }
+      tiles = wave_tree_sum_dpp(tiles);
+      smalls = wave_tree_sum_dpp(smalls);
+      rows = wave_tree_sum_dpp(rows) * a.heads;
+      const float time = kUnitStart + fmaxf(tiles > 0.f ? kTileChunk * t : 0.f,
+                                            smalls > 0.f ? kSmallRound / kRound * ts : 0.f);
+      const float load = tiles * (kUnitStart + kTileChunk * t) + smalls * kUnitStart +
+                         sums[2 * k + 1] * (kSmallRound / kRound);
+      const float estimate =
+          (tiles + smalls <= a.budget ? time : fmaxf(time, load / a.budget) + kSecond) +
+          kPartialRow * rows;
+      if (lane == 0)
+        atomicMin(reinterpret_cast<unsigned long long*>(&s_best),
+                  static_cast<unsigned long long>(__float_as_uint(estimate)) << 32 | (2 * i + k));
+    }
+    __syncthreads();
+    const float best = __uint_as_float(static_cast<uint32_t>(s_best >> 32));
+    __syncthreads();
+    if (kUnitStart + 0.5f * kTileChunk * (i0 + kSharedThreads / kWave) >= best) break;
+  }
+  const int choice = static_cast<int>(s_best & 0xffffffffu), kind = choice & 1;
+  const int per = tile_piece(kind, choice >> 1), per_small = small_piece(kind, choice >> 1);
+  auto small_entry = [&](int e) { return s_rows[e] <= kSmallRows[kind]; };
+  auto tiles_in = [&](int e) { return tiles_of(s_rows[e], small_entry(e)); };
+  auto pieces = [&](int e) { return cdiv(s_chunks[e], small_entry(e) ? per_small : per); };
+  auto units_of = [&](int e) { return tiles_in(e) * pieces(e); };
 
   // Exclusive scan of the entries' units, eight entries a thread.
   constexpr int kPer = kSharedEntries / kSharedThreads;
@@ -238,7 +262,7 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
       else
         hi = mid;
     }
-    const int e = lo, tile_count = abs(s_tiles[e]);
+    const int e = lo, tile_count = tiles_in(e);
     const int64_t count = pieces(e);
     const int local = u - s_start[e], piece = local / tile_count, tile = local - piece * tile_count;
     Unit x;
@@ -268,7 +292,7 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
         (begin >> 7) + static_cast<int>(static_cast<int64_t>(piece + 1) * s_chunks[e] / count);
     x.p_lo = max(begin, c0 << 7);
     x.p_hi = min(end, c1 << 7);
-    x.small = s_tiles[e] < 0;
+    x.small = small_entry(e);
     a.units[u] = x;
   }
   // Eight threads per request.
@@ -365,15 +389,12 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedMerg
   if (lane == 0) a.out_lse[row] = den > 0.f ? mx + logf(den) : -INFINITY;
 }
 
-// Units that a plan may hold: a tile's pieces pass its share of the budget by less than one, for
-// 128-row tiles (one per 128 rows and one more per entry) and for 16-row tiles (at most three per
-// entry, and one per 16 rows and one more per entry).
+// Units that a plan may hold: a tile's pieces pass its share of the budget by less than one, for the
+// tiles of either kind, of which there is one per 128 or 16 rows and one more per entry.
 int64_t shared_capacity(int64_t tokens, int64_t g, int64_t groups, int64_t max_reqs,
                         int64_t budget) {
   const int64_t entries = groups + (max_reqs < tokens ? max_reqs : tokens);
-  const int64_t tiles = 2 * (tokens * g / kRowsC) + entries;
-  const int64_t by_rows = 2 * (tokens * g / 16) + entries;
-  return 2 * budget + tiles + (by_rows < 3 * entries ? by_rows : 3 * entries);
+  return 2 * budget + 2 * (tokens * g / kRowsC) + 2 * (tokens * g / 16) + 2 * entries;
 }
 
 }  // namespace
@@ -411,7 +432,7 @@ extern "C" int oscar_shared_plan(const int32_t* qstarts, const int32_t* seq_lens
   const SharedPlanArgs a{qstarts, seq_lens, counts, group_starts, prefix_tokens,
                          reinterpret_cast<Unit*>(units), unit_count, token_slots,
                          static_cast<int32_t>(groups), static_cast<int32_t>(max_reqs), L.sink,
-                         L.recent, static_cast<int32_t>(g), static_cast<int32_t>(budget),
+                         L.recent, static_cast<int32_t>(g), L.kv_heads, static_cast<int32_t>(budget),
                          static_cast<int32_t>(capacity), slots, tokens};
   hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kSharedThreads), 0, as_stream(stream), a);
   return static_cast<int>(hipGetLastError());

@@ -65,12 +65,12 @@ def test_pages():
 def test_shared_prefixes():
     lib = _ext.library()
 
-    def plan(groups=2, reqs=8, tokens=8, hq=6, slots=64, lay=layout(), units=A, capacity=600,
+    def plan(groups=2, reqs=8, tokens=8, hq=6, slots=64, lay=layout(), units=A, capacity=700,
              starts=A):
         return lib.oscar_shared_plan(A, A, A, starts, A, groups, reqs, tokens, hq, slots, lay,
                                      units, capacity, A, A, None)
 
-    def attend(q=A, history=A, units=A, capacity=600, used=A, n=8, hq=6, slots=64, scale=1 / 16,
+    def attend(q=A, history=A, units=A, capacity=700, used=A, n=8, hq=6, slots=64, scale=1 / 16,
                lay=layout(), out=A, history_bytes=1 << 24):
         return lib.oscar_shared_history(q, 1536, 256, 1, history, history_bytes, A, 64, 64, A, units,
                                         capacity, A, used, n, hq, slots, scale, lay, A, A, 0, out,
