@@ -510,7 +510,8 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs& a, const Task& t, int
   const bool ok = out_row < rows && otok >= 0 && otok < a.n;
   const int64_t my_out = ok ? (otok * a.hq + head * a.g + (out_row - oqi * a.g)) : -1;
   if (ok && eg == 0)
-    a.lse[my_out * a.splits + split] = psum > 0.f ? (m + log2f(psum)) * kLn2 : -INFINITY;
+    a.lse[my_out * a.splits + split] =
+        (kCentred ? psum != 0.f : psum > 0.f) ? (m + log2f(psum)) * kLn2 : -INFINITY;
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
     const int src = 4 * eg + v;

@@ -183,10 +183,10 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
         r2[e] = ok ? r2[e] : -INFINITY;
       }
     }
-    float lm = r2[0];
+    float lm = max3(r2[0], r2[1], r2[2]);
 #pragma unroll
-    for (int e = 1; e < 16; ++e) lm = fmaxf(lm, r2[e]);
-    lm *= fq;
+    for (int e = 3; e < 15; e += 2) lm = max3(lm, r2[e], r2[e + 1]);
+    lm = fmaxf(lm, r2[15]) * fq;
     if (__any(lm > m + kTheta)) {  // lazy running max (history.hip)
       const float mn = fmaxf(m, max_xor32(max_xor16(lm)));
       const float alpha = mn == -INFINITY ? 1.0f : exp2f(m - mn);
@@ -202,26 +202,28 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
       }
     }
     const float nm = m == -INFINITY ? 0.f : -m;
-    float av[16];
+    float av[4][4];
     float amax = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float p = __builtin_amdgcn_exp2f(fmaf(r2[e], fq, nm));
       psum += p;
       zsum = fmaf(p, fmaf(1.5f, h16lo(vsz[e]), h16hi(vsz[e])), zsum);
-      av[e] = p * h16lo(vsz[e]);
-      amax = fmaxf(amax, av[e]);
+      av[e >> 2][e & 3] = fmaf(p, h16lo(vsz[e]), 0.0f);
+    }
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      amax = max3(amax, av[f][0], av[f][1]);
+      amax = max3(amax, av[f][2], av[f][3]);
     }
     amax = max_xor32(max_xor16(amax));
     const uint32_t eb = max(__float_as_uint(amax) >> 23, 7u);
-    const float mult = __uint_as_float((260u - eb) << 23);  // row max in [64, 128)
+    const float scale = __uint_as_float((eb - 6) << 23);  // row max / scale in [64, 128)
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
-      float x[4] = {av[4 * f] * mult, av[4 * f + 1] * mult, av[4 * f + 2] * mult,
-                    av[4 * f + 3] * mult};
-      hi[f] = fp8x4_take(x);
-      lo[f] = fp8x4(x[0], x[1], x[2], x[3]);
+      hi[f] = fp8x4_scaled_take(av[f], scale);
+      lo[f] = fp8x4_scaled_last(av[f], scale);
     }
     const i32x8 pa = {(int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3],
                       (int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3]};
@@ -313,7 +315,7 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
     for (int e = 0; e < 4; ++e) r[e] = fmaf(2.0f, sum[h][e], zs) * inv;
     *reinterpret_cast<f32x4*>(a.partials + out_row * kHeadDim + d0 + 128 * h) = r;
   }
-  if (d0 == 0) a.lse[out_row] = den > 0.f ? (mx + log2f(den)) * kLn2 : -INFINITY;
+  if (d0 == 0) a.lse[out_row] = den == 0.f ? -INFINITY : (mx + log2f(den)) * kLn2;
 }
 
 }  // namespace

@@ -339,12 +339,17 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedMerg
   __shared__ f32x4 s_sum[3][kWave];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int64_t row = blockIdx.x, token = row / a.hq;
-  const int used = token < a.counts[1] ? min(max(a.token_slots[token], 0), a.slots) : 0;
+  // The LSEs of every slot are read beside the count of those in use, not behind it.
   float w[kSharedSlots / kWave];
+#pragma unroll
+  for (int i = 0; i < kSharedSlots / kWave; ++i)
+    w[i] = kWave * i + lane < a.slots ? a.lse[row * a.slots + kWave * i + lane] : -INFINITY;
+  const int live = a.counts[1], held = a.token_slots[token];
+  const int used = token < live ? min(max(held, 0), a.slots) : 0;
   float mx = -INFINITY, den = 0.f;
 #pragma unroll
   for (int i = 0; i < kSharedSlots / kWave; ++i) {
-    w[i] = kWave * i + lane < used ? a.lse[row * a.slots + kWave * i + lane] : -INFINITY;
+    w[i] = kWave * i + lane < used ? w[i] : -INFINITY;
     mx = fmaxf(mx, w[i]);
   }
   mx = wave_max_dpp(mx);
@@ -386,7 +391,7 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedMerg
   else
     reinterpret_cast<uint2*>(a.out)[row * (kHeadDim / 4) + lane] =
         make_uint2(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]));
-  if (lane == 0) a.out_lse[row] = den > 0.f ? mx + logf(den) : -INFINITY;
+  if (lane == 0) a.out_lse[row] = den == 0.f ? -INFINITY : mx + logf(den);  // NaN stays NaN
 }
 
 // Units that a plan may hold: a tile's pieces pass its share of the budget by less than one, for the

@@ -215,6 +215,18 @@ def test_an_unmapped_block_holds_no_tokens():
     b.check(*b.run(), drop=[(0, 2176, 2304)])
 
 
+@pytest.mark.parametrize("members", [3, 200])
+def test_nan_in_a_query_stays_in_its_row(members):
+    requests, groups = spread_requests((1500, [300] * members, 1))
+    b = Batch(requests, groups)
+    clean, clean_lse = b.run()
+    b.q[1, 2, 77] = float("nan")
+    out, lse = b.run()
+    assert bool(out[1, 2].isnan().all()) and bool(lse[1, 2].isnan())
+    out[1, 2], lse[1, 2] = clean[1, 2], clean_lse[1, 2]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
 def test_agrees_with_the_unshared_launches():
     requests, groups = spread_requests((5000, [700] * 20, 1))
     b = Batch(requests, groups)
