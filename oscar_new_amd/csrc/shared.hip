@@ -58,31 +58,6 @@ struct SharedPlanArgs {
   int64_t tokens;
 };
 
-// Sums of four counts and a maximum over the workgroup (every thread gets them).
-__device__ __forceinline__ void plan_reduce(int64_t (&sum)[4], int& most) {
-  __shared__ int64_t s_sum[4][kSharedThreads / kWave];
-  __shared__ int s_most[kSharedThreads / kWave];
-  const int wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) sum[i] = wave_sum_i64(sum[i]);
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) most = max(most, __shfl_xor(most, m, kWave));
-  if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s_sum[i][wave] = sum[i];
-    s_most[wave] = most;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) sum[i] = 0;
-#pragma unroll
-  for (int w = 0; w < kSharedThreads / kWave; ++w) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += s_sum[i][w];
-    most = max(most, s_most[w]);
-  }
-}
-
 __device__ __forceinline__ int tiles_of(int rows, bool small) {
   return small ? (rows + 15) / 16 : (rows + kRowsC - 1) / kRowsC;
 }
@@ -141,25 +116,39 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
     }
   }
   __syncthreads();
-  int most = 0;  // chunks of one row's positions
   for (int r = tid; r < reqs; r += kSharedThreads) {
-    const int rows = rows_of(r, r + 1);
     s_chunks[groups + r] = chunks_of(s_own[r], s_end[r]);
-    s_rows[groups + r] = rows;
-    if (rows > 0)
-      most = max(most, s_chunks[groups + r] + (s_group[r] >= 0 ? s_chunks[s_group[r]] : 0));
+    s_rows[groups + r] = rows_of(r, r + 1);
   }
   __syncthreads();
-  // Tiles times chunks of either kind of tile, with the one and the other limit of small entries.
-  int64_t sums[4] = {};
-  for (int e = tid; e < entries; e += kSharedThreads)
+  // Tiles times chunks of either kind of tile, with the one and the other limit of small entries, and
+  // the most chunks of one row's positions: a wavefront each.
+  __shared__ int64_t s_sum[5];
+  if (wave < 5) {
+    int64_t sum = 0;
+    int most = 0;
+    if (wave < 4) {
+      for (int e = lane; e < entries; e += kWave) {
+        const bool small = s_rows[e] <= kSmallRows[wave >> 1];
+        if (small == ((wave & 1) != 0))
+          sum += static_cast<int64_t>(tiles_of(s_rows[e], small)) * s_chunks[e];
+      }
+      sum = wave_sum_i64(sum);
+    } else {
+      for (int r = lane; r < reqs; r += kWave)
+        if (s_rows[groups + r] > 0)
+          most = max(most, s_chunks[groups + r] + (s_group[r] >= 0 ? s_chunks[s_group[r]] : 0));
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const bool small = s_rows[e] <= kSmallRows[k];
-      sums[2 * k + (small ? 1 : 0)] +=
-          static_cast<int64_t>(tiles_of(s_rows[e], small)) * s_chunks[e];
+      for (int m = 32; m >= 1; m >>= 1) most = max(most, __shfl_xor(most, m, kWave));
+      sum = most;
     }
-  plan_reduce(sums, most);
+    if (lane == 0) s_sum[wave] = sum;
+  }
+  __shared__ uint64_t s_best;  // the least estimate's bits, then 2 i + k
+  if (tid == 0) s_best = ~0ull;
+  __syncthreads();
+  const int64_t sums[4] = {s_sum[0], s_sum[1], s_sum[2], s_sum[3]};
+  const int most = static_cast<int>(s_sum[4]);
   // Chunks of a piece of either kind of tile, from a time that grows by half chunks: no row in more
   // than `slots` pieces (its positions are two ranges, each with one uneven piece), and neither kind
   // in more than `budget` units by the average.
@@ -176,20 +165,17 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
   // The choice of least estimated time; the wavefronts estimate 16 at once, until the growing time
   // itself passes the best. Units that fit the CUs run side by side, one per CU, in the time of the
   // longest; more of them take their load and a short one's time behind another.
-  __shared__ uint64_t s_best;  // the estimate's bits, then 2 i + k
-  if (tid == 0) s_best = ~0ull;
-  __syncthreads();
+  const int kinds = sums[0] == sums[2] ? 1 : 2;  // no entry between the two limits
   for (int i0 = max(1, 2 * min(average[0], average[2]) - 6), end = i0 + 4096; i0 < end;
        i0 += kSharedThreads / kWave) {
     const int i = i0 + wave;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kinds; ++k) {
       const int t = tile_piece(k, i), ts = small_piece(k, i);
       float tiles = 0.f, smalls = 0.f, rows = 0.f;
-      const float per_t = 1.0f / t, per_ts = 1.0f / ts;
+      const float per_t = __builtin_amdgcn_rcpf(t), per_ts = __builtin_amdgcn_rcpf(ts);
       for (int e = lane; e < entries; e += kWave) {
         const bool small = s_rows[e] <= kSmallRows[k];
-        const float pieces = ceilf(s_chunks[e] * (small ? per_ts : per_t));
+        const float pieces = ceilf(s_chunks[e] * (small ? per_ts : per_t) - 1e-3f);
         const float units = tiles_of(s_rows[e], small) * pieces;
         tiles += small ? 0.f : units;
         smalls += small ? units : 0.f;
