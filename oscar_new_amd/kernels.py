@@ -548,6 +548,7 @@ class SharedPlan:
     slots: int
     query_heads: int
     requests: int  # rows of the block table that the units may name
+    tokens: int
     layout: object
     layout_struct: object  # its C form
 
@@ -564,9 +565,11 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
     ``meta.num_actual_tokens``; a padded graph step passes its rows). ``out``: a plan of the same
     sizes to fill again, so that a captured graph reads the new one.
     """
-    device = _same_device(meta.query_start_loc, group_starts=group_starts,
-                          prefix_tokens=prefix_tokens)
-    for name, t in (("group_starts", group_starts), ("prefix_tokens", prefix_tokens)):
+    device = _same_device(meta.query_start_loc, seq_lens=meta.seq_lens, counts=meta.counts,
+                          group_starts=group_starts, prefix_tokens=prefix_tokens)
+    for name, t in (("query_start_loc", meta.query_start_loc), ("seq_lens", meta.seq_lens),
+                    ("counts", meta.counts), ("group_starts", group_starts),
+                    ("prefix_tokens", prefix_tokens)):
         if _int32(t, name).dim() != 1 or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous vector")
     groups = prefix_tokens.shape[0]
@@ -574,7 +577,8 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
         raise ValueError("group_starts must hold one start per group and the end of the last")
     tokens = int(meta.num_actual_tokens if tokens is None else tokens)
     reqs, heads = int(meta.max_num_reqs), layout.kv_heads
-    if meta.query_start_loc.shape[0] < reqs + 1 or meta.seq_lens.shape[0] < reqs:
+    if (meta.query_start_loc.shape[0] < reqs + 1 or meta.seq_lens.shape[0] < reqs
+            or meta.counts.shape[0] < 2):
         raise ValueError("the metadata holds fewer requests than max_num_reqs")
     if hq <= 0 or hq % heads:
         raise ValueError("the query head count must be a multiple of the KV head count")
@@ -584,18 +588,17 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
         sizes = (8 * capacity, 1, max(tokens, 1))
         buffer = torch.empty(sum(sizes), dtype=torch.int32, device=device)
         units, count, used = buffer.split(sizes)
-        out = SharedPlan(units.view(capacity, 8), count, used, slots, hq, reqs, layout,
-                         layout_struct(layout))
-    elif (out.units.shape[0] != capacity or out.token_slots.shape[0] != max(tokens, 1)
+        out = SharedPlan(units.view(capacity, 8), count, used, slots, hq, reqs, tokens,
+                         layout, layout_struct(layout))
+    elif (out.units.shape[0] != capacity or out.tokens != tokens
           or out.slots != slots or out.query_heads != hq or out.requests != reqs
           or out.units.device != device or out.layout != layout):
         raise ValueError("the plan to fill again was made for other sizes")
     _launch(
         _ext.library().oscar_shared_plan, "prepare_shared", device,
-        _ptr(_int32(meta.query_start_loc, "query_start_loc")),
-        _ptr(_int32(meta.seq_lens, "seq_lens")), _ptr(_int32(meta.counts, "counts")),
-        _ptr(group_starts), _ptr(prefix_tokens), groups, reqs, tokens, hq, slots,
-        out.layout_struct, _ptr(out.units), capacity, _ptr(out.unit_count), _ptr(out.token_slots),
+        _ptr(meta.query_start_loc), _ptr(meta.seq_lens), _ptr(meta.counts), _ptr(group_starts),
+        _ptr(prefix_tokens), groups, reqs, tokens, hq, slots, out.layout_struct, _ptr(out.units),
+        capacity, _ptr(out.unit_count), _ptr(out.token_slots),
     )
     return out
 
@@ -610,13 +613,14 @@ def shared_history(query, history, meta, shared, layout, scale, merged=True):
     split's partials, ``(fp32 [n, hq, 1, 256], lse [n, hq, 1])``, for ``post_attention``.
     """
     n, hq, d = query.shape
-    if hq != shared.query_heads or n > shared.token_slots.shape[0]:
-        raise ValueError(f"the plan covers {shared.token_slots.shape[0]} tokens of "
+    if hq != shared.query_heads or n > shared.tokens:
+        raise ValueError(f"the plan covers {shared.tokens} tokens of "
                          f"{shared.query_heads} heads, got {n} of {hq}")
     if layout is not shared.layout and layout != shared.layout:
         raise ValueError("the plan was made for another cache layout")
     table = _int32(meta.block_tables, "block_tables")
-    device = _same_device(query, history=history, block_tables=table, units=shared.units)
+    device = _same_device(query, history=history, block_tables=table, counts=meta.counts,
+                          units=shared.units)
     if table.shape[0] < shared.requests or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError("block_tables must have contiguous rows, one per request of the plan")
     if history.dtype != torch.uint8 or not history.is_contiguous():

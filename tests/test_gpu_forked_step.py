@@ -98,7 +98,7 @@ class Server:
 
 
 @pytest.mark.parametrize("fused", [True, False])
-@pytest.mark.parametrize("qlen", [1, 4])
+@pytest.mark.parametrize("qlen", [1, 4, 70])
 def test_forked_requests_decode_alike_with_and_without_the_plan(qlen, fused):
     with_plan, without = Server(qlen, fused), Server(qlen, fused)
     got, want = with_plan.scenario(True), without.scenario(False)

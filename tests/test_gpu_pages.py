@@ -276,6 +276,25 @@ def test_captured_fork_replays_with_new_rows():
         w.check(stripes)
 
 
+def test_captured_compaction_replays():
+    w = World([1500, 300, 900], pool=30, rows=4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        pages.compact_pages(w.handle, w.table, w.seq_lens, w.counts)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            tables, live = pages.compact_pages(w.handle, w.table, w.seq_lens, w.counts)
+    torch.cuda.current_stream().wait_stream(side)
+    for count in (3, 1, 2, 3):
+        w.counts[0] = count
+        stripes, table, total = expect_compact(w, range(count))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert live.item() == total and np.array_equal(tables.cpu().numpy(), table)
+        w.check(stripes)
+
+
 def test_refusals():
     w = World([100], pool=4)
     other = World([100], pool=6)

@@ -280,6 +280,14 @@ def test_refusals():
         kernels.prepare_shared(b.meta, b.layout, 12, b.starts, b.prefix, out=plan)
     with pytest.raises(ValueError):
         kernels.prepare_shared(b.meta, b.layout, 33, b.starts, b.prefix)
+    for name in ("seq_lens", "counts", "query_start_loc"):
+        good = getattr(b.meta, name)
+        for bad, error in ((good.cpu(), RuntimeError), (good.long(), ValueError),
+                           (good[:1], ValueError)):
+            setattr(b.meta, name, bad)
+            with pytest.raises(error):
+                kernels.prepare_shared(b.meta, b.layout, 6, b.starts, b.prefix)
+        setattr(b.meta, name, good)
     many = torch.zeros(9001, dtype=torch.int32, device=DEV)
     with pytest.raises(ValueError):
         kernels.prepare_shared(b.meta, b.layout, 6, many, many[1:])
@@ -296,6 +304,11 @@ def test_refusals():
         with pytest.raises(ValueError):
             call(b.q, b.history, b.meta, plan, b.layout, 1 / 16)
     b.meta.block_tables = table
+    with pytest.raises(ValueError):
+        call(b.q, b.history, b.meta, plan, CacheLayout(1536), 1 / 16)
+    none = kernels.prepare_shared(b.meta, b.layout, 6, b.starts, b.prefix, tokens=0)
+    with pytest.raises(ValueError):
+        call(b.q[:1], b.history, b.meta, none, b.layout, 1 / 16)
     for scale in (0.0, -1.0, float("nan")):
         with pytest.raises(ValueError):
             call(b.q, b.history, b.meta, plan, b.layout, scale)
