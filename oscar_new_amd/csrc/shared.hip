@@ -34,7 +34,8 @@ constexpr int kSmallRows[2] = {48, 1024};
 // A unit's time in us: its start and end, a 128-token chunk of a 128-row tile, and a round of a 16-row
 // tile, in which each of the eight wavefronts takes 64 tokens (kRound chunks); what a short unit
 // behind another on its CU adds, and a partial row that is written and merged.
-constexpr float kUnitStart = 11.f, kTileChunk = 4.1f, kSmallRound = 2.75f, kSecond = 7.f;
+constexpr float kUnitStart = 11.f, kTileChunk = 4.2f, kSmallRound = 3.0f, kSecond = 7.f;
+constexpr float kUnitGap = 6.f;  // between two units of a CU, and a short one's uneven rounds
 constexpr float kPartialRow = 5.5e-4f;
 constexpr int kRound = kWavesC * 64 / kTokC;
 
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
       rows = wave_tree_sum_dpp(rows) * a.heads;
       const float time = kUnitStart + fmaxf(tiles > 0.f ? kTileChunk * t : 0.f,
                                             smalls > 0.f ? kSmallRound / kRound * ts : 0.f);
-      const float load = tiles * (kUnitStart + kTileChunk * t) + smalls * kUnitStart +
+      const float load = tiles * (kUnitStart + kTileChunk * t) + smalls * (kUnitStart + kUnitGap) +
                          sums[2 * k + 1] * (kSmallRound / kRound);
       const float estimate =
           (tiles + smalls <= a.budget ? time : fmaxf(time, load / a.budget) + kSecond) +
