@@ -59,8 +59,8 @@ class OscarAttentionBackend:
     @staticmethod
     def copy_blocks(*args, **kwargs):
         raise NotImplementedError(
-            "OSCAR pages belong to one request (its BF16 window lives in its first page); "
-            "pages cannot be copied or shared")
+            "OSCAR cannot copy single blocks (a request's BF16 window lives in its first page); "
+            "pages.fork_requests copies and shares the pages of whole requests")
 
     @staticmethod
     def swap_blocks(*args, **kwargs):

@@ -14,6 +14,12 @@
 // through DPP moves and one lane swap. A pair's other half is read again from memory (the row is
 // in the cache by then) rather than moved between lanes: one 16-byte load, in flight with the
 // lane's own, against four cross-lane moves behind it.
+//
+// What bounds it: without R_k the memory (16384 tokens of 7 heads, 120 MB: 25 to 26 us, 4.6 TB/s of
+// the 5.0 that a large copy reaches); with R_k vector issue and the hand-off of a block through LDS
+// (2048 tokens of 14 heads, 42 MB: 18.2 us; copies of the kernel without the norm took 5.4 us less,
+// without most of the products and of R_k's loads 3.9, without either output's stores 1.3); a decode
+// step its chain of loads (32 tokens of 7 heads: 5.2 us, 3.9 without R_k).
 #include <type_traits>
 
 #include "rotate.h"

@@ -158,8 +158,9 @@ class OscarMetadataBuilder:
 
     def _check(self, cm, common_prefix_len):
         if common_prefix_len:
-            raise ValueError("OSCAR cannot share a prefix between requests: each request's "
-                             "BF16 ring lives in its own first page")
+            raise ValueError("OSCAR cannot share a whole prefix between requests: each "
+                             "request's BF16 ring lives in its own first page (forked requests "
+                             "share the other pages: kernels.prepare_shared)")
         if not getattr(cm, "causal", True):
             raise ValueError("OSCAR serves causal decoder attention only")
         if cm.num_reqs > self.max_reqs or cm.num_actual_tokens > self.max_tokens:
