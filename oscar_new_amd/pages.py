@@ -11,7 +11,9 @@ Everything stays on the device: no call reads back, synchronizes or allocates an
 outputs, so calls can be captured in a graph. Page numbers are physical pages (a block table's entry
 divided by the kernel blocks of a page). All calls take the block table and the token counts of the
 scheduler's rows: row r holds ``seq_lens[r]`` tokens in the blocks of ``block_tables[r]``, and the
-rows below ``counts[0]`` are live.
+rows below ``counts[0]`` are live. Those tokens are the ones that stay: a fork of a request whose
+draft tokens are not yet accepted takes its count without them, since records of a shared page are
+not written again.
 """
 
 from __future__ import annotations

@@ -245,6 +245,43 @@ def test_large_pool_spans_several_scan_rounds():
     assert free[: count.item()].tolist() == [p for p in range(5000) if p not in taken]
 
 
+def test_pages_beyond_four_gigabytes():
+    layout = CacheLayout(768, kv_heads=1, config=OscarConfig(speculative_tokens=3))
+    pool, bpp, length = 12000, layout.blocks_per_page, 2 * 768 + 100
+    assert pool * layout.stripe_page_bytes > 1 << 32
+    stripes = [torch.empty(pool, layout.stripe_page_bytes, dtype=torch.uint8, device=DEV)
+               for _ in range(2)]
+    shape = (pool * bpp, 128, 1, 256)
+    caches = pages.PageCaches([tuple(t.view(torch.bfloat16).view(shape) for t in stripes)], layout)
+    owned = [11990, 11800, 11950]
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    for t in stripes:
+        t[owned] = torch.randint(0, 256, (3, t.shape[1]), generator=gen, device=DEV,
+                                 dtype=torch.uint8)
+    blocks = [p * bpp + b for p in owned for b in range(bpp)]
+    table, seq = i32([blocks, [-1] * len(blocks)]), i32([length, 0])
+    status = pages.fork_requests(caches, table, seq, i32([0]), i32([1]), i32([[11000, 11999]]))
+    assert status.tolist() == [1] and seq.tolist() == [length] * 2
+    assert table[1].tolist() == [p * bpp + b for p in (11000, 11800, 11999) for b in range(bpp)]
+    (history, window), cfg = stripes, layout.config
+    rows = (cfg.sink_tokens + cfg.ring_tokens) * 1024
+
+    def alike(first, last):
+        assert torch.equal(history[first, : 768 * 160], history[11990, : 768 * 160])
+        assert torch.equal(window[first, :rows], window[11990, :rows])
+        assert torch.equal(history[last, : 100 * 160], history[11950, : 100 * 160])
+
+    alike(11000, 11999)
+    # In use: 11000, 11800, 11950, 11990, 11999 -> pages 0 to 4 in that order.
+    tables, live = pages.compact_pages(caches, table, seq, i32([2, 0]))
+    assert live.item() == 5
+    assert tables[0].tolist() == [p * bpp + b for p in (3, 1, 2) for b in range(bpp)]
+    assert tables[1].tolist() == [p * bpp + b for p in (0, 1, 4) for b in range(bpp)]
+    alike(0, 4)
+    alike(3, 2)
+    assert torch.equal(history[1, : 768 * 160], history[11800, : 768 * 160])
+
+
 def test_captured_fork_replays_with_new_rows():
     w = World([1000, 700], pool=20, rows=6)
     parents, children = i32([0, 1]), i32([2, 3])
