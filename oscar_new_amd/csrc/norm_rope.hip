@@ -486,7 +486,10 @@ extern "C" int oscar_qk_norm_rope(const void* query, int64_t q_s0, int64_t q_s1,
   if (!query || !key || !q_weight || !k_weight || !positions || !q_out || !k_out ||
       (rotary_dim && !cos_sin) || !rk_t != !q_rot)
     return OSCAR_E_NULL;
-  if (hq > 0x7fffffffll / n || hk > 0x7fffffffll / n) return OSCAR_E_SHAPE;
+  // Rows are 32-bit, and a launch holds fewer than 2^32 threads (32 for a token's four heads).
+  if (hq > 0x7fffffffll / n || hk > 0x7fffffffll / n ||
+      (hq + 3) / 4 + (hk + 3) / 4 > 0xffffff00ll / 32 / n)
+    return OSCAR_E_SHAPE;
   if (q_s0 % 8 || q_s1 % 8 || k_s0 % 8 || k_s1 % 8 || !aligned16(query) || !aligned16(key) ||
       !aligned16(q_weight) || !aligned16(k_weight) || !aligned16(q_out) || !aligned16(k_out) ||
       (rk_t && (!aligned16(rk_t) || !aligned16(q_rot))))

@@ -293,6 +293,9 @@ __global__ __launch_bounds__(kSharedThreads) void shared_plan_kernel(const Share
     const int used = pieces(groups + r) + (s_group[r] >= 0 ? pieces(s_group[r]) : 0);
     for (int t = s_token[r] + (tid & 7); t < s_token[r + 1]; t += 8) a.token_slots[t] = used;
   }
+  // Tokens behind the last request's hold nothing.
+  for (int t = (reqs ? s_token[reqs] : 0) + tid; t < active; t += kSharedThreads)
+    a.token_slots[t] = 0;
 }
 
 __global__ __launch_bounds__(kThreadsC, 2) void shared_history_kernel(const AttnArgs a) {
@@ -457,7 +460,9 @@ extern "C" int oscar_shared_history(const void* query, int64_t q_s0, int64_t q_s
   if (st != OSCAR_OK || n == 0) return st;
   if (!token_slots || !out || !out_lse) return OSCAR_E_NULL;
   if (reinterpret_cast<uintptr_t>(out) % 16) return OSCAR_E_ALIGN;
-  if (hq > 0x7fffffffll / n || capacity > 0x7fffffffll / a.L.kv_heads) return OSCAR_E_SHAPE;
+  // A launch holds fewer than 2^32 threads.
+  if (hq > 0xffffffffll / kThreads / n || capacity > 0xffffffffll / kThreadsC / a.L.kv_heads)
+    return OSCAR_E_SHAPE;
   hipStream_t s = as_stream(stream);
   hipLaunchKernelGGL(shared_history_kernel, dim3(static_cast<unsigned>(capacity * a.L.kv_heads)),
                      dim3(kThreadsC), 0, s, a);

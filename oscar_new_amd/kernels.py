@@ -561,7 +561,8 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
     the device, ascending), whose first ``prefix_tokens[g]`` tokens (int32 [groups]) are the same:
     their history records are equal, in the same pages or in copies (``pages.fork_requests``).
     Requests of no group, and groups of one, share nothing; so does a step whose starts descend.
-    ``hq``: query heads; ``tokens``: most query tokens the plan's layers pass (default
+    ``hq``: query heads, at most 32 per KV head; groups and requests: at most 4096 together;
+    ``tokens``: most query tokens the plan's layers pass (default
     ``meta.num_actual_tokens``; a padded graph step passes its rows). ``out``: a plan of the same
     sizes to fill again, so that a captured graph reads the new one.
     """
@@ -583,6 +584,9 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
     if hq <= 0 or hq % heads:
         raise ValueError("the query head count must be a multiple of the KV head count")
     slots = choose_shared_slots(tokens, hq)
+    if tokens < 0 or reqs < 1:
+        raise ValueError(f"a plan needs at least one request and no negative tokens, got {reqs} "
+                         f"and {tokens}")
     capacity = _ext.library().oscar_shared_capacity(tokens, hq, groups, reqs, heads)
     if out is None:
         sizes = (8 * capacity, 1, max(tokens, 1))
@@ -613,6 +617,8 @@ def shared_history(query, history, meta, shared, layout, scale, merged=True):
     split's partials, ``(fp32 [n, hq, 1, 256], lse [n, hq, 1])``, for ``post_attention``.
     """
     n, hq, d = query.shape
+    if d != 256:
+        raise ValueError(f"the query must be [n, heads, 256], got {tuple(query.shape)}")
     if hq != shared.query_heads or n > shared.tokens:
         raise ValueError(f"the plan covers {shared.tokens} tokens of "
                          f"{shared.query_heads} heads, got {n} of {hq}")

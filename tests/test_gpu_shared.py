@@ -266,6 +266,87 @@ def test_captured_step_with_a_plan_filled_again():
         b.check(out, lse)
 
 
+def test_two_streams_use_one_plan_at_once():
+    requests, groups = spread_requests((3000, [300] * 30, 1), (900, [100, 800], 1))
+    b = Batch(requests, groups)
+    plan = kernels.prepare_shared(b.meta, b.layout, 6, b.starts, b.prefix)
+    queries = [b.q, b.q.flip(0).contiguous()]
+    want = [kernels.shared_history(q, b.history, b.meta, plan, b.layout, 1 / 16) for q in queries]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in queries]
+    got = []
+    for _ in range(5):
+        for q, side in zip(queries, sides):
+            with torch.cuda.stream(side):
+                got.append(kernels.shared_history(q, b.history, b.meta, plan, b.layout, 1 / 16))
+    torch.cuda.synchronize()
+    for i, (out, lse) in enumerate(got):
+        assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
+
+
+def test_tokens_of_no_request_hold_nothing():
+    requests, groups = spread_requests((900, [300, 400], 1))
+    b = Batch(requests, groups, pad=5)
+    b.meta.counts[1] += 5  # live by the count, but behind the last request's
+    out, lse = b.run()
+    b.check(out, lse)
+    b.meta.counts[0] = 0
+    out, lse = b.run()
+    assert not bool(out.any()) and bool((lse == -torch.inf).all())
+
+
+@pytest.mark.parametrize("qlen,reqs", [(1, 600), (200, 100)])
+def test_units_longer_than_their_offset_tables_far_in_a_pool(qlen, reqs):
+    """Requests that map the same 300000 tokens in pages beyond 4 GB of records and declare nothing
+    shared: more rows than the chip holds, so each unit is a whole row tile's positions. Either
+    tile's lanes add a quarter of the positions one by one, each sum off by at most 2^-24 of it."""
+    layout = CacheLayout(768, kv_heads=1, config=OscarConfig(sink_tokens=64, recent_tokens=256,
+                                                             speculative_tokens=3))
+    prefix, page = 300000, 768
+    need, pool = -(-(prefix + qlen) // page), 12000
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    data = records(need * page, gen)
+    order = pool - 1 - torch.randperm(need, generator=gen, device=DEV)
+    order[::5] = torch.arange(order[::5].numel(), device=DEV)  # and at the pool's start
+    history = torch.empty(pool, page * 512, dtype=torch.uint8, device=DEV)
+    history[order, : page * 160] = data.view(need, page * 160)
+    bpp = layout.blocks_per_page
+    row = (order[:, None] * bpp + torch.arange(bpp, device=DEV)).flatten().int()
+    tokens = reqs * qlen
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    meta = SimpleNamespace(
+        query_start_loc=i32(range(0, tokens + 1, qlen)), seq_lens=i32([prefix + qlen] * reqs),
+        block_tables=row.expand(reqs, -1).contiguous(), counts=i32([reqs, tokens]), num_reqs=reqs,
+        max_num_reqs=reqs, num_actual_tokens=tokens)
+    q = (12 * torch.randn(tokens, 6, 256, generator=gen, device=DEV)).bfloat16()
+    none = i32([])
+    plan = kernels.prepare_shared(meta, layout, 6, i32([0]), none)
+    units = plan.units[: plan.unit_count.item()]
+    assert bool((units[:, 5] - units[:, 4] == prefix - 256 - 64).all())
+    assert bool((units[:, 7] == (qlen == 1)).all())
+    out, lse = kernels.shared_history(q, history.view(-1), meta, plan, layout, 1 / 16)
+    half = []
+    for b in (0, 68):
+        d = data[64 : prefix - 256, b : b + 68]
+        codes = torch.stack([d[:, :64] >> s & 3 for s in (0, 2, 4, 6)], -1).flatten(1).double()
+        pair = d[:, 64:].contiguous().view(torch.float16).double()
+        half.append((codes, pair[:, :1], pair[:, 1:]))
+    (kc, ks, kz), (vc, vs, vz) = half
+    key, value, spread = kc * ks + kz, vc * vs + vz, vc * vs
+    rows = [0, tokens // 2, tokens - 1]
+    picked = q[rows].double().view(-1, 256)
+    score = picked @ key.T.contiguous() / 16
+    p = score.softmax(-1)
+    want = p @ value
+    shift = (2.0**-17 * picked.abs().amax(-1) * key.abs().sum(1).max() / 16 + 2.0**-14
+             + prefix / 4 * 2.0**-24)
+    bound = 2.0**-8 * (want.abs() + p @ spread) + 2 * shift[:, None] * (p @ value.abs())
+    err = (out[rows].double().view(-1, 256) - want).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+    err = (lse[rows].double().view(-1) - score.logsumexp(-1)).abs()
+    assert bool((err <= shift).all()), float((err / shift).max())
+
+
 def test_refusals():
     requests, groups = spread_requests((600, [300, 400], 1))
     b = Batch(requests, groups)

@@ -28,6 +28,7 @@ def test_qk_norm_rope():
     assert call(rotary=63) == -2 and call(rotary=258, stride=258) == -2 and call(rotary=-2) == -2
     assert call(stride=32) == -2 and call(rows=0) == -2
     assert call(n=1 << 31) == -2 and call(n=1 << 29) == -2
+    assert call(n=1 << 27, hq=1) == -2  # more threads than a launch holds
     assert call(q=None) == -1 and call(table=None) == -1 and call(positions=None) == -1
     assert call(rk_t=A) == -1 and call(q_rot=A) == -1
     assert call(q=A + 2) == -4 and call(q_s0=1537) == -4 and call(out=A + 8) == -4
@@ -86,6 +87,7 @@ def test_shared_prefixes():
     assert plan(lay=layout(page=1)) == -3
     assert attend(n=0) == 0
     assert attend(slots=3) == -2 and attend(slots=257) == -2 and attend(capacity=0) == -2
+    assert attend(n=1 << 22) == -2 and attend(capacity=1 << 23) == -2  # threads of a launch
     assert attend(n=-1) == -2 and attend(hq=0) == -2 and attend(history_bytes=64) == -2
     assert attend(q=None) == -1 and attend(used=None) == -1 and attend(out=None) == -1
     assert attend(q=A + 2) == -4 and attend(out=A + 4) == -4 and attend(history=A + 4) == -4
@@ -97,3 +99,10 @@ def test_tensors_on_the_host_are_refused():
     w = torch.zeros(256)
     with pytest.raises(RuntimeError):
         kernels.qk_norm_rope(q, q[:, :1], w, w, torch.zeros(4, 64), torch.zeros(2, dtype=torch.int64))
+
+
+def test_shared_history_takes_heads_of_256():
+    plan = kernels.SharedPlan(None, None, None, 4, 6, 1, 8, None, None)
+    for d in (128, 512):
+        with pytest.raises(ValueError, match="256"):
+            kernels.shared_history(torch.zeros(2, 6, d), None, None, plan, None, 1 / 16)
