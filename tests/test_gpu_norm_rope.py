@@ -79,6 +79,32 @@ def test_rows_against_64_bits(n, hq, hk, rotary, interleaved):
         assert torch.equal(turned[2], kernels.rotate(got[0], rk))
 
 
+@pytest.mark.parametrize("n,hq,hk,live", [(700, 6, 1, 700), (321, 6, 2, 300), (6001, 6, 1, 5500)])
+@pytest.mark.parametrize("rotary,interleaved", [(64, False), (128, False), (192, False),
+                                                (256, False), (0, False), (8, True), (96, True),
+                                                (256, True), (32, False)])
+def test_walks_of_many_rows(n, hq, hk, live, rotary, interleaved):
+    """Each wavefront's rows by itself, one block or several, against the formulas and with the bits
+    of the form without R_k and of ``rotate``."""
+    for table, weight, unit in ((torch.float32, torch.bfloat16, False),
+                                (torch.bfloat16, torch.float32, True)):
+        q, k, w, cs, pos, rk = make(n, hq, hk, rotary, table=table, weight=weight)
+        if live > 400 and rotary:
+            pos[400], pos[live - 1] = cs.shape[0], -1
+        counts = torch.tensor([1, live], dtype=torch.int32, device=DEV)
+        args = dict(counts=counts, eps=1e-6, unit_offset=unit, interleaved=interleaved)
+        got = kernels.qk_norm_rope(q, k, *w, cs, pos, **args)
+        turned = kernels.qk_norm_rope(q, k, *w, cs, pos, rk_t=rk.T.contiguous(), **args)
+        bad = [400, live - 1] if live > 400 and rotary else []
+        good = [t for t in range(live) if t not in bad]
+        for i, x in enumerate((q, k)):
+            check(turned[i][good].contiguous(), x[good], w[i], cs, pos[good], 1e-6, unit,
+                  interleaved)
+        for t, plain in zip(turned, (*got, kernels.rotate(got[0], rk))):
+            assert torch.equal(t[good], plain[good])
+            assert bool(t[bad].isnan().all()) and not bool(t[live:].any())
+
+
 @pytest.mark.parametrize("rotate", [False, True])
 @pytest.mark.parametrize("n,live", [(5, 3), (40, 0), (700, 511)])
 def test_rows_past_the_live_tokens_are_zero(n, live, rotate):
