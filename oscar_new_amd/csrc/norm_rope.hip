@@ -17,8 +17,8 @@
 //
 // What bounds it: without R_k the memory (16384 tokens of 7 heads, 120 MB: 25 to 26 us, 4.6 TB/s of
 // the 5.0 that a large copy reaches); with R_k the memory too for many rows (the same with R_k, 170 MB:
-// 36.5 us), the loads of rows and R_k and then R_k's reads from LDS for a chunk (2048 tokens of 14
-// heads, 42 MB: 14.5 us); a decode step its chain of loads (32 tokens of 7 heads: 5.2 us, 3.9 without
+// 36.4 us), the loads of rows and R_k and then R_k's reads from LDS for a chunk (2048 tokens of 14
+// heads, 42 MB: 14.3 us); a decode step its chain of loads (32 tokens of 7 heads: 5.2 us, 3.9 without
 // R_k).
 #include <type_traits>
 
@@ -629,7 +629,8 @@ __global__ __launch_bounds__(kWalkWaves * kWave, 2) void norm_rope_walk_kernel(
   }
   // Row 16 t + i of the LDS copy is the column of R_k that lane i's A operand of tile t reads, 32 (t / 2)
   // + 8 (i / 4) + 4 (t % 2) + i % 4, so that a lane ends with eight consecutive columns of a row in two
-  // tiles; its 16-byte piece p lies at p ^ i % 8, which the 8 lanes of a cycle read without conflicts.
+  // tiles; its 16-byte piece p lies at p ^ i, so that 16 lanes read 256 bytes of all banks (p ^ i % 8: 4
+  // cycles of conflicts a read, 0.2 us).
   if (blockIdx.x < q_blocks) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -637,7 +638,7 @@ __global__ __launch_bounds__(kWalkWaves * kWave, 2) void norm_rope_walk_kernel(
       const int col = 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) void*)(a.rk_t + col * kHeadDim +
-                                                          8 * ((lane & 31) ^ (r & 7))),
+                                                          8 * ((lane & 31) ^ i)),
           (__attribute__((address_space(3))) void*)(s_rk + 1024 * (16 * wave + j)), 16, 0, 0);
     }
   }
@@ -660,14 +661,15 @@ __global__ __launch_bounds__(kWalkWaves * kWave, 2) void norm_rope_walk_kernel(
       const int64_t row = 16 * b + n;
       uint16_t* out = a.q_rot + row * kHeadDim + 8 * g;
       // Eight operands (four products of two tiles) are read ahead of the eight in use.
-      const uint8_t* even = s_rk + 512 * n + 16 * (g ^ (n & 7));
-      const uint8_t* odd = s_rk + 512 * n + 16 * ((4 + g) ^ (n & 7));
+      const uint8_t* from[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) from[m] = s_rk + 512 * n + 16 * ((4 * m + g) ^ n);
       u32x4 f[2][8];
       auto read = [&](int i, u32x4 (&w)[8]) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           w[k] = *reinterpret_cast<const u32x4*>(
-              (k & 2 ? odd : even) + 8192 * (2 * (i >> 1) + (k & 1)) + 128 * (2 * (i & 1) + (k >> 2)));
+              from[k >> 1] + 8192 * (2 * (i >> 1) + (k & 1)) + 256 * (i & 1));
       };
       read(0, f[0]);
       f32x4 acc[2];
@@ -693,7 +695,7 @@ __global__ __launch_bounds__(kWalkWaves * kWave, 2) void norm_rope_walk_kernel(
 // With R_k: 16-row blocks up to which two workgroups of 8 wavefronts share each, all on CUs of their
 // own (300 tokens of 7 heads: 5.9 us, 6.3 by norm_rope_walk_kernel; 340, more workgroups than CUs: 7.6
 // and 6.4). Above, one workgroup per CU walks: wavefronts by themselves where a pair's dims lie in one
-// lane (2048 tokens of 14 heads 14.5 us, 18.2 by blocks through LDS; 16384 of 7 heads 36.5 and 50.4),
+// lane (2048 tokens of 14 heads 14.3 us, 18.2 by blocks through LDS; 16384 of 7 heads 36.4 and 50.4),
 // else blocks of 32 rows.
 constexpr int64_t kFewBlocks = 128, kRotateGroups = 256;
 
