@@ -26,6 +26,13 @@ struct RowTileLds {
 };
 static_assert(kWavesC * 16 * kHeadDim * 4 <= sizeof(RowTileLds::ring), "the merge fits the ring");
 
+// max(a, |b|, |c|) without the quieting of NaN operands (a row with one is NaN by its sum).
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // Rows [row_base, rows) (at most 16); everything else as chunk_tile.
 __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int head, int rows,
                                          int row_base, int p_lo, int p_hi, int slot,
@@ -98,12 +105,12 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
           const u32x4 w = *reinterpret_cast<const u32x4*>(src + 128 * h + 64 * b + 16 * g + 8 * q);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float x0 = valid ? bf16_to_float(w[i] & 0xffffu) : 0.f;
-            const float x1 = valid ? bf16_to_float(w[i] >> 16) : 0.f;
+            const uint32_t pair = valid ? w[i] : 0u;
+            const float x0 = __uint_as_float(pair << 16), x1 = __uint_as_float(pair & 0xffff0000u);
             sum += x0 + x1;
             x[h][b][8 * q + 2 * i] = x0;
             x[h][b][8 * q + 2 * i + 1] = x1;
-            mx = fmaxf(mx, fmaxf(fabsf(x0), fabsf(x1)));
+            mx = max3_abs(mx, x0, x1);
           }
         }
     mx = max_xor32(max_xor16(mx));
