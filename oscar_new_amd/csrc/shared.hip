@@ -19,7 +19,7 @@
 // each token.
 //
 // What bounds it (history launch and merge of a layer, us; unshared: the launches of history.hip and
-// their merge): a few samples of a short prompt their chain of loads, 6 of 2000 tokens 14.0 (unshared
+// their merge): a few samples of a short prompt their chain of loads, 6 of 2000 tokens 13.7 (unshared
 // 19.5); 16-row tiles vector issue, the rounds of their wavefronts and the start of a unit, about half
 // of its time, 32 of 32000 27.8 (38.2), three prompts of 9 samples with 4 query tokens 28.4 (48.0);
 // 128-row tiles the pipeline of chunk_tile.h, 4.2 a chunk, 256 of 32500 87.8 (259.5).
