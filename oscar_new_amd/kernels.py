@@ -422,6 +422,13 @@ def dequant_inverse_rotate(history, slots, rk, rv, layout):
 
 
 def _same_device(first, **others):
+    index = first.get_device()
+    for t in others.values():
+        if t is not None and t.get_device() != index:
+            break
+    else:
+        if index >= 0:
+            return first.device
     device = first.device
     if device.type != "cuda":
         raise RuntimeError("OSCAR kernels run on a ROCm GPU; got a tensor on " + str(device))
@@ -437,7 +444,7 @@ def _same_device(first, **others):
 def _launch(entry, what, device, *args):
     """Calls a C entry point on ``device`` and its current stream."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
@@ -454,24 +461,27 @@ def _vector(t, name):
     if t.dtype not in _VALUE_TYPES or t.shape != (256,):
         raise ValueError(f"{name} must be a bf16 or fp32 vector of 256, got {t.dtype} "
                          f"{tuple(t.shape)}")
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _rows_aligned(t):
-    """bf16 [n, h, 256] with 16-byte aligned rows, copying if needed."""
+    """bf16 [n, h, 256] with 16-byte aligned rows, copied if needed, and its first two strides."""
     s0, s1, s2 = t.stride()
     if t.dtype == torch.bfloat16 and s2 == 1 and not (s0 % 8 or s1 % 8 or t.data_ptr() % 16):
-        return t
+        return t, s0, s1
     t = _bf16(t).contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if t.data_ptr() % 16:
+        t = t.clone()
+    return t, *t.stride()[:2]
 
 
-def _rows_out(like, n, heads):
-    """New bf16 [n, heads, 256] rows on the device of ``like``."""
+def _rows_out(like):
+    """New contiguous bf16 rows of the shape and device of ``like``."""
     if like.dtype == torch.bfloat16:
-        return like.new_empty((n, heads, 256))
-    return torch.empty((n, heads, 256), dtype=torch.bfloat16, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    return torch.empty(like.shape, dtype=torch.bfloat16, device=like.device)
 
 
 def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None, eps=1e-6,
@@ -491,13 +501,8 @@ def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None
     Returns ``(query, key)``, contiguous bf16; with ``rk_t`` (R_k^T, contiguous bf16 [256, 256])
     ``(query, key, rotate(query, R_k))``, the third with the bits of ``rotate``.
     """
-    device = query.device
-    if (device.type != "cuda" or key.device != device or q_weight.device != device
-            or k_weight.device != device or cos_sin.device != device
-            or positions.device != device or counts is not None and counts.device != device
-            or rk_t is not None and rk_t.device != device):
-        _same_device(query, key=key, q_weight=q_weight, k_weight=k_weight, cos_sin=cos_sin,
-                     positions=positions, counts=counts, rk_t=rk_t)
+    device = _same_device(query, key=key, q_weight=q_weight, k_weight=k_weight, cos_sin=cos_sin,
+                          positions=positions, counts=counts, rk_t=rk_t)
     n, hq, d = query.shape
     hk = key.shape[1]
     if d != 256 or key.shape != (n, hk, 256):
@@ -520,13 +525,12 @@ def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None
     q_weight, k_weight = _vector(q_weight, "q_weight"), _vector(k_weight, "k_weight")
     if q_weight.dtype != k_weight.dtype:
         q_weight, k_weight = q_weight.float(), k_weight.float()
-    q_out, k_out = _rows_out(query, n, hq), _rows_out(query, n, hk)
-    q_rot = None if rk_t is None else _rows_out(query, n, hq)
+    q_out, k_out = _rows_out(query), _rows_out(key)
+    q_rot = None if rk_t is None else torch.empty_like(q_out)
     if n:
-        query, key = _rows_aligned(query), _rows_aligned(key)
-        positions = positions.contiguous()
-        q0, q1, _ = query.stride()
-        k0, k1, _ = key.stride()
+        (query, q0, q1), (key, k0, k1) = _rows_aligned(query), _rows_aligned(key)
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
         _launch(
             _ext.library().oscar_qk_norm_rope, "qk_norm_rope", device, query.data_ptr(), q0, q1,
             key.data_ptr(), k0, k1, n, hq, hk, q_weight.data_ptr(), k_weight.data_ptr(),
@@ -542,15 +546,34 @@ def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None
 class SharedPlan:
     """A step's units for ``shared_history`` (``prepare_shared``), in device buffers."""
 
-    units: torch.Tensor  # int32 [capacity, 8]
-    unit_count: torch.Tensor  # int32 [1]
-    token_slots: torch.Tensor  # int32 [tokens]: partial rows of each token
+    buffer: torch.Tensor  # int32: the units, their number, the partial rows of each token
+    capacity: int
     slots: int
     query_heads: int
     requests: int  # rows of the block table that the units may name
     tokens: int
     layout: object
     layout_struct: object  # its C form
+
+    @property
+    def units(self):
+        """int32 [capacity, 8]."""
+        return self.buffer[: 8 * self.capacity].view(self.capacity, 8)
+
+    @property
+    def unit_count(self):
+        """int32 [1]."""
+        return self.buffer[8 * self.capacity : 8 * self.capacity + 1]
+
+    @property
+    def token_slots(self):
+        """int32 [tokens]."""
+        return self.buffer[8 * self.capacity + 1 :][: self.tokens]
+
+    def addresses(self):
+        """Device addresses of the three parts."""
+        base = self.buffer.data_ptr()
+        return base, base + 32 * self.capacity, base + 32 * self.capacity + 4
 
 
 def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, out=None):
@@ -589,20 +612,18 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
                          f"and {tokens}")
     capacity = _ext.library().oscar_shared_capacity(tokens, hq, groups, reqs, heads)
     if out is None:
-        sizes = (8 * capacity, 1, max(tokens, 1))
-        buffer = torch.empty(sum(sizes), dtype=torch.int32, device=device)
-        units, count, used = buffer.split(sizes)
-        out = SharedPlan(units.view(capacity, 8), count, used, slots, hq, reqs, tokens,
-                         layout, layout_struct(layout))
-    elif (out.units.shape[0] != capacity or out.tokens != tokens
+        buffer = meta.seq_lens.new_empty(8 * capacity + 1 + max(tokens, 1))
+        out = SharedPlan(buffer, capacity, slots, hq, reqs, tokens, layout, layout_struct(layout))
+    elif (out.capacity != capacity or out.tokens != tokens
           or out.slots != slots or out.query_heads != hq or out.requests != reqs
-          or out.units.device != device or out.layout != layout):
+          or out.buffer.device != device or out.layout != layout):
         raise ValueError("the plan to fill again was made for other sizes")
+    units, unit_count, token_slots = out.addresses()
     _launch(
         _ext.library().oscar_shared_plan, "prepare_shared", device,
-        _ptr(meta.query_start_loc), _ptr(meta.seq_lens), _ptr(meta.counts), _ptr(group_starts),
-        _ptr(prefix_tokens), groups, reqs, tokens, hq, slots, out.layout_struct, _ptr(out.units),
-        capacity, _ptr(out.unit_count), _ptr(out.token_slots),
+        meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(), meta.counts.data_ptr(),
+        group_starts.data_ptr(), prefix_tokens.data_ptr(), groups, reqs, tokens, hq, slots,
+        out.layout_struct, units, capacity, unit_count, token_slots,
     )
     return out
 
@@ -626,7 +647,7 @@ def shared_history(query, history, meta, shared, layout, scale, merged=True):
         raise ValueError("the plan was made for another cache layout")
     table = _int32(meta.block_tables, "block_tables")
     device = _same_device(query, history=history, block_tables=table, counts=meta.counts,
-                          units=shared.units)
+                          plan=shared.buffer)
     if table.shape[0] < shared.requests or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError("block_tables must have contiguous rows, one per request of the plan")
     if history.dtype != torch.uint8 or not history.is_contiguous():
@@ -634,20 +655,20 @@ def shared_history(query, history, meta, shared, layout, scale, merged=True):
     slots = shared.slots
     out_lse = torch.empty((n, hq) if merged else (n, hq, 1), dtype=torch.float32, device=device)
     if merged:
-        out = _rows_out(query, n, hq)
+        out = _rows_out(query)
     else:
         out = out_lse.new_empty((n, hq, 1, d))
     if n == 0:
         return out, out_lse
+    units, unit_count, token_slots = shared.addresses()
     # One buffer: the partial rows, then their LSEs.
     partials = out_lse.new_empty(n * hq * slots * (d + 1))
-    query = _rows_aligned(query)
+    query, s0, s1 = _rows_aligned(query)
     _launch(
-        _ext.library().oscar_shared_history, "shared_history", device, query.data_ptr(),
-        *query.stride(), history.data_ptr(), history.numel(), table.data_ptr(), table.stride(0),
-        table.shape[1], _int32(meta.counts, "counts").data_ptr(), shared.units.data_ptr(),
-        shared.units.shape[0], shared.unit_count.data_ptr(), shared.token_slots.data_ptr(), n, hq,
-        slots, scale, shared.layout_struct, partials.data_ptr(),
+        _ext.library().oscar_shared_history, "shared_history", device, query.data_ptr(), s0, s1, 1,
+        history.data_ptr(), history.numel(), table.data_ptr(), table.stride(0),
+        table.shape[1], _int32(meta.counts, "counts").data_ptr(), units, shared.capacity,
+        unit_count, token_slots, n, hq, slots, scale, shared.layout_struct, partials.data_ptr(),
         partials.data_ptr() + 4 * n * hq * slots * d, not merged, out.data_ptr(),
         out_lse.data_ptr(),
     )

@@ -83,8 +83,8 @@ def free_pages(caches, block_tables, seq_lens, counts):
     """Pages that no token of a live row is mapped to: ``(pages, count)``, int32 ``[num_pages]`` with
     the free pages in ascending order and -1 behind them, and int32 ``[1]``."""
     table = _table(caches, block_tables, seq_lens, counts)
-    used = torch.empty(caches.num_pages, dtype=torch.int32, device=caches.device)
-    pages, count = used.new_empty(caches.num_pages), used.new_empty(1)
+    n = caches.num_pages
+    pages, count, used = seq_lens.new_empty(2 * n + 1).split((n, 1, n))
     _launch(
         _ext.library().oscar_free_pages, "free_pages", caches.device, caches.num_pages, *table,
         seq_lens.data_ptr(), counts.data_ptr(), caches.layout_struct, used.data_ptr(),
@@ -134,7 +134,7 @@ def compact_pages(caches, block_tables, seq_lens, counts):
     slot mappings made from it are stale.
     """
     table = _table(caches, block_tables, seq_lens, counts)
-    scratch = torch.empty(5 * caches.num_pages + 1, dtype=torch.int32, device=caches.device)
+    scratch = seq_lens.new_empty(5 * caches.num_pages + 1)
     tables, live = scratch.new_empty(block_tables.shape), scratch.new_empty(1)
     _launch(
         _ext.library().oscar_compact_pages, "compact_pages", caches.device,

@@ -102,7 +102,7 @@ def test_tensors_on_the_host_are_refused():
 
 
 def test_shared_history_takes_heads_of_256():
-    plan = kernels.SharedPlan(None, None, None, 4, 6, 1, 8, None, None)
+    plan = kernels.SharedPlan(None, 1, 4, 6, 1, 8, None, None)
     for d in (128, 512):
         with pytest.raises(ValueError, match="256"):
             kernels.shared_history(torch.zeros(2, 6, d), None, None, plan, None, 1 / 16)
