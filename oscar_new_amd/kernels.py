@@ -418,7 +418,7 @@ def dequant_inverse_rotate(history, slots, rk, rv, layout):
 
 # The operators below check and launch in as few Python steps as they can: in an eager decode step
 # a call's host time is longer than its kernel (qk_norm_rope of 32 tokens: 22 us of host time with
-# the helpers above, 5.6 us on the GPU).
+# the helpers above, 14 with these, 5.2 us on the GPU).
 
 
 def _same_device(first, **others):
