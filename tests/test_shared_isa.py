@@ -11,7 +11,8 @@ from tests.test_isa_hazards import HIPCC, ROOT, _late_sites
 
 
 @pytest.mark.skipif(not Path(HIPCC).exists(), reason="hipcc is not installed")
-@pytest.mark.parametrize("source,loads", [("shared.hip", 20), ("history_chunk.hip", 6)])
+@pytest.mark.parametrize("source,loads", [("shared.hip", 20), ("history_chunk.hip", 6),
+                                          ("norm_rope.hip", 16)])
 def test_tiles_keep_five_wait_states_before_every_dma(tmp_path, source, loads):
     out = tmp_path / "kernels.s"
     subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17",
