@@ -79,7 +79,6 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
     for (int i = 0; i < kDma; ++i) dma_x4_stream(base, voff[i], at + 1024 * i);
   };
   if (nmine > 0) issue(0, 0);
-  if (nmine > 1) issue(1, 1);
 
   // ---- the query rows as FP8 B operands, built by every wavefront for itself (chunk_tile.h).
   const int my_row = row_base + n;
@@ -132,6 +131,8 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
             qb[h][term][4 * b + d] = static_cast<int>(fp8x4_scaled_take(v, scale));
         }
   }
+
+  if (nmine > 1) issue(1, 1);
 
   // Offsets inside a stage (record r at kSkew + 144 r): QK operand of token 16 tt + n; scale | zero
   // of the lane's tokens 16 (e / 4) + 4 g + e % 4; transposed V reads of the rows that hold them.
