@@ -152,16 +152,40 @@ def test_unaligned_rows_and_far_token_strides():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_many_rows_far_apart_with_zero_infinite_and_nan_rows():
+    q, k, w, cs, pos, rk = make(700, 6, 1, 64)
+    q, k, rk_t = q.clone(), k.clone(), rk.T.contiguous()
+    q[100], k[101] = 0, 0
+    q[699, 0, 100] = float("inf")  # outside the turned dims: 0 times its weight, NaN in its place
+    q[350, 1, 7] = float("nan")
+    far = torch.empty(700, 1 << 22, dtype=torch.bfloat16, device=DEV)  # 5.9 GB from end to end
+    wide_q, wide_k = far[:, : 6 * 256].view(700, 6, 256), far[:, 4096:4352].view(700, 1, 256)
+    wide_q.copy_(q)
+    wide_k.copy_(k)
+    plain = kernels.qk_norm_rope(wide_q, wide_k, *w, cs, pos)
+    got = kernels.qk_norm_rope(wide_q, wide_k, *w, cs, pos, rk_t=rk_t)
+    for x, y in zip(got, (*plain, kernels.rotate(plain[0], rk))):
+        assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(), y.nan_to_num())
+    assert not bool(got[0][100].any()) and not bool(got[1][101].any())
+    assert got[0][699, 0].isnan().nonzero().flatten().tolist() == [100]
+    nan = got[0].isnan().flatten(0, 1)
+    assert bool(nan[350 * 6 + 1].all()) and int(nan.any(1).sum()) == 2
+    compact = kernels.qk_norm_rope(q, k, *w, cs, pos, rk_t=rk_t)
+    for x, y in zip(got, compact):
+        assert torch.equal(x.nan_to_num(), y.nan_to_num())
+
+
 def test_no_tokens():
     q, k, w, cs, pos, rk = make(3, 6, 1, 64)
     got = kernels.qk_norm_rope(q[:0], k[:0], *w, cs, pos[:0], rk_t=rk.T.contiguous())
     assert [tuple(t.shape) for t in got] == [(0, 6, 256), (0, 1, 256), (0, 6, 256)]
 
 
-def test_captured_and_on_another_stream():
-    q, k, w, cs, pos, rk = make(32, 6, 1, 64)
+@pytest.mark.parametrize("n", [32, 700])
+def test_captured_and_on_another_stream(n):
+    q, k, w, cs, pos, rk = make(n, 6, 1, 64)
     q, k, rk_t = q.clone(), k.clone(), rk.T.contiguous()
-    counts = torch.tensor([1, 32], dtype=torch.int32, device=DEV)
+    counts = torch.tensor([1, n], dtype=torch.int32, device=DEV)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -170,7 +194,7 @@ def test_captured_and_on_another_stream():
         with torch.cuda.graph(graph, stream=side):
             out = kernels.qk_norm_rope(q, k, *w, cs, pos, counts=counts, rk_t=rk_t)
     torch.cuda.current_stream().wait_stream(side)
-    for live in (32, 9, 31):
+    for live in (n, 9, n - 1):
         q.normal_()
         pos.random_(cs.shape[0])
         counts[1] = live
