@@ -562,7 +562,7 @@ int oscar_calibrated_rotations(const float* covariances, int32_t batch, int32_t 
  * the first rotary_dim dims (even, 0..256; dims i and i + rotary_dim / 2, or 2 i and 2 i + 1 when
  * interleaved) are turned by the angles of the token's position: cos_sin row `position` holds the
  * cosines of the pairs, then their sines (rows table_stride elements apart). fp32 arithmetic, one
- * rounding to bf16. query [n][hq][256], key [n][hk][256]: bf16, strides multiples of 8, rows
+ * rounding to bf16; a finite row whose squares leave fp32's range is scaled first. query [n][hq][256], key [n][hk][256]: bf16, strides multiples of 8, rows
  * contiguous and 16-byte aligned. Weights [256] and cos_sin: bf16 or fp32 (the flags). q_out, k_out:
  * contiguous bf16. counts (optional, as for the other entry points): rows of tokens at or past
  * counts[1] are zeroed and their positions not read. A live token whose position is outside

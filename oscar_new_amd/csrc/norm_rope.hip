@@ -84,6 +84,15 @@ __device__ __forceinline__ void unpack_eight(u32x4 w, float (&v)[8]) {
   }
 }
 
+// Eight packed values times a power of two (rounded where that leaves bf16's range).
+__device__ __forceinline__ u32x4 scale_eight(u32x4 w, float by) {
+  float v[8];
+  unpack_eight(w, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(v[2 * e] * by, v[2 * e + 1] * by);
+  return w;
+}
+
 // Partner of dim d, the index of its angle and the sign of the partner's term.
 __device__ __forceinline__ void pair_of(const NormRopeArgs& a, int d, int& pair, int& angle,
                                         float& sign) {
@@ -232,13 +241,17 @@ __device__ __forceinline__ void load_row(const NormRopeArgs& a, const uint16_t* 
   }
 }
 
+// What a row is multiplied by ahead of its norm: a power of two where fp32 does not hold its squares or
+// their mean with eps (magnitudes above 1e18, which would give zeros; below 4e-15 with as small an eps,
+// infinities), else 1. The scaled mean lies in [2^-114, 2^120], whatever the finite bf16 row.
+__device__ __forceinline__ float range_scale(float mean) {
+  return mean == INFINITY ? 0x1p-72f : mean < 0x1p-96f ? 0x1p80f : 1.f;
+}
+
 // 1 / sqrt(mean), NaN for a bad row: the hardware's reciprocal root (within one unit of the last
 // place), whose argument may not be subnormal.
 __device__ __forceinline__ float inverse_root(float mean, bool bad) {
-  const bool tiny = mean < 0x1p-96f;
-  mean = tiny ? mean * 0x1p96f : mean;
-  float inv = __builtin_amdgcn_rsqf(mean);
-  inv = tiny ? inv * 0x1p48f : inv;
+  const float inv = __builtin_amdgcn_rsqf(mean);
   return bad ? __uint_as_float(0x7fc00000u) : inv;
 }
 
@@ -248,8 +261,7 @@ template <int kMode, bool kFp32>
 __device__ __forceinline__ u32x4 finish_row(const NormRopeArgs& a, const float* s_weight,
                                             const Angles<kMode, kFp32>& t, const RowLoads& r,
                                             int l) {
-  float v[8], pair[8], own_w[8], pair_w[8], sum = 0.f;
-  unpack_eight(r.x, v);
+  float own_w[8], pair_w[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) own_w[e] = s_weight[8 * l + e];
   const int half = a.rotary >> 1;
@@ -268,20 +280,35 @@ __device__ __forceinline__ u32x4 finish_row(const NormRopeArgs& a, const float* 
       pair_w[e] = s_weight[p];
     }
   }
+  u32x4 own = r.x, other = r.pair;
+  auto mean_square = [&](float eps) {
+    float v[8], sum = 0.f;
+    unpack_eight(own, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
+    sum += dpp<kDppQuadXor1>(sum);
+    sum += dpp<kDppQuadXor2>(sum);
+    sum += dpp<kDppRowHalfMirror>(sum);
+    sum += dpp<kDppRowMirror>(sum);
+    sum = sum_xor16(sum);
+    return fmaf(sum, 1.0f / kHeadDim, eps);
+  };
+  float mean = mean_square(a.eps);
+  if (const float by = range_scale(mean); __builtin_expect(__any(by != 1.f), 0)) {
+    // The packed values are scaled, so that no register more is live across the branch.
+    own = scale_eight(own, by);
+    other = scale_eight(other, by);
+    mean = mean_square(a.eps * by * by);
+  }
+  const float inv = inverse_root(mean, t.bad);
+  float v[8], pair[8];
+  unpack_eight(own, v);
   if (kMode == kPairAdjacent) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) pair[e] = v[e ^ 1];
   } else {
-    unpack_eight(r.pair, pair);
+    unpack_eight(other, pair);
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
-  sum += dpp<kDppQuadXor1>(sum);
-  sum += dpp<kDppQuadXor2>(sum);
-  sum += dpp<kDppRowHalfMirror>(sum);
-  sum += dpp<kDppRowMirror>(sum);
-  sum = sum_xor16(sum);
-  const float inv = inverse_root(fmaf(sum, 1.0f / kHeadDim, a.eps), t.bad);
   const float pair_inv = kMode == kPairHalves && 8 * l < half ? -inv : inv;
   float o[8];
 #pragma unroll
@@ -522,18 +549,28 @@ __global__ __launch_bounds__(kWalkWaves * kWave, 2) void norm_rope_walk_kernel(
   u32x4 y[8];  // the finished rows
   auto finish = [&](int64_t b) {
     const float* w = s_weight[b < q_blocks ? 0 : 1] + 8 * g;
-    float v[8][8], sums[8];
+    float v[8][8];
+    auto mean_square = [&](float eps) {
+      float sums[8];
 #pragma unroll
-    for (int m = 0; m < 8; ++m) {
-      unpack_eight(x[m], v[m]);
-      float sum = 0.f;
+      for (int m = 0; m < 8; ++m) {
+        float sum = 0.f;
+        unpack_eight(x[m], v[m]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(v[m][e], v[m][e], sum);
-      sums[m] = sum_xor32(sum_xor16(sum));
+        for (int e = 0; e < 8; ++e) sum = fmaf(v[m][e], v[m][e], sum);
+        sums[m] = sum_xor32(sum_xor16(sum));
+      }
+      const float sum = ((sums[0] + sums[1]) + (sums[2] + sums[3])) +
+                        ((sums[4] + sums[5]) + (sums[6] + sums[7]));
+      return fmaf(sum, 1.0f / kHeadDim, eps);
+    };
+    float mean = mean_square(a.eps);
+    if (const float by = range_scale(mean); __any(by != 1.f)) {
+#pragma unroll
+      for (int m = 0; m < 8; ++m) x[m] = scale_eight(x[m], by);
+      mean = mean_square(a.eps * by * by);
     }
-    const float sum = ((sums[0] + sums[1]) + (sums[2] + sums[3])) +
-                      ((sums[4] + sums[5]) + (sums[6] + sums[7]));
-    const float inv = inverse_root(fmaf(sum, 1.0f / kHeadDim, a.eps), bad);
+    const float inv = inverse_root(mean, bad);
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
       const f32x4 lo = *reinterpret_cast<const f32x4*>(w + 32 * m);

@@ -221,3 +221,37 @@ def test_refusals():
             call(q, k, *w, cs, pos, eps=eps)
     with pytest.raises(RuntimeError):
         call(q.cpu(), k, *w, cs, pos)
+
+
+@pytest.mark.parametrize("n", [5, 700])  # blocks through LDS and wavefronts by themselves
+@pytest.mark.parametrize("rotary,interleaved", [(64, False), (256, False), (64, True), (20, False)])
+def test_finite_rows_whose_squares_leave_the_range_of_fp32(n, rotary, interleaved):
+    """Rows are normalized wherever their squares, sum or mean overflow or vanish in fp32. The bound
+    is the one above: every step but the scaling by a power of two is the same."""
+    q, k, w, cs, pos, rk = make(n, 4, 2, rotary)
+    q, k, rk_t = torch.randn(n, 4, 256, device=DEV), torch.randn(n, 2, 256, device=DEV), rk.T
+    for x in (q, k):
+        x[0] *= 1e19  # each square above the largest fp32 value, or their sum
+        x[1, 0] *= 3e17
+        x[1, 1, 100] = 3.3e38
+        x[2, 0, :] = 3.3e38
+        x[2, 1, 1:] = 0
+        x[2, 1, 0] = -3e38
+        x[3] *= 1e-24  # each square below the smallest
+        x[4, 0] *= 1e-19
+        x[4, 1] = 2.0**-133  # bf16's smallest
+    q, k, rk_t = q.bfloat16(), k.bfloat16(), rk_t.contiguous()
+    for eps in (0.0, 1e-32):
+        args = dict(eps=eps, interleaved=interleaved)
+        got = kernels.qk_norm_rope(q, k, *w, cs, pos, **args)
+        turned = kernels.qk_norm_rope(q, k, *w, cs, pos, rk_t=rk_t, **args)
+        for i, x in enumerate((q, k)):
+            check(got[i], x, w[i], cs, pos, eps, False, interleaved)
+        for t, plain in zip(turned, (*got, kernels.rotate(got[0], rk))):
+            assert torch.equal(t, plain)
+    # An eps that leaves the range with the mean: rows of tiny values, not zeros.
+    large = kernels.qk_norm_rope(q[:3], k[:3], *w, cs, pos[:3], eps=3e38, interleaved=interleaved)
+    for i, x in enumerate((q[:3], k[:3])):
+        want, largest = formula(x, w[i], cs, pos[:3], 3e38, False, interleaved)
+        bound = want.abs() * 2.0**-8 + largest * 2.0**-18 + 2.0**-134
+        assert bool(((large[i].double() - want).abs() <= bound).all())
