@@ -562,7 +562,8 @@ int oscar_calibrated_rotations(const float* covariances, int32_t batch, int32_t 
  * the first rotary_dim dims (even, 0..256; dims i and i + rotary_dim / 2, or 2 i and 2 i + 1 when
  * interleaved) are turned by the angles of the token's position: cos_sin row `position` holds the
  * cosines of the pairs, then their sines (rows table_stride elements apart). fp32 arithmetic, one
- * rounding to bf16; a finite row whose squares leave fp32's range is scaled first. query [n][hq][256], key [n][hk][256]: bf16, strides multiples of 8, rows
+ * rounding to bf16; a finite row whose squares leave fp32's range is scaled first. query
+ * [n][hq][256], key [n][hk][256]: bf16, strides multiples of 8, rows
  * contiguous and 16-byte aligned. Weights [256] and cos_sin: bf16 or fp32 (the flags). q_out, k_out:
  * contiguous bf16. counts (optional, as for the other entry points): rows of tokens at or past
  * counts[1] are zeroed and their positions not read. A live token whose position is outside
@@ -583,7 +584,8 @@ int oscar_qk_norm_rope(const void* query, int64_t q_s0, int64_t q_s1, const void
  * layer, num_pages physical pages each, 16-byte aligned; `table`: int32 block table (rows of
  * table_stride elements) whose entry j holds kernel block j of a request; seq_lens: tokens per row.
  * A page is in use when a row below counts[0] maps one of its seq_lens tokens to it; table entries
- * outside the pool are skipped.
+ * outside the pool are skipped. A page that a row maps past its tokens is free (for the pages of
+ * tokens to come, free_pages and compact_pages take a count that holds them).
  *
  * free_pages: `pages` [num_pages] receives the free pages in ascending order, then -1; count [1]
  * their number. `used`: scratch of num_pages.
@@ -613,8 +615,9 @@ int oscar_fork_requests(const void* stripes, int64_t layers, int64_t num_pages, 
  * compact_pages -- moves the pages in use to the pool's start: with `live` pages in use, those
  * below page `live` stay and the k-th one above moves to the k-th free one below (records and window
  * rows in use only; the old page keeps its bytes). new_table [rows][table_columns] receives the table
- * with the entries of live tokens' pages changed; live [1] the number of pages in use: every page
- * from there on is free. scratch: 5 num_pages + 1 values.
+ * with the entries of live tokens' pages changed and -1 behind them (their pages may hold another
+ * row's tokens now); rows from counts[0] on are copied as they are. live [1]: the number of pages in
+ * use; every page from there on is free. scratch: 5 num_pages + 1 values.
  */
 int oscar_compact_pages(const void* stripes, int64_t layers, int64_t num_pages,
                         const int32_t* table, int64_t table_stride, int64_t table_columns,

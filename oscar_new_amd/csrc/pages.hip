@@ -318,12 +318,15 @@ __global__ __launch_bounds__(kThreads) void compact_move_kernel(const CompactArg
   const int live = static_cast<int>(min(static_cast<int64_t>(max(a.t.counts[0], 0)), a.t.rows));
   for (int64_t r = blockIdx.x; r < a.t.rows; r += gridDim.x) {
     const int length = r < live ? a.t.seq_lens[r] : 0;
-    const int pages = length > 0 ? (length - 1) / L.bp + 1 : 0;
+    const int64_t held = static_cast<int64_t>(length > 0 ? (length - 1) / L.bp + 1 : 0) * L.bpp;
     for (int64_t c = threadIdx.x; c < a.t.columns; c += kThreads) {
       int block = a.t.table[r * a.t.stride + c];
       const int page = block >= 0 ? block / L.bpp : -1;
-      if (c < static_cast<int64_t>(pages) * L.bpp && page >= 0 && page < a.pool.num_pages)
-        block += (a.place[page] - page) * L.bpp;
+      if (c < held) {
+        if (page >= 0 && page < a.pool.num_pages) block += (a.place[page] - page) * L.bpp;
+      } else if (r < live) {
+        block = -1;  // a free page, in which another row's may lie now
+      }
       a.new_table[r * a.t.columns + c] = block;
     }
   }

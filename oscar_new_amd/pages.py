@@ -13,7 +13,8 @@ divided by the kernel blocks of a page). All calls take the block table and the 
 scheduler's rows: row r holds ``seq_lens[r]`` tokens in the blocks of ``block_tables[r]``, and the
 rows below ``counts[0]`` are live. Those tokens are the ones that stay: a fork of a request whose
 draft tokens are not yet accepted takes its count without them, since records of a shared page are
-not written again.
+not written again. A page that a row maps past its tokens counts as free: ``free_pages`` and
+``compact_pages`` take, for a row whose next tokens already have pages, the count with those tokens.
 """
 
 from __future__ import annotations
@@ -128,10 +129,11 @@ def compact_pages(caches, block_tables, seq_lens, counts):
     """Moves the pages in use to the pool's start in every layer.
 
     Returns ``(tables, live)``: int32 ``[1]`` the number of pages in use, and the block table with
-    every live token's blocks where they are now, all below page ``live``; the pages from there on
-    are free. Pages below ``live`` that were in use stay, the k-th one above moves to the k-th free
-    one below. ``block_tables`` is not changed (a caller with fixed buffers copies the new one in),
-    slot mappings made from it are stale.
+    every live token's blocks where they are now, all below page ``live``, and -1 behind a live row's
+    last page; the pages from there on are free. Rows that are not live come as they were. Pages below
+    ``live`` that were in use stay, the k-th one above moves to the k-th free one below.
+    ``block_tables`` is not changed (a caller with fixed buffers copies the new one in), slot
+    mappings made from it are stale.
     """
     table = _table(caches, block_tables, seq_lens, counts)
     scratch = seq_lens.new_empty(5 * caches.num_pages + 1)

@@ -362,3 +362,35 @@ def test_refusals():
     none = torch.zeros(0, dtype=torch.int32, device=DEV)
     assert pages.fork_requests(w.handle, w.table, w.seq_lens, none, none,
                                none.view(0, 2)).numel() == 0
+
+
+def test_compaction_leaves_no_block_of_a_page_that_it_gave_away():
+    """A row may map more pages than its tokens fill. Such a page is free: a moved page may lie in it,
+    so the new table does not name it any more. A count that holds the reserved tokens keeps it."""
+    w = World([2000, 900, 100], pool=24, rows=5)
+    bpp, table = w.bpp, w.table.cpu().numpy()
+    spare = [p for p in range(w.pool) if p not in sum(w.owned, [])]
+    reserved = [w.owned[0] + spare[:1], w.owned[1], w.owned[2] + spare[1:3]]
+    for r, owned in enumerate(reserved):
+        w.map(table, r, owned)
+    table[4, :bpp] = spare[3] * bpp + np.arange(bpp)  # a row that is not live keeps what it holds
+    w.table.copy_(torch.from_numpy(table))
+    stripes, want, total = expect_compact(w, range(3))
+    for r, owned in enumerate(w.owned):
+        want[r, bpp * len(owned) :] = -1
+    w_before = [[t.clone() for t in pair] for pair in w.caches]
+    tables, live = pages.compact_pages(w.handle, w.table, w.seq_lens, w.counts)
+    assert live.item() == total == 6 and np.array_equal(tables.cpu().numpy(), want)
+    w.check(stripes)
+    for pair, before in zip(w.caches, w_before):
+        for t, old in zip(pair, before):
+            t.copy_(old)
+    # The same with the reserved tokens counted: 2304 (three pages and one more), 1024, 2304.
+    w.owned, w.lengths = reserved, [2305, 900, 2304]
+    w.seq_lens[:3] = i32(w.lengths)
+    free = pages.free_pages(w.handle, w.table, w.seq_lens, w.counts)[0].tolist()
+    assert not set(free) & set(sum(reserved, []))
+    stripes, want, total = expect_compact(w, range(3))
+    tables, live = pages.compact_pages(w.handle, w.table, w.seq_lens, w.counts)
+    assert live.item() == total == 9 and np.array_equal(tables.cpu().numpy(), want)
+    w.check(stripes)
