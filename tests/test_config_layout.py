@@ -225,3 +225,14 @@ def test_device_rule_units_fit_the_budget(seed):
     t = device_split_tokens(int(lengths.sum()), tasks, heads, budget)
     units = sum(max(1, -(-int(l) // t)) for l in lengths)
     assert units <= max(-(-budget // heads), tasks + 1)
+
+
+def test_partial_rows_of_shared_prefixes_fit_the_scratch_and_a_wavefront():
+    from oscar_new_amd.config import SPLIT_ROW_BYTES, choose_shared_slots
+
+    assert choose_shared_slots(0, 6) == choose_shared_slots(1, 1) == choose_shared_slots(8, 6) == 256
+    assert choose_shared_slots(16384, 24) == 4  # the least, whatever the scratch
+    for tokens in (85, 86, 500, 2048, 5000):
+        slots = choose_shared_slots(tokens, 6)
+        assert 4 <= slots <= 256 and slots * tokens * 6 * SPLIT_ROW_BYTES <= 128 << 20
+        assert slots == 256 or (slots + 1) * tokens * 6 * SPLIT_ROW_BYTES > 128 << 20
