@@ -764,7 +764,7 @@ void launch_norm_rope(NormRopeArgs& a, hipStream_t s) {
   if (few)
     hipLaunchKernelGGL((norm_rope_rotate_kernel<kMode, kFp32, 8>), dim3(x, 2), dim3(8 * kWave), 0, s,
                        a);
-  else
+  else if constexpr (kMode != kPairAdjacent)  // of adjacent pairs the few rows alone get here
     hipLaunchKernelGGL((norm_rope_rotate_kernel<kMode, kFp32, 16>), dim3(x, 1), dim3(16 * kWave), 0,
                        s, a);
 }
