@@ -46,10 +46,23 @@ struct ChunkLds {
 static_assert(sizeof(ChunkLds) <= 160 * 1024, "one workgroup per CU");
 static_assert(kRawC % 16 == 0, "raw stages stay 16-byte aligned");
 
-// S^T tile += 2^(sb - 127) K (FP4) x Q (FP8), the scale per query row (column).
+// S^T tile += 2^(sb - 127) K (FP4) x Q (FP8), the scale per query row (column); kByte: the byte of sb
+// that holds it.
+template <int kByte = 0>
 __device__ __forceinline__ f32x4 mfma_qk_scaled(u32x4 k, const i32x8& q8, f32x4 c, int sb) {
   const i32x8 k4 = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k4, q8, c, 4, 0, 0, 127, 0, sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k4, q8, c, 4, 0, 0, 127, kByte, sb);
+}
+
+// Query terms of the shared-prefix tiles: the row's largest value is scaled to [8, 16) for the first
+// term and by 16 more for the second. The matrix instruction adds products in groups of eight and
+// keeps the bits down to 2^-13 of the largest product's power of two (measured); FP8 x FP4 products go
+// down to 2^-10, so either term's are all kept. With [128, 256) for both, a row's small values next to
+// a large one lost bits of their first term: errors of the LSE 1.1e-6 to 1.5e-6, now 2.0e-7 to 2.7e-7.
+constexpr int kQShift = 4;
+__device__ __forceinline__ f32x4 mfma_q_term(u32x4 k, const i32x8 (&q)[kQTerms], int term, f32x4 c,
+                                             int sb) {
+  return term == 0 ? mfma_qk_scaled<1>(k, q[0], c, sb) : mfma_qk_scaled<0>(k, q[1], c, sb);
 }
 
 typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
@@ -177,8 +190,8 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs& a, const Task& t, int
   for (int c = 0; c < ahead; ++c) issue(c, records(c));
 
   // ---- this wavefront's 16 query rows as FP8 B operands (kQTerms terms, nearly exact for bf16
-  // rows). Row n of lane (n, g), scaled to [128, 256) by a power of two that the MFMA takes back
-  // (sb). Byte e of dword d of half h: dim 128 h + 64 (d / 4) + 16 g + sigma(4 (d % 4) + e),
+  // rows). Row n of lane (n, g), scaled to [128, 256) (kCentred: mfma_q_term) by a power of two that
+  // the MFMA takes back (sb). Byte e of dword d of half h: dim 128 h + 64 (d / 4) + 16 g + sigma(4 (d % 4) + e),
   // sigma(j) = 2 (j % 8) + j / 8 (history.hip).
   const bool live = row_base + 16 * wave < rows;
   const int my_row = row_base + 16 * wave + n;
@@ -229,8 +242,10 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs& a, const Task& t, int
           for (int e = 0; e < 4; ++e) v[e] = x[h][b][2 * ((4 * d + e) & 7) + ((4 * d + e) >> 3)];
 #pragma unroll
           for (int term = 0; term < kQTerms; ++term)
-            qb[h][term][4 * b + d] = static_cast<int>(fp8x4_scaled_take(v, scale));
+            qb[h][term][4 * b + d] = static_cast<int>(
+                fp8x4_scaled_take(v, kCentred && term == 0 ? scale * (1 << kQShift) : scale));
         }
+    if (kCentred) sb |= (sb + kQShift) << 8;
   }
 
   // ---- spreading: K images of chunk c (wavefront w takes token tile w; below 4 also the scales
@@ -304,9 +319,11 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs& a, const Task& t, int
     const int h = i >> 3, tt = i & 7;
     const u32x4 f = lds.k[c & 1][h][tt][lane];
 #pragma unroll
-    for (int term = 0; term < kQTerms; ++term)
-      acc[tt] = mfma_qk_scaled(f, qb[h][term],
-                               h == 0 && term == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[tt], sb);
+    for (int term = 0; term < kQTerms; ++term) {
+      const f32x4 c0 = h == 0 && term == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[tt];
+      acc[tt] = kCentred ? mfma_q_term(f, qb[h], term, c0, sb)
+                         : mfma_qk_scaled(f, qb[h][term], c0, sb);
+    }
   };
   auto pv_step = [&](int c, int j) {
     const u32x4 f = lds.v[c & 1][j][lane];

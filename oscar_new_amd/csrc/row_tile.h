@@ -115,7 +115,7 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
     mx = max_xor32(max_xor16(mx));
     qs = 0.5f * sum_xor32(sum_xor16(sum));
     const uint32_t eb = max((__float_as_uint(mx) >> 23) & 0xffu, 8u);
-    const float scale = __uint_as_float((eb - 7) << 23);  // row max / scale in [128, 256)
+    const float scale = __uint_as_float((eb - 7) << 23);  // row max / scale in [128, 256): the second term's
     sb = static_cast<int>(eb) - 7;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -128,8 +128,10 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
           for (int e = 0; e < 4; ++e) v[e] = x[h][b][2 * ((4 * d + e) & 7) + ((4 * d + e) >> 3)];
 #pragma unroll
           for (int term = 0; term < kQTerms; ++term)
-            qb[h][term][4 * b + d] = static_cast<int>(fp8x4_scaled_take(v, scale));
+            qb[h][term][4 * b + d] = static_cast<int>(
+                fp8x4_scaled_take(v, term == 0 ? scale * (1 << kQShift) : scale));
         }
+    sb |= (sb + kQShift) << 8;
   }
 
   if (nmine > 1) issue(1, 1);
@@ -165,7 +167,7 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
 #pragma unroll
       for (int term = 0; term < kQTerms; ++term)
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) acc[tt] = mfma_qk_scaled(kf[tt], qb[h][term], acc[tt], sb);
+        for (int tt = 0; tt < 4; ++tt) acc[tt] = mfma_q_term(kf[tt], qb[h], term, acc[tt], sb);
     }
     uint32_t ksz[16], vsz[16];
 #pragma unroll

@@ -100,6 +100,20 @@ def check_step(b, drop=()):
     assert torch.equal(rows[:, :, 0].bfloat16(), out) and torch.equal(row_lse[..., 0], lse)
 
 
+def rewrite(b, at, values, share):
+    """Bytes from ``at`` on of every record become ``values(tokens)``, the first ``share`` alike."""
+    pages, bpp = b.history.view(-1, 768 * 512), b.layout.blocks_per_page
+    for r, data in enumerate(b.data):
+        new = values(data.shape[0])
+        data[:, at : at + new.shape[1]] = new
+        if r:
+            data[:share] = b.data[0][:share]
+        owned = b.meta.block_tables[r, ::bpp].tolist()
+        for j in range(-(-data.shape[0] // 768)):
+            part = data[768 * j : 768 * (j + 1)]
+            pages[owned[j] // bpp, : part.numel()] = part.reshape(-1)
+
+
 LARGE = {  # rows of the group's KV heads, all of more than 1024: 128-row tiles always
     "two heads, a partial last tile": dict(members=140, share=2500, n=2, heads=2, g=4),
     "a last tile that ends inside 16 rows": dict(members=211, share=3001, n=1, g=5, sink=4, recent=100),
@@ -147,21 +161,37 @@ def test_values_whose_codes_lie_close_to_their_middle(members):
     requests, groups = group(members, 2000, 1, low=300)
     b = Batch(requests, groups)
     gen = torch.Generator(device=DEV).manual_seed(8)
-    pages = b.history.view(-1, b.layout.physical_block_tokens * b.heads * 512)
     middle = torch.tensor([1, 2], dtype=torch.uint8, device=DEV)
-    for r, data in enumerate(b.data):
-        pick = middle[torch.randint(2, (data.shape[0], 64, 4), generator=gen, device=DEV)]
-        codes = pick[..., 0] | pick[..., 1] << 2 | pick[..., 2] << 4 | pick[..., 3] << 6
-        data[:, 68:132] = codes
-        if r:
-            data[:2000, 68:132] = b.data[0][:2000, 68:132]
-        blocks = b.meta.block_tables[r].view(-1, b.layout.blocks_per_page)[:, 0].tolist()
-        for j in range(-(-data.shape[0] // 768)):
-            part = data[768 * j : 768 * (j + 1)]
-            pages[blocks[j] // b.layout.blocks_per_page, : part.numel()] = part.reshape(-1)
+
+    def codes(t):
+        pick = middle[torch.randint(2, (t, 64, 4), generator=gen, device=DEV)]
+        return pick[..., 0] | pick[..., 1] << 2 | pick[..., 2] << 4 | pick[..., 3] << 6
+
+    rewrite(b, 68, codes, 2000)
     _, units = planned(b)
     assert bool(units[units[:, 5] <= 2000, 7].all()) == (members == 8)
     check_step(b)
+
+
+@pytest.mark.parametrize("members", [8, 200])
+def test_small_query_values_beside_large_ones(members):
+    """Large values of either sign and, 2^-14 of them, small ones of one sign that add up to a seventh
+    of a unit of the score: they are within the bound only if none is lost beside the large ones."""
+    requests, groups = group(members, 2000, 1, low=300)
+    b = Batch(requests, groups)
+    gen = torch.Generator(device=DEV).manual_seed(9)
+
+    def scale(t):  # keys of 0.8 times their codes
+        return torch.tensor([0.8, 0.0], device=DEV).half().view(torch.uint8).expand(t, 4)
+
+    rewrite(b, 64, scale, 2000)
+    large = torch.randint(2, b.q.shape, generator=gen, device=DEV) * 2 - 1
+    dim = torch.arange(256, device=DEV)
+    b.q = torch.where(dim % 16 < 2, 128.0 * large, 2.0**-7 * (1 + dim % 2)).bfloat16()
+    _, units = planned(b)
+    assert bool(units[units[:, 5] <= 2000, 7].all()) == (members == 8)
+    out, lse = b.run()
+    b.check(out, lse)
 
 
 def test_an_unmapped_block_of_a_shared_prefix():
