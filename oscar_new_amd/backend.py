@@ -25,7 +25,8 @@ import torch
 
 from . import kernels
 from .config import (OscarConfig, attention_programs, choose_chunk_splits, choose_device_partition,
-                     choose_history_partition, choose_splits, chunk_kernel_pays)
+                     choose_history_partition, choose_splits, chunk_kernel_pays,
+                     shared_prefix_pays)
 
 SPLIT_POLICIES = ("device", "reference", "mi355x")
 ENV_SPLIT_POLICY = "OSCAR_AMD_SPLIT_POLICY"
@@ -365,23 +366,31 @@ class OscarAttentionImpl:
             self._single_launch_step(q, k, v, meta, splits, split_tokens, rows, lse)
         return output
 
-    def _fused_step(self, q, k, v, meta, splits, split_tokens, rows, lse):
-        """With a plan of shared prefixes (``meta.shared``): pre-attention -> shared history ->
-        post. Otherwise the whole step in one launch (``layer_step``, where it applies); else, with
-        ``overlap``, the history launch carrying the pre-attention work (BF16 branch, K/V INT2
-        store and, with ``rotate_in_history``, the q rotation) -> post (split merge, inverse V
-        rotation, path merge, windows); else pre-attention -> history -> post, the last two in
-        one launch with ``one_launch_post``."""
-        layout = meta.layout
+    def _takes_shared(self, meta, tokens):
+        """Whether a fused step computes shared prefixes by the plan that the step has."""
         shared = getattr(meta, "shared", None)
-        if shared is not None:
+        if shared is None:
+            return False
+        longest, total = meta.max_query_len, getattr(meta, "total_seq_len", None)
+        return not isinstance(longest, int) or shared_prefix_pays(
+            tokens, meta.num_reqs, self.num_kv_heads, longest, total, shared.saved_tokens)
+
+    def _fused_step(self, q, k, v, meta, splits, split_tokens, rows, lse):
+        """With a plan of shared prefixes (``meta.shared``), where it pays (``shared_prefix_pays``):
+        pre-attention -> shared history -> post. Otherwise the whole step in one launch
+        (``layer_step``, where it applies); else, with ``overlap``, the history launch carrying the
+        pre-attention work (BF16 branch, K/V INT2 store and, with ``rotate_in_history``, the q
+        rotation) -> post (split merge, inverse V rotation, path merge, windows); else pre-attention
+        -> history -> post, the last two in one launch with ``one_launch_post``."""
+        layout = meta.layout
+        if self._takes_shared(meta, q.shape[0]):
             # Requests with common prefixes: the history branch computes the shared positions
             # once for all of them and comes merged, as one split.
             qrot, rp, rl = kernels.pre_attention(q, k, v, self.history, self.window, meta, layout,
                                                  self.scale, self.rk_t, self.rv_t,
                                                  raw=not kernels.chunk_raw_preferred(meta))
-            hp, hl = kernels.shared_history(qrot, self.history, meta, shared, layout, self.scale,
-                                            merged=False)
+            hp, hl = kernels.shared_history(qrot, self.history, meta, meta.shared, layout,
+                                            self.scale, merged=False)
             kernels.post_attention(hp, hl, rp, rl, self.rv, k, v, self.window, meta, layout, rows,
                                    lse)
             return

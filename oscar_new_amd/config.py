@@ -326,6 +326,34 @@ def chunk_kernel_pays(tokens, requests, num_kv_heads, q_heads, splits, max_seq_l
     return tile < task
 
 
+def shared_prefix_pays(tokens, requests, num_kv_heads, max_query_len, total_seq_len=None,
+                       saved_tokens=None):
+    """Whether a layer step takes less time with the shared positions of its requests computed once
+    (pre-attention, shared history, merge, post-attention) than with the history launch that carries
+    the BF16 branch and the store (no reference counterpart). Host-side values: ``saved_tokens`` sums
+    each group's shared tokens over its members but one; unknown, all requests count as one group
+    that shares everything. True when the lengths are not known either: then the caller decides.
+
+    Layer step without and with the plan (6 query heads, us). One query token: 6 samples of 2000
+    tokens 24.3 and 33.1, 32 of 32000 43.3 and 47.6, 96 of 16000 73.3 and 68.7, 256 of 32000 214 and
+    128; tokens that are not shared cost more with it: 64 requests of 16000 with 8000 of them shared
+    51 and 61, 256 of 16000 with 12000 135 and 112. Two to sixteen: few requests gain in any case
+    (8 of 2000, 4 tokens 60 and 46), many where half is shared (160 of 16000, 3 tokens, 800 shared
+    183 and 238, 8000 shared 182 and 160). Longer chunks fill 128-row tiles by themselves: 2 x 64
+    tokens of 32000 129 and 99, 2 x 256 199 and 222. Over 520 such steps the rule's choice took at most
+    1.06 of the time without the plan, 0.91 on average (the faster one's each time: 0.90)."""
+    if max_query_len > 16:
+        return tokens <= 256
+    if saved_tokens is None:
+        if total_seq_len is None:
+            return True
+        saved_tokens = total_seq_len - total_seq_len // max(1, requests)
+    own = 0 if total_seq_len is None else max(0, total_seq_len - saved_tokens)
+    if max_query_len > 1:
+        return requests <= 8 or saved_tokens >= 0.8 * own
+    return (saved_tokens - own) * num_kv_heads > 1_300_000
+
+
 def choose_shared_slots(tokens, q_heads, most=256, scratch_bytes=128 << 20):
     """Partial rows per query row of a step with shared prefixes (no reference counterpart): the
     pieces that a row's positions may be cut into, four per lane of the wavefront that merges them

@@ -554,6 +554,7 @@ class SharedPlan:
     tokens: int
     layout: object
     layout_struct: object  # its C form
+    saved_tokens: int | None = None  # positions computed once for several requests, where known
 
     @property
     def units(self):
@@ -576,7 +577,8 @@ class SharedPlan:
         return base, base + 32 * self.capacity, base + 32 * self.capacity + 4
 
 
-def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, out=None):
+def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, out=None,
+                   saved_tokens=None):
     """The plan of a step whose requests share prefixes, for every layer's ``shared_history``: one
     launch per step (no reference counterpart).
 
@@ -587,7 +589,9 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
     ``hq``: query heads, at most 32 per KV head; groups and requests: at most 4096 together;
     ``tokens``: most query tokens the plan's layers pass (default
     ``meta.num_actual_tokens``; a padded graph step passes its rows). ``out``: a plan of the same
-    sizes to fill again, so that a captured graph reads the new one.
+    sizes to fill again, so that a captured graph reads the new one. ``saved_tokens``: the host's sum
+    of each group's shared tokens over its members but one, for ``config.shared_prefix_pays``, by
+    which a layer step takes the plan or leaves it (a step that would leave it needs no plan).
     """
     device = _same_device(meta.query_start_loc, seq_lens=meta.seq_lens, counts=meta.counts,
                           group_starts=group_starts, prefix_tokens=prefix_tokens)
@@ -618,6 +622,7 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
           or out.slots != slots or out.query_heads != hq or out.requests != reqs
           or out.buffer.device != device or out.layout != layout):
         raise ValueError("the plan to fill again was made for other sizes")
+    out.saved_tokens = None if saved_tokens is None else int(saved_tokens)
     units, unit_count, token_slots = out.addresses()
     _launch(
         _ext.library().oscar_shared_plan, "prepare_shared", device,

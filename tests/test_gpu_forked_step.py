@@ -108,3 +108,22 @@ def test_forked_requests_decode_alike_with_and_without_the_plan(qlen, fused):
     for a, b in zip(with_plan.caches, without.caches):
         assert torch.equal(a[0].view(torch.int16), b[0].view(torch.int16))
         assert torch.equal(a[1].view(torch.int16), b[1].view(torch.int16))
+
+
+@pytest.mark.parametrize("taken", [True, False])
+@pytest.mark.parametrize("qlen", [1, 4, 70])
+def test_steps_that_take_the_plan_and_steps_that_leave_it(monkeypatch, qlen, taken):
+    calls, run = [], kernels.shared_history
+    monkeypatch.setattr("oscar_new_amd.backend.shared_prefix_pays", lambda *args: taken)
+    monkeypatch.setattr(kernels, "shared_history", lambda *a, **k: calls.append(1) or run(*a, **k))
+    with_plan, without = Server(qlen, True), Server(qlen, True)
+    got, want = with_plan.scenario(True), without.scenario(False)
+    assert len(calls) == (3 * LAYERS if taken else 0)
+    for a, b in zip(got, want):
+        if taken:  # bounds as above
+            assert float((a.float() - b.float()).norm() / b.float().norm()) < 1e-2
+        else:
+            assert torch.equal(a, b)
+    for a, b in zip(with_plan.caches, without.caches):
+        assert torch.equal(a[0].view(torch.int16), b[0].view(torch.int16))
+        assert torch.equal(a[1].view(torch.int16), b[1].view(torch.int16))
