@@ -191,8 +191,8 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs& a, const Task& t, int
 
   // ---- this wavefront's 16 query rows as FP8 B operands (kQTerms terms, nearly exact for bf16
   // rows). Row n of lane (n, g), scaled to [128, 256) (kCentred: mfma_q_term) by a power of two that
-  // the MFMA takes back (sb). Byte e of dword d of half h: dim 128 h + 64 (d / 4) + 16 g + sigma(4 (d % 4) + e),
-  // sigma(j) = 2 (j % 8) + j / 8 (history.hip).
+  // the MFMA takes back (sb). Byte e of dword d of half h: dim 128 h + 64 (d / 4) + 16 g +
+  // sigma(4 (d % 4) + e), sigma(j) = 2 (j % 8) + j / 8 (history.hip).
   const bool live = row_base + 16 * wave < rows;
   const int my_row = row_base + 16 * wave + n;
   const int qi = static_cast<int>(fastdiv(static_cast<uint32_t>(my_row), a.g_div));

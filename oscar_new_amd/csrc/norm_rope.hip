@@ -15,11 +15,11 @@
 // in the cache by then) rather than moved between lanes: one 16-byte load, in flight with the
 // lane's own, against four cross-lane moves behind it.
 //
-// What bounds it: without R_k the memory (16384 tokens of 7 heads, 120 MB: 25 to 26 us, 4.6 TB/s of
-// the 5.0 that a large copy reaches); with R_k the memory too for many rows (the same with R_k, 170 MB:
-// 36.4 us), the loads of rows and R_k and then R_k's reads from LDS for a chunk (2048 tokens of 14
-// heads, 42 MB: 14.3 us); a decode step its chain of loads (32 tokens of 7 heads: 5.2 us, 3.9 without
-// R_k).
+// What bounds it (us, calls back to back in a graph): without R_k the memory (16384 tokens of 7 heads,
+// 120 MB: 26.5, 4.5 TB/s; 31.6 where three inputs alternate and none is in the last-level cache); with
+// R_k the memory too for many rows (the same with R_k, 170 MB: 35.2), the loads of rows and R_k and then
+// R_k's reads from LDS for a chunk (2048 tokens of 14 heads, 42 MB: 14.1); a decode step its chain of
+// loads (32 tokens of 7 heads: 5.2, 4.3 without R_k).
 #include <type_traits>
 
 #include "dma.h"
@@ -732,7 +732,7 @@ __global__ __launch_bounds__(kWalkWaves * kWave, 2) void norm_rope_walk_kernel(
 // With R_k: 16-row blocks up to which two workgroups of 8 wavefronts share each, all on CUs of their
 // own (300 tokens of 7 heads: 5.9 us, 6.3 by norm_rope_walk_kernel; 340, more workgroups than CUs: 7.6
 // and 6.4). Above, one workgroup per CU walks: wavefronts by themselves where a pair's dims lie in one
-// lane (2048 tokens of 14 heads 14.3 us, 18.2 by blocks through LDS; 16384 of 7 heads 36.4 and 50.4),
+// lane (2048 tokens of 14 heads 14.1 us, 18.2 by blocks through LDS; 16384 of 7 heads 35.2 and 50.4),
 // else blocks of 32 rows.
 constexpr int64_t kFewBlocks = 128, kRotateGroups = 256;
 

@@ -8,11 +8,13 @@
 // unfinished last page.
 //
 // Copies are bounded by memory: 16 bytes a lane, only live records (a request's last page ends
-// inside) and live window rows. 96 forks in six layers, 356 MB read and written: 75.6 us, 4.7 TB/s of
-// the 5.0 that a large copy reaches; 8 forks of one parent in 16 layers 15.9 us (77 MB, the parent's
-// rows from the caches); 174 MB of moved pages 34.6 us. The bookkeeping is a few thousand integers
-// and runs in one workgroup (free pages 3.3 to 6.6 us, a compaction's plan 5.8 to 6.7), or in every
-// workgroup of a fork again, so that a call is one or two launches.
+// inside) and live window rows. 96 forks in six layers, 356 MB read and written: 75.7 us, 4.7 TB/s of
+// the 5.0 that a large copy reaches; 8 forks of one parent in 16 layers 16.1 us (77 MB, the parent's
+// rows from the caches); 174 MB of moved pages 34.2 us, about 45 where nothing of them is in the
+// last-level cache. The bookkeeping is a few integers per page and runs in one workgroup, or in every
+// workgroup of a fork again, so that a call is one or two launches. It grows with the pool (us, free
+// pages and a compaction in which nothing moves): 3.7 and 7.9 at 100 pages and 8 requests, 6.8 and 10.9
+// at 1000 and 60, 16 and 23 at 4000 and 200, 58 and 75 at 16000 and 800.
 #include "common.h"
 
 namespace oscar {

@@ -80,7 +80,8 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
   };
   if (nmine > 0) issue(0, 0);
 
-  // ---- the query rows as FP8 B operands, built by every wavefront for itself (chunk_tile.h).
+  // ---- the query rows as FP8 B operands, built by every wavefront for itself (chunk_tile.h; the
+  // first term at 2^kQShift times the scale).
   const int my_row = row_base + n;
   const int qi = static_cast<int>(fastdiv(static_cast<uint32_t>(my_row), a.g_div));
   const int64_t my_token = static_cast<int64_t>(t.qstart) + qi;
@@ -115,7 +116,7 @@ __device__ __forceinline__ void row_tile(const AttnArgs& a, const Task& t, int h
     mx = max_xor32(max_xor16(mx));
     qs = 0.5f * sum_xor32(sum_xor16(sum));
     const uint32_t eb = max((__float_as_uint(mx) >> 23) & 0xffu, 8u);
-    const float scale = __uint_as_float((eb - 7) << 23);  // row max / scale in [128, 256): the second term's
+    const float scale = __uint_as_float((eb - 7) << 23);  // row max / scale in [128, 256)
     sb = static_cast<int>(eb) - 7;
 #pragma unroll
     for (int h = 0; h < 2; ++h)

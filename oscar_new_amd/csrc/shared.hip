@@ -18,11 +18,13 @@
 // tile's pieces go to slots that the merge kernel joins by their LSEs, as many as the plan says for
 // each token.
 //
-// What bounds it (history launch and merge of a layer, us; unshared: the launches of history.hip and
-// their merge): a few samples of a short prompt their chain of loads, 6 of 2000 tokens 13.7 (unshared
+// What bounds it (history launch and merge of a layer, us, replayed back to back in a graph; the two
+// kernels' times in a trace add up to 1 to 5 us more; unshared: the launches of history.hip and their
+// merge, in a graph): a few samples of a short prompt their chain of loads, 6 of 2000 tokens 13.7 (unshared
 // 19.5); 16-row tiles vector issue, the rounds of their wavefronts and the start of a unit, about half
-// of its time, 32 of 32000 26.5 (38.2), three prompts of 9 samples with 4 query tokens 27.4 (48.0);
-// 128-row tiles the pipeline of chunk_tile.h, 4.2 a chunk, 256 of 32500 87.8 (259.5).
+// of its time, 32 of 32000 26.4 (38.3), three prompts of 9 samples with 4 query tokens 27.2 (48.6);
+// 128-row tiles the pipeline of chunk_tile.h, 4.2 a chunk, 256 of 32500 84 to 88 (261). Which layer
+// steps take it, in place of a history launch that carries more: config.shared_prefix_pays.
 #include "merge.h"
 #include "row_tile.h"
 
@@ -34,8 +36,8 @@ constexpr int kSharedEntries = 4096;  // groups and requests whose counts live i
 constexpr int kSharedSlots = 256;     // partial rows of a row: four per lane of a merging wavefront
 constexpr int kUnitWords = 8;
 // Rows up to which an entry's tiles are 16 rows: always, and where the plan finds that faster for the
-// step (32 samples of 32000 tokens, 192 rows: 26.7 us a layer against 34.4 with 128-row tiles, 96 of
-// 16000: 36.6 and 40.3, 128 of 32000: 58.6 and 55.6).
+// step (in a graph, 32 samples of 32000 tokens, 192 rows: 26.7 us a layer against 34.4 with 128-row
+// tiles, 96 of 16000: 36.6 and 40.3, 128 of 32000: 58.6 and 55.6).
 constexpr int kSmallRows[2] = {48, 1024};
 // A unit's time in us: its start and end, a 128-token chunk of a 128-row tile, and a round of a 16-row
 // tile, in which each of the eight wavefronts takes 64 tokens (kRound chunks); what a short unit
