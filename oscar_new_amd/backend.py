@@ -371,9 +371,11 @@ class OscarAttentionImpl:
         shared = getattr(meta, "shared", None)
         if shared is None:
             return False
-        longest, total = meta.max_query_len, getattr(meta, "total_seq_len", None)
+        longest = meta.max_query_len
         return not isinstance(longest, int) or shared_prefix_pays(
-            tokens, meta.num_reqs, self.num_kv_heads, longest, total, shared.saved_tokens)
+            tokens, meta.num_reqs, self.num_kv_heads, self.num_heads, longest,
+            getattr(meta, "total_seq_len", None), shared.saved_tokens, shared.groups,
+            getattr(meta, "total_query_keys", None), meta.layout.config.queries_per_tile)
 
     def _fused_step(self, q, k, v, meta, splits, split_tokens, rows, lse):
         """With a plan of shared prefixes (``meta.shared``), where it pays (``shared_prefix_pays``):

@@ -326,32 +326,55 @@ def chunk_kernel_pays(tokens, requests, num_kv_heads, q_heads, splits, max_seq_l
     return tile < task
 
 
-def shared_prefix_pays(tokens, requests, num_kv_heads, max_query_len, total_seq_len=None,
-                       saved_tokens=None):
+# Times of a layer step (us) by its query rows per history task, up to 8, 16 and 32, and of steps
+# with more than 16 query tokens in a request: without a plan of shared prefixes (start, per million
+# positions of a task's rows, per thousand query rows) and with it (start, per million positions of
+# 16 rows that a request has to itself, the same of a group, per thousand query rows).
+STEP_US = ((24.1, 23.3, 16.6), (42.3, 29.2, 8.9), (51.0, 40.2, 9.7), (73.3, 30.9, 3.6))
+SHARED_STEP_US = ((33.6, 35.9, 23.5, 19.3), (39.4, 33.8, 20.2, 11.3), (47.0, 26.7, 17.9, 9.2),
+                  (62.7, 18.9, 17.3, 5.8))
+
+
+@functools.lru_cache(maxsize=256)
+def shared_prefix_pays(tokens, requests, num_kv_heads, q_heads, max_query_len, total_seq_len=None,
+                       saved_tokens=None, groups=1, total_query_keys=None, queries_per_tile=4):
     """Whether a layer step takes less time with the shared positions of its requests computed once
     (pre-attention, shared history, merge, post-attention) than with the history launch that carries
     the BF16 branch and the store (no reference counterpart). Host-side values: ``saved_tokens`` sums
-    each group's shared tokens over its members but one; unknown, all requests count as one group
-    that shares everything. True when the lengths are not known either: then the caller decides.
+    each group's shared tokens over its members but one; unknown, the groups share everything.
+    ``total_query_keys`` sums query tokens times length. True when the lengths are not known: then
+    the caller decides.
 
-    Layer step without and with the plan (6 query heads, us). One query token: 6 samples of 2000
-    tokens 24.3 and 33.1, 32 of 32000 43.3 and 47.6, 96 of 16000 73.3 and 68.7, 256 of 32000 214 and
-    128; tokens that are not shared cost more with it: 64 requests of 16000 with 8000 of them shared
-    51 and 61, 256 of 16000 with 12000 135 and 112. Two to sixteen: few requests gain in any case
-    (8 of 2000, 4 tokens 60 and 46), many where half is shared (160 of 16000, 3 tokens, 800 shared
-    183 and 238, 8000 shared 182 and 160). Longer chunks fill 128-row tiles by themselves: 2 x 64
-    tokens of 32000 129 and 99, 2 x 256 199 and 222. Over 520 such steps the rule's choice took at most
-    1.06 of the time without the plan, 0.91 on average (the faster one's each time: 0.90)."""
-    if max_query_len > 16:
-        return tokens <= 256
+    A step with a plan is four launches and not three, and takes a request's own positions 16 rows at
+    a time, so it pays where much is shared: 6 samples of 2000 tokens 24.3 us without and 33.1 with
+    it, 32 of 32000 43.3 and 47.6, 256 of 32500 216 and 120; 64 requests of 16000 tokens with 4000 of
+    them shared 51 and 67; 160 of 16000, 3 query tokens, 800 shared 183 and 238, 8000 shared 182 and
+    160. Both times are estimated, linear in the positions and rows; the estimates are within a
+    quarter of most measured times, so the plan is taken where its one is below 0.85 of the other.
+    Over 890 steps of 1 to 4 KV heads and 4 to 8 query heads each the choice took at most 1.01 of the
+    time without the plan, 0.96 on average (the faster one's each time: 0.91)."""
+    if total_seq_len is None:
+        return True
+    requests, groups = max(1, requests), max(1, groups)
+    if requests <= groups:
+        return False
+    group = q_heads // num_kv_heads
     if saved_tokens is None:
-        if total_seq_len is None:
-            return True
-        saved_tokens = total_seq_len - total_seq_len // max(1, requests)
-    own = 0 if total_seq_len is None else max(0, total_seq_len - saved_tokens)
-    if max_query_len > 1:
-        return requests <= 8 or saved_tokens >= 0.8 * own
-    return (saved_tokens - own) * num_kv_heads > 1_300_000
+        saved_tokens = total_seq_len * (requests - groups) // requests
+    once = saved_tokens * groups / (requests - groups)  # shared positions, each group's once
+    own = max(0.0, total_seq_len - saved_tokens - once)
+    queries = total_query_keys / max(1, total_seq_len) if total_query_keys else max_query_len
+    rows = min(max_query_len, queries_per_tile) * group
+    kind = 3 if max_query_len > 16 else 0 if rows <= 8 else 1 if rows <= 16 else 2
+    tasks = math.ceil(queries / queries_per_tile)
+    own_tiles = math.ceil(queries * group / 16)
+    group_tiles = math.ceil(requests / groups * queries * group / 16)
+    million, thousand = num_kv_heads / 1e6, tokens * q_heads / 1e3
+    start, position, row = STEP_US[kind]
+    without = start + position * total_seq_len * tasks * million + row * thousand
+    start, alone, shared, row = SHARED_STEP_US[kind]
+    return (start + (alone * own * own_tiles + shared * once * group_tiles) * million
+            + row * thousand) < 0.85 * without
 
 
 def choose_shared_slots(tokens, q_heads, most=256, scratch_bytes=128 << 20):

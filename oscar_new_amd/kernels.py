@@ -554,6 +554,7 @@ class SharedPlan:
     tokens: int
     layout: object
     layout_struct: object  # its C form
+    groups: int = 1
     saved_tokens: int | None = None  # positions computed once for several requests, where known
 
     @property
@@ -617,7 +618,8 @@ def prepare_shared(meta, layout, hq, group_starts, prefix_tokens, tokens=None, o
     capacity = _ext.library().oscar_shared_capacity(tokens, hq, groups, reqs, heads)
     if out is None:
         buffer = meta.seq_lens.new_empty(8 * capacity + 1 + max(tokens, 1))
-        out = SharedPlan(buffer, capacity, slots, hq, reqs, tokens, layout, layout_struct(layout))
+        out = SharedPlan(buffer, capacity, slots, hq, reqs, tokens, layout, layout_struct(layout),
+                         groups)
     elif (out.capacity != capacity or out.tokens != tokens
           or out.slots != slots or out.query_heads != hq or out.requests != reqs
           or out.buffer.device != device or out.layout != layout):
