@@ -601,9 +601,10 @@ int oscar_free_pages(int64_t num_pages, const int32_t* table, int64_t table_stri
  * BF16 window (the page has one owner), and an unfinished last page (of several), which is copied
  * into fresh[i][1]. Only records and window rows of the parent's tokens are copied; table columns
  * past its last page keep their values. status[i]: 1, or 0 for a fork that was refused and wrote
- * nothing: a row outside the table, a parent that is some fork's child, a child row or a needed
- * fresh page that an earlier entry lists too, a needed fresh page outside the pool or among the
- * parent's, a parent's page outside the pool. Fresh pages must be free. forks <= 4096.
+ * nothing: a row outside the table, more tokens than its columns hold, a parent that is some fork's
+ * child, a child row or a needed fresh page that an earlier entry lists too, a needed fresh page
+ * outside the pool or among the parent's, a parent's page outside the pool. Fresh pages must be free.
+ * forks <= 4096.
  */
 int oscar_fork_requests(const void* stripes, int64_t layers, int64_t num_pages, int32_t* table,
                         int64_t table_stride, int64_t table_columns, int64_t rows,

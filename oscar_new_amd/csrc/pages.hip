@@ -208,7 +208,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(const ForkArgs a) {
   const int pages = length > 0 ? (length - 1) / L.bp + 1 : 0;
   const int tail = length - (pages - 1) * L.bp;
   const bool first = pages > 0, second = pages > 1 && tail < L.bp;
-  bad |= static_cast<int64_t>(pages) * L.bpp > a.columns;
+  bad |= length > 0 && (length - 1) / L.bk >= a.columns;  // a block of tokens without a column
   bad |= first && (p0 < 0 || p0 >= a.pool.num_pages);
   bad |= second && (p1 < 0 || p1 >= a.pool.num_pages || p1 == p0);
   for (int i = tid; i < a.forks; i += kThreads) {
@@ -240,7 +240,9 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(const ForkArgs a) {
   if (refused) return;
   if (lead) {
     int32_t* out = a.table + static_cast<int64_t>(child) * a.stride;
-    for (int c = tid; c < pages * L.bpp; c += kThreads) {
+    // The last page's blocks behind the tokens may have no columns.
+    const int columns = static_cast<int>(min(static_cast<int64_t>(pages) * L.bpp, a.columns));
+    for (int c = tid; c < columns; c += kThreads) {
       const int j = c / L.bpp, b = c - j * L.bpp;
       out[c] = j == 0 ? p0 * L.bpp + b
                       : (second && j == pages - 1 ? p1 * L.bpp + b : row[c]);

@@ -105,9 +105,9 @@ def fork_requests(caches, block_tables, seq_lens, parents, children, fresh):
     the parent's last page keep their values.
 
     Returns int32 ``[forks]``: 1, or 0 for a fork that was refused and wrote nothing (a row outside
-    the table, a parent that is also some fork's child, a child row or a needed page that an earlier
-    fork lists too, a needed page outside the pool or among the parent's own, a parent's page
-    outside the pool). At most 4096 forks a call.
+    the table, more tokens than its columns hold, a parent that is also some fork's child, a child
+    row or a needed page that an earlier fork lists too, a needed page outside the pool or among the
+    parent's own, a parent's page outside the pool). At most 4096 forks a call.
     """
     table = _table(caches, block_tables, seq_lens, parents=parents, children=children, fresh=fresh)
     forks = parents.numel()

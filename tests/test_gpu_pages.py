@@ -394,3 +394,22 @@ def test_compaction_leaves_no_block_of_a_page_that_it_gave_away():
     tables, live = pages.compact_pages(w.handle, w.table, w.seq_lens, w.counts)
     assert live.item() == total == 9 and np.array_equal(tables.cpu().numpy(), want)
     w.check(stripes)
+
+
+@pytest.mark.parametrize("length,columns,done", [(2000, 16, 1), (1920, 15, 1), (1921, 15, 0),
+                                                 (2304, 18, 1), (100, 1, 1), (129, 1, 0)])
+def test_forks_in_a_table_that_ends_inside_a_page(length, columns, done):
+    """A table needs a column for every block that holds tokens, not for whole pages."""
+    w = World([length, 50], pool=14, rows=4)
+    whole = w.table.clone()
+    w.table = w.table[:, :columns]
+    free = [p for p in range(w.pool) if p not in sum(w.owned, [])]
+    stripes, table, seq = w.stripes(), whole.cpu().numpy(), w.seq_lens.cpu().numpy()
+    before = table.copy()
+    if done:
+        expect_fork(w, stripes, table, seq, 0, 3, free[:2])
+    assert fork(w, [0], [3], [free[:2]]).tolist() == [done]
+    assert np.array_equal(w.table.cpu().numpy(), table[:, :columns])
+    assert np.array_equal(w.seq_lens.cpu().numpy(), seq)
+    assert np.array_equal(w.table._base.cpu().numpy()[:, columns:], before[:, columns:])
+    w.check(stripes)
