@@ -262,3 +262,33 @@ def test_infinite_queries_and_scales_stay_with_the_rows_that_see_them(members):
         out[rows] = clean[rows]
         assert torch.equal(out, clean)
         b.history.copy_(history)
+
+
+def test_captured_plan_and_history_of_changing_requests():
+    requests, groups = group(40, 3000, 2, low=300)
+    b = Batch(requests, groups, pad=4)
+    hq, m = b.heads * b.g, b.meta
+
+    def step(q):
+        plan = kernels.prepare_shared(m, b.layout, hq, b.starts, b.prefix, tokens=q.shape[0])
+        return kernels.shared_history(q, b.history, m, plan, b.layout, 1 / 16)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(b.q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out, lse = step(b.q)
+    torch.cuda.current_stream().wait_stream(side)
+    lengths = m.seq_lens.clone()
+    for live, share, less in ((40, 3000, 0), (7, 3000, 0), (40, 700, 0), (33, 3000, 2500), (40, 3000, 0)):
+        m.counts.copy_(torch.tensor([live, 2 * live], dtype=torch.int32))
+        m.seq_lens[:40] = lengths[:40] - less
+        b.prefix.fill_(share)
+        b.requests = [(p - less, n) for p, n in requests]
+        graph.replay()
+        want, want_lse = step(b.q)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        b.check(out, lse, live=live)
