@@ -43,14 +43,23 @@ typedef struct oscar_layout {
   int32_t kv_heads;              /* H */
   int32_t physical_block_tokens; /* Bp, tokens per physical page */
   int32_t kernel_block_tokens;   /* BK, tokens per block-table entry (power of two) */
-  int32_t slot_bytes;            /* 160 */
-  int32_t vector_bytes;          /* 68 */
+  int32_t slot_bytes;            /* 160; 272 for 4-bit records */
+  int32_t vector_bytes;          /* 68; 132 for 4-bit records */
   int32_t sink_tokens;           /* S */
   int32_t recent_tokens;         /* R */
   int32_t ring_tokens;           /* C = R + speculative + 1 */
   int32_t reserved;              /* 0 */
   int64_t stripe_page_bytes;     /* Bp * H * D * 2 */
 } oscar_layout;
+
+/*
+ * Records of 4-bit codes (no reference counterpart), per (token, KV head): bytes [0, 128) K codes,
+ * [128, 256) V codes (dim d in bits 4 (d % 2) of byte d / 2), then fp16 K scale, K zero, V scale and
+ * V zero, [264, 272) never written; the value of code c is zero + scale * c. oscar_rope_append writes
+ * them, oscar_history_int4 and oscar_read_records read them; the entry points that read no records, and
+ * those that copy whole ones (pages), take such a layout too. Every other one refuses it
+ * (OSCAR_E_LAYOUT).
+ */
 
 /* Clip configuration (reference: config.py:14-19; kernels.py:69-101). */
 enum oscar_clip_mode {
@@ -660,6 +669,57 @@ int oscar_shared_history(const void* query, int64_t q_s0, int64_t q_s1, int64_t 
                          const int32_t* token_slots, int64_t n, int64_t hq, int32_t slots,
                          float scale, const oscar_layout* layout, float* partials, float* lse,
                          int32_t fp32_out, void* out, float* out_lse, void* stream);
+
+/*
+ * rope_append -- rows of a packed projection on their way into the paged cache, in one launch (no
+ * reference counterpart as one call: what a model computes ahead of oscar_ascend/backend.py:125-140,
+ * then kernels.py:51-66 and 175-202). query (with q_out; optional, then hq = 0) [n][hq][256], key
+ * [n][hk][256] and value (optional: then nothing is stored) [n][hk][256]: bf16, strides multiples of 8,
+ * rows contiguous and 16-byte aligned.
+ *
+ * q_out and k_out (contiguous bf16): the rows of oscar_qk_norm_rope, with two additions. Without weights
+ * (both NULL) rows are not normed. With axis_count (1..32) > 1 a token has that many positions, axis a's
+ * at positions[a * position_stride + t], and pair j of the rotation takes its angle at the position of
+ * axis axes[j] (int32 [rotary_dim / 2]; a pair of no axis turns to NaN); a live token with a position
+ * outside [0, table_rows) gets NaN rows.
+ *
+ * q_rot (optional): rotate(q_out, R_k). With value: for every token t < counts[1] with slots[t] >= 0 the
+ * record of rotate(k_out, R_k) and rotate(value, R_v), clipped as `clip` says; 2-bit layouts get the
+ * bytes of oscar_store_int2. Live tokens' slots differ. rk_t, rv_t: R^T, contiguous bf16 [256][256].
+ * counts: optional without value.
+ */
+int oscar_rope_append(const void* query, int64_t q_s0, int64_t q_s1, const void* key, int64_t k_s0,
+                      int64_t k_s1, const void* value, int64_t v_s0, int64_t v_s1, int64_t n,
+                      int64_t hq, int64_t hk, const void* q_weight, const void* k_weight,
+                      int32_t weight_fp32, int32_t unit_offset, float eps, const void* cos_sin,
+                      int64_t table_rows, int64_t table_stride, int32_t table_fp32, int32_t rotary_dim,
+                      int32_t interleaved, const int64_t* positions, int64_t position_stride,
+                      int32_t axis_count, const int32_t* axes, const int32_t* counts, void* q_out,
+                      void* k_out, const void* rk_t, const void* rv_t, void* q_rot, void* history,
+                      int64_t history_bytes, const int64_t* slots, const oscar_layout* layout,
+                      const oscar_clip* clip, void* stream);
+
+/*
+ * read_records -- the values that the records of `slots` (int64 [n]) stand for, in the rotated basis:
+ * key_out, value_out bf16 [n][kv_heads][256]; zeros for a slot below 0 or outside the buffer. Either
+ * layout.
+ */
+int oscar_read_records(const void* history, int64_t history_bytes, const int64_t* slots, int64_t n,
+                       const oscar_layout* layout, void* key_out, void* value_out, void* stream);
+
+/*
+ * history_int4 -- oscar_attention_partials (raw = 0) over 4-bit records: the same tasks, masks, split
+ * rules, partial rows and LSEs. kernel_block_tokens >= 32. Under the device rule (split_tokens < 0) the
+ * split length is the least of eight tried ones with which all splits fit the budget.
+ */
+int oscar_history_int4(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_s2,
+                       const void* history, int64_t history_bytes, const int32_t* qstarts,
+                       const int32_t* seq_lens, const int32_t* block_tables, int64_t table_stride,
+                       int64_t table_columns, const int32_t* counts, const int32_t* tasks,
+                       const int32_t* task_count, int64_t n, int64_t hq, int64_t programs,
+                       int32_t splits, int32_t block_n, int32_t query_tile, int32_t max_query_len,
+                       float scale, int32_t split_tokens, const oscar_layout* layout,
+                       float* partials, float* lse, void* stream);
 
 #ifdef __cplusplus
 }

@@ -202,6 +202,21 @@ SIGNATURES = {
         _P, _I64, _P, _P, _I64, _I64, _I32, _F,  # units, capacity, count, slots of tokens, n ...
         POINTER(OscarLayout), _P, _P, _I32, _P, _P, _P,  # layout, partials, lse, fp32, outs, stream
     ],
+    "oscar_rope_append": [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64,  # query, key, value (+ row strides)
+        _I64, _I64, _I64, _P, _P, _I32, _I32, _F,  # n, hq, hk, weights, fp32, unit offset, eps
+        _P, _I64, _I64, _I32, _I32, _I32,  # cos_sin, rows, stride, fp32, rotary dim, interleaved
+        _P, _I64, _I32, _P, _P, _P, _P,  # positions, stride, axis count, axes, counts, q out, k out
+        _P, _P, _P, _P, _I64, _P,  # rk_t, rv_t, q rot, history, bytes, slots
+        POINTER(OscarLayout), POINTER(OscarClip), _P,
+    ],
+    "oscar_read_records": [_P, _I64, _P, _I64, POINTER(OscarLayout), _P, _P, _P],
+    "oscar_history_int4": [
+        _P, _I64, _I64, _I64, _P, _I64,  # query, history
+        _P, _P, _P, _I64, _I64, _P, _P, _P,  # qstarts .. table columns, counts, tasks, count
+        _I64, _I64, _I64, _I32, _I32, _I32, _I32, _F, _I32,  # n hq programs splits bn qt mql scale st
+        POINTER(OscarLayout), _P, _P, _P,  # layout, partials, lse, stream
+    ],
 }
 RESTYPES = {"oscar_noalloc_scratch_bytes": c_int64, "oscar_calibration_workspace_bytes": c_int64,
             "oscar_history_chunk_tiles": c_int64, "oscar_shared_capacity": c_int64}

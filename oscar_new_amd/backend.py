@@ -24,7 +24,7 @@ import os
 import torch
 
 from . import kernels
-from .config import (OscarConfig, attention_programs, choose_chunk_splits, choose_device_partition,
+from .config import (INT4_SLOTS, OscarConfig, attention_programs, choose_chunk_splits, choose_device_partition,
                      choose_history_partition, choose_splits, chunk_kernel_pays,
                      shared_prefix_pays)
 
@@ -246,7 +246,7 @@ class OscarAttentionImpl:
     def _roles_share_history_launch(self, meta):
         """Whether the step's history launch carries the pre-attention role workgroups."""
         layout = getattr(meta, "layout", None)
-        return (self.fused and self.overlap and not self.one_launch_post and not self.layer_step
+        return (self.cfg.history_bits == 2 and self.fused and self.overlap and not self.one_launch_post and not self.layer_step
                 and layout is not None
                 and kernels.history_pre_supported(meta, layout, self.num_heads))
 
@@ -255,7 +255,8 @@ class OscarAttentionImpl:
         branch and the K/V store as units of its own (MTP steps with token-bounded splits; the
         q rotation stays a launch of its own)."""
         layout = getattr(meta, "layout", None)
-        return (self.fused and self.overlap and not self.one_launch_post and not self.layer_step
+        return (self.cfg.history_bits == 2
+                and self.fused and self.overlap and not self.one_launch_post and not self.layer_step
                 and layout is not None and not self.rotate_in_history and not self.q_roles
                 and kernels.history_rows(meta, layout, self.num_heads) > 8
                 and kernels.history_pre_supported(meta, layout, self.num_heads, split_tokens,
@@ -276,6 +277,12 @@ class OscarAttentionImpl:
         if self.split_policy == "reference":
             return choose_splits(meta.num_reqs, self.num_kv_heads, meta.max_query_len), 0
         group = self.num_heads // self.num_kv_heads
+        if self.cfg.history_bits == 4:
+            n = int(meta.num_actual_tokens if tokens is None else tokens)
+            programs = attention_programs(n, meta.max_num_reqs, self.cfg.queries_per_tile)
+            return choose_device_partition(programs, self.num_kv_heads, meta.max_query_len, n,
+                                           self.num_heads, self.cfg.queries_per_tile,
+                                           slots=INT4_SLOTS)
         if meta.max_query_len > 16 and self.cfg.queries_per_tile * group > 8:
             n = int(meta.num_actual_tokens if tokens is None else tokens)
             longest = getattr(meta, "max_seq_len", None)
@@ -351,6 +358,16 @@ class OscarAttentionImpl:
         rows = output.view(n, -1)
         lse = getattr(meta, "merged_lse", None)
         layout = meta.layout
+        if layout.config.history_bits != self.cfg.history_bits:
+            raise ValueError(f"the layer keeps {self.cfg.history_bits}-bit records, the cache layout "
+                             f"{layout.config.history_bits}-bit ones")
+        if self.cfg.history_bits == 4:
+            # One launch for the rotated queries and the records of the step's tokens.
+            qrot = kernels.rope_append(
+                None if getattr(meta, "initial_prefill", False) else q, k, v, self.history,
+                meta.slot_mapping, meta.counts, layout, self.rk_t, self.rv_t)[2]
+            self._appended_step(q, k, v, qrot, meta, rows, lse)
+            return output
         if getattr(meta, "initial_prefill", False):
             # Every request starts here: INT2 store of all tokens, causal attention over each
             # request's own tokens (the reference's fused-infer call), then the windows.
@@ -365,6 +382,50 @@ class OscarAttentionImpl:
         else:
             self._single_launch_step(q, k, v, meta, splits, split_tokens, rows, lse)
         return output
+
+    def forward_appended(self, query, key, value, query_rot, kv_cache, attn_metadata, output):
+        """The rest of a layer step behind ``kernels.rope_append``, which has turned the queries and
+        keys, rotated the queries (not needed by an initial prefill) and written the step's records:
+        both attention branches, their merge and the windows. ``query`` and ``query_rot``
+        [n, heads, 256], ``key`` and ``value`` [n, kv_heads, 256]; returns ``output``
+        (contiguous, [n, heads * 256])."""
+        meta, n = attn_metadata, query.shape[0]
+        if self.rv is None:
+            raise RuntimeError("this OSCAR layer has no rotations: initialize_layer runs after "
+                               "weight loading")
+        if query.shape != (n, self.num_heads, 256) or any(
+                t.shape != (n, self.num_kv_heads, 256) for t in (key, value)):
+            raise ValueError("query, key and value must be [n, heads, 256] of the same tokens")
+        initial = getattr(meta, "initial_prefill", False)
+        if not initial and (query_rot is None or query_rot.shape != query.shape):
+            raise ValueError("a step with a history takes the queries rotated by R_k")
+        if meta.layout.config.history_bits != self.cfg.history_bits:
+            raise ValueError(f"the layer keeps {self.cfg.history_bits}-bit records, the cache layout "
+                             f"{meta.layout.config.history_bits}-bit ones")
+        if not output.is_contiguous():
+            raise ValueError("the attention output must be contiguous")
+        self._bind_cache(kv_cache, meta.layout)
+        if n:
+            self._appended_step(query, key, value, query_rot, meta, output.view(n, -1),
+                                getattr(meta, "merged_lse", None))
+        return output
+
+    def _appended_step(self, q, k, v, qrot, meta, rows, lse):
+        """Both branches and the merge of a step whose records are written."""
+        layout = meta.layout
+        if getattr(meta, "initial_prefill", False):
+            kernels.prefill_attention(q, k, v, self.window, meta, layout, self.scale, rows, lse)
+            kernels.store_windows(k, v, self.window, meta, layout)
+            return
+        splits, split_tokens = self.partition_for(meta, q.shape[0])
+        if kernels.chunk_raw_preferred(meta):
+            rp, rl = kernels.chunk_raw_attention(q, k, v, self.window, meta, layout, self.scale)
+        else:
+            rp, rl = kernels.attention_partials(q, k, v, self.history, self.window, meta, layout,
+                                                self.scale, 1, raw=True)
+        hp, hl = kernels.attention_partials(qrot, k, v, self.history, self.window, meta, layout,
+                                            self.scale, splits, raw=False, split_tokens=split_tokens)
+        kernels.post_attention(hp, hl, rp, rl, self.rv, k, v, self.window, meta, layout, rows, lse)
 
     def _takes_shared(self, meta, tokens):
         """Whether a fused step computes shared prefixes by the plan that the step has."""

@@ -38,6 +38,7 @@ class OscarConfig:
     v_rotation_path: str = ""
     block_n: int = 32
     queries_per_tile: int = 4
+    history_bits: int = 2  # per code of a history record: 2 (the reference's), or 4
 
     def __post_init__(self):
         for ok, message in _config_rules(self):
@@ -46,8 +47,8 @@ class OscarConfig:
 
     @property
     def data_bytes(self):
-        """Packed code bytes per vector: four 2-bit codes per byte."""
-        return self.head_dim // 4
+        """Packed code bytes per vector: four 2-bit or two 4-bit codes per byte."""
+        return self.head_dim * self.history_bits // 8
 
     @property
     def vector_bytes(self):
@@ -56,8 +57,10 @@ class OscarConfig:
 
     @property
     def slot_bytes(self):
-        """K and V vectors of one token-head, rounded up to a 32-byte multiple (160)."""
-        return ((2 * self.vector_bytes + 31) // 32) * 32
+        """K and V vectors of one token-head, rounded up to a 32-byte multiple (160). 4-bit records
+        are rounded to 16 bytes (272): their pieces are copied 16 bytes at a time."""
+        unit = 32 if self.history_bits == 2 else 16
+        return -(-2 * self.vector_bytes // unit) * unit
 
     @property
     def ring_tokens(self):
@@ -69,14 +72,19 @@ class OscarConfig:
 
     @classmethod
     def from_env(cls, speculative_tokens=3):
-        """Reference: config.py:65-81 (same variable names and defaults)."""
+        """Reference: config.py:65-81 (same variable names and defaults). ``OSCAR_AMD_HISTORY_BITS=4``
+        keeps the history in 4-bit records, which want less clipping: then the percentiles default to
+        0.99 (mean squared error of Gaussian rows 0.0110 of their own, at 0.96 0.0159)."""
+        bits = int(os.getenv("OSCAR_AMD_HISTORY_BITS", "2"))
+        k_ratio, v_ratio = ("0.96", "0.92") if bits == 2 else ("0.99", "0.99")
         return cls(
+            history_bits=bits,
             group_size=int(os.getenv("VLLM_OSCAR_GROUP_SIZE", "256")),
             sink_tokens=int(os.getenv("VLLM_OSCAR_SINK_TOKENS", "64")),
             recent_tokens=int(os.getenv("VLLM_OSCAR_RECENT_TOKENS", "256")),
             speculative_tokens=speculative_tokens,
-            k_clip_ratio=float(os.getenv("VLLM_OSCAR_K_CLIP_RATIO", "0.96")),
-            v_clip_ratio=float(os.getenv("VLLM_OSCAR_V_CLIP_RATIO", "0.92")),
+            k_clip_ratio=float(os.getenv("VLLM_OSCAR_K_CLIP_RATIO", k_ratio)),
+            v_clip_ratio=float(os.getenv("VLLM_OSCAR_V_CLIP_RATIO", v_ratio)),
             clip_mode=os.getenv("OSCAR_ASCEND_CLIP_MODE", "percentile"),
             k_clip_factor=float(os.getenv("OSCAR_ASCEND_K_CLIP_FACTOR", "1")),
             v_clip_factor=float(os.getenv("OSCAR_ASCEND_V_CLIP_FACTOR", "1")),
@@ -106,6 +114,7 @@ def _config_rules(cfg):
          "clip factors must lie in (0, 1]"),
         (cfg.block_n in (16, 32), "OSCAR_ASCEND_BLOCK_N must be 16 or 32"),
         (cfg.queries_per_tile in (1, 2, 4), "OSCAR_ASCEND_QUERY_TILE must be 1, 2 or 4"),
+        (cfg.history_bits in (2, 4), "history records hold 2-bit or 4-bit codes"),
     )
 
 
@@ -186,6 +195,8 @@ def choose_history_partition(num_tasks, num_kv_heads, max_query_len, max_seq_len
 # per CU, which measured best on the ragged MTP batch.
 HISTORY_SLOTS = 512
 QUEUE_SLOTS = 448
+# Of the 4-bit history kernel: one workgroup per CU.
+INT4_SLOTS = 256
 # Bytes of split scratch one split slot costs per query row (fp32 partial row + LSE).
 SPLIT_ROW_BYTES = 256 * 4 + 4
 
@@ -207,7 +218,7 @@ def device_split_tokens(history_total, tasks, num_kv_heads, budget, fit_grid=Tru
 
 def choose_device_partition(programs, num_kv_heads, max_query_len, tokens, q_heads,
                             queries_per_tile=4, reserved=0, max_splits=128,
-                            scratch_bytes=128 << 20):
+                            scratch_bytes=128 << 20, slots=None):
     """``(splits, split_tokens)`` of the device rule (no reference counterpart).
 
     Everything here is known when a graph is captured: the grid capacity ``programs``, the
@@ -224,12 +235,14 @@ def choose_device_partition(programs, num_kv_heads, max_query_len, tokens, q_hea
     takes a large share) it is bounded by ``scratch_bytes`` of split rows. A request that
     would need more splits gets longer ones. Steps with more than 16 query tokens in some request
     keep one split (config.py:86-87); above 8 rows per task their caller asks
-    ``choose_chunk_splits`` instead.
+    ``choose_chunk_splits`` instead. ``slots``: the launch's workgroup slots where they are not those of
+    the 2-bit kernels (``INT4_SLOTS``).
     """
     if max_query_len > 16:
         return 1, 0
     rows = min(max(int(max_query_len), 1), queries_per_tile) * (q_heads // num_kv_heads)
-    slots = QUEUE_SLOTS if rows > 16 else HISTORY_SLOTS
+    if slots is None:
+        slots = QUEUE_SLOTS if rows > 16 else HISTORY_SLOTS
     budget = max(1, slots - int(reserved))
     if rows > 16:
         per_split = max(1, int(tokens) * q_heads * SPLIT_ROW_BYTES)

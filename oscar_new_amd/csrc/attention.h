@@ -343,8 +343,8 @@ __device__ __forceinline__ void write_unused_splits(const AttnArgs& a, const Tas
 hipError_t launch_history(const AttnArgs& a, dim3 grid, int rows, hipStream_t stream,
                           int32_t* queue = nullptr);
 
-// The checks and fields of one attention_partials launch (attention.hip): OSCAR_OK with *out
-// filled and *qrows = query rows per task, or the entry point's error code. Nothing is
+// The checks and fields of one attention_partials launch (attention.hip) over records of `bits` bits
+// (history branch): OSCAR_OK with *out filled and *qrows = query rows per task, or the entry point's error code. Nothing is
 // launched when n == 0 (OSCAR_OK before the pointer checks).
 int make_attn_args(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_s2, const void* key,
                    int64_t k_s0, int64_t k_s1, int64_t k_s2, const void* value, int64_t v_s0,
@@ -355,6 +355,6 @@ int make_attn_args(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_s2, 
                    const int32_t* task_count, int64_t n, int64_t hq, int64_t programs,
                    int32_t splits, int32_t block_n, int32_t query_tile, int32_t max_query_len,
                    float scale, int32_t raw, int32_t split_tokens, const oscar_layout* layout,
-                   float* partials, float* lse, AttnArgs* out, int64_t* qrows);
+                   float* partials, float* lse, AttnArgs* out, int64_t* qrows, int32_t bits = 2);
 
 }  // namespace oscar

@@ -33,11 +33,13 @@ int make_attn_args(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_s2, 
                    const int32_t* task_count, int64_t n, int64_t hq, int64_t programs,
                    int32_t splits, int32_t block_n, int32_t query_tile, int32_t max_query_len,
                    float scale, int32_t raw, int32_t split_tokens, const oscar_layout* layout,
-                   float* partials, float* lse, AttnArgs* out, int64_t* qrows_out) {
+                   float* partials, float* lse, AttnArgs* out, int64_t* qrows_out, int32_t bits) {
   AttnArgs& a = *out;
   a = AttnArgs{};
-  const int st = make_layout(layout, &a.L);
+  // The BF16 branch reads no records; each history kernel those of its own width.
+  const int st = make_any_layout(layout, &a.L);
   if (st != OSCAR_OK) return st;
+  if (!raw && a.L.bits != bits) return OSCAR_E_LAYOUT;
   const int64_t h = a.L.kv_heads;
   if (n < 0 || hq <= 0 || hq % h || programs < 1 || splits < 1 || splits > 65535 ||
       block_n < 1 || query_tile < 1 || table_columns < 0 || programs > (1ll << 31) - 1)
@@ -63,10 +65,11 @@ int make_attn_args(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_s2, 
   } else {
     if (!history) return OSCAR_E_NULL;
     if (!aligned16(history)) return OSCAR_E_ALIGN;
-    // The history kernel streams 64-token chunks that never straddle a kernel block, and
-    // its masked (unmapped-block) chunks read the first 64 records of the buffer.
-    if (a.L.bk < 64) return OSCAR_E_UNSUPPORTED;
-    if (history_bytes < 64 * h * 160) return OSCAR_E_SHAPE;
+    // The history kernel streams chunks of 64 tokens (4-bit records: 32) that never straddle a kernel
+    // block, and its masked (unmapped-block) chunks read the first records of the buffer.
+    const int chunk = bits == 4 ? 32 : 64;
+    if (a.L.bk < chunk) return OSCAR_E_UNSUPPORTED;
+    if (history_bytes < chunk * h * a.L.slot_bytes) return OSCAR_E_SHAPE;
     if (!(scale > 0.f) || !(scale < INFINITY)) return OSCAR_E_UNSUPPORTED;
   }
   a.query = static_cast<const uint16_t*>(query);

@@ -186,6 +186,7 @@ struct Layout {
   int64_t page_bytes;  // stripe_page_bytes
   int32_t head_dim, kv_heads, bp, bk, bk_shift, bpp;
   int32_t slot_bytes, vector_bytes, sink, recent, ring;
+  int32_t bits;  // of a history code: 2 or 4
   FastDiv bpp_div;
   FastDiv ring_div;
   FastDiv bp_div;  // division by bp (slot -> page)
@@ -202,8 +203,10 @@ __device__ __forceinline__ int64_t slot_offset(const Layout& L, int64_t slot, in
   return page * L.page_bytes + (within * L.kv_heads + head) * L.slot_bytes;
 }
 
-// Returns OSCAR_OK or an argument error code.
+// Returns OSCAR_OK or an argument error code. make_layout takes layouts of 2-bit records, which most
+// kernels decode; make_any_layout those of 4-bit records too (kernels that copy records or read none).
 int make_layout(const oscar_layout* in, Layout* out);
+int make_any_layout(const oscar_layout* in, Layout* out);
 
 hipStream_t as_stream(void* s);
 

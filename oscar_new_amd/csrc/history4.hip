@@ -1,0 +1,515 @@
+// Attention of a step's tasks over the 4-bit history (the history branch of a layer whose cache holds
+// 4-bit records): per (task, KV head, split)
+//
+//   out[row] = sum_p e^{s_p} v_p / sum_p e^{s_p},  s_p = scale q . k_p,  k_p = z + s c  (record4.h)
+//
+// over the split's share of the positions [sink_len, recent_begin), with the rows' LSEs, for the split
+// merges of merge.h. The task table, splits and masks are those of history.hip; the reference has 2-bit
+// records only (oscar_ascend/kernels.py:290-482).
+//
+// Scale and zero fold out of the products: q . k = s (q . c) + z sum q, and sum p v = sum (p s) (c - 7.5)
+// + sum p (z + 7.5 s), in which the rounding of p s to bf16 weighs values of either sign: the products run
+// over c, and one more against ones gives the sum of the rounded p s. Codes and queries are exact in bf16.
+//
+// A workgroup of eight wavefronts, one per CU, takes up to 32 query rows. Wavefront w streams chunks of
+// 32 positions w, w + 8, ... of the split through an LDS ring of its own (direct-to-LDS copies, no barrier
+// in the loop); scores are computed transposed (positions by rows), so that a lane holds one row's
+// scores of eight positions and its probabilities are the P operand of the second product, whose other
+// operand comes from transposed LDS reads of 4-bit codes. The eight states are joined at the end.
+#include "dma.h"
+#include "history4.h"
+
+namespace oscar {
+namespace {
+
+constexpr int kChunk4 = 32;
+constexpr int kPieces4 = kSlot4 / 16;               // 17 pieces of a record
+constexpr int kStage4 = kChunk4 * kSlot4;           // 8704 bytes
+constexpr int kDma4 = (kChunk4 * kPieces4 + 63) / 64;  // 9 copies of a chunk, the last of 32 lanes
+constexpr int kTable4 = 512;                        // kernel blocks whose offsets live in LDS
+constexpr float kTheta4 = 8.0f;                     // slack of the running maximum, log2 units
+constexpr int kMaxTasks4 = 16384;                   // task rows of the device rule
+
+// A workgroup's form: RG groups of 16 query rows, W wavefronts with S ring stages each.
+template <int kRowGroups, int kWavesW, int kStagesS>
+struct Form4 {
+  static constexpr int RG = kRowGroups, W = kWavesW, S = kStagesS, kThreads = W * kWave;
+  struct Lds {
+    uint8_t ring[W][S][kStage4] __attribute__((aligned(16)));
+    uint8_t q[RG * 16 * kHeadDim * 2] __attribute__((aligned(16)));
+    uint32_t off[kTable4];
+    float red[4][W][16 * RG];  // per wavefront: row max, sum p, sum p (z + 7.5 s), sum of P
+  };
+  static_assert(W * 16 * kHeadDim * 4 <= sizeof(Lds::ring), "a row group's merge fits the ring");
+};
+
+// Waits until at most `chunks` chunks' copies are in flight.
+__device__ __forceinline__ void wait_chunks(int chunks) {
+  if (chunks >= 3)
+    OSCAR_WAIT_VM(3 * kDma4);
+  else if (chunks == 2)
+    OSCAR_WAIT_VM(2 * kDma4);
+  else if (chunks == 1)
+    OSCAR_WAIT_VM(kDma4);
+  else
+    OSCAR_WAIT_VM(0);
+}
+
+// The unit of workgroup slot u under the device rule: split lengths T such that the tasks' splits,
+// ceil(length / T) each, fit the budget's slots of one KV head (or one a task where it is smaller).
+// All splits run at once, one per CU, so the launch takes as long as T: eight lengths between the mean
+// share and the one that always fits are tried, one by each wavefront, and the least that fits is
+// taken (32 requests of 32704 positions on 256 slots: 8 splits of 4096 each). Multiples of kStep4, at
+// least kMinSplit4.
+constexpr int kMinSplit4 = 512, kStep4 = 64, kTried4 = 8;
+
+struct Unit4 {
+  Task t;
+  int split, nsplit, split_tokens;
+};
+
+template <int W>
+__device__ bool unit_of_slot(const AttnArgs& a, int programs, int u, int* lengths, Unit4& out) {
+  constexpr int kThreads4 = W * kWave;
+  __shared__ int64_t s_total[W];
+  __shared__ int s_fit[kTried4], s_carry[W], s_found[3];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t sum = 0;
+  for (int i = tid; i < programs; i += kThreads4) {
+    Task t;
+    const bool live = read_task(a, t, i);
+    const int len = live ? max(t.recent_begin - t.sink_len, 0) : -1;
+    lengths[i] = len;
+    sum += max(len, 0);
+  }
+  sum = wave_sum_i64(sum);
+  if (lane == 0) s_total[wave] = sum;
+  if (tid == 0) s_found[0] = -1;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) total += s_total[w];
+  const int count = max(min(a.task_count[0], programs), 0);
+  const int slots = max(-a.split_tokens / a.L.kv_heads, 1);
+  auto rounded = [](uint32_t per) {
+    return static_cast<int>(min(max((per + kStep4 - 1) / kStep4 * kStep4, uint32_t{kMinSplit4}),
+                                uint32_t{1} << 30));
+  };
+  // A 32-bit division where the batch allows it (its tokens are below 2^32 in all but absurd ones).
+  auto share = [&](uint32_t by) {
+    const uint64_t per = total >> 32 ? static_cast<uint64_t>(total) / by
+                                     : static_cast<uint32_t>(total) / by;
+    return static_cast<uint32_t>(min(per, uint64_t{1} << 30)) + 1;
+  };
+  const int least = rounded(share(slots));
+  const int most = rounded(share(max(slots - count, 1)));
+  auto tried = [&](int w) {
+    return w == kTried4 - 1 ? most : rounded(least + (most - least) / (kTried4 - 1) * w);
+  };
+  for (int k = wave; k < kTried4; k += W) {
+    const int t = tried(k);
+    int units = 0;
+    for (int i = lane; i < count; i += kWave) units += history_splits(a, max(lengths[i], 0), t);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) units += __shfl_xor(units, m, kWave);
+    if (lane == 0) s_fit[k] = units <= slots;
+  }
+  __syncthreads();
+  int st = most;
+#pragma unroll
+  for (int k = kTried4 - 1; k >= 0; --k)
+    if (s_fit[k]) st = tried(k);
+  // Exclusive scan of the split counts; the thread whose task holds slot u says so.
+  int carry = 0;
+  for (int c0 = 0; c0 < programs; c0 += kThreads4) {
+    const int i = c0 + tid;
+    const int ns = i < count && lengths[i] >= 0 ? history_splits(a, lengths[i], st) : 0;
+    int incl = ns;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int y = __shfl_up(incl, d, kWave);
+      incl += lane >= d ? y : 0;
+    }
+    if (lane == kWave - 1) s_carry[wave] = incl;
+    __syncthreads();
+    int before = carry, chunk = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      before += w < wave ? s_carry[w] : 0;
+      chunk += s_carry[w];
+    }
+    const int base = before + incl - ns;
+    if (ns > 0 && u >= base && u < base + ns) {
+      s_found[0] = i;
+      s_found[1] = u - base;
+      s_found[2] = ns;
+    }
+    carry += chunk;
+    __syncthreads();  // s_carry is read before the next round writes it
+  }
+  const int task = uniform(s_found[0]);
+  if (task < 0) return false;
+  out.split = uniform(s_found[1]);
+  out.nsplit = uniform(s_found[2]);
+  out.split_tokens = st;
+  // Its row again (the loads hit the cache), uniform for the workgroup.
+  Task t;
+  read_task(a, t, task);
+  out.t.req = uniform(t.req);
+  out.t.qoff = uniform(t.qoff);
+  out.t.qstart = uniform(t.qstart);
+  out.t.qlen = uniform(t.qlen);
+  out.t.prefix = uniform(t.prefix);
+  out.t.sink_len = uniform(t.sink_len);
+  out.t.recent_begin = uniform(t.recent_begin);
+  return true;
+}
+
+__device__ __forceinline__ f32x4 splat(float v) { return f32x4{v, v, v, v}; }
+
+// Rows 16 rg + n (rg < RG) of the task against positions [p_lo, p_hi), partial rows to `split`.
+template <class F>
+__device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, int head, int p_lo,
+                                              int p_hi, int split, typename F::Lds& lds) {
+  constexpr int RG = F::RG, W = F::W, S = F::S;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int first = p_lo / kChunk4;
+  const int nchunk = p_lo < p_hi ? (p_hi - 1) / kChunk4 - first + 1 : 0;
+  const int nmine = nchunk > wave ? (nchunk - wave + W - 1) / W : 0;
+  const int kb_first = p_lo >> a.L.bk_shift;
+  if (nchunk > 0) {
+    const int nkb = min(((p_hi - 1) >> a.L.bk_shift) - kb_first + 1, kTable4);
+    for (int j = tid; j < nkb; j += F::kThreads) lds.off[j] = block_offset4(a, t, head, kb_first + j);
+  }
+  // Query rows as they are, 16-byte piece p of row r at p ^ r % 16, two rows a copy. A row past the task's reads the buffer's first row and is zeroed below.
+  const uint32_t q_area = lds_addr(lds.q);
+#pragma unroll
+  for (int i = 0; i < RG * 8 / W; ++i) {
+    const int row0 = 2 * (i * W + wave), row = row0 + (lane >> 5);
+    const RowInfo ri = row_info(a, t, head, row);
+    const uint16_t* src = a.query + (ri.valid ? ri.token * a.qs0 + ri.qhead * a.qs1 : 0) +
+                          8 * ((lane & 31) ^ (row & 15));
+    dma_dwordx4(src, q_area + row0 * kHeadDim * 2);
+  }
+  barrier_lds();  // the offsets
+
+  // 16-byte piece c = 64 i + lane of a chunk is record c / 17, bytes 16 (c % 17).
+  const uint32_t tok_bytes = static_cast<uint32_t>(a.L.kv_heads) * kSlot4;
+  uint32_t voff[kDma4];
+#pragma unroll
+  for (int i = 0; i < kDma4; ++i) {
+    const int c = 64 * i + lane;
+    voff[i] = static_cast<uint32_t>(c / kPieces4) * tok_bytes + 16 * (c % kPieces4);
+  }
+  const uint32_t my_ring = lds_addr(lds.ring[wave][0]);
+  const uint32_t in_kb_mask = static_cast<uint32_t>(a.L.bk - 1);
+  uint32_t mapped = 0;  // bit s: stage s holds a mapped block's positions
+  auto issue = [&](int j, int s) {
+    const int t0 = (first + wave + W * j) * kChunk4;
+    const int local = (t0 >> a.L.bk_shift) - kb_first;
+    uint32_t off16 = lds.off[min(local, kTable4 - 1)];
+    if (local >= kTable4) off16 = block_offset4(a, t, head, t0 >> a.L.bk_shift);
+    off16 = uniform(off16);
+    const bool ok = off16 != kNoBlock4;  // an unmapped block copies the buffer's first records
+    const uint8_t* base = a.history;
+    if (ok)
+      base += (static_cast<uint64_t>(off16) << 4) + (static_cast<uint32_t>(t0) & in_kb_mask) * tok_bytes;
+    mapped = ok ? (mapped | 1u << s) : (mapped & ~(1u << s));
+    const uint32_t at = my_ring + s * kStage4;
+#pragma unroll
+    for (int i = 0; i < kDma4 - 1; ++i) dma_x4_stream(base, voff[i], at + 1024 * i);
+    if (lane < 32) dma_x4_stream(base, voff[kDma4 - 1], at + 1024 * (kDma4 - 1));
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s)
+    if (s < nmine) issue(s, s);
+  wait_chunks(min(nmine, S - 1));
+  barrier_lds();  // the query rows
+
+  // The rows' values in the order of the unpacked codes, in place.
+#pragma unroll
+  for (int i = 0; i < RG * 16; i += F::kThreads / 32) {
+    const int row = i + (tid >> 5);
+    u32x4* at = reinterpret_cast<u32x4*>(lds.q + row * kHeadDim * 2 + 16 * (tid & 31));
+    *at = row_info(a, t, head, row).valid ? code_order(*at) : u32x4{0u, 0u, 0u, 0u};
+  }
+  barrier_lds();
+  // B operand of k-step m: dims 64 g + 8 m .. + 7 of row n. One row group's stay in registers; two
+  // groups' are read from LDS as they are used (256 registers a lane hold the accumulators and no more).
+  auto q_operand = [&](int i, int m) {
+    return *reinterpret_cast<const u32x4*>(lds.q + (16 * i + n) * kHeadDim * 2 +
+                                           16 * ((8 * g + m) ^ n));
+  };
+  float qs[RG];
+  u32x4 qb[8];
+#pragma unroll
+  for (int i = 0; i < RG; ++i) {
+    float sum = 0.f;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      const u32x4 w = q_operand(i, m);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sum += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xffff0000u);
+      if (RG == 1) qb[m] = w;
+    }
+    qs[i] = sum_xor32(sum_xor16(sum));
+  }
+
+  const int k_off = kSlot4 * n + 32 * g;
+  const int side_off = kSlot4 * 4 * g + kSide4;
+  // Transposed reads: lane i of 16 names the row of position 16 (i / 4 % 2) + 4 g + i % 4, the one of two
+  // neighbouring groups of 16 dims for i < 8 and the other above, so that a lane gets one dim of its own
+  // eight positions in either.
+  const int v_off = kSlot4 * (16 * (n >> 2 & 1) + 4 * g + (n & 3)) + kCodes4 + 8 * (n >> 3);
+  const float fq = a.scale_log2;
+  float m_run[RG], psum[RG], zsum[RG];
+  f32x4 o[RG][16], ones_o[RG];  // o[c]: rows 4 g + v, dim 16 c + n
+#pragma unroll
+  for (int i = 0; i < RG; ++i) {
+    m_run[i] = -INFINITY;
+    psum[i] = zsum[i] = 0.f;
+    ones_o[i] = splat(0.f);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) o[i][c] = splat(0.f);
+  }
+
+  auto process = [&](int j, int s) {
+    const uint8_t* st = lds.ring[wave][s];
+    f32x4 acc[RG][2];
+#pragma unroll
+    for (int i = 0; i < RG; ++i) acc[i][0] = acc[i][1] = splat(0.f);
+    u32x4 kw[2][2];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        kw[tt][h] = *reinterpret_cast<const u32x4*>(st + k_off + 16 * kSlot4 * tt + 16 * h);
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      const u32x4 k0 = codes_bf16(kw[0][m >> 2][m & 3]), k1 = codes_bf16(kw[1][m >> 2][m & 3]);
+#pragma unroll
+      for (int i = 0; i < RG; ++i) {
+        const u32x4 q = RG == 1 ? qb[m] : q_operand(i, m);
+        acc[i][0] = mfma16x16x32(k0, q, acc[i][0]);
+        acc[i][1] = mfma16x16x32(k1, q, acc[i][1]);
+      }
+    }
+    uint2 side[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      side[e] = *reinterpret_cast<const uint2*>(st + side_off + kSlot4 * (16 * (e >> 2) + (e & 3)));
+    // A first or last chunk may be partial, or the block unmapped: positions outside get score -inf and
+    // a zero V scale and zero (their bytes may be NaN patterns).
+    const int t0 = (first + wave + W * j) * kChunk4;
+    const bool ok_block = mapped >> s & 1u;
+    const bool whole = ok_block && t0 >= p_lo && t0 + kChunk4 <= p_hi;
+    u32x4 pa[RG];
+#pragma unroll
+    for (int i = 0; i < RG; ++i) {
+      float r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        r[e] = fmaf(half_lo_to_float(side[e].x), acc[i][e >> 2][e & 3],
+                    half_hi_to_float(side[e].x) * qs[i]);
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int p = t0 + 16 * (e >> 2) + 4 * g + (e & 3);
+          const bool in = ok_block && p >= p_lo && p < p_hi;
+          r[e] = in ? r[e] : -INFINITY;
+          side[e].y = in ? side[e].y : 0u;
+        }
+      }
+      float lm = fmaxf(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])),
+                       fmaxf(fmaxf(r[4], r[5]), fmaxf(r[6], r[7]))) * fq;
+      if (__any(lm > m_run[i] + kTheta4)) {
+        const float mn = fmaxf(m_run[i], max_xor32(max_xor16(lm)));
+        const float alpha = mn == -INFINITY ? 1.0f : exp2f(m_run[i] - mn);
+        m_run[i] = mn;
+        psum[i] *= alpha;
+        zsum[i] *= alpha;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float av = __shfl(alpha, 4 * g + v, kWave);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) o[i][c][v] *= av;
+          ones_o[i][v] *= av;
+        }
+      }
+      const float nm = m_run[i] == -INFINITY ? 0.f : -m_run[i];
+      float pv[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(r[e], fq, nm));
+        const float sv = half_lo_to_float(side[e].y);
+        psum[i] += p;
+        zsum[i] = fmaf(p, fmaf(7.5f, sv, half_hi_to_float(side[e].y)), zsum[i]);
+        pv[e] = p * sv;
+      }
+      // Position e of the lane is nibble e of its transposed reads: the order of codes_bf16.
+      pa[i] = u32x4{pack_bf16x2(pv[0], pv[2]), pack_bf16x2(pv[4], pv[6]), pack_bf16x2(pv[1], pv[3]),
+                    pack_bf16x2(pv[5], pv[7])};
+      constexpr uint32_t kOnes = 0x3f803f80u;  // bf16 1, twice
+      ones_o[i] = mfma16x16x32(pa[i], u32x4{kOnes, kOnes, kOnes, kOnes}, ones_o[i]);
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2_ptr_t)(st + v_off + 16 * c));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u32x4 vf = codes_bf16(static_cast<uint32_t>(w[h]));
+#pragma unroll
+        for (int i = 0; i < RG; ++i) o[i][2 * c + h] = mfma16x16x32(pa[i], vf, o[i][2 * c + h]);
+      }
+    }
+  };
+
+  for (int j = 0, s = 0; j < nmine; ++j) {
+    // The stage that chunk j - 1 was read from (its reads have completed) takes chunk j + S - 1.
+    if (j + S - 1 < nmine) {
+      OSCAR_WAIT_LGKM();
+      issue(j + S - 1, s == 0 ? S - 1 : s - 1);
+    }
+    wait_chunks(min(nmine - 1 - j, S - 1));  // chunk j has landed
+    process(j, s);
+    s = s == S - 1 ? 0 : s + 1;
+  }
+
+  // ---- the wavefronts' states joined, normalized rows and LSEs written.
+#pragma unroll
+  for (int i = 0; i < RG; ++i) {
+    const float ps = sum_xor32(sum_xor16(psum[i])), zs = sum_xor32(sum_xor16(zsum[i]));
+    if (g == 0) {
+      lds.red[0][wave][16 * i + n] = m_run[i];
+      lds.red[1][wave][16 * i + n] = ps;
+      lds.red[2][wave][16 * i + n] = zs;
+    }
+    if (n == 0) *reinterpret_cast<f32x4*>(&lds.red[3][wave][16 * i + 4 * g]) = ones_o[i];
+  }
+  float* s_o = reinterpret_cast<float*>(&lds.ring[0][0][0]);  // [wavefront][16 rows][256]
+#pragma unroll
+  for (int i = 0; i < RG; ++i) {
+    __syncthreads();  // the ring (or the last rows' sums) has been read
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int row = 16 * i + 4 * g + v;
+      float mx = lds.red[0][0][row];
+#pragma unroll
+      for (int w = 1; w < W; ++w) mx = fmaxf(mx, lds.red[0][w][row]);
+      const float mw = lds.red[0][wave][row];
+      const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx);
+      float* dst = s_o + (wave * 16 + 4 * g + v) * kHeadDim + n;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) dst[16 * c] = o[i][c][v] * f;
+    }
+    __syncthreads();
+    // Thread -> row tid / 32, dims 4 (tid % 32) and 128 further on.
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += F::kThreads / 32) {
+    const int row16 = r0 + (tid >> 5), row = 16 * i + row16, d0 = 4 * (tid & 31);
+    const RowInfo ri = row_info(a, t, head, row);
+    if (!ri.valid) continue;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, lds.red[0][w][row]);
+    float den = 0.f, zs = 0.f;
+    f32x4 sum[2] = {};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float mw = lds.red[0][w][row];
+      const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx);
+      den = fmaf(f, lds.red[1][w][row], den);
+      zs = fmaf(f, fmaf(-7.5f, lds.red[3][w][row], lds.red[2][w][row]), zs);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        sum[h] += *reinterpret_cast<const f32x4*>(s_o + (w * 16 + row16) * kHeadDim + d0 + 128 * h);
+    }
+    const float inv = 1.0f / fmaxf(den, 1.0e-30f);
+    const int64_t out_row = (ri.token * a.hq + ri.qhead) * a.splits + split;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = (sum[h][e] + zs) * inv;
+      *reinterpret_cast<f32x4*>(a.partials + out_row * kHeadDim + d0 + 128 * h) = r;
+    }
+    if (d0 == 0) a.lse[out_row] = den == 0.f ? -INFINITY : (mx + log2f(den)) * kLn2;
+    }
+  }
+}
+
+template <class F>
+__global__ __launch_bounds__(F::kThreads) void history4_kernel(const AttnArgs a, int programs) {
+  __shared__ typename F::Lds lds;
+  const int head = blockIdx.y;
+  Task t;
+  int split, nsplit, split_tokens;
+  if (a.split_tokens < 0) {
+    Unit4 unit;
+    const int u = static_cast<int>(blockIdx.z) * programs + static_cast<int>(blockIdx.x);
+    if (!unit_of_slot<F::W>(a, programs, u, reinterpret_cast<int*>(&lds), unit)) return;
+    t = unit.t;
+    split = unit.split;
+    nsplit = unit.nsplit;
+    split_tokens = unit.split_tokens;
+    if (split == 0) write_unused_splits<F::kThreads>(a, t, head, nsplit, a.splits);
+    __syncthreads();  // the lengths have been read
+  } else {
+    if (!read_task(a, t, static_cast<int>(blockIdx.x))) return;
+    split = blockIdx.z;
+    split_tokens = a.split_tokens;
+    nsplit = history_splits(a, t.recent_begin - t.sink_len, split_tokens);
+    if (split >= nsplit) {
+      write_unused_split(a, t, head, split);
+      return;
+    }
+  }
+  int p_lo, p_hi;
+  history_positions(a, t, t.recent_begin - t.sink_len, nsplit, split, split_tokens, p_lo, p_hi);
+  history_rows4<F>(a, t, head, p_lo, p_hi, split, lds);
+}
+
+// One row group: eight wavefronts, two a SIMD, with two stages each. Two groups: four with four, so that
+// a wavefront has the registers for both.
+using OneGroup = Form4<1, 8, 2>;
+using TwoGroups = Form4<2, 4, 4>;
+
+}  // namespace
+}  // namespace oscar
+
+extern "C" int oscar_history_int4(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_s2,
+                                  const void* history, int64_t history_bytes, const int32_t* qstarts,
+                                  const int32_t* seq_lens, const int32_t* block_tables,
+                                  int64_t table_stride, int64_t table_columns, const int32_t* counts,
+                                  const int32_t* tasks, const int32_t* task_count, int64_t n,
+                                  int64_t hq, int64_t programs, int32_t splits, int32_t block_n,
+                                  int32_t query_tile, int32_t max_query_len, float scale,
+                                  int32_t split_tokens, const oscar_layout* layout, float* partials,
+                                  float* lse, void* stream) {
+  using namespace oscar;
+  AttnArgs a;
+  int64_t rows = 0;
+  const int st = make_attn_args(query, q_s0, q_s1, q_s2, nullptr, 0, 0, 1, nullptr, 0, 0, 1, history,
+                                history_bytes, nullptr, 0, qstarts, seq_lens, block_tables,
+                                table_stride, table_columns, counts, tasks, task_count, n, hq, programs,
+                                splits, block_n, query_tile, max_query_len, scale, 0, split_tokens,
+                                layout, partials, lse, &a, &rows, 4);
+  if (st != OSCAR_OK || n == 0) return st;
+  const int64_t z = split_tokens < 0 ? device_unit_slices(programs, a.L.kv_heads, split_tokens) : splits;
+  if (z > 65535 || a.L.kv_heads > 65535) return OSCAR_E_SHAPE;
+  // The lengths of the device rule's task rows lie in the ring.
+  if (split_tokens < 0 && programs > kMaxTasks4) return OSCAR_E_UNSUPPORTED;
+  if (programs * z > 0xffffffffll / OneGroup::kThreads / a.L.kv_heads) return OSCAR_E_SHAPE;
+  const dim3 grid(static_cast<unsigned>(programs), static_cast<unsigned>(a.L.kv_heads),
+                  static_cast<unsigned>(z));
+  hipStream_t s = as_stream(stream);
+  if (rows <= 16)
+    hipLaunchKernelGGL(history4_kernel<OneGroup>, grid, dim3(OneGroup::kThreads), 0, s, a,
+                       static_cast<int>(programs));
+  else
+    hipLaunchKernelGGL(history4_kernel<TwoGroups>, grid, dim3(TwoGroups::kThreads), 0, s, a,
+                       static_cast<int>(programs));
+  return static_cast<int>(hipGetLastError());
+}

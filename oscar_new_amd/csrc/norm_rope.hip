@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "dma.h"
+#include "norm_row.h"
 #include "rotate.h"
 
 namespace oscar {
@@ -52,46 +53,6 @@ struct NormRopeArgs {
   const uint16_t* rk_t;  // R_k^T [256][256]
   uint16_t* q_rot;
 };
-
-__device__ __forceinline__ float load_value(const void* p, int64_t i, int fp32) {
-  return fp32 ? static_cast<const float*>(p)[i]
-              : bf16_to_float(static_cast<const uint16_t*>(p)[i]);
-}
-// Eight consecutive values (16-byte aligned bf16, or fp32).
-__device__ __forceinline__ void load_eight(const void* p, int64_t i, int fp32, float (&v)[8]) {
-  if (fp32) {
-    const f32x4* s = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
-    const f32x4 lo = s[0], hi = s[1];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = lo[e];
-      v[4 + e] = hi[e];
-    }
-  } else {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + i);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[2 * e] = bf16_to_float(w[e] & 0xffffu);
-      v[2 * e + 1] = bf16_to_float(w[e] >> 16);
-    }
-  }
-}
-__device__ __forceinline__ void unpack_eight(u32x4 w, float (&v)[8]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[2 * e] = bf16_to_float(w[e] & 0xffffu);
-    v[2 * e + 1] = bf16_to_float(w[e] >> 16);
-  }
-}
-
-// Eight packed values times a power of two (rounded where that leaves bf16's range).
-__device__ __forceinline__ u32x4 scale_eight(u32x4 w, float by) {
-  float v[8];
-  unpack_eight(w, v);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(v[2 * e] * by, v[2 * e + 1] * by);
-  return w;
-}
 
 // Partner of dim d, the index of its angle and the sign of the partner's term.
 __device__ __forceinline__ void pair_of(const NormRopeArgs& a, int d, int& pair, int& angle,
@@ -239,20 +200,6 @@ __device__ __forceinline__ void load_row(const NormRopeArgs& a, const uint16_t* 
                              : (r.pair[e >> 1] & 0xffff0000u) | bits;
     }
   }
-}
-
-// What a row is multiplied by ahead of its norm: a power of two where fp32 does not hold its squares or
-// their mean with eps (magnitudes above 1e18, which would give zeros; below 4e-15 with as small an eps,
-// infinities), else 1. The scaled mean lies in [2^-114, 2^120], whatever the finite bf16 row.
-__device__ __forceinline__ float range_scale(float mean) {
-  return mean == INFINITY ? 0x1p-72f : mean < 0x1p-96f ? 0x1p80f : 1.f;
-}
-
-// 1 / sqrt(mean), NaN for a bad row: the hardware's reciprocal root (within one unit of the last
-// place), whose argument may not be subnormal.
-__device__ __forceinline__ float inverse_root(float mean, bool bad) {
-  const float inv = __builtin_amdgcn_rsqf(mean);
-  return bad ? __uint_as_float(0x7fc00000u) : inv;
 }
 
 // The row's 8 dims of this lane as bf16: zeros past the live tokens, NaN at a position outside the

@@ -338,7 +338,7 @@ __global__ __launch_bounds__(kThreads) void compact_move_kernel(const CompactArg
 
 int make_pool(const void* stripes, int64_t layers, int64_t num_pages, const oscar_layout* layout,
               PoolArgs* out) {
-  const int st = make_layout(layout, &out->L);
+  const int st = make_any_layout(layout, &out->L);
   if (st != OSCAR_OK) return st;
   if (layers <= 0 || layers > 65535 || num_pages <= 0) return OSCAR_E_SHAPE;
   if (num_pages > 0x7fffffffll / out->L.bpp) return OSCAR_E_SHAPE;
@@ -374,7 +374,7 @@ extern "C" int oscar_free_pages(int64_t num_pages, const int32_t* table, int64_t
                                 int32_t* pages, int32_t* count, void* stream) {
   using namespace oscar;
   Layout L;
-  int st = make_layout(layout, &L);
+  int st = make_any_layout(layout, &L);
   if (st != OSCAR_OK) return st;
   if (num_pages <= 0 || num_pages > 0x7fffffffll / L.bpp) return OSCAR_E_SHAPE;
   TableArgs t;

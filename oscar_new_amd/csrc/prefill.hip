@@ -476,7 +476,7 @@ extern "C" int oscar_prefill_attention(
     float* merged_lse, void* stream) {
   using namespace oscar;
   Layout L;
-  const int st = make_layout(layout, &L);
+  const int st = make_any_layout(layout, &L);
   if (st != OSCAR_OK) return st;
   const int64_t h = L.kv_heads;
   if (n < 0 || hq <= 0 || hq % h || max_reqs < 1 || max_reqs > 65535 || max_query_len < 0 ||
@@ -541,7 +541,7 @@ extern "C" int oscar_chunk_raw_attention(
     float* raw_partials, float* raw_lse, void* stream) {
   using namespace oscar;
   PrefillArgs a{};
-  const int st = make_layout(layout, &a.L);
+  const int st = make_any_layout(layout, &a.L);
   if (st != OSCAR_OK) return st;
   const int64_t h = a.L.kv_heads;
   if (n < 0 || hq <= 0 || hq % h || max_reqs < 1 || max_reqs > 65535 || max_query_len < 0 ||

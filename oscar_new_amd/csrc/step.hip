@@ -426,7 +426,7 @@ int make_post_args(const float* history_partials, const float* history_lse, int3
                    int64_t max_reqs, const oscar_layout* layout, PostArgs* out) {
   PostArgs& p = *out;
   p = PostArgs{};
-  const int st = make_layout(layout, &p.win.L);
+  const int st = make_any_layout(layout, &p.win.L);
   if (st != OSCAR_OK) return st;
   if (n < 0 || hq <= 0 || hq % p.win.L.kv_heads || splits < 1 || max_reqs < 0 ||
       window_elems < 0 || n * hq > 0x7fffffffll)

@@ -27,7 +27,7 @@ extern "C" int oscar_store_windows(const void* key, int64_t k_s0, int64_t k_s1, 
   using namespace oscar;
   if (n < 0 || max_reqs < 0 || window_elems < 0) return OSCAR_E_SHAPE;
   WindowArgs a{};
-  const int st = make_layout(layout, &a.L);
+  const int st = make_any_layout(layout, &a.L);
   if (st != OSCAR_OK) return st;
   const int64_t programs = n < max_reqs ? n : max_reqs;
   if (programs == 0) return OSCAR_OK;

@@ -28,6 +28,9 @@ __all__ = [
     "store_windows",
     "dequant_inverse_rotate",
     "qk_norm_rope",
+    "rope_append",
+    "rope_axes",
+    "read_records",
     "prepare_shared",
     "shared_history",
     "pre_attention",
@@ -270,11 +273,17 @@ def attention_partials(query, key, value, history, window, meta, layout, scale, 
     ``chunk`` (history branch under the reference split rule; no reference counterpart): the
     128-row-tile kernel of continuation chunks, within rounding of the others; by default where
     the metadata's host-side lengths say that it pays (``config.chunk_kernel_pays``).
+
+    With a layout of 4-bit records (``OscarConfig(history_bits=4)``) the history branch reads those,
+    under the same split rules; ``use_queue`` and ``chunk`` choose among the kernels of 2-bit records
+    and are ignored.
     """
     if raw and split_tokens:
         raise ValueError("split_tokens applies to the history branch only")
     if chunk and (raw or split_tokens):
         raise ValueError("chunk applies to the history branch under the reference split rule")
+    if not raw and layout.config.history_bits == 4:
+        return _attention_int4(query, history, meta, layout, scale, splits, split_tokens)
     _device_check(query, key, value, history, window)
     n, hq, d = query.shape
     cfg = layout.config
@@ -330,6 +339,46 @@ def attention_partials(query, key, value, history, window, meta, layout, scale, 
             _stream(query),
         ),
         "attention_partials",
+    )
+    return partials, lse
+
+
+def _attention_int4(query, history, meta, layout, scale, splits, split_tokens):
+    """The history branch of ``attention_partials`` over 4-bit records."""
+    table = _int32(meta.block_tables, "block_tables")
+    qstarts = _int32(meta.query_start_loc, "query_start_loc")
+    seq_lens, counts = _int32(meta.seq_lens, "seq_lens"), _int32(meta.counts, "counts")
+    tasks, task_count = _int32(meta.tasks, "tasks"), _int32(meta.task_count, "task_count")
+    device = _same_device(query, history=history, block_tables=table, query_start_loc=qstarts,
+                          seq_lens=seq_lens, counts=counts, tasks=tasks, task_count=task_count)
+    n, hq, d = query.shape
+    if d != 256:
+        raise ValueError(f"the query must be [n, heads, 256], got {tuple(query.shape)}")
+    if hq % layout.kv_heads:
+        raise ValueError("the query head count must be a multiple of the KV head count")
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("block_tables must have contiguous rows")
+    if history.dtype != torch.uint8 or not history.is_contiguous():
+        raise ValueError("history must be the contiguous bytes of the K stripe")
+    if splits < 1:
+        raise ValueError(f"a launch has at least one split, got {splits}")
+    lse = torch.empty((n, hq, splits), dtype=torch.float32, device=device)
+    partials = lse.new_empty((n, hq, splits, d))
+    if n == 0:
+        return partials, lse
+    cfg = layout.config
+    programs = attention_programs(n, meta.max_num_reqs, cfg.queries_per_tile)
+    if tasks.shape[0] < programs:
+        raise ValueError(f"task table holds {tasks.shape[0]} rows; the grid needs {programs}")
+    query, s0, s1 = _rows_aligned(query)
+    longest = getattr(meta, "max_query_len", None)
+    _launch(
+        _ext.library().oscar_history_int4, "attention_partials", device, query.data_ptr(), s0, s1, 1,
+        history.data_ptr(), history.numel(), qstarts.data_ptr(), seq_lens.data_ptr(),
+        table.data_ptr(), table.stride(0), table.shape[1], counts.data_ptr(), tasks.data_ptr(),
+        task_count.data_ptr(), n, hq, programs, splits, cfg.block_n, cfg.queries_per_tile,
+        longest if isinstance(longest, int) else 0, scale, int(split_tokens), layout_struct(layout),
+        partials.data_ptr(), lse.data_ptr(),
     )
     return partials, lse
 
@@ -402,6 +451,9 @@ def dequant_inverse_rotate(history, slots, rk, rv, layout):
     n, h, d = slots.numel(), layout.kv_heads, layout.config.head_dim
     if n > 4096:
         raise ValueError("Diagnostic dequant is limited to 4096 tokens; use fused attention")
+    if layout.config.history_bits == 4:
+        k, v = read_records(history, slots, layout)
+        return rotate(k, rk.T), rotate(v, rv.T)
     k = torch.empty((n, h, d), device=history.device, dtype=torch.bfloat16)
     v = torch.empty_like(k)
     if n:
@@ -485,7 +537,7 @@ def _rows_out(like):
 
 
 def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None, eps=1e-6,
-                 unit_offset=False, interleaved=False, rk_t=None):
+                 unit_offset=False, interleaved=False, rk_t=None, axes=None):
     """Norms of the queries and keys of each head with the position rotation in the same pass (no
     reference counterpart; what a model computes ahead of backend.py:125-140).
 
@@ -500,7 +552,19 @@ def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None
 
     Returns ``(query, key)``, contiguous bf16; with ``rk_t`` (R_k^T, contiguous bf16 [256, 256])
     ``(query, key, rotate(query, R_k))``, the third with the bits of ``rotate``.
+
+    ``axes`` (int32 [rotary / 2] on the device, ``rope_axes``): tokens have several positions (time,
+    height and width of images and video), ``positions`` is int64 [axes, n], and pair j takes its
+    angle from row ``positions[axes[j]][token]``. A pair whose axis is none of them turns to NaN.
     """
+    if axes is not None:
+        if q_weight is None or k_weight is None:
+            raise ValueError("qk_norm_rope takes the weights of both norms")
+        query, key, turned = rope_append(
+            query, key, None, None, None, counts, None, rk_t, None, cos_sin=cos_sin,
+            positions=positions, axes=axes, q_weight=q_weight, k_weight=k_weight, eps=eps,
+            unit_offset=unit_offset, interleaved=interleaved, rotate_query=rk_t is not None)
+        return (query, key) if rk_t is None else (query, key, turned)
     device = _same_device(query, key=key, q_weight=q_weight, k_weight=k_weight, cos_sin=cos_sin,
                           positions=positions, counts=counts, rk_t=rk_t)
     n, hq, d = query.shape
@@ -540,6 +604,167 @@ def qk_norm_rope(query, key, q_weight, k_weight, cos_sin, positions, counts=None
             k_out.data_ptr(), _ptr(rk_t), _ptr(q_rot),
         )
     return (q_out, k_out) if q_rot is None else (q_out, k_out, q_rot)
+
+
+def rope_axes(sections, interleaved=False, device=None):
+    """The axis of every pair, for ``qk_norm_rope`` and ``rope_append``: ``sections`` holds the pairs of
+    each axis (time first), which sum to half the rotary dims. Sections lie one after the other; with
+    ``interleaved`` the axes take turns (0 1 2 0 1 2 ...) while their sections last, and axis 0 has the
+    pairs that are left. Returns int32 [sum(sections)]."""
+    sections = [int(c) for c in sections]
+    if not sections or min(sections) < 0:
+        raise ValueError(f"sections must be counts of pairs, got {sections}")
+    if interleaved:
+        order, turn = [0] * sum(sections), len(sections)
+        for axis, count in enumerate(sections[1:], 1):
+            if count and axis + (count - 1) * turn >= len(order):
+                raise ValueError(f"axis {axis} has too many pairs to take turns, got {sections}")
+            order[axis : axis + count * turn : turn] = [axis] * count
+    else:
+        order = [axis for axis, count in enumerate(sections) for _ in range(count)]
+    return torch.tensor(order, dtype=torch.int32, device=device)
+
+
+def _rotation_check(r, name):
+    if r.dtype != torch.bfloat16 or not r.is_contiguous() or r.shape != (256, 256):
+        raise ValueError(f"{name} must be contiguous bf16 [256, 256] (R transposed)")
+
+
+def rope_append(query, key, value, history, slots, counts, layout, rk_t, rv_t, cos_sin=None,
+                positions=None, axes=None, q_weight=None, k_weight=None, eps=1e-6,
+                unit_offset=False, interleaved=False, rotate_query=True):
+    """Keys and values into the paged cache with the norms, the position rotation and the rotations by
+    R_k and R_v on the way, and the queries beside them, in one launch (no reference counterpart as
+    one call: a model's norms and rotary embedding, then backend.py:171-173 and 195).
+
+    ``query`` [n, hq, 256] (or None), ``key`` and ``value`` [n, kv_heads, 256]: bf16, any strides
+    (rows inside a packed projection output are read in place). ``cos_sin``, ``positions``, ``axes``,
+    ``interleaved``, ``eps``, ``unit_offset`` and the weights as for ``qk_norm_rope``; without
+    ``cos_sin`` nothing is turned, without weights nothing is normed. The record of every token below
+    ``counts[1]`` with ``slots[token] >= 0`` (int64, distinct) is written to ``history`` (the K stripe's
+    bytes) as ``layout`` says, with 2-bit or 4-bit codes; what ``rotate_store_int2`` of the returned
+    key and the value writes. ``value=None``: nothing is stored (then ``history``, ``slots``,
+    ``layout`` and ``rv_t`` are not read). The BF16 windows are not written: ``post_attention`` or
+    ``store_windows`` do that behind the attention.
+
+    Returns ``(query, key, query_rot)``, contiguous bf16 rows, zeros at or past ``counts[1]``;
+    ``query_rot`` is ``rotate(query, R_k)``, None without a query or with ``rotate_query=False``.
+    """
+    store = value is not None
+    device = _same_device(key, query=query, value=value, history=history if store else None,
+                          slots=slots if store else None, counts=counts, rk_t=rk_t,
+                          rv_t=rv_t if store else None, cos_sin=cos_sin, positions=positions,
+                          axes=axes, q_weight=q_weight, k_weight=k_weight)
+    n, hk, d = key.shape
+    hq = 0 if query is None else query.shape[1]
+    if d != 256 or (query is not None and query.shape != (n, hq, 256)) or (
+            store and value.shape != (n, hk, 256)):
+        raise ValueError("query, key and value must be [n, heads, 256] of the same tokens, with as "
+                         "many values as keys")
+    rows = rotary = stride = position_stride = 0
+    axis_count = 1
+    if cos_sin is not None:
+        if cos_sin.dim() != 2 or cos_sin.dtype not in _VALUE_TYPES:
+            raise ValueError("cos_sin must be a bf16 or fp32 [positions, rotary] table")
+        rows, rotary = cos_sin.shape
+        if rotary % 2 or rotary > 256 or (rotary and not rows):
+            raise ValueError(f"the rotary dims must be even and at most 256, got {rotary} of {rows} "
+                             "positions")
+        if not cos_sin.is_contiguous() and (cos_sin.stride(1) != 1 or cos_sin.stride(0) < rotary):
+            cos_sin = cos_sin.contiguous()
+        stride = max(cos_sin.stride(0), rotary)
+        if positions is None or positions.dtype != torch.int64:
+            raise ValueError("positions must be int64")
+        if axes is None:
+            if positions.shape != (n,):
+                raise ValueError("positions must be int64, one per token")
+        else:
+            if _int32(axes, "axes").shape != (rotary // 2,) or not axes.is_contiguous():
+                raise ValueError("axes must hold one axis per pair of the rotary dims")
+            if positions.dim() != 2 or positions.shape[1] != n or not 1 <= positions.shape[0] <= 32:
+                raise ValueError("positions must be int64 [axes, tokens], of at most 32 axes")
+            axis_count = positions.shape[0]
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        position_stride = n
+    elif positions is not None or axes is not None:
+        raise ValueError("positions and axes need the table cos_sin")
+    if counts is not None and (_int32(counts, "counts").numel() < 2 or not counts.is_contiguous()):
+        raise ValueError("counts must hold (requests, tokens)")
+    turn_query = rotate_query and query is not None
+    if (query is not None and (q_weight is None) != (k_weight is None)) or (
+            query is None and q_weight is not None):
+        raise ValueError("queries and keys are normed together: pass both weights or none")
+    if k_weight is not None:
+        k_weight = _vector(k_weight, "k_weight")
+        if q_weight is not None:
+            q_weight = _vector(q_weight, "q_weight")
+            if q_weight.dtype != k_weight.dtype:
+                q_weight, k_weight = q_weight.float(), k_weight.float()
+    if turn_query or store:
+        if rk_t is None:
+            raise ValueError("rk_t is needed to rotate queries and to store keys")
+        _rotation_check(rk_t, "rk_t")
+    lay = clip = None
+    size = 0
+    if store:
+        _rotation_check(rv_t, "rv_t")
+        if layout.kv_heads != hk:
+            raise ValueError(f"the layout has {layout.kv_heads} KV heads, got {hk}")
+        if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] < n or (
+                n > 1 and slots.stride(0) != 1):
+            raise ValueError("slots must be contiguous int64, one per token")
+        if counts is None:
+            raise ValueError("counts must hold (requests, tokens)")
+        if not history.is_contiguous():
+            raise ValueError("history must be the contiguous bytes of the K stripe")
+        lay, clip = layout_struct(layout), clip_struct(layout.config)
+        size = history.numel() * history.element_size()
+    k_out = _rows_out(key)
+    q_out = None if query is None else _rows_out(query)
+    q_rot = torch.empty_like(q_out) if turn_query else None
+    if n:
+        q0 = q1 = v0 = v1 = 0
+        key, k0, k1 = _rows_aligned(key)
+        if query is not None:
+            query, q0, q1 = _rows_aligned(query)
+        if store:
+            value, v0, v1 = _rows_aligned(value)
+        _launch(
+            _ext.library().oscar_rope_append, "rope_append", device, _ptr(query), q0, q1,
+            key.data_ptr(), k0, k1, _ptr(value), v0, v1, n, hq, hk, _ptr(q_weight), _ptr(k_weight),
+            k_weight is not None and k_weight.dtype == torch.float32, bool(unit_offset), eps,
+            _ptr(cos_sin), rows, stride, cos_sin is not None and cos_sin.dtype == torch.float32,
+            rotary, bool(interleaved), _ptr(positions), position_stride, axis_count, _ptr(axes),
+            _ptr(counts), _ptr(q_out), k_out.data_ptr(), _ptr(rk_t), _ptr(rv_t) if store else None,
+            _ptr(q_rot), _ptr(history) if store else None, size, _ptr(slots) if store else None, lay,
+            clip,
+        )
+    return q_out, k_out, q_rot
+
+
+def read_records(history, slots, layout):
+    """The values that records stand for (no reference counterpart; without the inverse rotations of
+    ``dequant_inverse_rotate`` and of any number of slots): ``(key, value)``, bf16
+    [n, kv_heads, 256] in the rotated basis, zeros for slots (int64 [n]) below 0 or outside the
+    buffer."""
+    device = _same_device(history, slots=slots)
+    if slots.dtype != torch.int64 or slots.dim() != 1:
+        raise ValueError("slots must be an int64 vector")
+    if not history.is_contiguous():
+        raise ValueError("history must be the contiguous bytes of the K stripe")
+    n = slots.shape[0]
+    key = torch.empty((n, layout.kv_heads, 256), dtype=torch.bfloat16, device=device)
+    value = torch.empty_like(key)
+    if n:
+        if not slots.is_contiguous():
+            slots = slots.contiguous()
+        _launch(
+            _ext.library().oscar_read_records, "read_records", device, history.data_ptr(),
+            history.numel() * history.element_size(), slots.data_ptr(), n, layout_struct(layout),
+            key.data_ptr(), value.data_ptr(),
+        )
+    return key, value
 
 
 @dataclass

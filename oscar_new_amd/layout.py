@@ -9,6 +9,9 @@ Per physical page (``Bp`` tokens, ``H`` kv heads, ``D`` = 256):
   slot ``s`` of head ``h`` starts at ``(s // Bp) * stripe + ((s % Bp) * H + h) * 160``;
   bytes [0,64) K codes, [64,66) K scale (fp16 LE), [66,68) K zero, [68,132) V codes,
   [132,134) V scale, [134,136) V zero, [136,160) untouched padding.
+  With ``history_bits=4`` a record is 272 bytes: [0,128) K codes, [128,256) V codes (dim ``d`` in
+  nibble ``d % 2`` of byte ``d // 2``), [256,264) K scale, K zero, V scale, V zero, [264,272)
+  untouched (no reference counterpart).
 * V stripe page of a request's FIRST physical page holds the BF16 window: sink tokens
   ``t < S`` at index ``t``, later tokens at ring index ``S + t % C``; each index stores K
   then V, ``H*D`` bf16 each.
@@ -41,7 +44,7 @@ class CacheLayout:
             )
         capacity = self.stripe_page_bytes
         if self.history_page_bytes > capacity:
-            raise ValueError("INT2 history slots exceed the native K stripe of a page")
+            raise ValueError("history slots exceed the native K stripe of a page")
         if self.window_page_bytes > capacity:
             raise ValueError(
                 f"the BF16 sink/ring window needs {self.window_page_bytes} bytes per owner "
@@ -69,7 +72,7 @@ class CacheLayout:
 
     # ---- addressing (layout.py:46-73)
     def slot_offset(self, slot, head=0):
-        """Byte offset of a token-head's 160-byte slot in the K stripe."""
+        """Byte offset of a token-head's record in the K stripe."""
         if slot < 0 or head < 0 or head >= self.kv_heads:
             raise ValueError("slot must be >= 0 and head inside [0, kv_heads)")
         page = slot // self.physical_block_tokens
