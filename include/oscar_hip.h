@@ -710,7 +710,10 @@ int oscar_read_records(const void* history, int64_t history_bytes, const int64_t
 /*
  * history_int4 -- oscar_attention_partials (raw = 0) over 4-bit records: the same tasks, masks, split
  * rules, partial rows and LSEs. kernel_block_tokens >= 32. Under the device rule (split_tokens < 0) the
- * split length is the least of eight tried ones with which all splits fit the budget.
+ * split length is the least of eight tried ones with which all splits fit the budget. row_tiles: the
+ * rows of a request in tiles of 32 instead of tasks (the tasks are not read), for steps with many query
+ * tokens in some request; split_tokens 0, equal splits of whole chunks of 32 positions; max_reqs bounds the
+ * requests (counts[0]).
  */
 int oscar_history_int4(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_s2,
                        const void* history, int64_t history_bytes, const int32_t* qstarts,
@@ -718,8 +721,8 @@ int oscar_history_int4(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_
                        int64_t table_columns, const int32_t* counts, const int32_t* tasks,
                        const int32_t* task_count, int64_t n, int64_t hq, int64_t programs,
                        int32_t splits, int32_t block_n, int32_t query_tile, int32_t max_query_len,
-                       float scale, int32_t split_tokens, const oscar_layout* layout,
-                       float* partials, float* lse, void* stream);
+                       float scale, int32_t split_tokens, int32_t row_tiles, int64_t max_reqs,
+                       const oscar_layout* layout, float* partials, float* lse, void* stream);
 
 #ifdef __cplusplus
 }

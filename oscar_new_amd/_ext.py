@@ -215,7 +215,7 @@ SIGNATURES = {
         _P, _I64, _I64, _I64, _P, _I64,  # query, history
         _P, _P, _P, _I64, _I64, _P, _P, _P,  # qstarts .. table columns, counts, tasks, count
         _I64, _I64, _I64, _I32, _I32, _I32, _I32, _F, _I32,  # n hq programs splits bn qt mql scale st
-        POINTER(OscarLayout), _P, _P, _P,  # layout, partials, lse, stream
+        _I32, _I64, POINTER(OscarLayout), _P, _P, _P,  # row tiles, max reqs, layout, partials, lse, stream
     ],
 }
 RESTYPES = {"oscar_noalloc_scratch_bytes": c_int64, "oscar_calibration_workspace_bytes": c_int64,

@@ -8,8 +8,11 @@
 // records only (oscar_ascend/kernels.py:290-482).
 //
 // Scale and zero fold out of the products: q . k = s (q . c) + z sum q, and sum p v = sum (p s) (c - 7.5)
-// + sum p (z + 7.5 s), in which the rounding of p s to bf16 weighs values of either sign: the products run
-// over c, and one more against ones gives the sum of the rounded p s. Codes and queries are exact in bf16.
+// + sum p (z + 7.5 s), in which the rounding of p s weighs values of either sign: the products run over c,
+// and one more against ones gives the sum of the rounded p s. Codes and queries are exact in bf16. p s is
+// rounded to fp16 (2^-11; bf16's 2^-8 made the error against 64 bits 0.0023 of the output where the
+// output's own rounding is 0.0017), times a power of two that each wavefront keeps for its largest s so
+// far: it lies below 2^15 then, and the smallest ones are off by 2^-31 of that s.
 //
 // A workgroup of eight wavefronts, one per CU, takes up to 32 query rows. Wavefront w streams chunks of
 // 32 positions w, w + 8, ... of the split through an LDS ring of its own (direct-to-LDS copies, no barrier
@@ -27,7 +30,7 @@ constexpr int kPieces4 = kSlot4 / 16;               // 17 pieces of a record
 constexpr int kStage4 = kChunk4 * kSlot4;           // 8704 bytes
 constexpr int kDma4 = (kChunk4 * kPieces4 + 63) / 64;  // 9 copies of a chunk, the last of 32 lanes
 constexpr int kTable4 = 512;                        // kernel blocks whose offsets live in LDS
-constexpr float kTheta4 = 8.0f;                     // slack of the running maximum, log2 units
+constexpr float kRoom4 = 13.0f;                     // of scores above a row's reference, log2 units
 constexpr int kMaxTasks4 = 16384;                   // task rows of the device rule
 
 // A workgroup's form: RG groups of 16 query rows, W wavefronts with S ring stages each.
@@ -38,7 +41,7 @@ struct Form4 {
     uint8_t ring[W][S][kStage4] __attribute__((aligned(16)));
     uint8_t q[RG * 16 * kHeadDim * 2] __attribute__((aligned(16)));
     uint32_t off[kTable4];
-    float red[4][W][16 * RG];  // per wavefront: row max, sum p, sum p (z + 7.5 s), sum of P
+    float red[3][W][16 * RG];  // per wavefront: reference score, sum p, sum p z
   };
   static_assert(W * 16 * kHeadDim * 4 <= sizeof(Lds::ring), "a row group's merge fits the ring");
 };
@@ -167,10 +170,27 @@ __device__ bool unit_of_slot(const AttnArgs& a, int programs, int u, int* length
 
 __device__ __forceinline__ f32x4 splat(float v) { return f32x4{v, v, v, v}; }
 
-// Rows 16 rg + n (rg < RG) of the task against positions [p_lo, p_hi), partial rows to `split`.
+// A workgroup's rows: row r (of 16 RG) is row base + r of the query tokens from token0 on times the group's
+// heads, where that lies below `end`.
+struct Rows4 {
+  int64_t token0;
+  int base, end;
+};
+__device__ __forceinline__ RowInfo row_of(const AttnArgs& a, const Rows4& rows, int head, int r) {
+  const int row = rows.base + r, qi = static_cast<int>(fastdiv(static_cast<uint32_t>(row), a.g_div));
+  RowInfo ri;
+  ri.qi = qi;
+  ri.token = rows.token0 + qi;
+  ri.valid = row < rows.end && ri.token >= 0 && ri.token < a.n;
+  ri.qhead = head * a.g + (row - qi * a.g);
+  return ri;
+}
+
+// The rows against positions [p_lo, p_hi) of request t.req, partial rows to `split`.
 template <class F>
-__device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, int head, int p_lo,
-                                              int p_hi, int split, typename F::Lds& lds) {
+__device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, const Rows4& rows,
+                                              int head, int p_lo, int p_hi, int split,
+                                              typename F::Lds& lds) {
   constexpr int RG = F::RG, W = F::W, S = F::S;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -187,7 +207,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
 #pragma unroll
   for (int i = 0; i < RG * 8 / W; ++i) {
     const int row0 = 2 * (i * W + wave), row = row0 + (lane >> 5);
-    const RowInfo ri = row_info(a, t, head, row);
+    const RowInfo ri = row_of(a, rows, head, row);
     const uint16_t* src = a.query + (ri.valid ? ri.token * a.qs0 + ri.qhead * a.qs1 : 0) +
                           8 * ((lane & 31) ^ (row & 15));
     dma_dwordx4(src, q_area + row0 * kHeadDim * 2);
@@ -221,9 +241,13 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     for (int i = 0; i < kDma4 - 1; ++i) dma_x4_stream(base, voff[i], at + 1024 * i);
     if (lane < 32) dma_x4_stream(base, voff[kDma4 - 1], at + 1024 * (kDma4 - 1));
   };
+  // The first chunks on their way, behind the query rows' copies.
+  auto start = [&]() {
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s)
-    if (s < nmine) issue(s, s);
+    for (int s = 0; s < S - 1; ++s)
+      if (s < nmine) issue(s, s);
+  };
+  start();
   wait_chunks(min(nmine, S - 1));
   barrier_lds();  // the query rows
 
@@ -232,7 +256,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
   for (int i = 0; i < RG * 16; i += F::kThreads / 32) {
     const int row = i + (tid >> 5);
     u32x4* at = reinterpret_cast<u32x4*>(lds.q + row * kHeadDim * 2 + 16 * (tid & 31));
-    *at = row_info(a, t, head, row).valid ? code_order(*at) : u32x4{0u, 0u, 0u, 0u};
+    *at = row_of(a, rows, head, row).valid ? code_order(*at) : u32x4{0u, 0u, 0u, 0u};
   }
   barrier_lds();
   // B operand of k-step m: dims 64 g + 8 m .. + 7 of row n. One row group's stay in registers; two
@@ -264,22 +288,19 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
   // eight positions in either.
   const int v_off = kSlot4 * (16 * (n >> 2 & 1) + 4 * g + (n & 3)) + kCodes4 + 8 * (n >> 3);
   const float fq = a.scale_log2;
-  float m_run[RG], psum[RG], zsum[RG];
-  f32x4 o[RG][16], ones_o[RG];  // o[c]: rows 4 g + v, dim 16 c + n
-#pragma unroll
-  for (int i = 0; i < RG; ++i) {
-    m_run[i] = -INFINITY;
-    psum[i] = zsum[i] = 0.f;
-    ones_o[i] = splat(0.f);
-#pragma unroll
-    for (int c = 0; c < 16; ++c) o[i][c] = splat(0.f);
-  }
 
-  auto process = [&](int j, int s) {
-    const uint8_t* st = lds.ring[wave][s];
+  // A chunk in stage s: the products of its K codes and the rows, and its scales and zeros.
+  struct Chunk {
     f32x4 acc[RG][2];
+    uint2 side[8];  // of the lane's positions 16 (e / 4) + 4 g + e % 4: K scale and zero, V scale and zero
+    bool whole;
+    uint32_t seen;  // bit e, where not whole
+    float top;      // largest V scale of the lane's
+  };
+  auto read_chunk = [&](int t0, int s, Chunk& c) {
+    const uint8_t* st = lds.ring[wave][s];
 #pragma unroll
-    for (int i = 0; i < RG; ++i) acc[i][0] = acc[i][1] = splat(0.f);
+    for (int i = 0; i < RG; ++i) c.acc[i][0] = c.acc[i][1] = splat(0.f);
     u32x4 kw[2][2];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
@@ -292,101 +313,169 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
 #pragma unroll
       for (int i = 0; i < RG; ++i) {
         const u32x4 q = RG == 1 ? qb[m] : q_operand(i, m);
-        acc[i][0] = mfma16x16x32(k0, q, acc[i][0]);
-        acc[i][1] = mfma16x16x32(k1, q, acc[i][1]);
+        c.acc[i][0] = mfma16x16x32(k0, q, c.acc[i][0]);
+        c.acc[i][1] = mfma16x16x32(k1, q, c.acc[i][1]);
       }
     }
-    uint2 side[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      side[e] = *reinterpret_cast<const uint2*>(st + side_off + kSlot4 * (16 * (e >> 2) + (e & 3)));
+      c.side[e] = *reinterpret_cast<const uint2*>(st + side_off + kSlot4 * (16 * (e >> 2) + (e & 3)));
     // A first or last chunk may be partial, or the block unmapped: positions outside get score -inf and
     // a zero V scale and zero (their bytes may be NaN patterns).
-    const int t0 = (first + wave + W * j) * kChunk4;
     const bool ok_block = mapped >> s & 1u;
-    const bool whole = ok_block && t0 >= p_lo && t0 + kChunk4 <= p_hi;
-    u32x4 pa[RG];
+    c.whole = ok_block && t0 >= p_lo && t0 + kChunk4 <= p_hi;
+    c.seen = 0u;
+    if (!c.whole) {
+      // The positions' bits, in a register that the compiler cannot know ahead of the branch.
+      const int from = max(p_lo - t0, 0), to = min(p_hi - t0, kChunk4);
+      uint32_t bits = ok_block ? (0xffffffffu << from) & (0xffffffffu >> (kChunk4 - to)) : 0u;
+      asm volatile("" : "+v"(bits));
+      c.seen = (bits >> (4 * g) & 0xfu) | (bits >> (12 + 4 * g) & 0xf0u);
 #pragma unroll
-    for (int i = 0; i < RG; ++i) {
-      float r[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        r[e] = fmaf(half_lo_to_float(side[e].x), acc[i][e >> 2][e & 3],
-                    half_hi_to_float(side[e].x) * qs[i]);
-      if (!whole) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int p = t0 + 16 * (e >> 2) + 4 * g + (e & 3);
-          const bool in = ok_block && p >= p_lo && p < p_hi;
-          r[e] = in ? r[e] : -INFINITY;
-          side[e].y = in ? side[e].y : 0u;
-        }
-      }
-      float lm = fmaxf(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])),
-                       fmaxf(fmaxf(r[4], r[5]), fmaxf(r[6], r[7]))) * fq;
-      if (__any(lm > m_run[i] + kTheta4)) {
-        const float mn = fmaxf(m_run[i], max_xor32(max_xor16(lm)));
-        const float alpha = mn == -INFINITY ? 1.0f : exp2f(m_run[i] - mn);
-        m_run[i] = mn;
-        psum[i] *= alpha;
-        zsum[i] *= alpha;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float av = __shfl(alpha, 4 * g + v, kWave);
-#pragma unroll
-          for (int c = 0; c < 16; ++c) o[i][c][v] *= av;
-          ones_o[i][v] *= av;
-        }
-      }
-      const float nm = m_run[i] == -INFINITY ? 0.f : -m_run[i];
-      float pv[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(r[e], fq, nm));
-        const float sv = half_lo_to_float(side[e].y);
-        psum[i] += p;
-        zsum[i] = fmaf(p, fmaf(7.5f, sv, half_hi_to_float(side[e].y)), zsum[i]);
-        pv[e] = p * sv;
-      }
-      // Position e of the lane is nibble e of its transposed reads: the order of codes_bf16.
-      pa[i] = u32x4{pack_bf16x2(pv[0], pv[2]), pack_bf16x2(pv[4], pv[6]), pack_bf16x2(pv[1], pv[3]),
-                    pack_bf16x2(pv[5], pv[7])};
-      constexpr uint32_t kOnes = 0x3f803f80u;  // bf16 1, twice
-      ones_o[i] = mfma16x16x32(pa[i], u32x4{kOnes, kOnes, kOnes, kOnes}, ones_o[i]);
+      for (int e = 0; e < 8; ++e) c.side[e].y = c.seen >> e & 1u ? c.side[e].y : 0u;
     }
+    c.top = 0.f;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2_ptr_t)(st + v_off + 16 * c));
+    for (int e = 0; e < 8; ++e) c.top = fmaxf(c.top, fabsf(half_lo_to_float(c.side[e].y)));
+  };
+  // Scores of row group i in units of fq, and their largest in log2 units.
+  auto row_scores = [&](Chunk& c, int i, float (&r)[8]) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const u32x4 vf = codes_bf16(static_cast<uint32_t>(w[h]));
+    for (int e = 0; e < 8; ++e)
+      r[e] = fmaf(half_lo_to_float(c.side[e].x), c.acc[i][e >> 2][e & 3],
+                  half_hi_to_float(c.side[e].x) * qs[i]);
+    if (!c.whole) {
+      asm volatile("" : "+v"(c.seen));
 #pragma unroll
-        for (int i = 0; i < RG; ++i) o[i][2 * c + h] = mfma16x16x32(pa[i], vf, o[i][2 * c + h]);
+      for (int e = 0; e < 8; ++e) r[e] = c.seen >> e & 1u ? r[e] : -INFINITY;
+    }
+    return fmaxf(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])),
+                 fmaxf(fmaxf(r[4], r[5]), fmaxf(r[6], r[7]))) * fq;
+  };
+  // This wavefront's chunks in turn through its ring (the first S - 1 are on their way), while `use` says
+  // to go on.
+  auto stream = [&](auto use) {
+    for (int j = 0, s = 0; j < nmine; ++j) {
+      // The stage that chunk j - 1 was read from (its reads have completed) takes chunk j + S - 1.
+      if (j + S - 1 < nmine) {
+        OSCAR_WAIT_LGKM();
+        issue(j + S - 1, s == 0 ? S - 1 : s - 1);
       }
+      wait_chunks(min(nmine - 1 - j, S - 1));  // chunk j has landed
+      if (!use((first + wave + W * j) * kChunk4, s)) return;
+      s = s == S - 1 ? 0 : s + 1;
     }
   };
 
-  for (int j = 0, s = 0; j < nmine; ++j) {
-    // The stage that chunk j - 1 was read from (its reads have completed) takes chunk j + S - 1.
-    if (j + S - 1 < nmine) {
-      OSCAR_WAIT_LGKM();
-      issue(j + S - 1, s == 0 ? S - 1 : s - 1);
+  // Weights are taken against a row's reference m_ref: the largest score of its first chunk here, with room
+  // for 2^kRoom4 above it, and V scales times v_by, with room for four times the first chunk's largest:
+  // then no sum is ever scaled again, and the accumulators stay where the matrix instructions want them
+  // (rescaling them as a running maximum grows made the compiler move them about: two row groups spilled
+  // registers). Should a score or scale need more room, the wavefront's chunks are gone through for the
+  // largest ones, and then again from the start with those.
+  float m_ref[RG], psum[RG], zsum[RG];
+  float v_limit = 0.f, v_by = 1.f;
+  f32x4 o[RG][16];  // o[c]: rows 4 g + v, dim 16 c + n
+  auto set_scale = [&](float top) {
+    const uint32_t eb = min(__float_as_uint(top) >> 23, 250u);
+    v_limit = __uint_as_float((eb + 3) << 23);           // 4 to 8 times the largest
+    v_by = __uint_as_float((127 + 126 - eb) << 23);      // p s v_by < 2^(13 + 3 - 1) = 2^15
+  };
+#pragma unroll
+  for (int i = 0; i < RG; ++i) m_ref[i] = -INFINITY;
+  bool exact = false, again;
+  do {
+    again = false;
+#pragma unroll
+    for (int i = 0; i < RG; ++i) {
+      psum[i] = zsum[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) o[i][c] = splat(0.f);
     }
-    wait_chunks(min(nmine - 1 - j, S - 1));  // chunk j has landed
-    process(j, s);
-    s = s == S - 1 ? 0 : s + 1;
-  }
+    stream([&](int t0, int s) {
+      Chunk c;
+      read_chunk(t0, s, c);
+      if (!exact && __any(c.top > v_limit)) {
+        if (v_limit == 0.f)
+          set_scale(max_xor32(max_xor16(c.top)));  // the same in every lane
+        else
+          again = true;
+      }
+      u32x4 pa[RG];
+      float vs[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vs[e] = half_lo_to_float(c.side[e].y) * v_by;
+#pragma unroll
+      for (int i = 0; i < RG; ++i) {
+        float r[8];
+        const float lm = row_scores(c, i, r);
+        if (!exact && __any(lm > m_ref[i] + kRoom4)) {
+          const float mx = max_xor32(max_xor16(lm));
+          again |= __any(m_ref[i] != -INFINITY && mx > m_ref[i] + kRoom4) != 0;
+          if (m_ref[i] == -INFINITY) m_ref[i] = mx;
+        }
+        const float nm = m_ref[i] == -INFINITY ? 0.f : -m_ref[i];
+        float pv[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(r[e], fq, nm));
+          psum[i] += p;
+          zsum[i] = fmaf(p, half_hi_to_float(c.side[e].y), zsum[i]);
+          pv[e] = p * vs[e];
+        }
+        // Position e of the lane is nibble e of its transposed reads: the order of codes_f16.
+        pa[i] = u32x4{pack_f16x2(pv[0], pv[2]), pack_f16x2(pv[4], pv[6]), pack_f16x2(pv[1], pv[3]),
+                      pack_f16x2(pv[5], pv[7])};
+      }
+      const uint8_t* st = lds.ring[wave][s];
+#pragma unroll
+      for (int c8 = 0; c8 < 8; ++c8) {
+        const i32x2 w =
+            __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2_ptr_t)(st + v_off + 16 * c8));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 vf = codes_f16(static_cast<uint32_t>(w[h]));
+#pragma unroll
+          for (int i = 0; i < RG; ++i) o[i][2 * c8 + h] = mfma16x16x32_f16(pa[i], vf, o[i][2 * c8 + h]);
+        }
+      }
+      return !again;
+    });
+    if (again) {
+      OSCAR_WAIT_VM(0);
+      OSCAR_WAIT_LGKM();
+      start();
+      float top = 0.f;
+      stream([&](int t0, int s) {
+        Chunk c;
+        read_chunk(t0, s, c);
+        top = fmaxf(top, c.top);
+#pragma unroll
+        for (int i = 0; i < RG; ++i) {
+          float r[8];
+          m_ref[i] = fmaxf(m_ref[i], row_scores(c, i, r));
+        }
+        return true;
+      });
+      OSCAR_WAIT_LGKM();
+      start();
+      set_scale(max_xor32(max_xor16(top)));
+#pragma unroll
+      for (int i = 0; i < RG; ++i) m_ref[i] = max_xor32(max_xor16(m_ref[i]));
+      exact = true;
+    }
+  } while (again);
 
   // ---- the wavefronts' states joined, normalized rows and LSEs written.
+  const float v_back = 1.0f / v_by;  // both powers of two
 #pragma unroll
   for (int i = 0; i < RG; ++i) {
     const float ps = sum_xor32(sum_xor16(psum[i])), zs = sum_xor32(sum_xor16(zsum[i]));
     if (g == 0) {
-      lds.red[0][wave][16 * i + n] = m_run[i];
+      lds.red[0][wave][16 * i + n] = m_ref[i];
       lds.red[1][wave][16 * i + n] = ps;
       lds.red[2][wave][16 * i + n] = zs;
     }
-    if (n == 0) *reinterpret_cast<f32x4*>(&lds.red[3][wave][16 * i + 4 * g]) = ones_o[i];
   }
   float* s_o = reinterpret_cast<float*>(&lds.ring[0][0][0]);  // [wavefront][16 rows][256]
 #pragma unroll
@@ -399,7 +488,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
 #pragma unroll
       for (int w = 1; w < W; ++w) mx = fmaxf(mx, lds.red[0][w][row]);
       const float mw = lds.red[0][wave][row];
-      const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx);
+      const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx) * v_back;
       float* dst = s_o + (wave * 16 + 4 * g + v) * kHeadDim + n;
 #pragma unroll
       for (int c = 0; c < 16; ++c) dst[16 * c] = o[i][c][v] * f;
@@ -409,7 +498,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
 #pragma unroll
     for (int r0 = 0; r0 < 16; r0 += F::kThreads / 32) {
     const int row16 = r0 + (tid >> 5), row = 16 * i + row16, d0 = 4 * (tid & 31);
-    const RowInfo ri = row_info(a, t, head, row);
+    const RowInfo ri = row_of(a, rows, head, row);
     if (!ri.valid) continue;
     float mx = -INFINITY;
 #pragma unroll
@@ -421,7 +510,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
       const float mw = lds.red[0][w][row];
       const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx);
       den = fmaf(f, lds.red[1][w][row], den);
-      zs = fmaf(f, fmaf(-7.5f, lds.red[3][w][row], lds.red[2][w][row]), zs);
+      zs = fmaf(f, lds.red[2][w][row], zs);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         sum[h] += *reinterpret_cast<const f32x4*>(s_o + (w * 16 + row16) * kHeadDim + d0 + 128 * h);
@@ -468,13 +557,89 @@ __global__ __launch_bounds__(F::kThreads) void history4_kernel(const AttnArgs a,
   }
   int p_lo, p_hi;
   history_positions(a, t, t.recent_begin - t.sink_len, nsplit, split, split_tokens, p_lo, p_hi);
-  history_rows4<F>(a, t, head, p_lo, p_hi, split, lds);
+  const Rows4 rows{t.qstart + t.qoff, 0, min(a.qt, t.qlen - t.qoff) * a.g};
+  history_rows4<F>(a, t, rows, head, p_lo, p_hi, split, lds);
+}
+
+// ---- steps with many query tokens in a request: tiles of 16 RG of its rows instead of tasks, so that a
+// tile's unpacked codes meet as many rows as a wavefront's registers hold sums of. The rows past a
+// request's last cost matrix products but hardly time where a tile has few: the records' copies
+// take as long.
+
+// Request and tile of tile slot x, the requests' tiles in order; false past the last. Every thread of the
+// workgroup calls it.
+template <class F>
+__device__ __forceinline__ bool find_tile4(const AttnArgs& a, int max_reqs, int x, int& req, int& tile) {
+  __shared__ int s_carry[F::W], s_found[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int reqs = max(min(a.counts[0], max_reqs), 0), active = a.counts[1];
+  if (tid == 0) s_found[0] = -1;
+  int carry = 0;
+  for (int c0 = 0; c0 < reqs && carry <= x; c0 += F::kThreads) {
+    const int r = c0 + tid;
+    int tiles = 0;
+    if (r < reqs) {
+      const int q0 = a.qstarts[r], rows = (min(a.qstarts[r + 1], active) - q0) * a.g;
+      tiles = rows > 0 ? (rows + 16 * F::RG - 1) / (16 * F::RG) : 0;
+    }
+    int incl = tiles;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int y = __shfl_up(incl, d, kWave);
+      incl += lane >= d ? y : 0;
+    }
+    if (lane == kWave - 1) s_carry[wave] = incl;
+    __syncthreads();
+    int before = carry, all = 0;
+#pragma unroll
+    for (int w = 0; w < F::W; ++w) {
+      before += w < wave ? s_carry[w] : 0;
+      all += s_carry[w];
+    }
+    const int base = before + incl - tiles;
+    if (x >= base && x < base + tiles) {
+      s_found[0] = r;
+      s_found[1] = x - base;
+    }
+    carry += all;
+    __syncthreads();  // s_carry is read before the next round writes it
+  }
+  if (reqs <= 0) return false;
+  req = uniform(s_found[0]);
+  tile = uniform(s_found[1]);
+  return req >= 0;
+}
+
+template <class F>
+__global__ __launch_bounds__(F::kThreads) void history4_tiles_kernel(const AttnArgs a, int max_reqs) {
+  __shared__ typename F::Lds lds;
+  // Workgroup ((tile, KV head), split): the tiles that exist dispatch first.
+  const int unit = static_cast<int>(blockIdx.x) / a.splits, h = a.L.kv_heads;
+  const int split = static_cast<int>(blockIdx.x) - unit * a.splits, head = unit % h;
+  Task t{};
+  int tile;
+  if (!find_tile4<F>(a, max_reqs, unit / h, t.req, tile)) return;
+  t.qstart = a.qstarts[t.req];
+  t.qlen = min(a.qstarts[t.req + 1], a.counts[1]) - t.qstart;
+  t.prefix = a.seq_lens[t.req] - t.qlen;
+  t.sink_len = min(a.L.sink, t.prefix);
+  t.recent_begin = max(t.sink_len, t.prefix - a.L.recent);
+  // Equal numbers of chunks for the splits (split_range's tiles of block_n positions, kernels.py:368-370,
+  // at whole chunks of absolute positions).
+  const int lo = max(t.sink_len, 0), hi = t.recent_begin;
+  const int c0 = lo / kChunk4, chunks = lo < hi ? (hi - 1) / kChunk4 - c0 + 1 : 0;
+  const int from = static_cast<int>(static_cast<int64_t>(chunks) * split / a.splits);
+  const int to = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / a.splits);
+  const int p_lo = max(lo, (c0 + from) * kChunk4), p_hi = min(hi, (c0 + to) * kChunk4);
+  const Rows4 rows{t.qstart, tile * 16 * F::RG, t.qlen * a.g};
+  history_rows4<F>(a, t, rows, head, p_lo, p_hi, split, lds);
 }
 
 // One row group: eight wavefronts, two a SIMD, with two stages each. Two groups: four with four, so that
 // a wavefront has the registers for both.
 using OneGroup = Form4<1, 8, 2>;
 using TwoGroups = Form4<2, 4, 4>;
+using RowTiles = Form4<2, 8, 2>;
 
 }  // namespace
 }  // namespace oscar
@@ -486,8 +651,9 @@ extern "C" int oscar_history_int4(const void* query, int64_t q_s0, int64_t q_s1,
                                   const int32_t* tasks, const int32_t* task_count, int64_t n,
                                   int64_t hq, int64_t programs, int32_t splits, int32_t block_n,
                                   int32_t query_tile, int32_t max_query_len, float scale,
-                                  int32_t split_tokens, const oscar_layout* layout, float* partials,
-                                  float* lse, void* stream) {
+                                  int32_t split_tokens, int32_t row_tiles, int64_t max_reqs,
+                                  const oscar_layout* layout, float* partials, float* lse,
+                                  void* stream) {
   using namespace oscar;
   AttnArgs a;
   int64_t rows = 0;
@@ -497,6 +663,21 @@ extern "C" int oscar_history_int4(const void* query, int64_t q_s0, int64_t q_s1,
                                 splits, block_n, query_tile, max_query_len, scale, 0, split_tokens,
                                 layout, partials, lse, &a, &rows, 4);
   if (st != OSCAR_OK || n == 0) return st;
+  hipStream_t s = as_stream(stream);
+  if (row_tiles) {
+    if (split_tokens) return OSCAR_E_UNSUPPORTED;
+    if (max_reqs < 1 || max_reqs > 0x7fffffffll) return OSCAR_E_SHAPE;
+    // A request of q tokens has at most q g / R + 1 tiles of R rows.
+    constexpr int64_t kRows = 16 * RowTiles::RG;
+    const int64_t reqs = n < max_reqs ? n : max_reqs;
+    if (n > 0x7fffffffll / hq) return OSCAR_E_SHAPE;
+    const int64_t tiles = n * a.g / kRows + reqs;
+    if (tiles > 0xffffffffll / RowTiles::kThreads / a.L.kv_heads / splits) return OSCAR_E_SHAPE;
+    hipLaunchKernelGGL(history4_tiles_kernel<RowTiles>,
+                       dim3(static_cast<unsigned>(tiles * a.L.kv_heads * splits)),
+                       dim3(RowTiles::kThreads), 0, s, a, static_cast<int>(max_reqs));
+    return static_cast<int>(hipGetLastError());
+  }
   const int64_t z = split_tokens < 0 ? device_unit_slices(programs, a.L.kv_heads, split_tokens) : splits;
   if (z > 65535 || a.L.kv_heads > 65535) return OSCAR_E_SHAPE;
   // The lengths of the device rule's task rows lie in the ring.
@@ -504,7 +685,6 @@ extern "C" int oscar_history_int4(const void* query, int64_t q_s0, int64_t q_s1,
   if (programs * z > 0xffffffffll / OneGroup::kThreads / a.L.kv_heads) return OSCAR_E_SHAPE;
   const dim3 grid(static_cast<unsigned>(programs), static_cast<unsigned>(a.L.kv_heads),
                   static_cast<unsigned>(z));
-  hipStream_t s = as_stream(stream);
   if (rows <= 16)
     hipLaunchKernelGGL(history4_kernel<OneGroup>, grid, dim3(OneGroup::kThreads), 0, s, a,
                        static_cast<int>(programs));

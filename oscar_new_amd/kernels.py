@@ -275,15 +275,15 @@ def attention_partials(query, key, value, history, window, meta, layout, scale, 
     the metadata's host-side lengths say that it pays (``config.chunk_kernel_pays``).
 
     With a layout of 4-bit records (``OscarConfig(history_bits=4)``) the history branch reads those,
-    under the same split rules; ``use_queue`` and ``chunk`` choose among the kernels of 2-bit records
-    and are ignored.
+    under the same split rules; ``use_queue`` does not apply, and ``chunk`` takes a request's rows in
+    tiles of 32 (by default with more than 16 query tokens in some request and no ``split_tokens``).
     """
     if raw and split_tokens:
         raise ValueError("split_tokens applies to the history branch only")
     if chunk and (raw or split_tokens):
         raise ValueError("chunk applies to the history branch under the reference split rule")
     if not raw and layout.config.history_bits == 4:
-        return _attention_int4(query, history, meta, layout, scale, splits, split_tokens)
+        return _attention_int4(query, history, meta, layout, scale, splits, split_tokens, chunk)
     _device_check(query, key, value, history, window)
     n, hq, d = query.shape
     cfg = layout.config
@@ -343,7 +343,7 @@ def attention_partials(query, key, value, history, window, meta, layout, scale, 
     return partials, lse
 
 
-def _attention_int4(query, history, meta, layout, scale, splits, split_tokens):
+def _attention_int4(query, history, meta, layout, scale, splits, split_tokens, chunk=None):
     """The history branch of ``attention_partials`` over 4-bit records."""
     table = _int32(meta.block_tables, "block_tables")
     qstarts = _int32(meta.query_start_loc, "query_start_loc")
@@ -368,16 +368,19 @@ def _attention_int4(query, history, meta, layout, scale, splits, split_tokens):
         return partials, lse
     cfg = layout.config
     programs = attention_programs(n, meta.max_num_reqs, cfg.queries_per_tile)
-    if tasks.shape[0] < programs:
+    longest = getattr(meta, "max_query_len", None)
+    longest = longest if isinstance(longest, int) else 0
+    if chunk is None:
+        chunk = longest > 16 and not split_tokens
+    if tasks.shape[0] < programs and not chunk:
         raise ValueError(f"task table holds {tasks.shape[0]} rows; the grid needs {programs}")
     query, s0, s1 = _rows_aligned(query)
-    longest = getattr(meta, "max_query_len", None)
     _launch(
         _ext.library().oscar_history_int4, "attention_partials", device, query.data_ptr(), s0, s1, 1,
         history.data_ptr(), history.numel(), qstarts.data_ptr(), seq_lens.data_ptr(),
         table.data_ptr(), table.stride(0), table.shape[1], counts.data_ptr(), tasks.data_ptr(),
         task_count.data_ptr(), n, hq, programs, splits, cfg.block_n, cfg.queries_per_tile,
-        longest if isinstance(longest, int) else 0, scale, int(split_tokens), layout_struct(layout),
+        longest, scale, int(split_tokens), bool(chunk), meta.max_num_reqs, layout_struct(layout),
         partials.data_ptr(), lse.data_ptr(),
     )
     return partials, lse

@@ -110,8 +110,9 @@ def exact(s, query, scale):
 
     The kernel's products of codes and queries are exact and summed in fp32 (256 terms and two more
     operations: at most 300 x 2^-24 of the sum of magnitudes), which moves a weight by e^d. The weights
-    times V's scale are rounded to bf16 (2^-8) against codes centred at 7.5; sums over L positions add at
-    most L / 256 chunk sums of 64 in fp32 on a path, and the states' and splits' joins a few more."""
+    times V's scale are rounded to fp16 (2^-11, or 2^-24 of the largest scale where they are small); sums
+    over L positions add at most L / 256 chunk sums of 32 terms in fp32 on a path, and the states' and
+    splits' joins a few more, of the codes' part and the zeros' part each."""
     n = query.shape[0]
     out = torch.zeros(n, s.hq, 256, dtype=torch.float64, device=DEV)
     lse = torch.full((n, s.hq), -math.inf, dtype=torch.float64, device=DEV)
@@ -132,10 +133,11 @@ def exact(s, query, scale):
                 w = score.softmax(-1)
                 out[t0 : t0 + q, rows] = w @ (vc * vs + vz)
                 lse[t0 : t0 + q, rows] = score.logsumexp(-1)
-                centred = w @ (vs * (vc - 7.5).abs())
-                whole = centred + w @ (vz + 7.5 * vs).abs()
+                codes = w @ (vs * vc)
+                whole = codes + w @ vz.abs()
                 sums = (64 + len(at) / 4) * 2.0**-24
-                slack[t0 : t0 + q, rows] = 2.0**-8 * centred + (2 * d[..., None] + sums) * whole
+                small = 15 * len(at) * 2.0**-24 * vs.amax()
+                slack[t0 : t0 + q, rows] = 2.0**-11 * codes + small + (2 * d[..., None] + sums) * whole
                 lse_slack[t0 : t0 + q, rows] = d + sums + 2.0**-21 * (1 + score.abs().amax(-1))
         t0 += q
     return out, lse, slack, lse_slack

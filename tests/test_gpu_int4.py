@@ -10,10 +10,10 @@ pytestmark = pytest.mark.gpu
 SCALE = 1 / 16
 
 
-def attend(s, splits=8, split_tokens=-256, query=None, merged=True):
+def attend(s, splits=8, split_tokens=-256, query=None, merged=True, chunk=None):
     query = s.query if query is None else query
     got = kernels.attention_partials(query, None, None, s.history, None, s.meta, s.layout, SCALE, splits,
-                                     raw=False, split_tokens=split_tokens)
+                                     raw=False, split_tokens=split_tokens, chunk=chunk)
     return kernels.merge_splits(*got, s.meta.counts) if merged else got
 
 
@@ -54,6 +54,27 @@ def test_split_rules(splits, split_tokens, qlens):
     check(s, attend(s, splits, split_tokens))
 
 
+@pytest.mark.parametrize("lengths,qlens", [([1], [1]), ([300], [300]), ([2000, 5, 40, 999], [31, 1, 2, 400]),
+                                           ([700], [17]), ([900, 900], [64, 65]), ([129], [128])])
+@pytest.mark.parametrize("heads,group", [(1, 6), (2, 5), (1, 1), (2, 8), (1, 32)])
+@pytest.mark.parametrize("splits", [1, 3, 16])
+def test_row_tiles(lengths, qlens, heads, group, splits):
+    s = world(lengths, qlens, layout_of(heads, queries_per_tile=1 if group > 8 else 4), group,
+              seed=splits, extra_rows=3)
+    check(s, attend(s, splits, 0, chunk=True))
+    s.meta.max_num_reqs = 700  # an engine's capacity: more tiles than there are
+    assert all(torch.equal(a[: sum(qlens)], b[: sum(qlens)]) for a, b in zip(
+        attend(s, splits, 0, chunk=True), attend(s, splits, 0, chunk=True)))
+    check(s, attend(s, splits, 0, chunk=True))
+
+
+def test_row_tiles_of_many_requests():
+    lengths = [1 + (i * 97) % 700 for i in range(300)]
+    qlens = [1 + (i * 31) % min(n, 40) for i, n in enumerate(lengths)]
+    s = world(lengths, qlens, layout_of(1), 6)
+    check(s, attend(s, 2, 0, chunk=True))
+
+
 @pytest.mark.parametrize("page,block", [(384, 128), (1536, 128), (768, 64), (768, 32), (96, 32)])
 def test_pages_and_blocks(page, block):
     s = world([1000, 97, 333], [1, 2, 1], layout_of(2, page, block, recent_tokens=17), 4)
@@ -70,6 +91,8 @@ def test_a_long_request():
     s = world([131072, 20], [1, 1], layout_of(1), 6)
     check(s, attend(s, 128))
     check(s, attend(s, 1, 0))  # one split: more kernel blocks than its table in LDS holds
+    s = world([131072], [40], layout_of(1), 6)
+    check(s, attend(s, 1, 0))
 
 
 def test_unmapped_blocks_are_masked():
@@ -134,6 +157,33 @@ def test_scales_of_any_size():
     side[..., 3] = torch.where(at % 3 == 0, -6e4, 2e-5).half()
     view[..., 256:264] = side.view(torch.uint8)
     check(s, attend(s))
+
+
+@pytest.mark.parametrize("qlen", [1, 4, 40])
+def test_scores_and_scales_that_grow(qlen):
+    """Weights are taken against a wavefront's first chunk: later ones far above it, far below it, and V
+    scales that grow a thousandfold keep every row's accuracy."""
+    for case in range(4):
+        s = world([9000], [qlen], layout_of(1), 6, seed=case, poison=False)
+        view = s.history.view(s.pool, -1)[:, : 768 * 272].view(s.pool, 768, 272)
+        side = view[..., 256:264].contiguous().view(torch.float16)
+        page = s.meta.block_tables[0, ::6][:12].long() // 6
+        at = torch.arange(12 * 768, device=DEV).view(12, 768)
+        if case == 0:  # a wavefront's first chunk tops the rest by 12 log2 units and more
+            big = at < 260
+            side[page, :, 0] = torch.where(big, 0.2, 0.002).half()
+            side[page, :, 1] = 0.0
+        elif case == 1:  # and lies below it, step by step
+            side[page, :, 0] = (0.001 * 1.002 ** (at / 4).float()).half()
+            side[page, :, 1] = 0.0
+        elif case == 2:  # V scales
+            side[page, :, 2] = (0.001 * 1.0008 ** at.float()).half()
+            side[page, :, 3] = (-0.0075 * 1.0008 ** at.float()).half()
+        else:  # the last position alone counts
+            side[page, :, 0] = torch.where(at == 8950, 30.0, 0.01).half()
+        view[..., 256:264] = side.view(torch.uint8)
+        check(s, attend(s, split_tokens=0, splits=1))
+        check(s, attend(s, split_tokens=0, splits=3, chunk=qlen > 16))
 
 
 def test_records_beyond_4_gb():

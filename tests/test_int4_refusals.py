@@ -79,10 +79,10 @@ def test_append():
 
 def test_history():
     def attend(q=A, q_s0=1536, history=A, size=1 << 24, table=A, n=8, hq=6, programs=8, splits=8, bn=32,
-               qt=4, mql=1, scale=1 / 16, st=-256, lay=layout(), partials=A, lse=A, tasks=A):
+               qt=4, mql=1, scale=1 / 16, st=-256, lay=layout(), partials=A, lse=A, tasks=A, tiles=0, reqs=8):
         return _ext.library().oscar_history_int4(q, q_s0, 256, 1, history, size, A, A, table, 64, 64, A,
                                                  tasks, A, n, hq, programs, splits, bn, qt, mql, scale, st,
-                                                 lay, partials, lse, None)
+                                                 tiles, reqs, lay, partials, lse, None)
 
     assert attend(n=0) == 0
     assert attend(n=-1) == -2 and attend(hq=0) == -2 and attend(programs=0) == -2
@@ -95,6 +95,8 @@ def test_history():
     assert attend(scale=0.0) == -5 and attend(hq=33) == -5 and attend(hq=9, mql=4) == -5
     assert attend(programs=16385) == -5  # task rows of the device rule
     assert attend(programs=1 << 24, st=0) == -2 and attend(st=-(1 << 30)) == -2
+    assert attend(tiles=1) == -5 and attend(tiles=1, st=0, reqs=0) == -2
+    assert attend(tiles=1, st=0, n=1 << 30) == -2 and attend(tiles=1, st=0, n=1 << 27, splits=64) == -2
 
 
 def test_read():
