@@ -25,7 +25,8 @@ import torch
 
 from . import kernels
 from .config import (INT4_SLOTS, OscarConfig, attention_programs, choose_chunk_splits, choose_device_partition,
-                     choose_history_partition, choose_splits, chunk_kernel_pays,
+                     choose_history_partition, choose_int4_splits, choose_splits,
+                     chunk_kernel_pays,
                      shared_prefix_pays)
 
 SPLIT_POLICIES = ("device", "reference", "mi355x")
@@ -279,6 +280,10 @@ class OscarAttentionImpl:
         group = self.num_heads // self.num_kv_heads
         if self.cfg.history_bits == 4:
             n = int(meta.num_actual_tokens if tokens is None else tokens)
+            if meta.max_query_len > 16:
+                longest = getattr(meta, "max_seq_len", None)
+                return choose_int4_splits(n, meta.num_reqs, self.num_kv_heads, self.num_heads,
+                                          longest if isinstance(longest, int) else None), 0
             programs = attention_programs(n, meta.max_num_reqs, self.cfg.queries_per_tile)
             return choose_device_partition(programs, self.num_kv_heads, meta.max_query_len, n,
                                            self.num_heads, self.cfg.queries_per_tile,

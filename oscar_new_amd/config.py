@@ -290,6 +290,32 @@ def choose_chunk_splits(tokens, requests, num_kv_heads, q_heads, max_seq_len, co
     return min(range(1, min(max_splits, steps) + 1), key=cost)
 
 
+# The same of a 32-row tile of 4-bit records and its round of 256 positions.
+INT4_TILE_ROWS, INT4_ROUND_TOKENS, INT4_ROUND_US, INT4_START_US = 32, 256, 2.45, 12.0
+
+
+@functools.lru_cache(maxsize=256)
+def choose_int4_splits(tokens, requests, num_kv_heads, q_heads, max_seq_len, compute_units=256,
+                       max_splits=16, scratch_bytes=128 << 20):
+    """Split count of the 4-bit history branch in steps with more than 16 query tokens in some request:
+    ``choose_chunk_splits`` with the times of that kernel's tiles (2048 tokens over 32768, six heads, 384
+    tiles: 716 / 530 / 576 / 553 / 613 us with 1 / 2 / 3 / 4 / 5 splits, 1.5 to 3 rounds over the CUs; 64
+    over 16000: 171 / 94 / 57 / 39 / 33 with 1 / 2 / 4 / 8 / 16)."""
+    if not max_seq_len:
+        return 1
+    group = q_heads // num_kv_heads
+    tiles = num_kv_heads * (-(-tokens * group // INT4_TILE_ROWS) + max(1, requests) - 1)
+    most = max(1, min(max_splits, scratch_bytes // max(1, tokens * q_heads * SPLIT_ROW_BYTES)))
+    steps = -(-int(max_seq_len) // INT4_ROUND_TOKENS)
+
+    def cost(splits):
+        rounds = -(-tiles * splits // compute_units)
+        return (rounds * (-(-steps // splits) * INT4_ROUND_US + INT4_START_US)
+                + tokens * q_heads * splits * CHUNK_ROW_US)
+
+    return min(range(1, min(most, steps) + 1), key=cost)
+
+
 # The start of a workgroup among others of the launch, most of it beside their work.
 CHUNK_SHORT_US = 6.0
 # The task-shaped history kernels (us): a 64-token chunk of one task on its CU, and the share of a

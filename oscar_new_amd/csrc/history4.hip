@@ -64,7 +64,7 @@ __device__ __forceinline__ void wait_chunks(int chunks) {
 // share and the one that always fits are tried, one by each wavefront, and the least that fits is
 // taken (32 requests of 32704 positions on 256 slots: 8 splits of 4096 each). Multiples of kStep4, at
 // least kMinSplit4.
-constexpr int kMinSplit4 = 512, kStep4 = 64, kTried4 = 8;
+constexpr int kMinSplit4 = 256, kStep4 = 64, kTried4 = 8;
 
 struct Unit4 {
   Task t;
@@ -75,15 +75,19 @@ template <int W>
 __device__ bool unit_of_slot(const AttnArgs& a, int programs, int u, int* lengths, Unit4& out) {
   constexpr int kThreads4 = W * kWave;
   __shared__ int64_t s_total[W];
-  __shared__ int s_fit[kTried4], s_carry[W], s_found[3];
+  __shared__ int s_fit[kTried4], s_carry[W], s_found[10];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int64_t sum = 0;
+  Task mine{};  // of the thread's last task: with at most one a thread, its owner has the row of the unit's
+  int mine_task = -1;
   for (int i = tid; i < programs; i += kThreads4) {
     Task t;
     const bool live = read_task(a, t, i);
     const int len = live ? max(t.recent_begin - t.sink_len, 0) : -1;
     lengths[i] = len;
     sum += max(len, 0);
+    mine = t;
+    mine_task = i;
   }
   sum = wave_sum_i64(sum);
   if (lane == 0) s_total[wave] = sum;
@@ -143,28 +147,27 @@ __device__ bool unit_of_slot(const AttnArgs& a, int programs, int u, int* length
     }
     const int base = before + incl - ns;
     if (ns > 0 && u >= base && u < base + ns) {
-      s_found[0] = i;
-      s_found[1] = u - base;
-      s_found[2] = ns;
+      Task t = mine;
+      if (i != mine_task) read_task(a, t, i);
+      const int row[10] = {i, u - base, ns, t.req, t.qoff, t.qstart, t.qlen, t.prefix, t.sink_len,
+                           t.recent_begin};
+#pragma unroll
+      for (int k = 0; k < 10; ++k) s_found[k] = row[k];
     }
     carry += chunk;
     __syncthreads();  // s_carry is read before the next round writes it
   }
-  const int task = uniform(s_found[0]);
-  if (task < 0) return false;
+  if (uniform(s_found[0]) < 0) return false;
   out.split = uniform(s_found[1]);
   out.nsplit = uniform(s_found[2]);
   out.split_tokens = st;
-  // Its row again (the loads hit the cache), uniform for the workgroup.
-  Task t;
-  read_task(a, t, task);
-  out.t.req = uniform(t.req);
-  out.t.qoff = uniform(t.qoff);
-  out.t.qstart = uniform(t.qstart);
-  out.t.qlen = uniform(t.qlen);
-  out.t.prefix = uniform(t.prefix);
-  out.t.sink_len = uniform(t.sink_len);
-  out.t.recent_begin = uniform(t.recent_begin);
+  out.t.req = uniform(s_found[3]);
+  out.t.qoff = uniform(s_found[4]);
+  out.t.qstart = uniform(s_found[5]);
+  out.t.qlen = uniform(s_found[6]);
+  out.t.prefix = uniform(s_found[7]);
+  out.t.sink_len = uniform(s_found[8]);
+  out.t.recent_begin = uniform(s_found[9]);
   return true;
 }
 
@@ -635,11 +638,10 @@ __global__ __launch_bounds__(F::kThreads) void history4_tiles_kernel(const AttnA
   history_rows4<F>(a, t, rows, head, p_lo, p_hi, split, lds);
 }
 
-// One row group: eight wavefronts, two a SIMD, with two stages each. Two groups: four with four, so that
-// a wavefront has the registers for both.
+// Eight wavefronts, two a SIMD, with two stages each.
 using OneGroup = Form4<1, 8, 2>;
-using TwoGroups = Form4<2, 4, 4>;
-using RowTiles = Form4<2, 8, 2>;
+using TwoGroups = Form4<2, 8, 2>;
+using RowTiles = TwoGroups;
 
 }  // namespace
 }  // namespace oscar

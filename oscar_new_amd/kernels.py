@@ -76,9 +76,12 @@ def _rows_contiguous(t):
 
 
 def layout_struct(layout):
-    """``CacheLayout`` -> C ``oscar_layout``."""
+    """``CacheLayout`` -> C ``oscar_layout`` (made once for a layout, which never changes)."""
+    made = layout.__dict__.get("_struct")
+    if made is not None:
+        return made
     cfg = layout.config
-    return _ext.OscarLayout(
+    made = _ext.OscarLayout(
         cfg.head_dim,
         layout.kv_heads,
         layout.physical_block_tokens,
@@ -91,6 +94,8 @@ def layout_struct(layout):
         0,
         layout.stripe_page_bytes,
     )
+    object.__setattr__(layout, "_struct", made)
+    return made
 
 
 def clip_struct(cfg):
@@ -388,20 +393,18 @@ def _attention_int4(query, history, meta, layout, scale, splits, split_tokens, c
 
 def merge_splits(partials, lse, counts):
     """LSE merge of split partials (reference kernels.py:506-511) -> (bf16 out, logsum)."""
-    _device_check(partials, lse, counts)
+    device = _same_device(partials, lse=lse, counts=counts)
     n, hq, splits, d = partials.shape
-    out = torch.empty((n, hq, d), dtype=torch.bfloat16, device=partials.device)
-    logsum = torch.empty((n, hq), dtype=torch.float32, device=partials.device)
+    out = torch.empty((n, hq, d), dtype=torch.bfloat16, device=device)
+    logsum = partials.new_empty((n, hq), dtype=torch.float32)
     if n:
-        partials = partials.contiguous()
-        lse = lse.contiguous()
-        _ext.check(
-            _ext.library().oscar_merge_splits(
-                _ptr(partials), _ptr(lse), _ptr(_int32(counts, "counts")), n, hq, splits, d,
-                _ptr(out), _ptr(logsum), _stream(partials),
-            ),
-            "merge_splits",
-        )
+        if not partials.is_contiguous():
+            partials = partials.contiguous()
+        if not lse.is_contiguous():
+            lse = lse.contiguous()
+        _launch(_ext.library().oscar_merge_splits, "merge_splits", device, partials.data_ptr(),
+                lse.data_ptr(), _int32(counts, "counts").data_ptr(), n, hq, splits, d, out.data_ptr(),
+                logsum.data_ptr())
     return out, logsum
 
 
