@@ -13,6 +13,7 @@
 // A block of rows (token, head) is one workgroup: half a wavefront per row, 32 lanes of 8 dims. The
 // block's angles are gathered into LDS first, each pair from the table row of its axis' position, in
 // flight with the rows: so several axes, any table type and any pair order cost the rows nothing.
+#include "dma.h"
 #include "norm_row.h"
 #include "quant4.h"
 #include "rotate.h"
@@ -341,8 +342,468 @@ void append_kernel(const AppendArgs a, int64_t q_blocks, int64_t k_blocks) {
 // Rows up to which blocks hold 16 of them instead of 32, so that the blocks of a decode step lie on as
 // many CUs as they can.
 constexpr int64_t kSmallAppendRows = 16 * 256;
+constexpr unsigned kWalkGroups = 256;  // one per CU
 
-// ---- records back to values: a wavefront per vector.
+// ---- the same for many rows of 4-bit layouts: workgroups of 8 wavefronts, one per CU, with one of the
+// rotations in LDS (queries and keys by R_k, values by R_v, the CUs divided by their work); each wavefront
+// walks 16-row blocks of its own and needs no other. A lane loads the eight 16-byte pieces 32 m + 8 g of
+// row lane % 16 (g = lane / 16), which is what the products read as B operand, and ends with the same
+// pieces of the rotated row, so that a row goes from memory to its record in registers: 16 rows are
+// quantized at a time, four lanes each. Pairs of halves 32 dims or a multiple of it apart, and adjacent
+// ones, lie in one lane.
+constexpr int kWalkWaves = 8, kWalkThreads = kWalkWaves * kWave;
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 as_u16x2(uint32_t v) { return __builtin_bit_cast(u16x2, v); }
+__device__ __forceinline__ uint32_t as_u32(u16x2 v) { return __builtin_bit_cast(uint32_t, v); }
+
+// Sum and maximum over the four lanes of a row.
+__device__ __forceinline__ uint32_t row_sum(uint32_t v) {
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = r[0] + r[1];
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return r[0] + r[1];
+}
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(r[0], r[1]);
+}
+
+// quantize_store4 (percentile or factor) of 16 rows, four lanes each: z[m] holds dims 32 m + 8 g .. + 7 as
+// bf16. The quantile's order statistics come from a bisection of the 15-bit magnitudes, between the
+// largest one and four powers of two below it where that holds enough values.
+__device__ __forceinline__ void quantize_rows4(const u32x4 (&z)[8], int mode, float ratio, float factor,
+                                               uint8_t* codes, uint8_t* side, int g) {
+#pragma clang fp contract(off)
+  constexpr uint32_t kMagnitude = 0x7fff7fffu, kTop = 0x80008000u;
+  u16x2 top2 = as_u16x2(0u);
+  float mn = INFINITY, mx = -INFINITY;
+#pragma unroll
+  for (int m = 0; m < 8; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      top2 = __builtin_elementwise_max(top2, as_u16x2(z[m][e] & kMagnitude));
+      const float lo = __uint_as_float(z[m][e] << 16), hi = __uint_as_float(z[m][e] & 0xffff0000u);
+      mn = fminf(mn, fminf(lo, hi));
+      mx = fmaxf(mx, fmaxf(lo, hi));
+    }
+  const uint32_t top = row_max(max(static_cast<uint32_t>(top2[0]), static_cast<uint32_t>(top2[1])));
+  mn = -max_xor32(max_xor16(-mn));
+  mx = max_xor32(max_xor16(mx));
+  float thr = INFINITY;
+  if (mode == OSCAR_CLIP_FACTOR) {
+    thr = __uint_as_float(top << 16) * factor;
+  } else if (ratio != 0.0f) {
+    auto count = [&](uint32_t from) {  // magnitudes at or above `from` (1 .. 0x8000)
+      const u16x2 add = as_u16x2((0x8000u - from) * 0x10001u);
+      uint32_t c = 0;
+#pragma unroll
+      for (int m = 0; m < 8; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          c += __builtin_popcount(as_u32(as_u16x2(z[m][e] & kMagnitude) + add) & kTop);
+      return row_sum(c);
+    };
+    const float rank = ratio * 255.0f;
+    const int lo_idx = static_cast<int>(floorf(rank)), hi_idx = static_cast<int>(ceilf(rank));
+    const float weight = rank - static_cast<float>(lo_idx);
+    const uint32_t need = static_cast<uint32_t>(kHeadDim - lo_idx);
+    // count(lo) >= need > count(hi).
+    uint32_t lo = 0, hi = top + 1;
+    uint32_t mid = top > 512 ? top - 512 : (top + 1) >> 1;
+    while (__any(hi - lo > 1)) {
+      const bool open = hi - lo > 1;
+      const bool enough = count(open ? mid : 1) >= need;
+      lo = open && enough ? mid : lo;
+      hi = open && !enough ? mid : hi;
+      mid = (lo + hi) >> 1;
+    }
+    const float below = __uint_as_float(lo << 16);
+    float above = below;
+    if (hi_idx != lo_idx) {
+      const uint32_t more = count(lo + 1);
+      u16x2 next = as_u16x2(0xffffffffu);
+      const u16x2 sub = as_u16x2((lo + 1) * 0x10001u);
+#pragma unroll
+      for (int m = 0; m < 8; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          next = __builtin_elementwise_min(next, as_u16x2(z[m][e] & kMagnitude) - sub);
+      const uint32_t least = 0xffffu - row_max(0xffffu - min(static_cast<uint32_t>(next[0]),
+                                                             static_cast<uint32_t>(next[1])));
+      if (more >= static_cast<uint32_t>(kHeadDim - hi_idx)) above = __uint_as_float((least + lo + 1) << 16);
+    }
+    thr = __fmaf_rn(weight, above - below, below);
+  }
+  if (thr != INFINITY) {
+    mn = clamp1(mn, thr);
+    mx = clamp1(mx, thr);
+  }
+  float spread = (mx - mn) / 15.0f;
+  spread = spread < 6.103515625e-05f ? 6.103515625e-05f : spread;
+  if (top > 0x7f80u) spread = mn = __uint_as_float(0x7fc00000u);  // a NaN: so are the record's values
+  const uint32_t zero = float_to_f16_bits(mn), scale = float_to_f16_bits(spread);
+  const float zf = f16_bits_to_float(zero), sf = f16_bits_to_float(scale);
+  const float r = scale_rcp(sf);
+#pragma unroll
+  for (int m = 0; m < 8; ++m) {
+    float d[8], y[8];
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t w = z[m][e >> 1];
+      float x = __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+      x = __builtin_amdgcn_fmed3f(x, -thr, thr);
+      d[e] = x - zf;
+      y[e] = __builtin_fmaf(d[e], r, 0.5f);
+      near |= fabsf(y[e] - rintf(y[e])) < 1.52587890625e-05f;  // quant4.h
+    }
+    if (__any(near)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = d[e] / sf + 0.5f;
+    }
+    uint32_t packed = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      int c = static_cast<int>(y[e]);
+      c = c < 0 ? 0 : (c > 15 ? 15 : c);
+      packed |= static_cast<uint32_t>(c) << (4 * e);
+    }
+    if (codes) *reinterpret_cast<uint32_t*>(codes + 16 * m + 4 * g) = packed;
+  }
+  if (codes && g == 0) *reinterpret_cast<uint32_t*>(side) = scale | (zero << 16);
+}
+
+template <bool kAdjacent, bool kFp32>
+__global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const AppendArgs a,
+                                                                      int value_groups) {
+  __shared__ __attribute__((aligned(16))) uint8_t s_r[kHeadDim * kHeadDim * 2];
+  __shared__ __attribute__((aligned(16))) float s_weight[2][kHeadDim];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int64_t active = live_tokens(a);
+  // The last workgroups take the values, the others the keys and then the queries.
+  const int groups = static_cast<int>(gridDim.x);
+  const bool is_v = static_cast<int>(blockIdx.x) >= groups - value_groups;
+  const int mine = is_v ? groups - value_groups : 0;
+  const int64_t k_blocks = is_v ? 0 : (a.set[1].rows + 15) / 16;
+  const int64_t blocks = is_v ? (a.set[2].rows + 15) / 16 : k_blocks + (a.set[0].rows + 15) / 16;
+  const int64_t width = is_v ? value_groups : groups - value_groups;
+  const int64_t first = static_cast<int64_t>(wave) * width + (blockIdx.x - mine);
+  const int64_t step = kWalkWaves * width;
+  const int half = a.rotary >> 1;
+  auto set_of = [&](int64_t b) { return is_v ? 2 : b < k_blocks ? 1 : 0; };
+
+  u32x4 x[8];
+  int64_t row = 0, position = 0;
+  uint32_t token = 0;
+  int head = 0;
+  bool live = false, bad = false;
+  constexpr int kBytes = kFp32 ? 4 : 2, kLoads = kFp32 ? 2 : 1;
+  // Packed angles of eight consecutive dims of a half, or of the four pairs of eight adjacent dims.
+  constexpr int kWords = kAdjacent ? 2 * kLoads : 4 * kLoads;
+  auto load_words = [&](const char* at, uint32_t (&w)[kWords]) {
+    if constexpr (kWords == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(at);
+      w[0] = v.x;
+      w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const u32x4 v = reinterpret_cast<const u32x4*>(at)[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
+      }
+    }
+  };
+  auto word_value = [](const uint32_t (&w)[kWords], int i) {
+    if (kFp32) return __uint_as_float(w[i]);
+    return bf16_to_float(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
+  };
+  const char* turn = nullptr;          // the angles' table row, from the lane's first dim on
+  uint32_t cos0[kWords], sin0[kWords];  // of the first group of dims, with the row's loads
+
+  // The lane's row of block b: its token (and position), then its values.
+  auto place = [&](int64_t b) {
+    const int which = set_of(b);
+    const RowSet& t = a.set[which];
+    row = (which == 0 ? b - k_blocks : b) * 16 + n;
+    const uint32_t safe = row < t.rows ? static_cast<uint32_t>(row) : 0u;
+    token = fastdiv(safe, t.h_div);
+    head = static_cast<int>(safe - token * static_cast<uint32_t>(t.heads));
+    live = row < t.rows && token < active;
+    position = which < 2 && a.rotary && live ? a.positions[token] : 0;
+    const uint16_t* src = t.x + static_cast<int64_t>(token) * t.s0 + static_cast<int64_t>(head) * t.s1 + 8 * g;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) x[m] = *reinterpret_cast<const u32x4*>(src + 32 * m);
+  };
+  auto load_angles = [&](int64_t b) {
+    if (set_of(b) == 2) return;
+    bad = a.rotary > 0 && (position < 0 || position >= a.table_rows);
+    turn = static_cast<const char*>(a.table) +
+           ((bad ? 0 : position) * a.table_stride + (kAdjacent ? 4 * g : 8 * g)) * kBytes;
+    if (8 * g < a.rotary) {
+      load_words(turn, cos0);
+      load_words(turn + half * kBytes, sin0);
+    }
+  };
+
+  u32x4 y[8];  // the finished rows
+  // The arithmetic of norm_rope.hip's walking kernel.
+  auto finish = [&](int which) {
+    if (which == 2) {
+#pragma unroll
+      for (int m = 0; m < 8; ++m) y[m] = x[m];
+      return;
+    }
+    const float* w = s_weight[which] + 8 * g;
+    float v[8][8];
+    float inv = bad ? __uint_as_float(0x7fc00000u) : 1.f;
+    const bool norm = a.set[which].weight != nullptr;
+    if (norm) {
+      auto mean_square = [&](float eps) {
+        float sums[8];
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          float sum = 0.f;
+          unpack_eight(x[m], v[m]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum = fmaf(v[m][e], v[m][e], sum);
+          sums[m] = sum_xor32(sum_xor16(sum));
+        }
+        const float sum = ((sums[0] + sums[1]) + (sums[2] + sums[3])) +
+                          ((sums[4] + sums[5]) + (sums[6] + sums[7]));
+        return fmaf(sum, 1.0f / kHeadDim, eps);
+      };
+      float mean = mean_square(a.eps);
+      if (const float by = range_scale(mean); __any(by != 1.f)) {
+#pragma unroll
+        for (int m = 0; m < 8; ++m) x[m] = scale_eight(x[m], by);
+        mean = mean_square(a.eps * by * by);
+      }
+      inv = inverse_root(mean, bad);
+    }
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      unpack_eight(x[m], v[m]);
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(w + 32 * m);
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(w + 32 * m + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[m][e] = norm ? v[m][e] * inv * (e < 4 ? lo[e & 3] : hi[e & 3]) : v[m][e] * inv;
+    }
+    if constexpr (!kAdjacent) {
+      const int apart = half >> 5;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j >= apart) break;
+        uint32_t c[kWords], s[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          c[i] = cos0[i];
+          s[i] = sin0[i];
+        }
+        if (j) {
+          load_words(turn + 32 * j * kBytes, c);
+          load_words(turn + (32 * j + half) * kBytes, s);
+        }
+        auto rotate_pair = [&](float (&lo)[8], float (&hi)[8]) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float co = word_value(c, e), si = word_value(s, e);
+            const float l = lo[e], h = hi[e];
+            lo[e] = fmaf(l, co, -h * si);
+            hi[e] = fmaf(h, co, l * si);
+          }
+        };
+        // The other half is 1 to 4 pieces on: constant indexes, so that the rows stay in registers.
+        if (apart == 1)
+          rotate_pair(v[j], v[j + 1]);
+        else if (apart == 2)
+          rotate_pair(v[j], v[j + 2]);
+        else if (apart == 3)
+          rotate_pair(v[j], v[j + 3]);
+        else
+          rotate_pair(v[j], v[j + 4]);
+      }
+    } else {
+#pragma unroll
+      for (int m = 0; m < 8; ++m) {
+        if (32 * m + 8 * g < a.rotary) {
+          uint32_t c[kWords], s[kWords];
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            c[i] = cos0[i];
+            s[i] = sin0[i];
+          }
+          if (m) {
+            load_words(turn + 16 * m * kBytes, c);
+            load_words(turn + (16 * m + half) * kBytes, s);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float co = word_value(c, e >> 1), si = word_value(s, e >> 1);
+            const float l = v[m][e], h = v[m][e + 1];
+            v[m][e] = fmaf(l, co, -h * si);
+            v[m][e + 1] = fmaf(h, co, l * si);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < 8; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[m][e] = live ? pack_bf16x2(v[m][2 * e], v[m][2 * e + 1]) : 0u;
+  };
+
+  if (first < blocks) place(first);
+  float weight[8];
+  const bool stages = tid < 64 && a.set[tid >> 5].weight;
+  if (stages) load_eight(a.set[tid >> 5].weight, 8 * (tid & 31), a.weight_fp32, weight);
+  if (first < blocks) load_angles(first);
+  // Row 16 t + i of the LDS copy is the column of R that lane i's A operand of tile t reads, 32 (t / 2)
+  // + 8 (i / 4) + 4 (t % 2) + i % 4, so that a lane ends with eight consecutive columns of a row in two
+  // tiles; its 16-byte piece p lies at p ^ i (norm_rope.hip).
+  const uint16_t* rt = a.rt[is_v ? 2 : 1];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int q = 2 * (16 * wave + j) + (lane >> 5), t = q >> 4, i = q & 15;
+    const int col = 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(rt + col * kHeadDim + 8 * ((lane & 31) ^ i)),
+        (__attribute__((address_space(3))) void*)(s_r + 1024 * (16 * wave + j)), 16, 0, 0);
+  }
+  if (stages)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_weight[tid >> 5][8 * (tid & 31) + e] = weight[e] + a.offset;
+  OSCAR_WAIT_VM0_SEEN();
+  __syncthreads();  // R and the weights
+  for (int64_t b = first; b < blocks; b += step) {
+    const int which = set_of(b);
+    finish(which);
+    const int64_t my_row = row;
+    const int64_t slot = which && live ? a.slots[token] : -1;
+    const int my_head = head;
+    if (b + step < blocks) {
+      place(b + step);
+      load_angles(b + step);
+    }
+    const RowSet& t = a.set[which];
+    const bool in = my_row < t.rows;
+    if (which < 2 && in) {
+      uint16_t* out = t.out + my_row * kHeadDim + 8 * g;
+#pragma unroll
+      for (int m = 0; m < 8; ++m) *reinterpret_cast<u32x4*>(out + 32 * m) = y[m];
+    }
+    if (!which && !a.q_rot) continue;
+    u32x4 z[8];
+    const uint8_t* from[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) from[m] = s_r + 512 * n + 16 * ((4 * m + g) ^ n);
+    // Eight operands (four products of two tiles) are read ahead of the eight in use.
+    u32x4 f[2][8];
+    auto read = [&](int i, u32x4 (&w)[8]) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        w[k] = *reinterpret_cast<const u32x4*>(from[k >> 1] + 8192 * (2 * (i >> 1) + (k & 1)) +
+                                               256 * (i & 1));
+    };
+    read(0, f[0]);
+    f32x4 acc[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i < 15) read(i + 1, f[(i + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (!(i & 1)) acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        acc[k & 1] = mfma16x16x32(f[i & 1][k], y[4 * (i & 1) + (k >> 1)], acc[k & 1]);
+      if (i & 1)
+        z[i >> 1] = u32x4{pack_bf16x2(acc[0][0], acc[0][1]), pack_bf16x2(acc[0][2], acc[0][3]),
+                          pack_bf16x2(acc[1][0], acc[1][1]), pack_bf16x2(acc[1][2], acc[1][3])};
+    }
+    if (!which) {
+      uint16_t* out = a.q_rot + my_row * kHeadDim + 8 * g;
+      if (in)
+#pragma unroll
+        for (int m = 0; m < 8; ++m) *reinterpret_cast<u32x4*>(out + 32 * m) = z[m];
+      continue;
+    }
+    uint8_t* record = nullptr;
+    if (slot >= 0 && slot < a.history_bytes) {
+      const int64_t at = slot_offset(a.L, slot, my_head);
+      if (at + a.L.slot_bytes <= a.history_bytes) record = a.history + at;
+    }
+    uint8_t* codes = record ? record + (which - 1) * kCodes4 : nullptr;
+    quantize_rows4(z, a.mode, a.ratio[which], a.factor[which], codes,
+                   record ? record + kSide4 + 4 * (which - 1) : nullptr, g);
+  }
+}
+
+// ---- the angles of tokens with several positions as a table of their own, one row per token, and its row
+// numbers (-1 where a position lies outside the table): then every kernel of single positions serves them.
+struct ComposeArgs {
+  const void* table;
+  int64_t table_rows, table_stride;
+  const int64_t* positions;
+  int64_t position_stride, n;
+  const int32_t* axes;
+  const int32_t* counts;
+  int32_t axis_count, rotary, fp32;
+  FastDiv rotary_div;
+  void* out;
+  int64_t* rows;
+};
+
+// kPer elements a thread (8: of one half, and 16-byte stores; 1: any rotary dims).
+template <int kPer>
+__global__ __launch_bounds__(kThreads) void compose_angles_kernel(const ComposeArgs a) {
+  const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t token = fastdiv(i, a.rotary_div);  // by the threads of a token
+  const int64_t active = a.counts ? min(static_cast<int64_t>(max(a.counts[1], 0)), a.n) : a.n;
+  if (token >= active) return;
+  const int e0 = static_cast<int>(i - token * a.rotary_div.divisor) * kPer, half = a.rotary >> 1;
+  const int pair = e0 < half ? e0 : e0 - half;
+  int axis[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) axis[k] = a.axes[pair + k];
+  float v[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const bool known = axis[k] >= 0 && axis[k] < a.axis_count;
+    const int64_t p = known ? a.positions[axis[k] * a.position_stride + token] : -1;
+    v[k] = p >= 0 && p < a.table_rows ? load_value(a.table, p * a.table_stride + e0 + k, a.fp32)
+                                      : __uint_as_float(0x7fc00000u);
+  }
+  const int64_t at = static_cast<int64_t>(token) * a.rotary + e0;
+  if constexpr (kPer == 8) {
+    if (a.fp32) {
+      f32x4* out = reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at);
+      out[0] = f32x4{v[0], v[1], v[2], v[3]};
+      out[1] = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + at) =
+          u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                pack_bf16x2(v[6], v[7])};
+    }
+  } else if (a.fp32) {
+    static_cast<float*>(a.out)[at] = v[0];
+  } else {
+    static_cast<uint16_t*>(a.out)[at] = static_cast<uint16_t>(float_to_bf16(v[0]));
+  }
+  if (e0 == 0) {
+    bool bad = false;
+    for (int k = 0; k < a.axis_count; ++k) {
+      const int64_t p = a.positions[k * a.position_stride + token];
+      bad |= p < 0 || p >= a.table_rows;
+    }
+    a.rows[token] = bad ? -1 : static_cast<int64_t>(token);
+  }
+}
+
+// ---- records back to values: half a wavefront per record, 8 dims a lane of either vector, two records.
 struct ReadArgs {
   const uint8_t* history;
   int64_t history_bytes;
@@ -352,40 +813,54 @@ struct ReadArgs {
   Layout L;
   uint16_t* out[2];
 };
+constexpr int kReadPer = 2, kReadItems = 8 * kReadPer;  // records of a half wavefront, of a workgroup
 
+template <int kBits>
 __global__ __launch_bounds__(kThreads) void read_records_kernel(const ReadArgs a) {
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 2 + (wave >> 1);
-  const int is_v = wave & 1;
-  if (item >= a.items) return;
-  const uint32_t token = fastdiv(static_cast<uint32_t>(item), a.h_div);
-  const int head = static_cast<int>(item - static_cast<int64_t>(token) * a.L.kv_heads);
-  const int64_t slot = a.slots[token];
-  uint2 bits = make_uint2(0u, 0u);
-  if (slot >= 0 && slot < a.history_bytes) {
-    const int64_t at = slot_offset(a.L, slot, head);
-    if (at + a.L.slot_bytes <= a.history_bytes) {
-      const uint8_t* p = a.history + at;
-      uint32_t codes, side;
-      float value[4];
-      if (a.L.bits == 4) {
-        codes = reinterpret_cast<const uint16_t*>(p + is_v * kCodes4)[lane];
-        side = *reinterpret_cast<const uint32_t*>(p + kSide4 + 4 * is_v);
-      } else {
-        codes = p[is_v * a.L.vector_bytes + lane];
-        side = *reinterpret_cast<const uint32_t*>(p + is_v * a.L.vector_bytes + kHeadDim / 4);
-      }
-      const float scale = half_lo_to_float(side), zero = half_hi_to_float(side);
+  const int l = threadIdx.x & 31, mine = threadIdx.x >> 5;
+  const int64_t item0 = static_cast<int64_t>(blockIdx.x) * kReadItems + mine;
+  uint32_t codes[kReadPer][2] = {}, side[kReadPer][2] = {};  // no record: zeros
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t c = a.L.bits == 4 ? codes >> (4 * e) & 15u : codes >> (2 * e) & 3u;
-        // As the oracle decodes: the product is rounded before the sum.
-        value[e] = __fadd_rn(__fmul_rn(static_cast<float>(c), scale), zero);
+  for (int i = 0; i < kReadPer; ++i) {
+    const int64_t item = item0 + 8 * i;
+    if (item >= a.items) break;
+    const uint32_t token = fastdiv(static_cast<uint32_t>(item), a.h_div);
+    const int64_t slot = a.slots[token];
+    if (slot < 0 || slot >= a.history_bytes) continue;
+    const int64_t at = slot_offset(
+        a.L, slot, static_cast<int>(item - static_cast<int64_t>(token) * a.L.kv_heads));
+    if (at + a.L.slot_bytes > a.history_bytes) continue;
+    const uint8_t* p = a.history + at;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      if (kBits == 4) {
+        codes[i][v] = reinterpret_cast<const uint32_t*>(p + v * kCodes4)[l];
+        side[i][v] = *reinterpret_cast<const uint32_t*>(p + kSide4 + 4 * v);
+      } else {
+        codes[i][v] = reinterpret_cast<const uint16_t*>(p + v * a.L.vector_bytes)[l];
+        side[i][v] = *reinterpret_cast<const uint32_t*>(p + v * a.L.vector_bytes + kHeadDim / 4);
       }
-      bits = make_uint2(pack_bf16x2(value[0], value[1]), pack_bf16x2(value[2], value[3]));
     }
   }
-  *reinterpret_cast<uint2*>(a.out[is_v] + item * kHeadDim + 4 * lane) = bits;
+#pragma unroll
+  for (int i = 0; i < kReadPer; ++i) {
+    const int64_t item = item0 + 8 * i;
+    if (item >= a.items) break;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const float scale = half_lo_to_float(side[i][v]), zero = half_hi_to_float(side[i][v]);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t c = codes[i][v] >> (kBits * e) & ((1u << kBits) - 1);
+        // As the oracle decodes: the product is rounded before the sum.
+        x[e] = __fadd_rn(__fmul_rn(static_cast<float>(c), scale), zero);
+      }
+      *reinterpret_cast<u32x4*>(a.out[v] + item * kHeadDim + 8 * l) =
+          u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                pack_bf16x2(x[6], x[7])};
+    }
+  }
 }
 
 inline bool aligned(const void* p, uintptr_t by) { return reinterpret_cast<uintptr_t>(p) % by == 0; }
@@ -396,8 +871,44 @@ RowSet row_set(const void* x, int64_t s0, int64_t s1, const void* weight, void* 
           static_cast<int32_t>(heads), make_fastdiv(static_cast<uint32_t>(heads))};
 }
 
+// The workgroups for the values such that the longer of both kinds' walks is shortest: rounds of the
+// wavefronts, in which a block of keys or values (with the quantizer) costs about twice one of queries that
+// are rotated, which costs twice those that are not.
+int value_groups_of(int64_t q_blocks, int64_t kv_blocks, bool rotated) {
+  const int64_t q_cost = rotated ? 2 : 1;
+  auto rounds = [](int64_t b, int64_t groups) { return (b + kWalkWaves * groups - 1) / (kWalkWaves * groups); };
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int g = 1; g < static_cast<int>(kWalkGroups); ++g) {
+    const int64_t rest = kWalkGroups - g, keys = rounds(kv_blocks, rest);
+    const int64_t qk = 4 * keys + q_cost * (rounds(q_blocks + kv_blocks, rest) - keys);
+    const int64_t v = 4 * rounds(kv_blocks, g), time = v > qk ? v : qk;
+    if (time < least) {
+      least = time;
+      best = g;
+    }
+  }
+  return best;
+}
+
+// Whether append_walk_kernel serves the call: 4-bit records, no clip search, and pairs in one lane.
+bool walks(const AppendArgs& a) {
+  const bool rows16 = !a.rotary || (aligned(a.table, 16) && a.table_stride % 8 == 0);
+  return a.set[2].rows && a.L.bits == 4 && a.mode != OSCAR_CLIP_SEARCH && rows16 &&
+         (a.adjacent ? a.rotary % 8 == 0 : a.rotary % 64 == 0) && a.axis_count <= 1;
+}
+
 }  // namespace
 }  // namespace oscar
+
+extern "C" int64_t oscar_rope_scratch_bytes(int64_t n, int64_t hq, int64_t hk, int32_t store,
+                                            int32_t rotary_dim, int32_t table_fp32,
+                                            int32_t axis_count) {
+  using namespace oscar;
+  if (axis_count < 2 || rotary_dim <= 0 || n * (hq + hk + (store ? hk : 0)) <= kSmallAppendRows)
+    return 0;
+  return (n * 8 + 15) / 16 * 16 + n * rotary_dim * (table_fp32 ? 4 : 2);
+}
 
 extern "C" int oscar_rope_append(
     const void* query, int64_t q_s0, int64_t q_s1, const void* key, int64_t k_s0, int64_t k_s1,
@@ -407,7 +918,8 @@ extern "C" int oscar_rope_append(
     int32_t rotary_dim, int32_t interleaved, const int64_t* positions, int64_t position_stride,
     int32_t axis_count, const int32_t* axes, const int32_t* counts, void* q_out, void* k_out,
     const void* rk_t, const void* rv_t, void* q_rot, void* history, int64_t history_bytes,
-    const int64_t* slots, const oscar_layout* layout, const oscar_clip* clip, void* stream) {
+    const int64_t* slots, const oscar_layout* layout, const oscar_clip* clip, void* scratch,
+    int64_t scratch_bytes, void* stream) {
   using namespace oscar;
   const bool store = value != nullptr;
   AppendArgs a{};
@@ -442,6 +954,39 @@ extern "C" int oscar_rope_append(
   if (store && (v_s0 % 8 || v_s1 % 8 || !aligned(value, 16) || !aligned(rv_t, 16) ||
                 !aligned(history, 16)))
     return OSCAR_E_ALIGN;
+  const int64_t need = oscar_rope_scratch_bytes(n, hq, hk, store, rotary_dim, table_fp32, axis_count);
+  if (need && n > (0xffffffffll - kThreads) / rotary_dim) return OSCAR_E_SHAPE;
+  if (need && !scratch) return OSCAR_E_NULL;
+  if (scratch_bytes < need) return OSCAR_E_SHAPE;
+  if (need && !aligned(scratch, 16)) return OSCAR_E_ALIGN;
+  hipStream_t s = as_stream(stream);
+  if (need) {
+    // Row numbers, then the angles.
+    const int64_t rows_bytes = (n * 8 + 15) / 16 * 16;
+    ComposeArgs c{cos_sin, table_rows, table_stride, positions, position_stride, n, axes, counts,
+                  axis_count, rotary_dim, table_fp32 ? 1 : 0, {},
+                  static_cast<char*>(scratch) + rows_bytes, static_cast<int64_t*>(scratch)};
+    auto compose = [&](auto kernel, int per) {
+      c.rotary_div = make_fastdiv(static_cast<uint32_t>(rotary_dim / per));
+      const int64_t threads = n * (rotary_dim / per);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((threads + kThreads - 1) / kThreads)),
+                         dim3(kThreads), 0, s, c);
+    };
+    rotary_dim % 16 ? compose(compose_angles_kernel<1>, 1) : compose(compose_angles_kernel<8>, 8);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return static_cast<int>(err);
+    cos_sin = c.out;
+    table_rows = n;
+    table_stride = rotary_dim;
+    positions = c.rows;
+    axis_count = 1;
+  }
+  const int64_t all = n * (hq + hk + (store ? hk : 0));
+  if (!store && query && q_weight && rotary_dim && all > kSmallAppendRows)
+    return oscar_qk_norm_rope(query, q_s0, q_s1, key, k_s0, k_s1, n, hq, hk, q_weight, k_weight,
+                              weight_fp32, unit_offset, eps, cos_sin, table_rows, table_stride,
+                              table_fp32, rotary_dim, interleaved, positions, counts, q_out, k_out,
+                              q_rot ? rk_t : nullptr, q_rot, stream);
   if (query) a.set[0] = row_set(query, q_s0, q_s1, q_weight, q_out, n, hq);
   a.set[1] = row_set(key, k_s0, k_s1, k_weight, k_out, n, hk);
   if (store) a.set[2] = row_set(value, v_s0, v_s1, nullptr, nullptr, n, hk);
@@ -475,14 +1020,21 @@ extern "C" int oscar_rope_append(
     a.factor[1] = clip->k_factor;
     a.factor[2] = clip->v_factor;
   }
-  hipStream_t s = as_stream(stream);
-  const int64_t all = a.set[0].rows + a.set[1].rows + a.set[2].rows;
   auto blocks = [&](int i, int64_t rows) { return (a.set[i].rows + rows - 1) / rows; };
   auto lds = [&](int rows) { return static_cast<uint32_t>(rows * rotary_dim * sizeof(float)); };
   if (!q_rot && !store) {
     const int64_t q = blocks(0, kTurnRows), grid = q + blocks(1, kTurnRows);
     hipLaunchKernelGGL(turn_rows_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
                        lds(kTurnRows + 8), s, a, q);
+  } else if (all > kSmallAppendRows && walks(a)) {
+    const int value_groups = value_groups_of(blocks(0, 16), blocks(1, 16), q_rot != nullptr);
+    auto walk = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(kWalkGroups), dim3(kWalkThreads), 0, s, a, value_groups);
+    };
+    if (a.adjacent || !rotary_dim)
+      table_fp32 ? walk(append_walk_kernel<true, true>) : walk(append_walk_kernel<true, false>);
+    else
+      table_fp32 ? walk(append_walk_kernel<false, true>) : walk(append_walk_kernel<false, false>);
   } else if (all <= kSmallAppendRows) {
     const int64_t q = blocks(0, 16), k = blocks(1, 16);
     hipLaunchKernelGGL(append_kernel<1>, dim3(static_cast<unsigned>(q + k + blocks(2, 16))),
@@ -505,9 +1057,9 @@ extern "C" int oscar_read_records(const void* history, int64_t history_bytes, co
   if (st != OSCAR_OK) return st;
   if (n == 0) return OSCAR_OK;
   if (!history || !slots || !key_out || !value_out) return OSCAR_E_NULL;
-  // 128 threads an item, fewer than 2^32 a launch.
-  if (a.L.kv_heads > 0x1ffffffll / n) return OSCAR_E_SHAPE;
-  if (!aligned(history, 4) || !aligned(key_out, 8) || !aligned(value_out, 8)) return OSCAR_E_ALIGN;
+  // 16 threads an item, fewer than 2^32 a launch.
+  if (a.L.kv_heads > 0x7ffffffll / n) return OSCAR_E_SHAPE;
+  if (!aligned(history, 4) || !aligned(key_out, 16) || !aligned(value_out, 16)) return OSCAR_E_ALIGN;
   a.history = static_cast<const uint8_t*>(history);
   a.history_bytes = history_bytes;
   a.slots = slots;
@@ -515,7 +1067,10 @@ extern "C" int oscar_read_records(const void* history, int64_t history_bytes, co
   a.h_div = make_fastdiv(static_cast<uint32_t>(a.L.kv_heads));
   a.out[0] = static_cast<uint16_t*>(key_out);
   a.out[1] = static_cast<uint16_t*>(value_out);
-  hipLaunchKernelGGL(read_records_kernel, dim3(static_cast<unsigned>((a.items + 1) / 2)),
-                     dim3(kThreads), 0, as_stream(stream), a);
+  const dim3 grid(static_cast<unsigned>((a.items + kReadItems - 1) / kReadItems));
+  if (a.L.bits == 4)
+    hipLaunchKernelGGL(read_records_kernel<4>, grid, dim3(kThreads), 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL(read_records_kernel<2>, grid, dim3(kThreads), 0, as_stream(stream), a);
   return static_cast<int>(hipGetLastError());
 }

@@ -24,6 +24,7 @@ struct Quantized4 {
 __device__ __forceinline__ Quantized4 quantize4(const float x[4], float thr, float mn, float mx,
                                                 float (&code)[4], float& sf, float& zf) {
 #pragma clang fp contract(off)
+  const bool whole = mn == mn && mx == mx;  // no NaN (wave_min_max has one as an extreme)
   float xc[4];
   if (thr == INFINITY) {
 #pragma unroll
@@ -35,6 +36,7 @@ __device__ __forceinline__ Quantized4 quantize4(const float x[4], float thr, flo
   }
   float spread = (mx - mn) / 15.0f;
   spread = spread < 6.103515625e-05f ? 6.103515625e-05f : spread;
+  if (!whole) spread = mn = __uint_as_float(0x7fc00000u);  // so are the record's values
   Quantized4 q;
   q.zero = float_to_f16_bits(mn);
   q.scale = float_to_f16_bits(spread);

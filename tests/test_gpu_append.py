@@ -219,14 +219,51 @@ def test_rows_and_records(n, live, hq, hk, norm, rotary, interleaved, bits):
         assert not bool(got_rows[dead].any())
 
 
+@pytest.mark.parametrize("rotary,interleaved", [(64, False), (128, False), (192, False), (256, False), (0, False),
+                                                (8, True), (96, True), (256, True), (32, False), (20, False)])
+@pytest.mark.parametrize("n,live,hq,hk,axes", [(700, 700, 6, 1, 1), (1100, 1001, 3, 2, 3), (5000, 4999, 1, 1, 2)])
+def test_many_rows(rotary, interleaved, n, live, hq, hk, axes):
+    """The walk over many rows gives what few rows at a time give, bit for bit, NaN rows and all."""
+    for table, weight, norm, rotate in ((torch.float32, torch.bfloat16, True, True),
+                                        (torch.bfloat16, torch.float32, True, False),
+                                        (torch.bfloat16, torch.float32, False, True)):
+        m = list(make(n, hq, hk, rotary, axes, table=table, weight=weight))
+        layout = layout_of(hk, k_clip_ratio=0.97, v_clip_ratio=0.99)
+        history, slots = cache(n, layout, n // 768 + 2)
+        slots[live // 3] = -1
+        if rotary:
+            m[5][axes - 1, 400], m[5][0, 90] = m[4].shape[0], -1
+        if rotary == 0:
+            m[4] = torch.zeros(1, 0, device=DEV)
+        args = dict(norm=norm, axes=axes > 1, interleaved=interleaved, rotate_query=rotate)
+        got = append(m, layout, history, slots, counts_of(live), **args)
+        small = torch.full_like(history, 171)
+        rows = [None if x is None else torch.empty_like(x) for x in got]
+        step = 300
+        for t0 in range(0, n, step):
+            part = [x[t0 : t0 + step] for x in m[:3]] + m[3:5] + [m[5][:, t0 : t0 + step]] + m[6:]
+            one = append(part, layout, small, slots[t0 : t0 + step].clone(),
+                         counts_of(max(0, min(live - t0, step))), **args)
+            for x, y in zip(rows, one):
+                if x is not None:
+                    x[t0 : t0 + step] = y
+        for x, y in zip(got, rows):
+            assert (x is None and y is None) or torch.equal(x.view(torch.int16), y.view(torch.int16))
+        assert torch.equal(history, small)
+        if rotary:
+            assert bool(got[1][400].isnan().all()) and bool(got[1][90].isnan().all())
+            key, value = kernels.read_records(history, slots, layout)
+            assert bool(key[400].isnan().all()) and bool(value[400].isfinite().all())
+
+
 @pytest.mark.parametrize("mode,k,v", [("factor", 0.8, 1.0), ("percentile", 0, 0.875), ("percentile", 1.0, 0.93)])
-def test_clip_modes(mode, k, v):
-    n = 70
+@pytest.mark.parametrize("n", [70, 1500])
+def test_clip_modes(mode, k, v, n):
     m = make(n, 3, 1, 64)
     config = (dict(k_clip_factor=k, v_clip_factor=v) if mode == "factor"
               else dict(k_clip_ratio=k, v_clip_ratio=v))
     layout = layout_of(1, clip_mode=mode, **config)
-    history, slots = cache(n, layout, 2)
+    history, slots = cache(n, layout, 3)
     got = append(m, layout, history, slots, counts_of(n), axes=False)
     rotated = kernels.rotate(got[1], m[7].T), kernels.rotate(m[2], m[8].T)
     parts, _ = record_parts(history, layout, slots)
@@ -314,14 +351,16 @@ def test_strides_and_slots_outside_the_buffer():
     assert not bool(key[3:5].any()) and not bool(value[3:5].any())
 
 
-def test_extreme_rows():
+@pytest.mark.parametrize("n", [8, 1400])
+def test_extreme_rows(n):
     """Rows of zeros, equal values, tiny and huge ones: records of the same steps in torch."""
-    n = 8
     m = list(make(n, 1, 1, 64))
     value = m[2].clone()
     value[0], value[1], value[2], value[3] = 0, 1.5, value[2] * 2.0**-30, value[3] * 2.0**12
     value[4], value[5, 0, 0] = -value[4].abs(), 3e4
     m[2] = value
+    value[6] = 0  # nearly every value equal, a few far out: a threshold in the lowest bits
+    value[6, 0, 3:9] = 2.0**20
     layout = layout_of(1)
     history, slots = cache(n, layout, 2)
     append(m, layout, history, slots, counts_of(n), axes=False)
@@ -330,10 +369,13 @@ def test_extreme_rows():
     want = codes_of(x, layout.config, layout.config.v_clip_ratio, 1.0)
     assert torch.equal(scale, want[1][..., 0]) and torch.equal(zero, want[2][..., 0])
     assert torch.equal(codes, want[0].to(torch.uint8))
+    m[2][7, 0, 17] = float("nan")
+    append(m, layout, history, slots, counts_of(n), axes=False)
+    assert bool(kernels.read_records(history, slots[7:8], layout)[1].isnan().all())
 
 
-def test_a_captured_append_replays():
-    n = 40
+@pytest.mark.parametrize("n", [40, 900])
+def test_a_captured_append_replays(n):
     m = make(n, 6, 1, 64, 3)
     layout = layout_of(1)
     history, slots = cache(n, layout, 2)
@@ -342,7 +384,7 @@ def test_a_captured_append_replays():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         got = append(m, layout, history, slots, counts)
-    for live in (40, 1, 0, 33, 40):
+    for live in (n, 1, 0, 33, n):
         counts[1] = live
         m[5].copy_(m[5].roll(1, 1))
         slots.copy_(slots.roll(3))
