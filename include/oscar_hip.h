@@ -686,11 +686,8 @@ int oscar_shared_history(const void* query, int64_t q_s0, int64_t q_s1, int64_t 
  * q_rot (optional): rotate(q_out, R_k). With value: for every token t < counts[1] with slots[t] >= 0 the
  * record of rotate(k_out, R_k) and rotate(value, R_v), clipped as `clip` says; 2-bit layouts get the
  * bytes of oscar_store_int2. Live tokens' slots differ. rk_t, rv_t: R^T, contiguous bf16 [256][256].
- * counts: optional without value. scratch (16-byte aligned): oscar_rope_scratch_bytes of the same sizes
- * (store: whether value is given), 0 for few rows and for one position a token.
+ * counts: optional without value.
  */
-int64_t oscar_rope_scratch_bytes(int64_t n, int64_t hq, int64_t hk, int32_t store, int32_t rotary_dim,
-                                 int32_t table_fp32, int32_t axis_count);
 int oscar_rope_append(const void* query, int64_t q_s0, int64_t q_s1, const void* key, int64_t k_s0,
                       int64_t k_s1, const void* value, int64_t v_s0, int64_t v_s1, int64_t n,
                       int64_t hq, int64_t hk, const void* q_weight, const void* k_weight,
@@ -700,7 +697,7 @@ int oscar_rope_append(const void* query, int64_t q_s0, int64_t q_s1, const void*
                       int32_t axis_count, const int32_t* axes, const int32_t* counts, void* q_out,
                       void* k_out, const void* rk_t, const void* rv_t, void* q_rot, void* history,
                       int64_t history_bytes, const int64_t* slots, const oscar_layout* layout,
-                      const oscar_clip* clip, void* scratch, int64_t scratch_bytes, void* stream);
+                      const oscar_clip* clip, void* stream);
 
 /*
  * read_records -- the values that the records of `slots` (int64 [n]) stand for, in the rotated basis:

@@ -208,9 +208,8 @@ SIGNATURES = {
         _P, _I64, _I64, _I32, _I32, _I32,  # cos_sin, rows, stride, fp32, rotary dim, interleaved
         _P, _I64, _I32, _P, _P, _P, _P,  # positions, stride, axis count, axes, counts, q out, k out
         _P, _P, _P, _P, _I64, _P,  # rk_t, rv_t, q rot, history, bytes, slots
-        POINTER(OscarLayout), POINTER(OscarClip), _P, _I64, _P,  # layout, clip, scratch, bytes, stream
+        POINTER(OscarLayout), POINTER(OscarClip), _P,  # layout, clip, stream
     ],
-    "oscar_rope_scratch_bytes": [_I64, _I64, _I64, _I32, _I32, _I32, _I32],
     "oscar_read_records": [_P, _I64, _P, _I64, POINTER(OscarLayout), _P, _P, _P],
     "oscar_history_int4": [
         _P, _I64, _I64, _I64, _P, _I64,  # query, history
@@ -220,7 +219,7 @@ SIGNATURES = {
     ],
 }
 RESTYPES = {"oscar_noalloc_scratch_bytes": c_int64, "oscar_calibration_workspace_bytes": c_int64,
-            "oscar_history_chunk_tiles": c_int64, "oscar_rope_scratch_bytes": c_int64, "oscar_shared_capacity": c_int64}
+            "oscar_history_chunk_tiles": c_int64, "oscar_shared_capacity": c_int64}
 NOALLOC_SCRATCH_BYTES = 32 << 20  # OSCAR_NOALLOC_SCRATCH_BYTES
 
 _lib = None

@@ -19,6 +19,13 @@
 #include "rotate.h"
 
 namespace oscar {
+
+bool launch_norm_rope_axes(const void* query, int64_t q_s0, int64_t q_s1, const void* key, int64_t k_s0,
+                           int64_t k_s1, int64_t n, int64_t hq, int64_t hk, const void* q_weight,
+                           const void* k_weight, bool weight_fp32, bool unit_offset, float eps,
+                           bool table_fp32, bool interleaved, const int32_t* counts, void* q_out,
+                           void* k_out, const AxisTable& axes, hipStream_t s);  // norm_rope.hip
+
 namespace {
 
 constexpr int kMostAxes = 32;  // a lane of the half wavefront checks an axis' position
@@ -35,14 +42,10 @@ struct RowSet {
 
 struct AppendArgs {
   RowSet set[3];      // queries, keys, values
-  const void* table;  // [table_rows][rotary]: cos of every pair, then sin
-  int64_t table_rows, table_stride;
-  const int64_t* positions;  // axis a of token t at a * position_stride + t
-  int64_t position_stride;
-  const int32_t* axes;  // axis of every pair; null: axis 0
+  AxisTable angles;   // axes null: axis 0 of every pair
   const int32_t* counts;
   int64_t n;
-  int32_t axis_count, rotary, table_fp32, weight_fp32, adjacent;
+  int32_t rotary, table_fp32, weight_fp32, adjacent;
   FastDiv rotary_div;
   float offset, eps;
   const uint16_t* rt[3];  // R^T of each set, contiguous [256][256]; null: no rotation
@@ -69,12 +72,13 @@ __device__ __forceinline__ void gather_angles(const AppendArgs& a, int64_t first
   for (int i = threadIdx.x; i < tokens * a.rotary; i += kThreadsA) {
     const int t = static_cast<int>(fastdiv(static_cast<uint32_t>(i), a.rotary_div));
     const int e = i - t * a.rotary;
-    const int axis = a.axes ? a.axes[e < half ? e : e - half] : 0;
+    const AxisTable& table = a.angles;
+    const int axis = table.axes ? table.axes[e < half ? e : e - half] : 0;
     const int64_t token = first_token + t;
     float v = __uint_as_float(0x7fc00000u);
-    if (token < active && axis >= 0 && axis < a.axis_count) {
-      const int64_t p = a.positions[axis * a.position_stride + token];
-      if (p >= 0 && p < a.table_rows) v = load_value(a.table, p * a.table_stride + e, a.table_fp32);
+    if (token < active && axis >= 0 && axis < table.count) {
+      const int64_t p = table.positions[axis * table.position_stride + token];
+      if (p >= 0 && p < table.rows) v = load_value(table.table, p * table.stride + e, a.table_fp32);
     }
     s_turn[i] = v;
   }
@@ -170,12 +174,8 @@ __device__ __forceinline__ void load_weights(const AppendArgs& a, const RowSet& 
 }
 
 // Whether some position of the token lies outside the table (the same for the half wavefront).
-__device__ __forceinline__ bool bad_position(const AppendArgs& a, int64_t token, bool live, int l) {
-  bool out = false;
-  if (a.rotary && live && l < a.axis_count) {
-    const int64_t p = a.positions[l * a.position_stride + token];
-    out = p < 0 || p >= a.table_rows;
-  }
+__device__ __forceinline__ bool bad_token(const AppendArgs& a, int64_t token, bool live, int l) {
+  const bool out = a.rotary && live && l < a.angles.count && bad_position(a.angles, token, l);
   const uint64_t any = __ballot(out);
   return ((any >> (threadIdx.x & 32)) & 0xffffffffull) != 0;
 }
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void turn_rows_kernel(const AppendArgs a,
   const int tokens = static_cast<int>(fastdiv(static_cast<uint32_t>(last_row), t.h_div) - first) + 1;
 #pragma unroll
   for (int i = 0; i < kTurnPerHalf; ++i)
-    bad[i] = bad_position(a, token[i], token[i] < active, l);
+    bad[i] = bad_token(a, token[i], token[i] < active, l);
   gather_angles<kThreads>(a, first, tokens, active, s_angles);
   __syncthreads();
   float* s_y = s_angles + kTurnRows * a.rotary + mine * a.rotary;
@@ -288,7 +288,7 @@ void append_kernel(const AppendArgs a, int64_t q_blocks, int64_t k_blocks) {
       const int64_t last_row = min(r0 + kRows, t.rows) - 1;
       const int tokens =
           static_cast<int>(fastdiv(static_cast<uint32_t>(last_row), t.h_div) - first) + 1;
-      bad = bad_position(a, token, has_row && token < active, l);
+      bad = bad_token(a, token, has_row && token < active, l);
       gather_angles<kAppendThreads>(a, first, tokens, active, s_angles);
       __syncthreads();
     }
@@ -476,7 +476,7 @@ __device__ __forceinline__ void quantize_rows4(const u32x4 (&z)[8], int mode, fl
   if (codes && g == 0) *reinterpret_cast<uint32_t*>(side) = scale | (zero << 16);
 }
 
-template <bool kAdjacent, bool kFp32>
+template <bool kAdjacent, bool kFp32, bool kAxes>
 __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const AppendArgs a,
                                                                       int value_groups) {
   __shared__ __attribute__((aligned(16))) uint8_t s_r[kHeadDim * kHeadDim * 2];
@@ -504,25 +504,40 @@ __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const Appe
   constexpr int kBytes = kFp32 ? 4 : 2, kLoads = kFp32 ? 2 : 1;
   // Packed angles of eight consecutive dims of a half, or of the four pairs of eight adjacent dims.
   constexpr int kWords = kAdjacent ? 2 * kLoads : 4 * kLoads;
-  auto load_words = [&](const char* at, uint32_t (&w)[kWords]) {
-    if constexpr (kWords == 2) {
-      const uint2 v = *reinterpret_cast<const uint2*>(at);
-      w[0] = v.x;
-      w[1] = v.y;
+  const char* turn = nullptr;  // the angles' table row
+  int64_t turn_token = 0;      // or the token that has several
+  // Angles of the lane's group j of dims (32 j + 8 g on).
+  auto load_words = [&](int j, uint32_t (&c)[kWords], uint32_t (&sn)[kWords]) {
+    const int pair = kAdjacent ? 16 * j + 4 * g : 32 * j + 8 * g;
+    if constexpr (kAxes) {
+      constexpr int kN = kAdjacent ? 4 : 8;
+      axis_words<kN, kFp32>(
+          a.angles,
+          [&](int axis) { return a.angles.positions[axis * a.angles.position_stride + turn_token]; },
+          pair, pair_axes<kN>(a.angles, pair), c, sn);
     } else {
+      auto load = [](const char* at, uint32_t (&w)[kWords]) {
+        if constexpr (kWords == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(at);
+          w[0] = v.x;
+          w[1] = v.y;
+        } else {
 #pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) {
-        const u32x4 v = reinterpret_cast<const u32x4*>(at)[i];
+          for (int i = 0; i < kWords / 4; ++i) {
+            const u32x4 v = reinterpret_cast<const u32x4*>(at)[i];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
-      }
+            for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
+          }
+        }
+      };
+      load(turn + pair * kBytes, c);
+      load(turn + (pair + half) * kBytes, sn);
     }
   };
   auto word_value = [](const uint32_t (&w)[kWords], int i) {
     if (kFp32) return __uint_as_float(w[i]);
     return bf16_to_float(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
   };
-  const char* turn = nullptr;          // the angles' table row, from the lane's first dim on
   uint32_t cos0[kWords], sin0[kWords];  // of the first group of dims, with the row's loads
 
   // The lane's row of block b: its token (and position), then its values.
@@ -534,20 +549,23 @@ __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const Appe
     token = fastdiv(safe, t.h_div);
     head = static_cast<int>(safe - token * static_cast<uint32_t>(t.heads));
     live = row < t.rows && token < active;
-    position = which < 2 && a.rotary && live ? a.positions[token] : 0;
+    position = !kAxes && which < 2 && a.rotary && live ? a.angles.positions[token] : 0;
     const uint16_t* src = t.x + static_cast<int64_t>(token) * t.s0 + static_cast<int64_t>(head) * t.s1 + 8 * g;
 #pragma unroll
     for (int m = 0; m < 8; ++m) x[m] = *reinterpret_cast<const u32x4*>(src + 32 * m);
   };
   auto load_angles = [&](int64_t b) {
     if (set_of(b) == 2) return;
-    bad = a.rotary > 0 && (position < 0 || position >= a.table_rows);
-    turn = static_cast<const char*>(a.table) +
-           ((bad ? 0 : position) * a.table_stride + (kAdjacent ? 4 * g : 8 * g)) * kBytes;
-    if (8 * g < a.rotary) {
-      load_words(turn, cos0);
-      load_words(turn + half * kBytes, sin0);
+    if constexpr (kAxes) {
+      bad = false;
+      for (int k = g; live && k < a.angles.count; k += 4) bad |= bad_position(a.angles, token, k);
+      bad = row_max(bad) != 0;
+      turn_token = live ? token : 0;  // a dead row's angles are those of a token that exists
+    } else {
+      bad = a.rotary > 0 && (position < 0 || position >= a.angles.rows);
+      turn = static_cast<const char*>(a.angles.table) + (bad ? 0 : position) * a.angles.stride * kBytes;
     }
+    if (8 * g < a.rotary) load_words(0, cos0, sin0);
   };
 
   u32x4 y[8];  // the finished rows
@@ -605,10 +623,7 @@ __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const Appe
           c[i] = cos0[i];
           s[i] = sin0[i];
         }
-        if (j) {
-          load_words(turn + 32 * j * kBytes, c);
-          load_words(turn + (32 * j + half) * kBytes, s);
-        }
+        if (j) load_words(j, c, s);
         auto rotate_pair = [&](float (&lo)[8], float (&hi)[8]) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -638,10 +653,7 @@ __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const Appe
             c[i] = cos0[i];
             s[i] = sin0[i];
           }
-          if (m) {
-            load_words(turn + 16 * m * kBytes, c);
-            load_words(turn + (16 * m + half) * kBytes, s);
-          }
+          if (m) load_words(m, c, s);
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
             const float co = word_value(c, e >> 1), si = word_value(s, e >> 1);
@@ -742,67 +754,6 @@ __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const Appe
   }
 }
 
-// ---- the angles of tokens with several positions as a table of their own, one row per token, and its row
-// numbers (-1 where a position lies outside the table): then every kernel of single positions serves them.
-struct ComposeArgs {
-  const void* table;
-  int64_t table_rows, table_stride;
-  const int64_t* positions;
-  int64_t position_stride, n;
-  const int32_t* axes;
-  const int32_t* counts;
-  int32_t axis_count, rotary, fp32;
-  FastDiv rotary_div;
-  void* out;
-  int64_t* rows;
-};
-
-// kPer elements a thread (8: of one half, and 16-byte stores; 1: any rotary dims).
-template <int kPer>
-__global__ __launch_bounds__(kThreads) void compose_angles_kernel(const ComposeArgs a) {
-  const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
-  const uint32_t token = fastdiv(i, a.rotary_div);  // by the threads of a token
-  const int64_t active = a.counts ? min(static_cast<int64_t>(max(a.counts[1], 0)), a.n) : a.n;
-  if (token >= active) return;
-  const int e0 = static_cast<int>(i - token * a.rotary_div.divisor) * kPer, half = a.rotary >> 1;
-  const int pair = e0 < half ? e0 : e0 - half;
-  int axis[kPer];
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) axis[k] = a.axes[pair + k];
-  float v[kPer];
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const bool known = axis[k] >= 0 && axis[k] < a.axis_count;
-    const int64_t p = known ? a.positions[axis[k] * a.position_stride + token] : -1;
-    v[k] = p >= 0 && p < a.table_rows ? load_value(a.table, p * a.table_stride + e0 + k, a.fp32)
-                                      : __uint_as_float(0x7fc00000u);
-  }
-  const int64_t at = static_cast<int64_t>(token) * a.rotary + e0;
-  if constexpr (kPer == 8) {
-    if (a.fp32) {
-      f32x4* out = reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at);
-      out[0] = f32x4{v[0], v[1], v[2], v[3]};
-      out[1] = f32x4{v[4], v[5], v[6], v[7]};
-    } else {
-      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + at) =
-          u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                pack_bf16x2(v[6], v[7])};
-    }
-  } else if (a.fp32) {
-    static_cast<float*>(a.out)[at] = v[0];
-  } else {
-    static_cast<uint16_t*>(a.out)[at] = static_cast<uint16_t>(float_to_bf16(v[0]));
-  }
-  if (e0 == 0) {
-    bool bad = false;
-    for (int k = 0; k < a.axis_count; ++k) {
-      const int64_t p = a.positions[k * a.position_stride + token];
-      bad |= p < 0 || p >= a.table_rows;
-    }
-    a.rows[token] = bad ? -1 : static_cast<int64_t>(token);
-  }
-}
-
 // ---- records back to values: half a wavefront per record, 8 dims a lane of either vector, two records.
 struct ReadArgs {
   const uint8_t* history;
@@ -893,22 +844,14 @@ int value_groups_of(int64_t q_blocks, int64_t kv_blocks, bool rotated) {
 
 // Whether append_walk_kernel serves the call: 4-bit records, no clip search, and pairs in one lane.
 bool walks(const AppendArgs& a) {
-  const bool rows16 = !a.rotary || (aligned(a.table, 16) && a.table_stride % 8 == 0);
+  const bool rows16 = !a.rotary || (aligned(a.angles.table, 16) && a.angles.stride % 8 == 0 &&
+                                    aligned(a.angles.axes, 16));
   return a.set[2].rows && a.L.bits == 4 && a.mode != OSCAR_CLIP_SEARCH && rows16 &&
-         (a.adjacent ? a.rotary % 8 == 0 : a.rotary % 64 == 0) && a.axis_count <= 1;
+         (a.adjacent ? a.rotary % 8 == 0 : a.rotary % 64 == 0);
 }
 
 }  // namespace
 }  // namespace oscar
-
-extern "C" int64_t oscar_rope_scratch_bytes(int64_t n, int64_t hq, int64_t hk, int32_t store,
-                                            int32_t rotary_dim, int32_t table_fp32,
-                                            int32_t axis_count) {
-  using namespace oscar;
-  if (axis_count < 2 || rotary_dim <= 0 || n * (hq + hk + (store ? hk : 0)) <= kSmallAppendRows)
-    return 0;
-  return (n * 8 + 15) / 16 * 16 + n * rotary_dim * (table_fp32 ? 4 : 2);
-}
 
 extern "C" int oscar_rope_append(
     const void* query, int64_t q_s0, int64_t q_s1, const void* key, int64_t k_s0, int64_t k_s1,
@@ -918,8 +861,7 @@ extern "C" int oscar_rope_append(
     int32_t rotary_dim, int32_t interleaved, const int64_t* positions, int64_t position_stride,
     int32_t axis_count, const int32_t* axes, const int32_t* counts, void* q_out, void* k_out,
     const void* rk_t, const void* rv_t, void* q_rot, void* history, int64_t history_bytes,
-    const int64_t* slots, const oscar_layout* layout, const oscar_clip* clip, void* scratch,
-    int64_t scratch_bytes, void* stream) {
+    const int64_t* slots, const oscar_layout* layout, const oscar_clip* clip, void* stream) {
   using namespace oscar;
   const bool store = value != nullptr;
   AppendArgs a{};
@@ -954,49 +896,20 @@ extern "C" int oscar_rope_append(
   if (store && (v_s0 % 8 || v_s1 % 8 || !aligned(value, 16) || !aligned(rv_t, 16) ||
                 !aligned(history, 16)))
     return OSCAR_E_ALIGN;
-  const int64_t need = oscar_rope_scratch_bytes(n, hq, hk, store, rotary_dim, table_fp32, axis_count);
-  if (need && n > (0xffffffffll - kThreads) / rotary_dim) return OSCAR_E_SHAPE;
-  if (need && !scratch) return OSCAR_E_NULL;
-  if (scratch_bytes < need) return OSCAR_E_SHAPE;
-  if (need && !aligned(scratch, 16)) return OSCAR_E_ALIGN;
   hipStream_t s = as_stream(stream);
-  if (need) {
-    // Row numbers, then the angles.
-    const int64_t rows_bytes = (n * 8 + 15) / 16 * 16;
-    ComposeArgs c{cos_sin, table_rows, table_stride, positions, position_stride, n, axes, counts,
-                  axis_count, rotary_dim, table_fp32 ? 1 : 0, {},
-                  static_cast<char*>(scratch) + rows_bytes, static_cast<int64_t*>(scratch)};
-    auto compose = [&](auto kernel, int per) {
-      c.rotary_div = make_fastdiv(static_cast<uint32_t>(rotary_dim / per));
-      const int64_t threads = n * (rotary_dim / per);
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((threads + kThreads - 1) / kThreads)),
-                         dim3(kThreads), 0, s, c);
-    };
-    rotary_dim % 16 ? compose(compose_angles_kernel<1>, 1) : compose(compose_angles_kernel<8>, 8);
-    const hipError_t err = hipGetLastError();
-    if (err != hipSuccess) return static_cast<int>(err);
-    cos_sin = c.out;
-    table_rows = n;
-    table_stride = rotary_dim;
-    positions = c.rows;
-    axis_count = 1;
-  }
   const int64_t all = n * (hq + hk + (store ? hk : 0));
-  if (!store && query && q_weight && rotary_dim && all > kSmallAppendRows)
-    return oscar_qk_norm_rope(query, q_s0, q_s1, key, k_s0, k_s1, n, hq, hk, q_weight, k_weight,
-                              weight_fp32, unit_offset, eps, cos_sin, table_rows, table_stride,
-                              table_fp32, rotary_dim, interleaved, positions, counts, q_out, k_out,
-                              q_rot ? rk_t : nullptr, q_rot, stream);
+  // Rows of several positions without R_k: norm_rope.hip's streaming kernel.
+  if (axes && !store && !q_rot && query && q_weight && rotary_dim &&
+      launch_norm_rope_axes(query, q_s0, q_s1, key, k_s0, k_s1, n, hq, hk, q_weight, k_weight,
+                            weight_fp32, unit_offset, eps, table_fp32, interleaved, counts, q_out,
+                            k_out, {cos_sin, table_rows, table_stride, positions, position_stride, axes,
+                                    axis_count, rotary_dim}, s))
+    return static_cast<int>(hipGetLastError());
   if (query) a.set[0] = row_set(query, q_s0, q_s1, q_weight, q_out, n, hq);
   a.set[1] = row_set(key, k_s0, k_s1, k_weight, k_out, n, hk);
   if (store) a.set[2] = row_set(value, v_s0, v_s1, nullptr, nullptr, n, hk);
-  a.table = cos_sin;
-  a.table_rows = table_rows;
-  a.table_stride = table_stride;
-  a.positions = positions;
-  a.position_stride = position_stride;
-  a.axes = axis_count > 1 ? axes : nullptr;
-  a.axis_count = axis_count;
+  a.angles = {cos_sin, table_rows, table_stride, positions, position_stride,
+              rotary_dim ? axes : nullptr, axis_count, rotary_dim};
   a.counts = counts;
   a.n = n;
   a.rotary = rotary_dim;
@@ -1031,10 +944,19 @@ extern "C" int oscar_rope_append(
     auto walk = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(kWalkGroups), dim3(kWalkThreads), 0, s, a, value_groups);
     };
+    auto by_axes = [&](auto adjacent, auto fp32) {
+      constexpr bool kAdjacent = decltype(adjacent)::value, kFp32 = decltype(fp32)::value;
+      if (a.angles.axes)
+        walk(append_walk_kernel<kAdjacent, kFp32, true>);
+      else
+        walk(append_walk_kernel<kAdjacent, kFp32, false>);
+    };
     if (a.adjacent || !rotary_dim)
-      table_fp32 ? walk(append_walk_kernel<true, true>) : walk(append_walk_kernel<true, false>);
+      table_fp32 ? by_axes(std::true_type(), std::true_type())
+                 : by_axes(std::true_type(), std::false_type());
     else
-      table_fp32 ? walk(append_walk_kernel<false, true>) : walk(append_walk_kernel<false, false>);
+      table_fp32 ? by_axes(std::false_type(), std::true_type())
+                 : by_axes(std::false_type(), std::false_type());
   } else if (all <= kSmallAppendRows) {
     const int64_t q = blocks(0, 16), k = blocks(1, 16);
     hipLaunchKernelGGL(append_kernel<1>, dim3(static_cast<unsigned>(q + k + blocks(2, 16))),

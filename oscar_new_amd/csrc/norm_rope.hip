@@ -52,6 +52,7 @@ struct NormRopeArgs {
   float offset, eps;
   const uint16_t* rk_t;  // R_k^T [256][256]
   uint16_t* q_rot;
+  AxisTable axes;  // tokens with several positions (norm_rope_axes_kernel)
 };
 
 // Partner of dim d, the index of its angle and the sign of the partner's term.
@@ -315,6 +316,88 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeArgs 
   for (int i = 0; i < kRopeHeads; ++i)
     if (i < count)
       *reinterpret_cast<u32x4*>(out + i * kHeadDim) = finish_row(a, s_weight, angles, r[i], l);
+}
+
+// ---- tokens with several positions, no rotation by R_k: half a wavefront takes up to eight of a token's
+// rows, queries and keys in one list, since its angles cost more here: a position per axis, and a load of
+// each axis' table row for the lanes that have a pair of it.
+constexpr int kAxesHeads = 8;
+
+template <int kMode, bool kFp32>
+__global__ __launch_bounds__(kThreads) void norm_rope_axes_kernel(const NormRopeArgs a,
+                                                                  FastDiv per_token) {
+  static_assert(kMode != kPairGeneric, "pairs of eight dims");
+  constexpr int kN = kMode == kPairHalves ? 8 : 4, kWords = kFp32 ? kN : kN / 2;
+  __shared__ float s_weight[2][kHeadDim + 8];
+  const int l = threadIdx.x & 31;
+  const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t index = fastdiv(item, per_token);
+  const int64_t token = index;
+  const int h0 = static_cast<int>(item - index * per_token.divisor) * kAxesHeads;
+  const int count = token < a.n ? min(kAxesHeads, a.q.heads + a.k.heads - h0) : 0;
+  const int64_t active = live_tokens(a);
+  const bool live = token < active;
+  const int half = a.rotary >> 1;
+  const int pair0 = kMode == kPairAdjacent ? 4 * l : 8 * l < half ? 8 * l : 8 * l - half;
+  // The position on axis l, the pairs' axes, and the rows: in flight together.
+  int64_t position = 0;
+  if (live && l < a.axes.count) position = a.axes.positions[l * a.axes.position_stride + token];
+  PairAxes<kN> pairs;
+  if (8 * l < a.rotary) pairs = pair_axes<kN>(a.axes, pair0);
+  RowLoads r[kAxesHeads];
+  Angles<kMode, kFp32> angles;
+  auto row_at = [&](int i, int64_t (&at)[2]) {  // source and output of row i of the list
+    const int head = h0 + i;
+    const bool is_k = head >= a.q.heads;
+    const NormArgs& t = is_k ? a.k : a.q;
+    const int h = is_k ? head - a.q.heads : head;
+    at[0] = reinterpret_cast<int64_t>(t.x + token * t.s0 + h * t.s1);
+    at[1] = reinterpret_cast<int64_t>(t.out + (token * t.heads + h) * kHeadDim + 8 * l);
+    return is_k;
+  };
+#pragma unroll
+  for (int i = 0; i < kAxesHeads; ++i) start_row(angles, r[i]);
+#pragma unroll
+  for (int i = 0; i < kAxesHeads; ++i)
+    if (i < count) {
+      int64_t at[2];
+      row_at(i, at);
+      load_row<kMode>(a, reinterpret_cast<const uint16_t*>(at[0]), l, r[i]);
+    }
+  stage_weights(a, a.q.weight, s_weight[0], 0);
+  stage_weights(a, a.k.weight, s_weight[1], 32);
+  angles.live = live;
+  const bool outside = live && l < a.axes.count && (position < 0 || position >= a.axes.rows);
+  angles.bad = a.rotary > 0 && (__ballot(outside) >> (threadIdx.x & 32) & 0xffffffffull) != 0;
+  auto position_on = [&](int axis) {
+    const int lo = __shfl(static_cast<int>(position), axis, 32);
+    const int hi = __shfl(static_cast<int>(position >> 32), axis, 32);
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 |
+                                static_cast<uint32_t>(lo));
+  };
+  // Every lane of the wavefront takes part (its exchanges read other lanes'); lanes past the rotary dims
+  // keep their identity turn.
+  if (8 * l >= a.rotary) {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) pairs.axis[e] = 0;
+    pairs.one = true;
+  }
+  uint32_t c[kWords], s[kWords];
+  axis_words<kN, kFp32>(a.axes, position_on, 8 * l < a.rotary ? pair0 : 0, pairs, c, s);
+  if (8 * l < a.rotary)
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      angles.c[w >> 2][w & 3] = c[w];
+      angles.s[w >> 2][w & 3] = s[w];
+    }
+  __syncthreads();  // the weights
+#pragma unroll
+  for (int i = 0; i < kAxesHeads; ++i)
+    if (i < count) {
+      int64_t at[2];
+      const bool is_k = row_at(i, at);
+      *reinterpret_cast<u32x4*>(at[1]) = finish_row(a, s_weight[is_k], angles, r[i], l);
+    }
 }
 
 // ---- with the rotation, few rows or pairs that lie further apart: workgroups of kWaves wavefronts
@@ -781,3 +864,44 @@ extern "C" int oscar_qk_norm_rope(const void* query, int64_t q_s0, int64_t q_s1,
     launch(std::integral_constant<int, kPairGeneric>());
   return static_cast<int>(hipGetLastError());
 }
+
+namespace oscar {
+
+// The form for tokens with several positions, without R_k: oscar_rope_append has checked the arguments.
+// False where its pairs do not lie eight dims a lane (then it takes another kernel).
+bool launch_norm_rope_axes(const void* query, int64_t q_s0, int64_t q_s1, const void* key, int64_t k_s0,
+                           int64_t k_s1, int64_t n, int64_t hq, int64_t hk, const void* q_weight,
+                           const void* k_weight, bool weight_fp32, bool unit_offset, float eps,
+                           bool table_fp32, bool interleaved, const int32_t* counts, void* q_out,
+                           void* k_out, const AxisTable& axes, hipStream_t s) {
+  if (axes.rotary % (interleaved ? 8 : 16) || !aligned16(axes.table) || axes.stride % 8 ||
+      !aligned16(axes.axes))
+    return false;
+  NormRopeArgs a{};
+  a.q = {static_cast<const uint16_t*>(query), q_s0, q_s1, q_weight, static_cast<uint16_t*>(q_out),
+         n * hq, static_cast<int32_t>(hq), make_fastdiv(static_cast<uint32_t>(hq))};
+  a.k = {static_cast<const uint16_t*>(key), k_s0, k_s1, k_weight, static_cast<uint16_t*>(k_out),
+         n * hk, static_cast<int32_t>(hk), make_fastdiv(static_cast<uint32_t>(hk))};
+  a.axes = axes;
+  a.counts = counts;
+  a.n = n;
+  a.rotary = axes.rotary;
+  a.weight_fp32 = weight_fp32 ? 1 : 0;
+  a.adjacent = interleaved ? 1 : 0;
+  a.offset = unit_offset ? 1.f : 0.f;
+  a.eps = eps;
+  const int64_t per = (hq + hk + kAxesHeads - 1) / kAxesHeads;
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((n * per + 7) / 8)), dim3(kThreads), 0, s, a,
+                       make_fastdiv(static_cast<uint32_t>(per)));
+  };
+  if (interleaved)
+    table_fp32 ? launch(norm_rope_axes_kernel<kPairAdjacent, true>)
+               : launch(norm_rope_axes_kernel<kPairAdjacent, false>);
+  else
+    table_fp32 ? launch(norm_rope_axes_kernel<kPairHalves, true>)
+               : launch(norm_rope_axes_kernel<kPairHalves, false>);
+  return true;
+}
+
+}  // namespace oscar

@@ -736,12 +736,6 @@ def rope_append(query, key, value, history, slots, counts, layout, rk_t, rv_t, c
             query, q0, q1 = _rows_aligned(query)
         if store:
             value, v0, v1 = _rows_aligned(value)
-        scratch, scratch_bytes = None, 0
-        if axis_count > 1:
-            scratch_bytes = _ext.library().oscar_rope_scratch_bytes(
-                n, hq, hk, store, rotary, cos_sin.dtype == torch.float32, axis_count)
-            if scratch_bytes:
-                scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)
         _launch(
             _ext.library().oscar_rope_append, "rope_append", device, _ptr(query), q0, q1,
             key.data_ptr(), k0, k1, _ptr(value), v0, v1, n, hq, hk, _ptr(q_weight), _ptr(k_weight),
@@ -750,7 +744,7 @@ def rope_append(query, key, value, history, slots, counts, layout, rk_t, rv_t, c
             rotary, bool(interleaved), _ptr(positions), position_stride, axis_count, _ptr(axes),
             _ptr(counts), _ptr(q_out), k_out.data_ptr(), _ptr(rk_t), _ptr(rv_t) if store else None,
             _ptr(q_rot), _ptr(history) if store else None, size, _ptr(slots) if store else None, lay,
-            clip, _ptr(scratch), scratch_bytes,
+            clip,
         )
     return q_out, k_out, q_rot
 

@@ -138,6 +138,28 @@ def test_rows_of_several_axes(n, hq, hk, rotary, interleaved):
         assert torch.equal(turned[2], kernels.rotate(got[0], rk_t.T))
 
 
+@pytest.mark.parametrize("rotary,interleaved", [(64, False), (128, False), (128, True), (32, False)])
+@pytest.mark.parametrize("sections", [(16, 24, 24), (5, 6, 5), (7, 1, 8)])
+@pytest.mark.parametrize("cycle", [False, True])
+def test_sections(rotary, interleaved, sections, cycle):
+    """Axes in sections (whole lanes of one axis, or borders inside them) and in turns, many rows."""
+    total = sum(sections)
+    counts = [c * (rotary // 2) // total for c in sections]
+    counts[0] += rotary // 2 - sum(counts)
+    if cycle and 3 * max(counts[1:]) > rotary // 2:  # more than their turns
+        counts = [rotary // 2 - 2 * (rotary // 6)] + [rotary // 6] * 2
+    for table in (torch.float32, torch.bfloat16):
+        q, k, _, w, cs, pos, _, rk_t, _ = make(900, 5, 2, rotary, 3, table=table)
+        order = kernels.rope_axes(counts, cycle, DEV)
+        args = dict(eps=1e-5, interleaved=interleaved, axes=order)
+        got = kernels.qk_norm_rope(q, k, *w, cs, pos, **args)
+        for x, y, weight in ((got[0], q, w[0]), (got[1], k, w[1])):
+            check(x, y, weight, cs, pos, order, 1e-5, False, interleaved)
+        turned = kernels.qk_norm_rope(q, k, *w, cs, pos, rk_t=rk_t, **args)
+        assert torch.equal(turned[0], got[0]) and torch.equal(turned[1], got[1])
+        assert torch.equal(turned[2], kernels.rotate(got[0], rk_t.T))
+
+
 @pytest.mark.parametrize("rotary,interleaved", [(64, False), (256, True), (20, False), (6, True), (0, False)])
 @pytest.mark.parametrize("rotate", [False, True])
 def test_one_axis_has_the_bits_of_the_plain_call(rotary, interleaved, rotate):
@@ -163,7 +185,11 @@ def test_positions_and_axes_outside():
         assert bool(x[good].isfinite().all())
     order = order.clone()
     order[3], order[9] = 3, -1  # pairs (3, 35) and (9, 41) belong to no axis
-    wrong = kernels.qk_norm_rope(q, k, *w, cs, pos, axes=order, counts=counts_of(30))
+    wrong = kernels.qk_norm_rope(q, k, *w, cs, pos, axes=order, counts=counts_of(30), rk_t=rk_t)[:2]
+    again = kernels.qk_norm_rope(q, k, *w, cs, pos, axes=order, counts=counts_of(30))
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(wrong, again))
+    alone = kernels.qk_norm_rope(q, k, *w, cs, pos[:1], axes=order, counts=counts_of(30))
+    assert bool(alone[0][good][..., [3, 35, 9, 41]].isnan().all())
     dims = torch.zeros(256, dtype=torch.bool, device=DEV)
     dims[[3, 35, 9, 41]] = True
     for x, y in zip(wrong, got):

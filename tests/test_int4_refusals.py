@@ -49,11 +49,11 @@ def test_environment(monkeypatch):
 def append(query=A, q_s0=1536, key=A, value=A, n=4, hq=6, hk=1, qw=A, kw=A, eps=1e-6, table=A,
            rows=100, stride=64, fp32=0, rotary=64, positions=A, pos_stride=4, count=3, axes=A, counts=A,
            q_out=A, k_out=A, rk_t=A, rv_t=A, q_rot=A, history=A, size=1 << 24, slots=A, lay=layout(),
-           clip=CLIP, scratch=A, scratch_bytes=1 << 30):
+           clip=CLIP):
     return _ext.library().oscar_rope_append(
         query, q_s0, 256, key, 256, 256, value, 256, 256, n, hq, hk, qw, kw, 0, 0, eps, table, rows,
         stride, fp32, rotary, 0, positions, pos_stride, count, axes, counts, q_out, k_out, rk_t, rv_t,
-        q_rot, history, size, slots, lay, clip, scratch, scratch_bytes, None)
+        q_rot, history, size, slots, lay, clip, None)
 
 
 def test_append():
@@ -74,13 +74,6 @@ def test_append():
     for name in ("query", "key", "value", "history", "q_out", "k_out", "rk_t", "rv_t", "q_rot", "qw", "kw"):
         assert append(**{name: A + 8}) == -4, name
     assert append(q_s0=1537) == -4 and append(table=A + 1) == -4 and append(table=A + 2, fp32=1) == -4
-    need = _ext.library().oscar_rope_scratch_bytes(600, 6, 1, 1, 64, 0, 3)
-    assert need == 600 * 8 + 600 * 64 * 2  # rows' numbers and angles of many rows with several axes
-    assert _ext.library().oscar_rope_scratch_bytes(600, 6, 1, 1, 64, 0, 1) == 0
-    assert _ext.library().oscar_rope_scratch_bytes(32, 6, 1, 1, 64, 0, 3) == 0
-    many = dict(n=600, pos_stride=600)
-    assert append(scratch=None, **many) == -1 and append(scratch_bytes=need - 1, **many) == -2
-    assert append(scratch=A + 8, **many) == -4
     assert append(eps=-1.0) == -5 and append(eps=float("nan")) == -5
 
 
