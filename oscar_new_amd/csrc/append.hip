@@ -354,7 +354,9 @@ constexpr unsigned kWalkGroups = 256;  // one per CU
 constexpr int kWalkWaves = 8, kWalkThreads = kWalkWaves * kWave;
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u16x2 as_u16x2(uint32_t v) { return __builtin_bit_cast(u16x2, v); }
+__device__ __forceinline__ i16x2 as_i16x2(uint32_t v) { return __builtin_bit_cast(i16x2, v); }
 __device__ __forceinline__ uint32_t as_u32(u16x2 v) { return __builtin_bit_cast(uint32_t, v); }
 
 // Sum and maximum over the four lanes of a row.
@@ -371,71 +373,173 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
   return max(r[0], r[1]);
 }
 
-// quantize_store4 (percentile or factor) of 16 rows, four lanes each: z[m] holds dims 32 m + 8 g .. + 7 as
-// bf16. The quantile's order statistics come from a bisection of the 15-bit magnitudes, between the
-// largest one and four powers of two below it where that holds enough values.
-__device__ __forceinline__ void quantize_rows4(const u32x4 (&z)[8], int mode, float ratio, float factor,
-                                               uint8_t* codes, uint8_t* side, int g) {
-#pragma clang fp contract(off)
-  constexpr uint32_t kMagnitude = 0x7fff7fffu, kTop = 0x80008000u;
-  u16x2 top2 = as_u16x2(0u);
-  float mn = INFINITY, mx = -INFINITY;
+// The kLargest largest magnitudes of a row whose lanes hold z, in descending order: a sorted list per lane
+// and half word, into which every pair is sorted, then lists joined: the largest of two descending lists
+// are the larger of a[i] and b[last - i], which two steps of compares put in order.
+constexpr uint32_t kLargest = 4;
+__device__ __forceinline__ void largest_of_row(const u32x4 (&z)[8], uint32_t (&most)[kLargest]) {
+  u16x2 s[kLargest];
+#pragma unroll
+  for (uint32_t i = 0; i < kLargest; ++i) s[i] = as_u16x2(0u);
 #pragma unroll
   for (int m = 0; m < 8; ++m)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      top2 = __builtin_elementwise_max(top2, as_u16x2(z[m][e] & kMagnitude));
-      const float lo = __uint_as_float(z[m][e] << 16), hi = __uint_as_float(z[m][e] & 0xffff0000u);
-      mn = fminf(mn, fminf(lo, hi));
-      mx = fmaxf(mx, fmaxf(lo, hi));
+      u16x2 t = as_u16x2(z[m][e] & 0x7fff7fffu);
+#pragma unroll
+      for (uint32_t i = 0; i < kLargest; ++i) {
+        const u16x2 larger = __builtin_elementwise_max(s[i], t);
+        t = __builtin_elementwise_min(s[i], t);
+        s[i] = larger;
+      }
     }
-  const uint32_t top = row_max(max(static_cast<uint32_t>(top2[0]), static_cast<uint32_t>(top2[1])));
-  mn = -max_xor32(max_xor16(-mn));
-  mx = max_xor32(max_xor16(mx));
+  auto join = [&](const uint32_t (&a)[kLargest], const uint32_t (&b)[kLargest]) {
+    uint32_t c[kLargest];
+#pragma unroll
+    for (uint32_t i = 0; i < kLargest; ++i) c[i] = max(a[i], b[kLargest - 1 - i]);
+    auto order = [&](int i, int j) {
+      const uint32_t larger = max(c[i], c[j]);
+      c[j] = min(c[i], c[j]);
+      c[i] = larger;
+    };
+    order(0, 2);
+    order(1, 3);
+    order(0, 1);
+    order(2, 3);
+#pragma unroll
+    for (uint32_t i = 0; i < kLargest; ++i) most[i] = c[i];
+  };
+  uint32_t a[kLargest], b[kLargest];
+#pragma unroll
+  for (uint32_t i = 0; i < kLargest; ++i) {
+    a[i] = s[i][0];
+    b[i] = s[i][1];
+  }
+  join(a, b);
+#pragma unroll
+  for (uint32_t i = 0; i < kLargest; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(most[i], most[i], false, false);
+    a[i] = r[0];
+    b[i] = r[1];
+  }
+  join(a, b);
+#pragma unroll
+  for (uint32_t i = 0; i < kLargest; ++i) {
+    const auto r = __builtin_amdgcn_permlane32_swap(most[i], most[i], false, false);
+    a[i] = r[0];
+    b[i] = r[1];
+  }
+  join(a, b);
+}
+
+// The need-th largest magnitude of a row and the one before it (need >= 2): first in bins of four below the
+// row's largest, `top`, a byte each (127: a bin of all that lie 508, four powers of two, below), whose
+// number is bisected four values at a time, then inside the bin that holds it.
+__device__ __forceinline__ void statistics_of_row(const u32x4 (&z)[8], uint32_t top, uint32_t need,
+                                                  uint32_t& below, uint32_t& above) {
+  u16x2 mag[32];
+  uint32_t bins[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    u16x2 b[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mag[2 * k + i] = as_u16x2(z[k >> 1][2 * (k & 1) + i] & 0x7fff7fffu);
+      b[i] = __builtin_elementwise_min((as_u16x2(top * 0x10001u) - mag[2 * k + i]) >> u16x2{2, 2},
+                                       u16x2{127, 127});
+    }
+    bins[k] = as_u32(b[0]) | as_u32(b[1]) << 8;
+  }
+  // Up to bin `low` there are `larger` < need values, up to bin `high` at least need.
+  int low = -1, high = 127;
+  uint32_t larger = 0;
+#pragma unroll 1
+  for (int i = 0; i < 7; ++i) {
+    const int mid = (low + high) >> 1;
+    const uint32_t add = static_cast<uint32_t>(127 - mid) * 0x01010101u;
+    uint32_t c = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) c += __builtin_popcount((bins[k] + add) & 0x80808080u);
+    const uint32_t upto = kHeadDim - row_sum(c);
+    const bool enough = upto >= need;
+    high = enough ? mid : high;
+    low = enough ? low : mid;
+    larger = enough ? larger : upto;
+  }
+  // At or above `lo` there are at least need, at or above `hi` `larger` < need.
+  uint32_t hi = top - 4 * high + 1;
+  uint32_t lo = high == 127 || hi < 4 ? 0 : hi - 4;
+  while (__any(hi - lo > 1)) {
+    const uint32_t mid = (lo + hi) >> 1;  // lo where they are next to each other: it stays
+    const u16x2 add = as_u16x2((0x8000u - mid) * 0x10001u);
+    uint32_t c = 0;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) c += __builtin_popcount(as_u32(mag[k] + add) & 0x80008000u);
+    c = row_sum(c);
+    const bool enough = c >= need || mid == lo;
+    lo = enough ? mid : lo;
+    hi = enough ? hi : mid;
+    larger = enough ? larger : c;
+  }
+  u16x2 next = as_u16x2(0xffffffffu);
+  const u16x2 sub = as_u16x2((lo + 1) * 0x10001u);
+#pragma unroll
+  for (int k = 0; k < 32; ++k) next = __builtin_elementwise_min(next, mag[k] - sub);
+  const uint32_t least = 0xffffu - row_max(0xffffu - min(uint32_t{next[0]}, uint32_t{next[1]}));
+  below = lo;
+  above = larger == need - 1 ? least + lo + 1 : lo;
+}
+
+// quantize_store4 (percentile or factor) of 16 rows, four lanes each: z[m] holds dims 32 m + 8 g .. + 7 as
+// bf16. The quantile's two order statistics are among the kLargest largest magnitudes where it is near 1
+// (0.9883 on).
+__device__ __forceinline__ void quantize_rows4(const u32x4 (&z)[8], int mode, float ratio, float factor,
+                                               uint8_t* codes, uint8_t* side, int g) {
+#pragma clang fp contract(off)
+  // Two bf16 values a word: as signed numbers the largest is the row's maximum unless all are negative, as
+  // unsigned ones the largest is its minimum unless none is.
+  i16x2 largest2 = {INT16_MIN, INT16_MIN};
+  u16x2 most2 = as_u16x2(0u), least2 = as_u16x2(0xffffffffu);
+#pragma unroll
+  for (int m = 0; m < 8; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      largest2 = __builtin_elementwise_max(largest2, as_i16x2(z[m][e]));
+      most2 = __builtin_elementwise_max(most2, as_u16x2(z[m][e]));
+      least2 = __builtin_elementwise_min(least2, as_u16x2(z[m][e]));
+    }
+  const int largest = static_cast<int>(row_max(static_cast<uint32_t>(
+                          max(int{largest2[0]}, int{largest2[1]}) + 0x8000))) - 0x8000;
+  const uint32_t most = row_max(max(uint32_t{most2[0]}, uint32_t{most2[1]}));
+  const uint32_t least = 0xffffu - row_max(0xffffu - min(uint32_t{least2[0]}, uint32_t{least2[1]}));
+  const uint32_t top = max(static_cast<uint32_t>(max(largest, 0)), most & 0x8000u ? most & 0x7fffu : 0u);
+  float mx = __uint_as_float((largest >= 0 ? static_cast<uint32_t>(largest) : least) << 16);
+  float mn = __uint_as_float((most & 0x8000u ? most : least) << 16);
   float thr = INFINITY;
   if (mode == OSCAR_CLIP_FACTOR) {
     thr = __uint_as_float(top << 16) * factor;
   } else if (ratio != 0.0f) {
-    auto count = [&](uint32_t from) {  // magnitudes at or above `from` (1 .. 0x8000)
-      const u16x2 add = as_u16x2((0x8000u - from) * 0x10001u);
-      uint32_t c = 0;
-#pragma unroll
-      for (int m = 0; m < 8; ++m)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          c += __builtin_popcount(as_u32(as_u16x2(z[m][e] & kMagnitude) + add) & kTop);
-      return row_sum(c);
-    };
     const float rank = ratio * 255.0f;
     const int lo_idx = static_cast<int>(floorf(rank)), hi_idx = static_cast<int>(ceilf(rank));
     const float weight = rank - static_cast<float>(lo_idx);
     const uint32_t need = static_cast<uint32_t>(kHeadDim - lo_idx);
-    // count(lo) >= need > count(hi).
-    uint32_t lo = 0, hi = top + 1;
-    uint32_t mid = top > 512 ? top - 512 : (top + 1) >> 1;
-    while (__any(hi - lo > 1)) {
-      const bool open = hi - lo > 1;
-      const bool enough = count(open ? mid : 1) >= need;
-      lo = open && enough ? mid : lo;
-      hi = open && !enough ? mid : hi;
-      mid = (lo + hi) >> 1;
-    }
-    const float below = __uint_as_float(lo << 16);
-    float above = below;
-    if (hi_idx != lo_idx) {
-      const uint32_t more = count(lo + 1);
-      u16x2 next = as_u16x2(0xffffffffu);
-      const u16x2 sub = as_u16x2((lo + 1) * 0x10001u);
+    uint32_t below, above;
+    if (need <= kLargest) {
+      uint32_t first[kLargest];
+      largest_of_row(z, first);
+      const uint32_t more = static_cast<uint32_t>(kHeadDim - hi_idx);  // need or one less
+      below = above = first[0];
 #pragma unroll
-      for (int m = 0; m < 8; ++m)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          next = __builtin_elementwise_min(next, as_u16x2(z[m][e] & kMagnitude) - sub);
-      const uint32_t least = 0xffffu - row_max(0xffffu - min(static_cast<uint32_t>(next[0]),
-                                                             static_cast<uint32_t>(next[1])));
-      if (more >= static_cast<uint32_t>(kHeadDim - hi_idx)) above = __uint_as_float((least + lo + 1) << 16);
+      for (uint32_t i = 1; i < kLargest; ++i) {
+        below = need == i + 1 ? first[i] : below;
+        above = more == i + 1 ? first[i] : above;
+      }
+    } else {
+      statistics_of_row(z, top, need, below, above);
+      if (hi_idx == lo_idx) above = below;
     }
-    thr = __fmaf_rn(weight, above - below, below);
+    const float under = __uint_as_float(below << 16);
+    thr = __fmaf_rn(weight, __uint_as_float(above << 16) - under, under);
   }
   if (thr != INFINITY) {
     mn = clamp1(mn, thr);
