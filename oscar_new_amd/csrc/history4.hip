@@ -7,18 +7,24 @@
 // merges of merge.h. The task table, splits and masks are those of history.hip; the reference has 2-bit
 // records only (oscar_ascend/kernels.py:290-482).
 //
-// Scale and zero fold out of the products: q . k = s (q . c) + z sum q, and sum p v = sum (p s) (c - 7.5)
-// + sum p (z + 7.5 s), in which the rounding of p s weighs values of either sign: the products run over c,
-// and one more against ones gives the sum of the rounded p s. Codes and queries are exact in bf16. p s is
-// rounded to fp16 (2^-11; bf16's 2^-8 made the error against 64 bits 0.0023 of the output where the
-// output's own rounding is 0.0017), times a power of two that each wavefront keeps for its largest s so
-// far: it lies below 2^15 then, and the smallest ones are off by 2^-31 of that s.
+// Scale and zero fold out of the products: q . k = s (q . c) + z sum q, and sum p v = sum (p s) c + sum p z,
+// so that the matrix instructions run over codes as they unpack. K's are exact in bf16, as the queries
+// are; V's in fp16, and p s is rounded to fp16: by 2^-11 of itself (bf16's 2^-8 made the error against 64
+// bits 0.0023 of the output's norm; now it is the 0.0017 of the output's own rounding), or, the smallest,
+// by 2^-24 of the largest V scale of a wavefront's first chunk (see v_by). Sums are fp32.
 //
 // A workgroup of eight wavefronts, one per CU, takes up to 32 query rows. Wavefront w streams chunks of
 // 32 positions w, w + 8, ... of the split through an LDS ring of its own (direct-to-LDS copies, no barrier
 // in the loop); scores are computed transposed (positions by rows), so that a lane holds one row's
 // scores of eight positions and its probabilities are the P operand of the second product, whose other
 // operand comes from transposed LDS reads of 4-bit codes. The eight states are joined at the end.
+//
+// Up to 16 rows the records' bytes bound it: 32 requests of 32704 positions (285 MB) take 52 us, 5.5 TB/s
+// where a large copy moves 5.2 (reads alone reach 7). Tiles of 32 rows are bound by the vector units, which
+// issue in 72 % of the cycles (the matrix units' share is 34 %): a wavefront's 32 positions cost 450
+// vector instructions and 61 matrix instructions, of which the unpacking, 200, is paid once per tile:
+// 2048 tokens of 6 heads against 32768 positions 505 us, 0.82 PFLOP/s. Tiles of 48 or 64 rows would halve
+// the unpacking's share but spill: a row group's sums are 64 registers of a lane.
 #include "dma.h"
 #include "history4.h"
 
@@ -205,7 +211,8 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     const int nkb = min(((p_hi - 1) >> a.L.bk_shift) - kb_first + 1, kTable4);
     for (int j = tid; j < nkb; j += F::kThreads) lds.off[j] = block_offset4(a, t, head, kb_first + j);
   }
-  // Query rows as they are, 16-byte piece p of row r at p ^ r % 16, two rows a copy. A row past the task's reads the buffer's first row and is zeroed below.
+  // Query rows as they are, 16-byte piece p of row r at p ^ r % 16, two rows a copy. A row past the task's
+  // reads the buffer's first row and is zeroed below.
   const uint32_t q_area = lds_addr(lds.q);
 #pragma unroll
   for (int i = 0; i < RG * 8 / W; ++i) {
@@ -500,34 +507,34 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     // Thread -> row tid / 32, dims 4 (tid % 32) and 128 further on.
 #pragma unroll
     for (int r0 = 0; r0 < 16; r0 += F::kThreads / 32) {
-    const int row16 = r0 + (tid >> 5), row = 16 * i + row16, d0 = 4 * (tid & 31);
-    const RowInfo ri = row_of(a, rows, head, row);
-    if (!ri.valid) continue;
-    float mx = -INFINITY;
+      const int row16 = r0 + (tid >> 5), row = 16 * i + row16, d0 = 4 * (tid & 31);
+      const RowInfo ri = row_of(a, rows, head, row);
+      if (!ri.valid) continue;
+      float mx = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < W; ++w) mx = fmaxf(mx, lds.red[0][w][row]);
-    float den = 0.f, zs = 0.f;
-    f32x4 sum[2] = {};
+      for (int w = 0; w < W; ++w) mx = fmaxf(mx, lds.red[0][w][row]);
+      float den = 0.f, zs = 0.f;
+      f32x4 sum[2] = {};
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float mw = lds.red[0][w][row];
-      const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx);
-      den = fmaf(f, lds.red[1][w][row], den);
-      zs = fmaf(f, lds.red[2][w][row], zs);
+      for (int w = 0; w < W; ++w) {
+        const float mw = lds.red[0][w][row];
+        const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx);
+        den = fmaf(f, lds.red[1][w][row], den);
+        zs = fmaf(f, lds.red[2][w][row], zs);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        sum[h] += *reinterpret_cast<const f32x4*>(s_o + (w * 16 + row16) * kHeadDim + d0 + 128 * h);
-    }
-    const float inv = 1.0f / fmaxf(den, 1.0e-30f);
-    const int64_t out_row = (ri.token * a.hq + ri.qhead) * a.splits + split;
+        for (int h = 0; h < 2; ++h)
+          sum[h] += *reinterpret_cast<const f32x4*>(s_o + (w * 16 + row16) * kHeadDim + d0 + 128 * h);
+      }
+      const float inv = 1.0f / fmaxf(den, 1.0e-30f);
+      const int64_t out_row = (ri.token * a.hq + ri.qhead) * a.splits + split;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 r;
+      for (int h = 0; h < 2; ++h) {
+        f32x4 r;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = (sum[h][e] + zs) * inv;
-      *reinterpret_cast<f32x4*>(a.partials + out_row * kHeadDim + d0 + 128 * h) = r;
-    }
-    if (d0 == 0) a.lse[out_row] = den == 0.f ? -INFINITY : (mx + log2f(den)) * kLn2;
+        for (int e = 0; e < 4; ++e) r[e] = (sum[h][e] + zs) * inv;
+        *reinterpret_cast<f32x4*>(a.partials + out_row * kHeadDim + d0 + 128 * h) = r;
+      }
+      if (d0 == 0) a.lse[out_row] = den == 0.f ? -INFINITY : (mx + log2f(den)) * kLn2;
     }
   }
 }
@@ -664,7 +671,9 @@ extern "C" int oscar_history_int4(const void* query, int64_t q_s0, int64_t q_s1,
                                 table_stride, table_columns, counts, tasks, task_count, n, hq, programs,
                                 splits, block_n, query_tile, max_query_len, scale, 0, split_tokens,
                                 layout, partials, lse, &a, &rows, 4);
-  if (st != OSCAR_OK || n == 0) return st;
+  if (st != OSCAR_OK) return st;
+  if (history_bytes > 16ll * kNoBlock4) return OSCAR_E_UNSUPPORTED;  // block offsets are 32 bits of 16 bytes
+  if (n == 0) return OSCAR_OK;
   hipStream_t s = as_stream(stream);
   if (row_tiles) {
     if (split_tokens) return OSCAR_E_UNSUPPORTED;

@@ -88,6 +88,7 @@ def test_history():
     assert attend(n=-1) == -2 and attend(hq=0) == -2 and attend(programs=0) == -2
     assert attend(splits=0) == -2 and attend(splits=65536) == -2 and attend(qt=0) == -2
     assert attend(size=32 * 272 - 1) == -2  # fewer bytes than a masked chunk reads
+    assert attend(size=(1 << 36) + 1, n=0) == -5  # block offsets of 32 bits
     assert attend(q=None) == -1 and attend(history=None) == -1 and attend(tasks=None) == -1
     assert attend(partials=None) == -1 and attend(lse=None) == -1
     assert attend(lay=layout(2)) == -3 and attend(lay=layout(slot=264)) == -3
