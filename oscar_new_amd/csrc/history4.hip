@@ -37,6 +37,7 @@ constexpr int kStage4 = kChunk4 * kSlot4;           // 8704 bytes
 constexpr int kDma4 = (kChunk4 * kPieces4 + 63) / 64;  // 9 copies of a chunk, the last of 32 lanes
 constexpr int kTable4 = 512;                        // kernel blocks whose offsets live in LDS
 constexpr float kRoom4 = 13.0f;                     // of scores above a row's reference, log2 units
+constexpr float kScaleRoom4 = 4.0f;                 // of scaled V scales
 constexpr int kMaxTasks4 = 16384;                   // task rows of the device rule
 
 // A workgroup's form: RG groups of 16 query rows, W wavefronts with S ring stages each.
@@ -177,6 +178,18 @@ __device__ bool unit_of_slot(const AttnArgs& a, int programs, int u, int* length
   return true;
 }
 
+// fmaxf keeps its operands quiet with an instruction each where it does not know them to be.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
 __device__ __forceinline__ f32x4 splat(float v) { return f32x4{v, v, v, v}; }
 
 // A workgroup's rows: row r (of 16 RG) is row base + r of the query tokens from token0 on times the group's
@@ -275,6 +288,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     return *reinterpret_cast<const u32x4*>(lds.q + (16 * i + n) * kHeadDim * 2 +
                                            16 * ((8 * g + m) ^ n));
   };
+  const float fq = a.scale_log2;
   float qs[RG];
   u32x4 qb[8];
 #pragma unroll
@@ -288,7 +302,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
         sum += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xffff0000u);
       if (RG == 1) qb[m] = w;
     }
-    qs[i] = sum_xor32(sum_xor16(sum));
+    qs[i] = sum_xor32(sum_xor16(sum)) * fq;
   }
 
   const int k_off = kSlot4 * n + 32 * g;
@@ -297,7 +311,6 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
   // neighbouring groups of 16 dims for i < 8 and the other above, so that a lane gets one dim of its own
   // eight positions in either.
   const int v_off = kSlot4 * (16 * (n >> 2 & 1) + 4 * g + (n & 3)) + kCodes4 + 8 * (n >> 3);
-  const float fq = a.scale_log2;
 
   // A chunk in stage s: the products of its K codes and the rows, and its scales and zeros.
   struct Chunk {
@@ -305,10 +318,22 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     uint2 side[8];  // of the lane's positions 16 (e / 4) + 4 g + e % 4: K scale and zero, V scale and zero
     bool whole;
     uint32_t seen;  // bit e, where not whole
-    float top;      // largest V scale of the lane's
   };
   auto read_chunk = [&](int t0, int s, Chunk& c) {
-    const uint8_t* st = lds.ring[wave][s];
+    uint8_t* st = lds.ring[wave][s];
+    // A first or last chunk may be partial, or the block unmapped: positions outside get score -inf and,
+    // in LDS, a zero V scale and zero (their bytes may be NaN patterns).
+    const bool ok_block = mapped >> s & 1u;
+    c.whole = ok_block && t0 >= p_lo && t0 + kChunk4 <= p_hi;
+    if (!c.whole) {
+      // The positions' bits, in a register that the compiler cannot know ahead of the branch.
+      const int from = max(p_lo - t0, 0), to = min(p_hi - t0, kChunk4);
+      uint32_t bits = ok_block ? (0xffffffffu << from) & (0xffffffffu >> (kChunk4 - to)) : 0u;
+      asm volatile("" : "+v"(bits));
+      c.seen = (bits >> (4 * g) & 0xfu) | (bits >> (12 + 4 * g) & 0xf0u);
+      if (lane < kChunk4 && !(bits >> lane & 1u))
+        *reinterpret_cast<uint32_t*>(st + kSlot4 * lane + kSide4 + 4) = 0u;
+    }
 #pragma unroll
     for (int i = 0; i < RG; ++i) c.acc[i][0] = c.acc[i][1] = splat(0.f);
     u32x4 kw[2][2];
@@ -330,40 +355,25 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       c.side[e] = *reinterpret_cast<const uint2*>(st + side_off + kSlot4 * (16 * (e >> 2) + (e & 3)));
-    // A first or last chunk may be partial, or the block unmapped: positions outside get score -inf and
-    // a zero V scale and zero (their bytes may be NaN patterns).
-    const bool ok_block = mapped >> s & 1u;
-    c.whole = ok_block && t0 >= p_lo && t0 + kChunk4 <= p_hi;
-    c.seen = 0u;
-    if (!c.whole) {
-      // The positions' bits, in a register that the compiler cannot know ahead of the branch.
-      const int from = max(p_lo - t0, 0), to = min(p_hi - t0, kChunk4);
-      uint32_t bits = ok_block ? (0xffffffffu << from) & (0xffffffffu >> (kChunk4 - to)) : 0u;
-      asm volatile("" : "+v"(bits));
-      c.seen = (bits >> (4 * g) & 0xfu) | (bits >> (12 + 4 * g) & 0xf0u);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) c.side[e].y = c.seen >> e & 1u ? c.side[e].y : 0u;
-    }
-    c.top = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c.top = fmaxf(c.top, fabsf(half_lo_to_float(c.side[e].y)));
   };
-  // Scores of row group i in units of fq, and their largest in log2 units.
-  auto row_scores = [&](Chunk& c, int i, float (&r)[8]) {
+  // Scores of row group i in log2 units, less m.
+  auto row_scores = [&](Chunk& c, const float (&ks)[8], int i, float m, float (&r)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      r[e] = fmaf(half_lo_to_float(c.side[e].x), c.acc[i][e >> 2][e & 3],
-                  half_hi_to_float(c.side[e].x) * qs[i]);
+      r[e] = fmaf(ks[e], c.acc[i][e >> 2][e & 3], fmaf(half_hi_to_float(c.side[e].x), qs[i], -m));
     if (!c.whole) {
       asm volatile("" : "+v"(c.seen));
 #pragma unroll
       for (int e = 0; e < 8; ++e) r[e] = c.seen >> e & 1u ? r[e] : -INFINITY;
     }
-    return fmaxf(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])),
-                 fmaxf(fmaxf(r[4], r[5]), fmaxf(r[6], r[7]))) * fq;
   };
-  // This wavefront's chunks in turn through its ring (the first S - 1 are on their way), while `use` says
-  // to go on.
+  auto largest = [](const float (&r)[8], float m) {
+    return max3(max3(max3(max3(m, r[0], r[1]), r[2], r[3]), r[4], r[5]), r[6], r[7]);
+  };
+  auto largest_abs = [](const float (&r)[8], float m) {
+    return max3_abs(max3_abs(max3_abs(max3_abs(m, r[0], r[1]), r[2], r[3]), r[4], r[5]), r[6], r[7]);
+  };
+  // This wavefront's chunks in turn through its ring (the first S - 1 are on their way).
   auto stream = [&](auto use) {
     for (int j = 0, s = 0; j < nmine; ++j) {
       // The stage that chunk j - 1 was read from (its reads have completed) takes chunk j + S - 1.
@@ -372,7 +382,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
         issue(j + S - 1, s == 0 ? S - 1 : s - 1);
       }
       wait_chunks(min(nmine - 1 - j, S - 1));  // chunk j has landed
-      if (!use((first + wave + W * j) * kChunk4, s)) return;
+      use((first + wave + W * j) * kChunk4, s);
       s = s == S - 1 ? 0 : s + 1;
     }
   };
@@ -381,54 +391,62 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
   // for 2^kRoom4 above it, and V scales times v_by, with room for four times the first chunk's largest:
   // then no sum is ever scaled again, and the accumulators stay where the matrix instructions want them
   // (rescaling them as a running maximum grows made the compiler move them about: two row groups spilled
-  // registers). Should a score or scale need more room, the wavefront's chunks are gone through for the
-  // largest ones, and then again from the start with those.
-  float m_ref[RG], psum[RG], zsum[RG];
-  float v_limit = 0.f, v_by = 1.f;
+  // registers). Should a later score or scale have needed more room, the wavefront goes through its chunks
+  // again, with the largest ones, which it knows by then.
+  float m_ref[RG], m_less[RG], psum[RG], zsum[RG];
+  float v_by = 1.f;
   f32x4 o[RG][16];  // o[c]: rows 4 g + v, dim 16 c + n
   auto set_scale = [&](float top) {
     const uint32_t eb = min(__float_as_uint(top) >> 23, 250u);
-    v_limit = __uint_as_float((eb + 3) << 23);           // 4 to 8 times the largest
-    v_by = __uint_as_float((127 + 126 - eb) << 23);      // p s v_by < 2^(13 + 3 - 1) = 2^15
+    v_by = __uint_as_float((127 + 126 - eb) << 23);  // the largest lies in [0.5, 1)
   };
 #pragma unroll
-  for (int i = 0; i < RG; ++i) m_ref[i] = -INFINITY;
-  bool exact = false, again;
+  for (int i = 0; i < RG; ++i) {
+    m_ref[i] = -INFINITY;
+    m_less[i] = 0.f;
+  }
+  bool placed = false, again = false;
   do {
-    again = false;
+    // The largest so far of the lane's positions, scores less their reference and scaled V scales.
+    float m_top[RG], v_top = 0.f;
 #pragma unroll
     for (int i = 0; i < RG; ++i) {
       psum[i] = zsum[i] = 0.f;
+      m_top[i] = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 16; ++c) o[i][c] = splat(0.f);
     }
     stream([&](int t0, int s) {
       Chunk c;
       read_chunk(t0, s, c);
-      if (!exact && __any(c.top > v_limit)) {
-        if (v_limit == 0.f)
-          set_scale(max_xor32(max_xor16(c.top)));  // the same in every lane
-        else
-          again = true;
-      }
-      u32x4 pa[RG];
-      float vs[8];
+      float ks[8], vs[8];  // products with zero added: one instruction with the conversion
 #pragma unroll
-      for (int e = 0; e < 8; ++e) vs[e] = half_lo_to_float(c.side[e].y) * v_by;
+      for (int e = 0; e < 8; ++e) ks[e] = fmaf(half_lo_to_float(c.side[e].x), fq, 0.f);
+      if (!placed && (mapped >> s & 1u)) {
+        placed = true;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vs[e] = half_lo_to_float(c.side[e].y);
+        set_scale(max_xor32(max_xor16(largest_abs(vs, 0.f))));  // the same in every lane
+#pragma unroll
+        for (int i = 0; i < RG; ++i) {
+          float r[8];
+          row_scores(c, ks, i, 0.f, r);
+          m_ref[i] = max_xor32(max_xor16(largest(r, -INFINITY)));
+          m_less[i] = m_ref[i] == -INFINITY ? 0.f : m_ref[i];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vs[e] = fmaf(half_lo_to_float(c.side[e].y), v_by, 0.f);
+      v_top = largest_abs(vs, v_top);
+      u32x4 pa[RG];
 #pragma unroll
       for (int i = 0; i < RG; ++i) {
-        float r[8];
-        const float lm = row_scores(c, i, r);
-        if (!exact && __any(lm > m_ref[i] + kRoom4)) {
-          const float mx = max_xor32(max_xor16(lm));
-          again |= __any(m_ref[i] != -INFINITY && mx > m_ref[i] + kRoom4) != 0;
-          if (m_ref[i] == -INFINITY) m_ref[i] = mx;
-        }
-        const float nm = m_ref[i] == -INFINITY ? 0.f : -m_ref[i];
-        float pv[8];
+        float r[8], pv[8];
+        row_scores(c, ks, i, m_less[i], r);
+        m_top[i] = largest(r, m_top[i]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(r[e], fq, nm));
+          const float p = __builtin_amdgcn_exp2f(r[e]);
           psum[i] += p;
           zsum[i] = fmaf(p, half_hi_to_float(c.side[e].y), zsum[i]);
           pv[e] = p * vs[e];
@@ -449,30 +467,26 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
           for (int i = 0; i < RG; ++i) o[i][2 * c8 + h] = mfma16x16x32_f16(pa[i], vf, o[i][2 * c8 + h]);
         }
       }
-      return !again;
     });
+    if (again) break;
+    v_top = max_xor32(max_xor16(v_top));
+    again = __any(v_top > kScaleRoom4) != 0;  // else p s v_by < 2^(13 + 2)
+#pragma unroll
+    for (int i = 0; i < RG; ++i) {
+      const float above = max_xor32(max_xor16(m_top[i]));
+      // A first chunk of nothing but -inf has no reference, and later scores are as they are.
+      again |= __any(above > (m_ref[i] == -INFINITY ? -INFINITY : kRoom4)) != 0;
+      m_top[i] = m_ref[i] == -INFINITY ? above : fmaxf(m_ref[i], m_ref[i] + above);
+    }
     if (again) {
-      OSCAR_WAIT_VM(0);
+#pragma unroll
+      for (int i = 0; i < RG; ++i) {
+        m_ref[i] = m_top[i];
+        m_less[i] = m_ref[i] == -INFINITY ? 0.f : m_ref[i];
+      }
+      set_scale(v_top / v_by);
       OSCAR_WAIT_LGKM();
       start();
-      float top = 0.f;
-      stream([&](int t0, int s) {
-        Chunk c;
-        read_chunk(t0, s, c);
-        top = fmaxf(top, c.top);
-#pragma unroll
-        for (int i = 0; i < RG; ++i) {
-          float r[8];
-          m_ref[i] = fmaxf(m_ref[i], row_scores(c, i, r));
-        }
-        return true;
-      });
-      OSCAR_WAIT_LGKM();
-      start();
-      set_scale(max_xor32(max_xor16(top)));
-#pragma unroll
-      for (int i = 0; i < RG; ++i) m_ref[i] = max_xor32(max_xor16(m_ref[i]));
-      exact = true;
     }
   } while (again);
 
