@@ -224,15 +224,17 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     const int nkb = min(((p_hi - 1) >> a.L.bk_shift) - kb_first + 1, kTable4);
     for (int j = tid; j < nkb; j += F::kThreads) lds.off[j] = block_offset4(a, t, head, kb_first + j);
   }
-  // Query rows as they are, 16-byte piece p of row r at p ^ r % 16, two rows a copy. A row past the task's
-  // reads the buffer's first row and is zeroed below.
+  // Query rows as they are, two rows a copy; 16-byte piece 8 g + m of row r at (16 (g % 2) + 8 (g / 2) + m)
+  // ^ r % 16, for the banks of the reads below, in which a quarter of a wavefront is lanes of two g. A row past
+  // the task's reads the buffer's first row and is zeroed below.
   const uint32_t q_area = lds_addr(lds.q);
 #pragma unroll
   for (int i = 0; i < RG * 8 / W; ++i) {
     const int row0 = 2 * (i * W + wave), row = row0 + (lane >> 5);
     const RowInfo ri = row_of(a, rows, head, row);
+    const int at = (lane & 31) ^ (row & 15);
     const uint16_t* src = a.query + (ri.valid ? ri.token * a.qs0 + ri.qhead * a.qs1 : 0) +
-                          8 * ((lane & 31) ^ (row & 15));
+                          8 * ((at >> 1 & 8) | (at << 1 & 16) | (at & 7));
     dma_dwordx4(src, q_area + row0 * kHeadDim * 2);
   }
   barrier_lds();  // the offsets
@@ -286,7 +288,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
   // groups' are read from LDS as they are used (256 registers a lane hold the accumulators and no more).
   auto q_operand = [&](int i, int m) {
     return *reinterpret_cast<const u32x4*>(lds.q + (16 * i + n) * kHeadDim * 2 +
-                                           16 * ((8 * g + m) ^ n));
+                                           16 * ((16 * (g & 1) + 8 * (g >> 1) + m) ^ n));
   };
   const float fq = a.scale_log2;
   float qs[RG];
@@ -305,17 +307,20 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     qs[i] = sum_xor32(sum_xor16(sum)) * fq;
   }
 
-  const int k_off = kSlot4 * n + 32 * g;
-  const int side_off = kSlot4 * 4 * g + kSide4;
-  // Transposed reads: lane i of 16 names the row of position 16 (i / 4 % 2) + 4 g + i % 4, the one of two
-  // neighbouring groups of 16 dims for i < 8 and the other above, so that a lane gets one dim of its own
+  // Row r of score tile 0 is position r of a chunk, of tile 1 position 16 + (r ^ 8): then the eight
+  // positions that a lane has, and all that either half wavefront reads at a time, lie in LDS banks of their
+  // own (with 16 + r, records 16 apart shared theirs: 101 cycles of conflicts a chunk).
+  const int k_off[2] = {kSlot4 * n + 32 * g, kSlot4 * (16 + (n ^ 8)) + 32 * g};
+  const int side_off[2] = {kSlot4 * 4 * g + kSide4, kSlot4 * (16 + (4 * g ^ 8)) + kSide4};
+  // Transposed reads: lane i of 16 names the row of position i % 4 of its four in tile i / 4 % 2, the one of
+  // two neighbouring groups of 16 dims for i < 8 and the other above, so that a lane gets one dim of its own
   // eight positions in either.
-  const int v_off = kSlot4 * (16 * (n >> 2 & 1) + 4 * g + (n & 3)) + kCodes4 + 8 * (n >> 3);
+  const int v_off = kSlot4 * ((n >> 2 & 1 ? 16 + (4 * g ^ 8) : 4 * g) + (n & 3)) + kCodes4 + 8 * (n >> 3);
 
   // A chunk in stage s: the products of its K codes and the rows, and its scales and zeros.
   struct Chunk {
     f32x4 acc[RG][2];
-    uint2 side[8];  // of the lane's positions 16 (e / 4) + 4 g + e % 4: K scale and zero, V scale and zero
+    uint2 side[8];  // of the lane's positions, row 4 g + e % 4 of tile e / 4: K scale and zero, V scale and zero
     bool whole;
     uint32_t seen;  // bit e, where not whole
   };
@@ -330,7 +335,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
       const int from = max(p_lo - t0, 0), to = min(p_hi - t0, kChunk4);
       uint32_t bits = ok_block ? (0xffffffffu << from) & (0xffffffffu >> (kChunk4 - to)) : 0u;
       asm volatile("" : "+v"(bits));
-      c.seen = (bits >> (4 * g) & 0xfu) | (bits >> (12 + 4 * g) & 0xf0u);
+      c.seen = (bits >> (4 * g) & 0xfu) | (bits >> (12 + (4 * g ^ 8)) & 0xf0u);
       if (lane < kChunk4 && !(bits >> lane & 1u))
         *reinterpret_cast<uint32_t*>(st + kSlot4 * lane + kSide4 + 4) = 0u;
     }
@@ -341,7 +346,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        kw[tt][h] = *reinterpret_cast<const u32x4*>(st + k_off + 16 * kSlot4 * tt + 16 * h);
+        kw[tt][h] = *reinterpret_cast<const u32x4*>(st + k_off[tt] + 16 * h);
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
       const u32x4 k0 = codes_bf16(kw[0][m >> 2][m & 3]), k1 = codes_bf16(kw[1][m >> 2][m & 3]);
@@ -354,7 +359,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      c.side[e] = *reinterpret_cast<const uint2*>(st + side_off + kSlot4 * (16 * (e >> 2) + (e & 3)));
+      c.side[e] = *reinterpret_cast<const uint2*>(st + side_off[e >> 2] + kSlot4 * (e & 3));
   };
   // Scores of row group i in log2 units, less m.
   auto row_scores = [&](Chunk& c, const float (&ks)[8], int i, float m, float (&r)[8]) {
