@@ -291,7 +291,7 @@ def choose_chunk_splits(tokens, requests, num_kv_heads, q_heads, max_seq_len, co
 
 
 # The same of a 32-row tile of 4-bit records and its round of 256 positions.
-INT4_TILE_ROWS, INT4_ROUND_TOKENS, INT4_ROUND_US, INT4_START_US = 32, 256, 2.45, 12.0
+INT4_TILE_ROWS, INT4_ROUND_TOKENS, INT4_ROUND_US, INT4_START_US = 32, 256, 2.1, 12.0
 
 
 @functools.lru_cache(maxsize=256)
@@ -299,8 +299,7 @@ def choose_int4_splits(tokens, requests, num_kv_heads, q_heads, max_seq_len, com
                        max_splits=16, scratch_bytes=128 << 20):
     """Split count of the 4-bit history branch in steps with more than 16 query tokens in some request:
     ``choose_chunk_splits`` with the times of that kernel's tiles (2048 tokens over 32768, six heads, 384
-    tiles: 716 / 530 / 576 / 553 / 613 us with 1 / 2 / 3 / 4 / 5 splits, 1.5 to 3 rounds over the CUs; 64
-    over 16000: 171 / 94 / 57 / 39 / 33 with 1 / 2 / 4 / 8 / 16)."""
+    tiles: 567 / 448 / 505 / 471 / 541 us with 1 / 2 / 3 / 4 / 5 splits, 1.5 to 3 rounds over the CUs)."""
     if not max_seq_len:
         return 1
     group = q_heads // num_kv_heads

@@ -21,10 +21,13 @@
 //
 // Up to 16 rows the records' bytes bound it: 32 requests of 32704 positions (285 MB) take 52 us, 5.5 TB/s
 // where a large copy moves 5.2 (reads alone reach 7). Tiles of 32 rows are bound by the vector units, which
-// issue in 72 % of the cycles (the matrix units' share is 34 %): a wavefront's 32 positions cost 450
-// vector instructions and 61 matrix instructions, of which the unpacking, 200, is paid once per tile:
-// 2048 tokens of 6 heads against 32768 positions 505 us, 0.82 PFLOP/s. Tiles of 48 or 64 rows would halve
-// the unpacking's share but spill: a row group's sums are 64 registers of a lane.
+// issue in 78 % of the cycles (the matrix units' share is 38 %): a wavefront's 32 positions cost 400 vector
+// instructions, of which the unpacking, 224, is paid once per tile, and 64 matrix instructions: 2048 tokens
+// of 6 heads against 32768 positions take 447 us, 0.92 PFLOP/s. Tiles of 48 or 64 rows, on one wavefront a
+// SIMD with 512 registers, halve the unpacking's share but have no second wavefront that fills the waits:
+// 617 and 632 us. Codes as fp16 subnormals (five instructions for eight instead of seven) lose the low bits
+// of the products (errors 2.5e-5 of the sum of magnitudes, which the matrix instruction aligns as if the
+// codes were normal).
 #include "dma.h"
 #include "history4.h"
 
@@ -424,6 +427,10 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
     stream([&](int t0, int s) {
       Chunk c;
       read_chunk(t0, s, c);
+      // From here to most of the second products this wavefront goes ahead of its SIMD's other one, so that
+      // one's vector instructions run beside the other's matrix instructions (2048 tokens against 32768
+      // positions 493 -> 453 us; to the end of the products 458, from the products on 481).
+      __builtin_amdgcn_s_setprio(1);
       float ks[8], vs[8];  // products with zero added: one instruction with the conversion
 #pragma unroll
       for (int e = 0; e < 8; ++e) ks[e] = fmaf(half_lo_to_float(c.side[e].x), fq, 0.f);
@@ -467,6 +474,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
             __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2_ptr_t)(st + v_off + 16 * c8));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          if (c8 == 6 && h == 0) __builtin_amdgcn_s_setprio(0);
           const u32x4 vf = codes_f16(static_cast<uint32_t>(w[h]));
 #pragma unroll
           for (int i = 0; i < RG; ++i) o[i][2 * c8 + h] = mfma16x16x32_f16(pa[i], vf, o[i][2 * c8 + h]);
