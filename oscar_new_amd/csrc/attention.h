@@ -344,8 +344,8 @@ hipError_t launch_history(const AttnArgs& a, dim3 grid, int rows, hipStream_t st
                           int32_t* queue = nullptr);
 
 // The checks and fields of one attention_partials launch (attention.hip) over records of `bits` bits
-// (history branch): OSCAR_OK with *out filled and *qrows = query rows per task, or the entry point's error code. Nothing is
-// launched when n == 0 (OSCAR_OK before the pointer checks).
+// (history branch): OSCAR_OK with *out filled and *qrows = query rows per task, or the entry point's error
+// code. Nothing is launched when n == 0 (OSCAR_OK before the pointer checks).
 int make_attn_args(const void* query, int64_t q_s0, int64_t q_s1, int64_t q_s2, const void* key,
                    int64_t k_s0, int64_t k_s1, int64_t k_s2, const void* value, int64_t v_s0,
                    int64_t v_s1, int64_t v_s2, const void* history, int64_t history_bytes,

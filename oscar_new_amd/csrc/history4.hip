@@ -53,16 +53,13 @@ struct Form4 {
     uint32_t off[kTable4];
     float red[3][W][16 * RG];  // per wavefront: reference score, sum p, sum p z
   };
+  static_assert(S == 2);  // wait_chunks
   static_assert(W * 16 * kHeadDim * 4 <= sizeof(Lds::ring), "a row group's merge fits the ring");
 };
 
-// Waits until at most `chunks` chunks' copies are in flight.
+// Waits until at most `chunks` chunks' copies (0 or 1) are in flight.
 __device__ __forceinline__ void wait_chunks(int chunks) {
-  if (chunks >= 3)
-    OSCAR_WAIT_VM(3 * kDma4);
-  else if (chunks == 2)
-    OSCAR_WAIT_VM(2 * kDma4);
-  else if (chunks == 1)
+  if (chunks)
     OSCAR_WAIT_VM(kDma4);
   else
     OSCAR_WAIT_VM(0);
@@ -73,8 +70,9 @@ __device__ __forceinline__ void wait_chunks(int chunks) {
 // All splits run at once, one per CU, so the launch takes as long as T: eight lengths between the mean
 // share and the one that always fits are tried, one by each wavefront, and the least that fits is
 // taken (32 requests of 32704 positions on 256 slots: 8 splits of 4096 each). Multiples of kStep4, at
-// least kMinSplit4.
-constexpr int kMinSplit4 = 256, kStep4 = 64, kTried4 = 8;
+// least kMinSplit4, one chunk for a wavefront of each SIMD (one request of 900 positions with its merge: 15.9
+// us in splits of 128, 16.8 of 256).
+constexpr int kMinSplit4 = 128, kStep4 = 64, kTried4 = 8;
 
 struct Unit4 {
   Task t;
@@ -518,50 +516,47 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
 #pragma unroll
   for (int i = 0; i < RG; ++i) {
     __syncthreads();  // the ring (or the last rows' sums) has been read
+    const int live = min(rows.end - rows.base - 16 * i, 16);
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
+      if (4 * g + v >= live) continue;
       const int row = 16 * i + 4 * g + v;
       float mx = lds.red[0][0][row];
 #pragma unroll
       for (int w = 1; w < W; ++w) mx = fmaxf(mx, lds.red[0][w][row]);
       const float mw = lds.red[0][wave][row];
-      const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx) * v_back;
+      const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mx) * v_back;
       float* dst = s_o + (wave * 16 + 4 * g + v) * kHeadDim + n;
 #pragma unroll
       for (int c = 0; c < 16; ++c) dst[16 * c] = o[i][c][v] * f;
     }
     __syncthreads();
-    // Thread -> row tid / 32, dims 4 (tid % 32) and 128 further on.
+    // A wavefront takes a row, a lane four dims of it.
 #pragma unroll
-    for (int r0 = 0; r0 < 16; r0 += F::kThreads / 32) {
-      const int row16 = r0 + (tid >> 5), row = 16 * i + row16, d0 = 4 * (tid & 31);
+    for (int r0 = 0; r0 < 16; r0 += W) {
+      const int row16 = r0 + wave, row = 16 * i + row16, d0 = 4 * lane;
       const RowInfo ri = row_of(a, rows, head, row);
       if (!ri.valid) continue;
       float mx = -INFINITY;
 #pragma unroll
       for (int w = 0; w < W; ++w) mx = fmaxf(mx, lds.red[0][w][row]);
       float den = 0.f, zs = 0.f;
-      f32x4 sum[2] = {};
+      f32x4 sum = {};
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         const float mw = lds.red[0][w][row];
-        const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx);
+        const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mx);
         den = fmaf(f, lds.red[1][w][row], den);
         zs = fmaf(f, lds.red[2][w][row], zs);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          sum[h] += *reinterpret_cast<const f32x4*>(s_o + (w * 16 + row16) * kHeadDim + d0 + 128 * h);
+        sum += *reinterpret_cast<const f32x4*>(s_o + (w * 16 + row16) * kHeadDim + d0);
       }
       const float inv = 1.0f / fmaxf(den, 1.0e-30f);
       const int64_t out_row = (ri.token * a.hq + ri.qhead) * a.splits + split;
+      f32x4 r;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f32x4 r;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = (sum[h][e] + zs) * inv;
-        *reinterpret_cast<f32x4*>(a.partials + out_row * kHeadDim + d0 + 128 * h) = r;
-      }
-      if (d0 == 0) a.lse[out_row] = den == 0.f ? -INFINITY : (mx + log2f(den)) * kLn2;
+      for (int e = 0; e < 4; ++e) r[e] = (sum[e] + zs) * inv;
+      *reinterpret_cast<f32x4*>(a.partials + out_row * kHeadDim + d0) = r;
+      if (lane == 0) a.lse[out_row] = den == 0.f ? -INFINITY : (mx + log2f(den)) * kLn2;
     }
   }
 }
@@ -580,7 +575,6 @@ __global__ __launch_bounds__(F::kThreads) void history4_kernel(const AttnArgs a,
     split = unit.split;
     nsplit = unit.nsplit;
     split_tokens = unit.split_tokens;
-    if (split == 0) write_unused_splits<F::kThreads>(a, t, head, nsplit, a.splits);
     __syncthreads();  // the lengths have been read
   } else {
     if (!read_task(a, t, static_cast<int>(blockIdx.x))) return;
@@ -596,6 +590,8 @@ __global__ __launch_bounds__(F::kThreads) void history4_kernel(const AttnArgs a,
   history_positions(a, t, t.recent_begin - t.sink_len, nsplit, split, split_tokens, p_lo, p_hi);
   const Rows4 rows{t.qstart + t.qoff, 0, min(a.qt, t.qlen - t.qoff) * a.g};
   history_rows4<F>(a, t, rows, head, p_lo, p_hi, split, lds);
+  // Last, as the other rows' copies would wait for these stores.
+  if (a.split_tokens < 0 && split == 0) write_unused_splits<F::kThreads>(a, t, head, nsplit, a.splits);
 }
 
 // ---- steps with many query tokens in a request: tiles of 16 RG of its rows instead of tasks, so that a
