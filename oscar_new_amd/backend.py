@@ -24,10 +24,9 @@ import os
 import torch
 
 from . import kernels
-from .config import (INT4_SLOTS, OscarConfig, attention_programs, choose_chunk_splits, choose_device_partition,
-                     choose_history_partition, choose_int4_splits, choose_splits,
-                     chunk_kernel_pays,
-                     shared_prefix_pays)
+from .config import (INT4_SLOTS, OscarConfig, attention_programs, choose_chunk_splits,
+                     choose_device_partition, choose_history_partition, choose_int4_splits,
+                     choose_splits, chunk_kernel_pays, shared_prefix_pays)
 
 SPLIT_POLICIES = ("device", "reference", "mi355x")
 ENV_SPLIT_POLICY = "OSCAR_AMD_SPLIT_POLICY"
@@ -247,8 +246,8 @@ class OscarAttentionImpl:
     def _roles_share_history_launch(self, meta):
         """Whether the step's history launch carries the pre-attention role workgroups."""
         layout = getattr(meta, "layout", None)
-        return (self.cfg.history_bits == 2 and self.fused and self.overlap and not self.one_launch_post and not self.layer_step
-                and layout is not None
+        return (self.cfg.history_bits == 2 and self.fused and self.overlap
+                and not self.one_launch_post and not self.layer_step and layout is not None
                 and kernels.history_pre_supported(meta, layout, self.num_heads))
 
     def _queue_roles(self, meta, split_tokens, tokens):

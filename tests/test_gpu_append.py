@@ -69,7 +69,9 @@ def codes_of(x, cfg, ratio, factor):
     def quantize(limit):
         c = x if limit is None else torch.minimum(torch.maximum(x, -limit), limit)
         low, high = c.amin(-1, keepdim=True), c.amax(-1, keepdim=True)
-        scale = ((high - low) / 15).clamp(min=2.0**-14).half()
+        # By a tensor: torch multiplies by a scalar's reciprocal, which misses the ties of fp16, as
+        # 6.0443115234375 / 15 = 1650.5 x 2^-12.
+        scale = ((high - low) / torch.full_like(high, 15)).clamp(min=2.0**-14).half()
         zero = low.half()
         codes = ((c - zero.float()) / scale.float() + 0.5).trunc().clamp(0, 15)
         return codes, scale, zero
@@ -398,6 +400,30 @@ def test_extreme_rows(n):
     m[2][7, 0, 17] = float("nan")
     append(m, layout, history, slots, counts_of(n), axes=False)
     assert bool(kernels.read_records(history, slots[7:8], layout)[1].isnan().all())
+
+
+@pytest.mark.parametrize("n", [8, 1400, 2200])
+@pytest.mark.parametrize("ratio", [1.0, 0.997, 0.99, 252 / 255, 0.985, 0.9, 0.875])
+def test_order_statistics(n, ratio):
+    """Rows of one sign, of few different values, of magnitudes over many powers of two, unturned."""
+    m = list(make(n, 1, 1, 0))
+    one = torch.eye(256, dtype=torch.bfloat16, device=DEV)
+    x = m[2].float()
+    x[0::8], x[1::8] = x[0::8].abs() + 0.01, -x[1::8].abs() - 0.01
+    x[2::8] = (x[2::8] * 2).round() / 2  # many equal ones, zeros of either sign
+    x[3::8] *= 2.0 ** torch.randint(-12, 3, x[3::8].shape, device=DEV)
+    x[4::8] = x[4::8].sign() * 2.0**-100
+    x[5::8, :, 5] = 1e30
+    value = x.bfloat16()
+    layout = layout_of(1, k_clip_ratio=ratio, v_clip_ratio=ratio)
+    history, slots = cache(n, layout, n // 768 + 2)
+    kernels.rope_append(None, value.flip(-1), value, history, slots, counts_of(n), layout, one, one)
+    parts, _ = record_parts(history, layout, slots)
+    for (codes, scale, zero), rows in zip(parts, (value.flip(-1), value)):
+        want = codes_of(rows, layout.config, ratio, 1.0)
+        # A zero point of zero is one of either sign.
+        assert torch.equal(scale, want[1][..., 0]) and bool((zero == want[2][..., 0]).all())
+        assert torch.equal(codes, want[0].to(torch.uint8))
 
 
 @pytest.mark.parametrize("n", [40, 900])

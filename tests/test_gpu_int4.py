@@ -186,6 +186,25 @@ def test_scores_and_scales_that_grow(qlen):
         check(s, attend(s, split_tokens=0, splits=3, chunk=qlen > 16))
 
 
+@pytest.mark.parametrize("qlen", [1, 4, 40])
+def test_first_chunks_of_no_weight(qlen):
+    """Positions of score -inf (keys of -inf, queries above zero) count nothing, a wavefront's first chunks
+    among them, whose largest score is no reference then."""
+    s = world([2000], [qlen], layout_of(1), 6, poison=False)
+    s.query = s.query.abs() + 0.01
+    lo, hi = s.spans[0]
+    view = s.history.view(s.pool, -1)[:, : 768 * 272].view(s.pool, 768, 272)
+    side = view[..., 256:264].contiguous().view(torch.float16)
+    page = s.meta.block_tables[0, ::6][:3].long() // 6
+    at = torch.arange(3 * 768, device=DEV).view(3, 768)
+    side[page, :, 1] = torch.where(at < lo + 1000, -torch.inf, side[page, :, 1].float()).half()
+    view[..., 256:264] = side.view(torch.uint8)
+    got = [attend(s), attend(s, split_tokens=0, splits=1), attend(s, split_tokens=0, splits=3, chunk=qlen > 16)]
+    s.spans = [(lo + 1000, hi)]
+    for g in got:
+        check(s, g)
+
+
 def test_records_beyond_4_gb():
     layout = layout_of(2)
     s = world([3000, 800], [1, 1], layout, 6, extra_pages=5600, high=True, poison=False)
