@@ -298,7 +298,7 @@ INT4_TILE_ROWS, INT4_ROUND_TOKENS, INT4_ROUND_US, INT4_START_US = 32, 256, 2.1, 
 def choose_int4_splits(tokens, requests, num_kv_heads, q_heads, max_seq_len, compute_units=256,
                        max_splits=16, scratch_bytes=128 << 20):
     """Split count of the 4-bit history branch in steps with more than 16 query tokens in some request:
-    ``choose_chunk_splits`` with the times of that kernel's tiles (2048 tokens over 32768, six heads, 384
+    ``choose_chunk_splits`` with the times of that kernel's tiles (2048 tokens over 30400, six heads, 384
     tiles: 567 / 448 / 505 / 471 / 541 us with 1 / 2 / 3 / 4 / 5 splits, 1.5 to 3 rounds over the CUs)."""
     if not max_seq_len:
         return 1

@@ -19,11 +19,13 @@
 // scores of eight positions and its probabilities are the P operand of the second product, whose other
 // operand comes from transposed LDS reads of 4-bit codes. The eight states are joined at the end.
 //
-// Up to 16 rows the records' bytes bound it: 32 requests of 32704 positions (285 MB) take 52 us, 5.5 TB/s
-// where a large copy moves 5.2 (reads alone reach 7). Tiles of 32 rows are bound by the vector units, which
+// Up to 16 rows the records' bytes bound it: 32 requests of 32636 positions (284 MB) take 52 us, 5.5 TB/s
+// where a large copy moves 5.2 (reads alone reach 7); a small step its chain (one request of 579 positions 10.8
+// us: 3.3 until the unit is known, 1.5 until its records are there, 0.7 for the query operands, 2 for a
+// wavefront's chunk, 3 for the join). Tiles of 32 rows are bound by the vector units, which
 // issue in 78 % of the cycles (the matrix units' share is 38 %): a wavefront's 32 positions cost 400 vector
 // instructions, of which the unpacking, 224, is paid once per tile, and 64 matrix instructions: 2048 tokens
-// of 6 heads against 32768 positions take 447 us, 0.92 PFLOP/s. Tiles of 48 or 64 rows, on one wavefront a
+// of 6 heads against 30400 positions take 447 us, 0.86 PFLOP/s. Tiles of 48 or 64 rows, on one wavefront a
 // SIMD with 512 registers, halve the unpacking's share but have no second wavefront that fills the waits:
 // 617 and 632 us. Codes as fp16 subnormals (five instructions for eight instead of seven) lose the low bits
 // of the products (errors 2.5e-5 of the sum of magnitudes, which the matrix instruction aligns as if the
@@ -69,8 +71,8 @@ __device__ __forceinline__ void wait_chunks(int chunks) {
 // ceil(length / T) each, fit the budget's slots of one KV head (or one a task where it is smaller).
 // All splits run at once, one per CU, so the launch takes as long as T: eight lengths between the mean
 // share and the one that always fits are tried, one by each wavefront, and the least that fits is
-// taken (32 requests of 32704 positions on 256 slots: 8 splits of 4096 each). Multiples of kStep4, at
-// least kMinSplit4, one chunk for a wavefront of each SIMD (one request of 900 positions with its merge: 15.9
+// taken (32 requests of 32636 positions on 256 slots: 8 splits of 4096 each). Multiples of kStep4, at
+// least kMinSplit4, one chunk for a wavefront of each SIMD (one request of 579 positions with its merge: 15.9
 // us in splits of 128, 16.8 of 256).
 constexpr int kMinSplit4 = 128, kStep4 = 64, kTried4 = 8;
 
@@ -426,7 +428,7 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
       Chunk c;
       read_chunk(t0, s, c);
       // From here to most of the second products this wavefront goes ahead of its SIMD's other one, so that
-      // one's vector instructions run beside the other's matrix instructions (2048 tokens against 32768
+      // one's vector instructions run beside the other's matrix instructions (2048 tokens against 30400
       // positions 493 -> 453 us; to the end of the products 458, from the products on 481).
       __builtin_amdgcn_s_setprio(1);
       float ks[8], vs[8];  // products with zero added: one instruction with the conversion
