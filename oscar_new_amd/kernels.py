@@ -350,10 +350,12 @@ def attention_partials(query, key, value, history, window, meta, layout, scale, 
 
 def _attention_int4(query, history, meta, layout, scale, splits, split_tokens, chunk=None):
     """The history branch of ``attention_partials`` over 4-bit records."""
-    table = _int32(meta.block_tables, "block_tables")
-    qstarts = _int32(meta.query_start_loc, "query_start_loc")
-    seq_lens, counts = _int32(meta.seq_lens, "seq_lens"), _int32(meta.counts, "counts")
-    tasks, task_count = _int32(meta.tasks, "tasks"), _int32(meta.task_count, "task_count")
+    table, qstarts, seq_lens = meta.block_tables, meta.query_start_loc, meta.seq_lens
+    counts, tasks, task_count = meta.counts, meta.tasks, meta.task_count
+    if not (table.dtype == qstarts.dtype == seq_lens.dtype == counts.dtype == tasks.dtype
+            == task_count.dtype == torch.int32):
+        for name in ("block_tables", "query_start_loc", "seq_lens", "counts", "tasks", "task_count"):
+            _int32(getattr(meta, name), name)
     device = _same_device(query, history=history, block_tables=table, query_start_loc=qstarts,
                           seq_lens=seq_lens, counts=counts, tasks=tasks, task_count=task_count)
     n, hq, d = query.shape
@@ -367,7 +369,7 @@ def _attention_int4(query, history, meta, layout, scale, splits, split_tokens, c
         raise ValueError("history must be the contiguous bytes of the K stripe")
     if splits < 1:
         raise ValueError(f"a launch has at least one split, got {splits}")
-    lse = torch.empty((n, hq, splits), dtype=torch.float32, device=device)
+    lse = query.new_empty((n, hq, splits), dtype=torch.float32)
     partials = lse.new_empty((n, hq, splits, d))
     if n == 0:
         return partials, lse
@@ -395,7 +397,7 @@ def merge_splits(partials, lse, counts):
     """LSE merge of split partials (reference kernels.py:506-511) -> (bf16 out, logsum)."""
     device = _same_device(partials, lse=lse, counts=counts)
     n, hq, splits, d = partials.shape
-    out = torch.empty((n, hq, d), dtype=torch.bfloat16, device=device)
+    out = partials.new_empty((n, hq, d), dtype=torch.bfloat16)
     logsum = partials.new_empty((n, hq), dtype=torch.float32)
     if n:
         if not partials.is_contiguous():
@@ -730,21 +732,30 @@ def rope_append(query, key, value, history, slots, counts, layout, rk_t, rv_t, c
     q_out = None if query is None else _rows_out(query)
     q_rot = torch.empty_like(q_out) if turn_query else None
     if n:
-        q0 = q1 = v0 = v1 = 0
+        q = v = (None, 0, 0)
+        out = turned = records = at = matrix = weight = table = places = None
         key, k0, k1 = _rows_aligned(key)
         if query is not None:
             query, q0, q1 = _rows_aligned(query)
+            q, out = (query.data_ptr(), q0, q1), q_out.data_ptr()
+            if turn_query:
+                turned = q_rot.data_ptr()
         if store:
             value, v0, v1 = _rows_aligned(value)
+            v, matrix = (value.data_ptr(), v0, v1), rv_t.data_ptr()
+            records, at = history.data_ptr(), slots.data_ptr()
+        if cos_sin is not None:
+            table, places = cos_sin.data_ptr(), positions.data_ptr()
+        if k_weight is not None:
+            weight = k_weight.data_ptr()
         _launch(
-            _ext.library().oscar_rope_append, "rope_append", device, _ptr(query), q0, q1,
-            key.data_ptr(), k0, k1, _ptr(value), v0, v1, n, hq, hk, _ptr(q_weight), _ptr(k_weight),
-            k_weight is not None and k_weight.dtype == torch.float32, bool(unit_offset), eps,
-            _ptr(cos_sin), rows, stride, cos_sin is not None and cos_sin.dtype == torch.float32,
-            rotary, bool(interleaved), _ptr(positions), position_stride, axis_count, _ptr(axes),
-            _ptr(counts), _ptr(q_out), k_out.data_ptr(), _ptr(rk_t), _ptr(rv_t) if store else None,
-            _ptr(q_rot), _ptr(history) if store else None, size, _ptr(slots) if store else None, lay,
-            clip,
+            _ext.library().oscar_rope_append, "rope_append", device, *q, key.data_ptr(), k0, k1, *v, n,
+            hq, hk, None if q_weight is None else q_weight.data_ptr(), weight,
+            weight is not None and k_weight.dtype == torch.float32, bool(unit_offset), eps, table, rows,
+            stride, table is not None and cos_sin.dtype == torch.float32, rotary, bool(interleaved),
+            places, position_stride, axis_count, None if axes is None else axes.data_ptr(),
+            None if counts is None else counts.data_ptr(), out, k_out.data_ptr(),
+            None if rk_t is None else rk_t.data_ptr(), matrix, turned, records, size, at, lay, clip,
         )
     return q_out, k_out, q_rot
 
@@ -760,7 +771,7 @@ def read_records(history, slots, layout):
     if not history.is_contiguous():
         raise ValueError("history must be the contiguous bytes of the K stripe")
     n = slots.shape[0]
-    key = torch.empty((n, layout.kv_heads, 256), dtype=torch.bfloat16, device=device)
+    key = history.new_empty((n, layout.kv_heads, 256), dtype=torch.bfloat16)
     value = torch.empty_like(key)
     if n:
         if not slots.is_contiguous():
