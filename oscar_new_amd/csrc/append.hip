@@ -950,19 +950,21 @@ RowSet row_set(const void* x, int64_t s0, int64_t s1, const void* weight, void* 
           static_cast<int32_t>(heads), make_fastdiv(static_cast<uint32_t>(heads))};
 }
 
-// The workgroups for the values such that the longer of both kinds' walks is shortest: rounds of the
-// wavefronts, in which a block of keys or values (with the quantizer) costs about twice one of queries that
-// are rotated, which costs twice those that are not.
-int value_groups_of(int64_t q_blocks, int64_t kv_blocks, bool rotated) {
-  const int64_t q_cost = rotated ? 2 : 1;
-  auto rounds = [](int64_t b, int64_t groups) { return (b + kWalkWaves * groups - 1) / (kWalkWaves * groups); };
+// The workgroups for the values such that the longer of both kinds' walks is shortest. A CU's wavefronts
+// share its four SIMDs, so the largest number of blocks of a SIMD counts, each at its cost in units of about
+// 1 us: a value 6 (product and quantizer), a key 6, a query 3, a norm 2 more, a query's product 3. 16384
+// tokens of 6 heads, normed and rotated: 32 workgroups 71.5 us, 24 71.7, 64 78.6; 4 heads that are only
+// turned: 64 32.1, 52 32.8, 44 38.5, 80 34.5; 2048 tokens of 12: 32 22.3, 28 23.1, 36 28.6.
+int value_groups_of(int64_t q_blocks, int64_t kv_blocks, bool rotated, bool normed) {
+  const int64_t k_cost = normed ? 8 : 6, q_cost = 3 + (normed ? 2 : 0) + (rotated ? 3 : 0);
+  auto of_simd = [](int64_t blocks, int64_t groups) { return (blocks + 4 * groups - 1) / (4 * groups); };
   int best = 1;
   int64_t least = INT64_MAX;
   for (int g = 1; g < static_cast<int>(kWalkGroups); ++g) {
-    const int64_t rest = kWalkGroups - g, keys = rounds(kv_blocks, rest);
-    const int64_t qk = 4 * keys + q_cost * (rounds(q_blocks + kv_blocks, rest) - keys);
-    const int64_t v = 4 * rounds(kv_blocks, g), time = v > qk ? v : qk;
-    if (time < least) {
+    const int64_t rest = kWalkGroups - g, keys = of_simd(kv_blocks, rest);
+    const int64_t qk = k_cost * keys + q_cost * (of_simd(q_blocks + kv_blocks, rest) - keys);
+    const int64_t v = 6 * of_simd(kv_blocks, g), time = v > qk ? v : qk;
+    if (time <= least) {
       least = time;
       best = g;
     }
@@ -1068,7 +1070,8 @@ extern "C" int oscar_rope_append(
     hipLaunchKernelGGL(turn_rows_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
                        lds(kTurnRows + 8), s, a, q);
   } else if (all > kSmallAppendRows && walks(a)) {
-    const int value_groups = value_groups_of(blocks(0, 16), blocks(1, 16), q_rot != nullptr);
+    const int value_groups = value_groups_of(blocks(0, 16), blocks(1, 16), q_rot != nullptr,
+                                             k_weight != nullptr);
     auto walk = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(kWalkGroups), dim3(kWalkThreads), 0, s, a, value_groups);
     };
