@@ -12,8 +12,8 @@
 //
 // Three forms. Few rows: blocks of 16 (token, head) rows on as many CUs as there are blocks, bound by the
 // chain counts - positions - angles - norm - product - quantile - record (10.5 us for 32 tokens of 6 + 1
-// heads, 11.3 for 512). Many rows of 4-bit layouts: wavefronts that walk 16-row blocks (15.8 us for 2048
-// tokens, 53 for 16384, 181 MB). Rows that are turned only: no product, the rows' bytes.
+// heads, 11.3 for 512). Many rows of 4-bit layouts: wavefronts that walk 16-row blocks (15.2 us for 2048
+// tokens, 52 for 16384, 181 MB). Rows that are turned only: no product, the rows' bytes.
 #include "dma.h"
 #include "norm_row.h"
 #include "quant4.h"
@@ -342,7 +342,7 @@ void append_kernel(const AppendArgs a, int64_t q_blocks, int64_t k_blocks) {
 }
 
 // Rows up to which blocks of 16 find a CU each. 512 tokens of 8 rows: 11.3 us, against 15.4 in blocks of 32
-// and 13.8 by walking wavefronts; 768: 17.6, 15.9 and 14.2; 2048: 31, 24 and 15.8. Blocks of 32 remain for
+// and 13 by walking wavefronts; 768: 17.6, 15.9 and 13; 2048: 31, 24 and 15.2. Blocks of 32 remain for
 // what the walk does not serve (`walks`).
 constexpr int64_t kSmallAppendRows = 16 * 256;
 constexpr unsigned kWalkGroups = 256;  // one per CU
@@ -353,9 +353,10 @@ constexpr unsigned kWalkGroups = 256;  // one per CU
 // row lane % 16 (g = lane / 16), which is what the products read as B operand, and ends with the same
 // pieces of the rotated row, so that a row goes from memory to its record in registers: 16 rows are
 // quantized at a time, four lanes each. Pairs of halves 32 dims or a multiple of it apart, and adjacent
-// ones, lie in one lane. 16384 tokens of 8 rows are bound by the rows' bytes; 2048, one block a wavefront, by
-// what a block takes: 5 to 7 us until R and the angles are there, 4 for the norm and the turn, 3 for the
-// products, 4 for the records (two wavefronts a SIMD).
+// ones, lie in one lane. 2048 tokens of 8 rows, one block a wavefront, are bound by what a block takes: 5 to
+// 7 us until R and the angles are there, 4 for the norm and the turn, 3 for the products (whose operands,
+// 128 KB a block, LDS hands over in 2), 4 for the records; 16384 by the same a block later, at 60 to 70 % of
+// what the rows' bytes would take.
 constexpr int kWalkWaves = 8, kWalkThreads = kWalkWaves * kWave;
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
@@ -502,8 +503,11 @@ __device__ __forceinline__ void statistics_of_row(const u32x4 (&z)[8], uint32_t 
 // quantize_store4 (percentile or factor) of 16 rows, four lanes each: z[m] holds dims 32 m + 8 g .. + 7 as
 // bf16. The quantile's two order statistics are among the kLargest largest magnitudes where it is near 1
 // (0.9726 on).
+// `record_of`: the row's record or null, asked for when the statistics are known (its slot is on the way
+// until then).
+template <class Record>
 __device__ __forceinline__ void quantize_rows4(const u32x4 (&z)[8], int mode, float ratio, float factor,
-                                               uint8_t* codes, uint8_t* side, int g) {
+                                               bool is_v, int g, Record record_of) {
 #pragma clang fp contract(off)
   // Two bf16 values a word: as signed numbers the largest is the row's maximum unless all are negative, as
   // unsigned ones the largest is its minimum unless none is.
@@ -560,6 +564,8 @@ __device__ __forceinline__ void quantize_rows4(const u32x4 (&z)[8], int mode, fl
   const uint32_t zero = float_to_f16_bits(mn), scale = float_to_f16_bits(spread);
   const float zf = f16_bits_to_float(zero), sf = f16_bits_to_float(scale);
   const float r = scale_rcp(sf);
+  uint8_t* const record = record_of();
+  uint8_t* const codes = record + is_v * kCodes4;
 #pragma unroll
   for (int m = 0; m < 8; ++m) {
     float d[8], y[8];
@@ -584,9 +590,10 @@ __device__ __forceinline__ void quantize_rows4(const u32x4 (&z)[8], int mode, fl
       c = c < 0 ? 0 : (c > 15 ? 15 : c);
       packed |= static_cast<uint32_t>(c) << (4 * e);
     }
-    if (codes) *reinterpret_cast<uint32_t*>(codes + 16 * m + 4 * g) = packed;
+    if (record) *reinterpret_cast<uint32_t*>(codes + 16 * m + 4 * g) = packed;
   }
-  if (codes && g == 0) *reinterpret_cast<uint32_t*>(side) = scale | (zero << 16);
+  if (record && g == 0)
+    *reinterpret_cast<uint32_t*>(record + kSide4 + 4 * is_v) = scale | (zero << 16);
 }
 
 template <bool kAdjacent, bool kFp32, bool kAxes>
@@ -618,7 +625,7 @@ __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const Appe
   // Packed angles of eight consecutive dims of a half, or of the four pairs of eight adjacent dims.
   constexpr int kWords = kAdjacent ? 2 * kLoads : 4 * kLoads;
   const char* turn = nullptr;  // the angles' table row
-  int64_t turn_token = 0;      // or the token that has several
+  uint32_t turn_token = 0;     // or the token that has several
   // Angles of the lane's group j of dims (32 j + 8 g on).
   auto load_words = [&](int j, uint32_t (&c)[kWords], uint32_t (&sn)[kWords]) {
     const int pair = kAdjacent ? 16 * j + 4 * g : 32 * j + 8 * g;
@@ -823,7 +830,8 @@ __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const Appe
     const int which = set_of(b);
     finish(which);
     const int64_t my_row = row;
-    const int64_t slot = which && live ? a.slots[token] : -1;
+    const uint32_t my_token = token;
+    const bool my_live = live;
     const int my_head = head;
     if (b + step < blocks) {
       place(b + step);
@@ -870,14 +878,12 @@ __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const Appe
         for (int m = 0; m < 8; ++m) *reinterpret_cast<u32x4*>(out + 32 * m) = z[m];
       continue;
     }
-    uint8_t* record = nullptr;
-    if (slot >= 0 && slot < a.history_bytes) {
+    const int64_t slot = my_live ? a.slots[my_token] : -1;
+    quantize_rows4(z, a.mode, a.ratio[which], a.factor[which], is_v, g, [&]() -> uint8_t* {
+      if (slot < 0 || slot >= a.history_bytes) return nullptr;
       const int64_t at = slot_offset(a.L, slot, my_head);
-      if (at + a.L.slot_bytes <= a.history_bytes) record = a.history + at;
-    }
-    uint8_t* codes = record ? record + (which - 1) * kCodes4 : nullptr;
-    quantize_rows4(z, a.mode, a.ratio[which], a.factor[which], codes,
-                   record ? record + kSide4 + 4 * (which - 1) : nullptr, g);
+      return at + a.L.slot_bytes <= a.history_bytes ? a.history + at : nullptr;
+    });
   }
 }
 
