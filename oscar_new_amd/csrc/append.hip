@@ -355,8 +355,8 @@ constexpr unsigned kWalkGroups = 256;  // one per CU
 // quantized at a time, four lanes each. Pairs of halves 32 dims or a multiple of it apart, and adjacent
 // ones, lie in one lane. 2048 tokens of 8 rows, one block a wavefront, are bound by what a block takes: 5 to
 // 7 us until R and the angles are there, 4 for the norm and the turn, 3 for the products (whose operands,
-// 128 KB a block, LDS hands over in 2), 4 for the records; 16384 by the same a block later, at 60 to 70 % of
-// what the rows' bytes would take.
+// 128 KB a block, LDS hands over in 2), 4 for the records. 16384 move their bytes at 60 to 70 % of a copy's
+// rate: a wavefront's next rows are on the way while it works on a block, and no more fit its registers.
 constexpr int kWalkWaves = 8, kWalkThreads = kWalkWaves * kWave;
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
