@@ -426,6 +426,32 @@ def test_order_statistics(n, ratio):
         assert torch.equal(codes, want[0].to(torch.uint8))
 
 
+@pytest.mark.parametrize("clip", [dict(v_clip_ratio=1.0), dict(v_clip_ratio=0.99), dict(v_clip_ratio=0.9),
+                                  dict(v_clip_ratio=0), dict(clip_mode="factor", v_clip_factor=0.8)])
+def test_rows_that_are_not_finite(clip):
+    """Infinities, overflows and NaN: many rows at a time and few give the same bytes, and other rows keep
+    theirs."""
+    n = 2400
+    m = list(make(n, 1, 1, 0))
+    value = m[2].clone()
+    value[0::7, 0, 3], value[1::7, 0, 5] = float("inf"), float("-inf")
+    value[2::7, 0, 90:101:10], value[3::7], value[4::7, 0, 9] = 3e38, value[3::7] * 1e38, float("nan")
+    layout = layout_of(1, **clip)
+    for rv_t in (m[8], torch.eye(256, dtype=torch.bfloat16, device=DEV)):
+        history, slots = cache(n, layout, n // 768 + 2)
+        few = history.clone()
+        finite = history.clone()
+        kernels.rope_append(None, m[1], value, history, slots, counts_of(n), layout, m[7], rv_t)
+        for a in range(0, n, 400):
+            part = slice(a, a + 400)
+            kernels.rope_append(None, m[1][part], value[part], few, slots[part].contiguous(), counts_of(400),
+                                layout, m[7], rv_t)
+        kernels.rope_append(None, m[1], m[2], finite, slots, counts_of(n), layout, m[7], rv_t)
+        assert torch.equal(history, few)
+        rows = [record_parts(h, layout, slots)[1][5::7] for h in (history, finite)]
+        assert torch.equal(*rows)
+
+
 @pytest.mark.parametrize("n", [40, 900])
 def test_a_captured_append_replays(n):
     m = make(n, 6, 1, 64, 3)
