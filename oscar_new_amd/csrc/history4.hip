@@ -67,6 +67,28 @@ __device__ __forceinline__ void wait_chunks(int chunks) {
     OSCAR_WAIT_VM(0);
 }
 
+// Sum over the wavefront and inclusive sums of its lanes, through data-parallel primitives: a launch waits for
+// these chains (with exchanges through LDS one request of 579 positions took 0.7 us more).
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
+  v += dpp_u32<kDppQuadXor1>(v);
+  v += dpp_u32<kDppQuadXor2>(v);
+  v += dpp_u32<kDppRowHalfMirror>(v);
+  v += dpp_u32<kDppRowMirror>(v);
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = r[0] + r[1];
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return r[0] + r[1];
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  constexpr int kShr1 = 0x111, kBcast15 = 0x142, kBcast31 = 0x143;
+  v += __builtin_amdgcn_update_dpp(0, v, kShr1, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, kShr1 + 1, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, kShr1 + 3, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, kShr1 + 7, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, kBcast15, 0xa, 0xf, false);  // rows 1 and 3: the row below's last
+  return v + __builtin_amdgcn_update_dpp(0, v, kBcast31, 0xc, 0xf, false);  // the upper half: lane 31's
+}
+
 // The unit of workgroup slot u under the device rule: split lengths T such that the tasks' splits,
 // ceil(length / T) each, fit the budget's slots of one KV head (or one a task where it is smaller).
 // All splits run at once, one per CU, so the launch takes as long as T: eight lengths between the mean
@@ -99,7 +121,9 @@ __device__ bool unit_of_slot(const AttnArgs& a, int programs, int u, int* length
     mine = t;
     mine_task = i;
   }
-  sum = wave_sum_i64(sum);
+  // A thread has at most 32 lengths below 2^31.
+  sum = (static_cast<int64_t>(wave_sum_u32(static_cast<uint32_t>(sum >> 20))) << 20) +
+        wave_sum_u32(static_cast<uint32_t>(sum) & 0xfffffu);
   if (lane == 0) s_total[wave] = sum;
   if (tid == 0) s_found[0] = -1;
   __syncthreads();
@@ -127,8 +151,7 @@ __device__ bool unit_of_slot(const AttnArgs& a, int programs, int u, int* length
     const int t = tried(k);
     int units = 0;
     for (int i = lane; i < count; i += kWave) units += history_splits(a, max(lengths[i], 0), t);
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) units += __shfl_xor(units, m, kWave);
+    units = static_cast<int>(wave_sum_u32(static_cast<uint32_t>(units)));
     if (lane == 0) s_fit[k] = units <= slots;
   }
   __syncthreads();
@@ -141,12 +164,7 @@ __device__ bool unit_of_slot(const AttnArgs& a, int programs, int u, int* length
   for (int c0 = 0; c0 < programs; c0 += kThreads4) {
     const int i = c0 + tid;
     const int ns = i < count && lengths[i] >= 0 ? history_splits(a, lengths[i], st) : 0;
-    int incl = ns;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int y = __shfl_up(incl, d, kWave);
-      incl += lane >= d ? y : 0;
-    }
+    const int incl = wave_scan(ns);
     if (lane == kWave - 1) s_carry[wave] = incl;
     __syncthreads();
     int before = carry, chunk = 0;
@@ -617,12 +635,7 @@ __device__ __forceinline__ bool find_tile4(const AttnArgs& a, int max_reqs, int 
       const int q0 = a.qstarts[r], rows = (min(a.qstarts[r + 1], active) - q0) * a.g;
       tiles = rows > 0 ? (rows + 16 * F::RG - 1) / (16 * F::RG) : 0;
     }
-    int incl = tiles;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int y = __shfl_up(incl, d, kWave);
-      incl += lane >= d ? y : 0;
-    }
+    const int incl = wave_scan(tiles);
     if (lane == kWave - 1) s_carry[wave] = incl;
     __syncthreads();
     int before = carry, all = 0;
