@@ -20,9 +20,9 @@
 // operand comes from transposed LDS reads of 4-bit codes. The eight states are joined at the end.
 //
 // Up to 16 rows the records' bytes bound it: 32 requests of 32636 positions (284 MB) take 52 us, 5.5 TB/s
-// where a large copy moves 5.2 (reads alone reach 7); a small step its chain (one request of 579 positions 10.8
-// us: 3.3 until the unit is known, 1.5 until its records are there, 0.7 for the query operands, 2 for a
-// wavefront's chunk, 3 for the join). Tiles of 32 rows are bound by the vector units, which
+// where a large copy moves 5.2 (reads alone reach 7); a small step its chain (one request of 579 positions 10.1
+// us: 2.5 until the unit is known, 1.6 until its records are there, 0.6 for the query operands, 1.7 for a
+// wavefront's chunk, 2.6 for the join). Tiles of 32 rows are bound by the vector units, which
 // issue in 78 % of the cycles (the matrix units' share is 38 %): a wavefront's 32 positions cost 400 vector
 // instructions, of which the unpacking, 224, is paid once per tile, and 64 matrix instructions: 2048 tokens
 // of 6 heads against 30400 positions take 447 us, 0.86 PFLOP/s. Tiles of 48 or 64 rows, on one wavefront a
@@ -94,8 +94,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 // All splits run at once, one per CU, so the launch takes as long as T: eight lengths between the mean
 // share and the one that always fits are tried, one by each wavefront, and the least that fits is
 // taken (32 requests of 32636 positions on 256 slots: 8 splits of 4096 each). Multiples of kStep4, at
-// least kMinSplit4, one chunk for a wavefront of each SIMD (one request of 579 positions with its merge: 15.9
-// us in splits of 128, 16.8 of 256).
+// least kMinSplit4, one chunk for a wavefront of each SIMD (one request of 579 positions with its merge: 0.9
+// us less than in splits of 256).
 constexpr int kMinSplit4 = 128, kStep4 = 64, kTried4 = 8;
 
 struct Unit4 {
