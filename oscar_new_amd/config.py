@@ -18,6 +18,9 @@ from dataclasses import dataclass
 
 # Clip modes as passed across the C ABI.
 CLIP_MODES = {"percentile": 0, "factor": 1, "search": 2}
+# Percentiles of K and V by the bits of a record: the reference's for 2 bits. 4-bit records want less
+# clipping (mean squared error of Gaussian rows at 0.99 0.0110 of their own, at 0.96 0.0159, at 0.92 0.0277).
+CLIP_RATIOS = {2: (0.96, 0.92), 4: (0.99, 0.99)}
 
 
 @dataclass(frozen=True)
@@ -29,8 +32,8 @@ class OscarConfig:
     sink_tokens: int = 64
     recent_tokens: int = 256
     speculative_tokens: int = 3
-    k_clip_ratio: float = 0.96
-    v_clip_ratio: float = 0.92
+    k_clip_ratio: float | None = None  # None: CLIP_RATIOS of history_bits
+    v_clip_ratio: float | None = None
     clip_mode: str = "percentile"
     k_clip_factor: float = 1.0
     v_clip_factor: float = 1.0
@@ -41,6 +44,10 @@ class OscarConfig:
     history_bits: int = 2  # per code of a history record: 2 (the reference's), or 4
 
     def __post_init__(self):
+        for name, ratio in zip(("k_clip_ratio", "v_clip_ratio"),
+                               CLIP_RATIOS.get(self.history_bits, CLIP_RATIOS[2])):
+            if getattr(self, name) is None:
+                object.__setattr__(self, name, ratio)
         for ok, message in _config_rules(self):
             if not ok:
                 raise ValueError(message)
@@ -73,18 +80,20 @@ class OscarConfig:
     @classmethod
     def from_env(cls, speculative_tokens=3):
         """Reference: config.py:65-81 (same variable names and defaults). ``OSCAR_AMD_HISTORY_BITS=4``
-        keeps the history in 4-bit records, which want less clipping: then the percentiles default to
-        0.99 (mean squared error of Gaussian rows 0.0110 of their own, at 0.96 0.0159)."""
-        bits = int(os.getenv("OSCAR_AMD_HISTORY_BITS", "2"))
-        k_ratio, v_ratio = ("0.96", "0.92") if bits == 2 else ("0.99", "0.99")
+        keeps the history in 4-bit records."""
+
+        def ratio(name):
+            value = os.getenv(name)
+            return None if value is None else float(value)
+
         return cls(
-            history_bits=bits,
+            history_bits=int(os.getenv("OSCAR_AMD_HISTORY_BITS", "2")),
             group_size=int(os.getenv("VLLM_OSCAR_GROUP_SIZE", "256")),
             sink_tokens=int(os.getenv("VLLM_OSCAR_SINK_TOKENS", "64")),
             recent_tokens=int(os.getenv("VLLM_OSCAR_RECENT_TOKENS", "256")),
             speculative_tokens=speculative_tokens,
-            k_clip_ratio=float(os.getenv("VLLM_OSCAR_K_CLIP_RATIO", k_ratio)),
-            v_clip_ratio=float(os.getenv("VLLM_OSCAR_V_CLIP_RATIO", v_ratio)),
+            k_clip_ratio=ratio("VLLM_OSCAR_K_CLIP_RATIO"),
+            v_clip_ratio=ratio("VLLM_OSCAR_V_CLIP_RATIO"),
             clip_mode=os.getenv("OSCAR_ASCEND_CLIP_MODE", "percentile"),
             k_clip_factor=float(os.getenv("OSCAR_ASCEND_K_CLIP_FACTOR", "1")),
             v_clip_factor=float(os.getenv("OSCAR_ASCEND_V_CLIP_FACTOR", "1")),
