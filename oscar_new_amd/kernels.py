@@ -460,7 +460,7 @@ def dequant_inverse_rotate(history, slots, rk, rv, layout):
     if n > 4096:
         raise ValueError("Diagnostic dequant is limited to 4096 tokens; use fused attention")
     if layout.config.history_bits == 4:
-        k, v = read_records(history, slots, layout)
+        k, v = read_records(history, slots.to(torch.int64).reshape(-1), layout)
         return rotate(k, rk.T), rotate(v, rv.T)
     k = torch.empty((n, h, d), device=history.device, dtype=torch.bfloat16)
     v = torch.empty_like(k)
