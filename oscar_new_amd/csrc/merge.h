@@ -206,8 +206,10 @@ __device__ __forceinline__ uint2 merge_splits_out(const SplitMerge& r) {
   return make_uint2(pack_bf16x2(r.acc[0] / dn, r.acc[1] / dn),
                     pack_bf16x2(r.acc[2] / dn, r.acc[3] / dn));
 }
+// -inf where no split has weight; NaN where a split's LSE is, as the merged row is then.
 __device__ __forceinline__ float merge_splits_lse(const SplitMerge& r) {
-  return r.den > 0.f ? r.mx + logf(fmaxf(r.den, kDenFloor)) : -INFINITY;
+  if (r.den == 0.f) return -INFINITY;
+  return r.den > 0.f ? r.mx + logf(fmaxf(r.den, kDenFloor)) : r.den;
 }
 
 // kernels.py:514-527: (e^{la-M} a + e^{lb-M} b) / (e^{la-M} + e^{lb-M}), M = max(la, lb)
@@ -228,7 +230,9 @@ __device__ __forceinline__ float path_merge(const PathWeights& w, float a, float
   return fmaf(w.wa, a, w.wb * b) / w.den;
 }
 __device__ __forceinline__ float path_lse(const PathWeights& w) {
-  return (w.wa + w.wb) > 0.f ? w.mx + logf(w.wa + w.wb) : -INFINITY;
+  const float sum = w.wa + w.wb;
+  if (sum == 0.f) return -INFINITY;
+  return sum > 0.f ? w.mx + logf(sum) : sum;  // NaN stays NaN
 }
 
 }  // namespace oscar
