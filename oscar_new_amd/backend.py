@@ -393,6 +393,8 @@ class OscarAttentionImpl:
         both attention branches, their merge and the windows. ``query`` and ``query_rot``
         [n, heads, 256], ``key`` and ``value`` [n, kv_heads, 256]; returns ``output``
         (contiguous, [n, heads * 256])."""
+        if attn_metadata is None:  # profiling run: nothing scheduled
+            return output.zero_()
         meta, n = attn_metadata, query.shape[0]
         if self.rv is None:
             raise RuntimeError("this OSCAR layer has no rotations: initialize_layer runs after "
