@@ -423,7 +423,8 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
   float v_by = 1.f;
   f32x4 o[RG][16];  // o[c]: rows 4 g + v, dim 16 c + n
   auto set_scale = [&](float top) {
-    const uint32_t eb = min(__float_as_uint(top) >> 23, 250u);
+    // From fp16's least value, 2^-24, on: with a first chunk of zeros the scaled V scales stay finite.
+    const uint32_t eb = min(max(__float_as_uint(top) >> 23, 127u - 24u), 250u);
     v_by = __uint_as_float((127 + 126 - eb) << 23);  // the largest lies in [0.5, 1)
   };
 #pragma unroll
