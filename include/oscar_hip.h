@@ -209,7 +209,8 @@ int64_t oscar_history_chunk_tiles(int64_t n, int64_t max_reqs, int64_t programs,
 /*
  * merge_splits -- replaces kernels.py:506-511 `merge_splits(partials, lse, counts)`.
  * out[t, q, :] = sum_s e^{lse_s - M} P_s / sum_s e^{lse_s - M} (bf16) and
- * logsum[t, q] = M + log(sum) or -inf; rows t >= counts[1] become 0 / -inf.
+ * logsum[t, q] = M + log(sum) or -inf; NaN (as the row) where a split's LSE is; rows t >= counts[1] become
+ * 0 / -inf.
  */
 int oscar_merge_splits(const float* partials, const float* lse, const int32_t* counts, int64_t n,
                        int64_t hq, int32_t splits, int32_t d, void* out, float* logsum,

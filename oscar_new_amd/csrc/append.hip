@@ -11,9 +11,10 @@
 // ones those of oscar_rotate and 2-bit records the bytes of oscar_store_int2.
 //
 // Three forms. Few rows: blocks of 16 (token, head) rows on as many CUs as there are blocks, bound by the
-// chain counts - positions - angles - norm - product - quantile - record (10.5 us for 32 tokens of 6 + 1
-// heads, 11.3 for 512). Many rows of 4-bit layouts: wavefronts that walk 16-row blocks (15.2 us for 2048
-// tokens, 52 for 16384, 181 MB). Rows that are turned only: no product, the rows' bytes.
+// chain counts - positions - angles - norm - product - quantile - record (11.6 us for 32 tokens of 6 + 1
+// heads, 12.2 for 512; kernel times here and below). Many rows of 4-bit layouts: wavefronts that walk 16-row
+// blocks (15.7 us for 2048 tokens, 50 to 52 for 16384, 181 MB). Rows that are turned only: no product, the
+// rows' bytes.
 #include "dma.h"
 #include "norm_row.h"
 #include "quant4.h"
@@ -341,9 +342,10 @@ void append_kernel(const AppendArgs a, int64_t q_blocks, int64_t k_blocks) {
   }
 }
 
-// Rows up to which blocks of 16 find a CU each. 512 tokens of 8 rows: 11.3 us, against 15.4 in blocks of 32
-// and 13 by walking wavefronts; 768: 17.6, 15.9 and 13; 2048: 31, 24 and 15.2. Blocks of 32 remain for
-// what the walk does not serve (`walks`).
+// Rows up to which blocks of 16 find a CU each. 512 tokens of 8 rows: 12.2 us, against 15.9 in blocks of 32
+// and 13.0 by walking wavefronts; 768: 18.5, 16.3 and 13.4; 2048: 33, 25.9 and 15.7. Blocks of 32 remain for
+// what the walk does not serve (`walks`), and load R anew each: 16384 tokens with 96 rotary dims in halves
+// 149 us, with 2-bit records 145.
 constexpr int64_t kSmallAppendRows = 16 * 256;
 constexpr unsigned kWalkGroups = 256;  // one per CU
 
@@ -888,7 +890,7 @@ __global__ __launch_bounds__(kWalkThreads, 2) void append_walk_kernel(const Appe
 }
 
 // ---- records back to values: half a wavefront per record, 8 dims a lane of either vector, two records in
-// flight. 2048 records take 3.1 us, 16384 6.0 (21 MB, 3.5 TB/s).
+// flight. 2048 records take 3.4 us, 16384 6.0 (21 MB, 3.5 TB/s) to 6.8.
 struct ReadArgs {
   const uint8_t* history;
   int64_t history_bytes;
@@ -959,8 +961,9 @@ RowSet row_set(const void* x, int64_t s0, int64_t s1, const void* weight, void* 
 // The workgroups for the values such that the longer of both kinds' walks is shortest. A CU's wavefronts
 // share its four SIMDs, so the largest number of blocks of a SIMD counts, each at its cost in units of about
 // 1 us: a value 6 (product and quantizer), a key 6, a query 3, a norm 2 more, a query's product 3. 16384
-// tokens of 6 heads, normed and rotated: 32 workgroups 71.5 us, 24 71.7, 64 78.6; 4 heads that are only
-// turned: 64 32.1, 52 32.8, 44 38.5, 80 34.5; 2048 tokens of 12: 32 22.3, 28 23.1, 36 28.6.
+// tokens of 6 heads, normed and rotated: 32 workgroups 50.6 us, 28 55.9, 40 52.8, 64 56.0; 4 heads that are only
+// turned: 64 27.8, 52 29.8, 44 35.5, 80 29.0; 2048 tokens of 12: 32 19.7, 28 22.0, 36 21.7. The 255
+// trials take the host 2.7 us a call.
 int value_groups_of(int64_t q_blocks, int64_t kv_blocks, bool rotated, bool normed) {
   const int64_t k_cost = normed ? 8 : 6, q_cost = 3 + (normed ? 2 : 0) + (rotated ? 3 : 0);
   auto of_simd = [](int64_t blocks, int64_t groups) { return (blocks + 4 * groups - 1) / (4 * groups); };

@@ -25,7 +25,7 @@
 // wavefront's chunk, 2.6 for the join). Tiles of 32 rows are bound by the vector units, which
 // issue in 78 % of the cycles (the matrix units' share is 38 %): a wavefront's 32 positions cost 400 vector
 // instructions, of which the unpacking, 224, is paid once per tile, and 64 matrix instructions: 2048 tokens
-// of 6 heads against 30400 positions take 447 us, 0.86 PFLOP/s. Tiles of 48 or 64 rows, on one wavefront a
+// of 6 heads against 30400 positions take 456 us, 0.84 PFLOP/s. Tiles of 48 or 64 rows, on one wavefront a
 // SIMD with 512 registers, halve the unpacking's share but have no second wavefront that fills the waits:
 // 617 and 632 us. Codes as fp16 subnormals (five instructions for eight instead of seven) lose the low bits
 // of the products (errors 2.5e-5 of the sum of magnitudes, which the matrix instruction aligns as if the
@@ -418,7 +418,8 @@ __device__ __forceinline__ void history_rows4(const AttnArgs& a, const Task& t, 
   // then no sum is ever scaled again, and the accumulators stay where the matrix instructions want them
   // (rescaling them as a running maximum grows made the compiler move them about: two row groups spilled
   // registers). Should a later score or scale have needed more room, the wavefront goes through its chunks
-  // again, with the largest ones, which it knows by then.
+  // again, with the largest ones, which it knows by then (32 requests of 32636 positions, one late position of
+  // each with scores 15 nats above the mean: 63 us instead of 52).
   float m_ref[RG], m_less[RG], psum[RG], zsum[RG];
   float v_by = 1.f;
   f32x4 o[RG][16];  // o[c]: rows 4 g + v, dim 16 c + n
