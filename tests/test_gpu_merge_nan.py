@@ -6,7 +6,7 @@ import torch
 
 from oscar_new_amd import kernels
 from tests._int4 import DEV, layout_of, world
-from tests.test_gpu_int4 import SCALE, attend
+from tests.test_gpu_int4 import attend, check
 from tests.test_gpu_int4_step import Served
 
 pytestmark = pytest.mark.gpu
@@ -88,6 +88,20 @@ def test_one_nan_record(qlens, splits, split_tokens, chunk, value):
     assert torch.equal(out[~bad], want[~bad]) and torch.equal(lse[~bad], want_lse[~bad])
     assert torch.equal(lse.isnan(), bad & (not value))  # weights are whole where a value is not
     assert value is False or torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("splits,split_tokens", [(8, -256), (40, 128), (1, 0)])
+def test_queries_that_are_not_finite(splits, split_tokens):
+    """An infinite score makes its wavefront take all of its rows against another reference: the others stay
+    within rounding."""
+    s = world([700, 3000], [1, 1], layout_of(2), 4)
+    query = s.query.clone()
+    query[0, 3, 7], query[1, 0, 0], query[1, 5, 9] = float("nan"), float("inf"), float("-inf")
+    out, lse = attend(s, splits, split_tokens, query=query)
+    bad = torch.zeros(2, 8, dtype=torch.bool, device=DEV)
+    bad[0, 3] = bad[1, 0] = bad[1, 5] = True
+    assert torch.equal(out.isnan().all(-1), bad) and torch.equal(lse.isnan(), bad)
+    check(s, (out, lse), but=bad)
 
 
 @pytest.mark.parametrize("counts", [[1, 1, 1], [3, 1, 4], [40, 1, 2]])
